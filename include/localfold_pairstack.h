@@ -558,6 +558,120 @@ LF_API lf_status lf_peer_buffer_destroy(lf_context* ctx, void* ptr);
 LF_API lf_status lf_pair_transpose_scatter(lf_context* ctx, const void* src, int32_t rows, int32_t length,
                                            int32_t vector_bytes, int32_t ranks, int32_t rank, void* const* dst);
 
+/* ------------------------------------------------------------------------------------------
+ * Training and 8-bit operators.  The reference runs the stack forward only and keeps nothing in
+ * 8 bits: no counterpart there.
+ *
+ * Every buffer of these calls is device memory of the context's GPU, tensors may start at any
+ * element, and nothing is allocated or kept by the library: what a call needs besides its tensors is the
+ * `workspace` that its *_workspace function gives the size of (16-byte aligned; its content
+ * means nothing between calls).  So a call can be captured into a CUDA graph as it is, and two
+ * graphs with workspaces of their own are independent.  Rows of tensors follow one another without gaps.
+ * ------------------------------------------------------------------------------------------ */
+
+/* The 8-bit form of a float matrix [rows][channels].  128 consecutive channels of a row share one
+ * power of two: the least that brings the largest finite magnitude of the block to the format's
+ * largest code (448 or 57344), 2^-126 at least.  A code is the value over that power, rounded to
+ * nearest; NaN stays NaN, an infinity becomes NaN in E4M3 (which has none) and stays one in E5M2.
+ * codes: [rows][channels rounded up to 16], zeros behind the last channel.  exponents: the
+ * powers' biased bytes (value + 127), tiles of 512 bytes [ceil(channels / 512)][ceil(rows / 128)],
+ * in a tile [row % 32][row % 128 / 32][channel % 512 / 128].  Both start on 16-byte boundaries; bytes
+ * of exponents that belong to no block are of no account.  codes null: no matrix. */
+typedef enum lf_float8_format { LF_FLOAT8_E4M3 = 0, LF_FLOAT8_E5M2 = 1 } lf_float8_format;
+typedef struct lf_float8_matrix {
+  int64_t rows;
+  int32_t channels, format;
+  void* codes;
+  void* exponents;
+} lf_float8_matrix;
+LF_API uint64_t lf_float8_code_bytes(int64_t rows, int32_t channels);
+LF_API uint64_t lf_float8_exponent_bytes(int64_t rows, int32_t channels);
+
+/* source [out.rows][out.channels] of `dtype` -> out.  block_rows 128 (weights) makes one power of
+ * two for 128 x 128 elements, and `transposed` (codes null: none) then receives the same values with rows and
+ * channels exchanged. */
+typedef struct lf_float8_encode_desc {
+  lf_float8_matrix out, transposed;
+  int32_t dtype, block_rows;
+  const void* source;
+} lf_float8_encode_desc;
+LF_API lf_status lf_float8_encode(lf_context* ctx, const lf_float8_encode_desc* d, lf_result* r);
+/* out [source.rows][source.channels] of `dtype` = the values of source (exact in either type). */
+typedef struct lf_float8_decode_desc {
+  lf_float8_matrix source;
+  int32_t dtype, reserved;
+  void* out;
+} lf_float8_decode_desc;
+LF_API lf_status lf_float8_decode(lf_context* ctx, const lf_float8_decode_desc* d, lf_result* r);
+
+/* LayerNorm over the channels of each row, at most 8192: y = (x - mean) inverse_deviation scale + offset, inverse_deviation =
+ * 1 / sqrt(variance + epsilon), statistics in float32 over two passes whatever `variance` says.
+ * Any of the results may be left out, but not both of out and encoded: out of act_dtype (may be
+ * activations itself), the statistics [rows] float32 (both or neither), the input's 8-bit form
+ * (checkpoint) for the backward pass, the output's 8-bit form (encoded, of y before it is rounded
+ * to act_dtype) for a projection on 8-bit operands. */
+typedef struct lf_layer_norm_desc {
+  int64_t rows;
+  int32_t channels, variance, act_dtype;
+  float epsilon;
+  const void* activations;
+  const float* scale;             /* [channels] */
+  const float* offset;            /* [channels] */
+  void* out;
+  float* mean;
+  float* inverse_deviation;
+  lf_float8_matrix checkpoint, encoded;
+} lf_layer_norm_desc;
+LF_API lf_status lf_layer_norm_run(lf_context* ctx, const lf_layer_norm_desc* d, lf_result* r);
+/* Its gradients from gradient = dL/dy (act_dtype) and the statistics of the forward pass: out = dL/dx
+ * (act_dtype; may be gradient itself), dL/dscale and dL/doffset [channels] float32.  The input is given whole
+ * (activations, act_dtype) or as the checkpoint.  Results do not depend on how the GPU schedules the
+ * blocks. */
+typedef struct lf_layer_norm_backward_desc {
+  int64_t rows;
+  int32_t channels, act_dtype;
+  const void* gradient;
+  const void* activations;        /* or null: */
+  lf_float8_matrix checkpoint;
+  const float* mean;
+  const float* inverse_deviation;
+  const float* scale;
+  void* out;
+  float* scale_gradient;
+  float* offset_gradient;
+  void* workspace;
+  uint64_t workspace_bytes;
+} lf_layer_norm_backward_desc;
+LF_API uint64_t lf_layer_norm_backward_workspace(const lf_context* ctx, int64_t rows, int32_t channels);
+LF_API lf_status lf_layer_norm_backward_run(lf_context* ctx, const lf_layer_norm_backward_desc* d, lf_result* r);
+
+/* out[m][n] = sum_k activations[m][k] weights[n][k] (+ bias[n]), float32 sums, out_dtype rows.  The
+ * gradient of a projection's input is the same call on the encoded gradient and the transposed
+ * weights. */
+typedef struct lf_float8_linear_desc {
+  lf_float8_matrix activations;   /* [rows][channels] */
+  lf_float8_matrix weights;       /* [out channels][channels] */
+  const float* bias;              /* [out channels] or null */
+  int32_t out_dtype, reserved;
+  void* out;
+} lf_float8_linear_desc;
+LF_API lf_status lf_float8_linear_run(lf_context* ctx, const lf_float8_linear_desc* d, lf_result* r);
+/* weight_gradient [out channels][channels] = sum over rows of gradient[row][n] activations[row][k], bias_gradient [out channels]
+ * (or null) = sum of gradient[row][n], float32.  gradient: bf16 rows, or its 8-bit form; activations: the 8-bit
+ * form that the forward pass multiplied with. */
+typedef struct lf_float8_weight_gradient_desc {
+  lf_float8_matrix activations;
+  const void* gradient;           /* bf16, or null: */
+  lf_float8_matrix encoded_gradient;
+  int32_t out_channels, reserved;
+  float* weight_gradient;
+  float* bias_gradient;
+  void* workspace;
+  uint64_t workspace_bytes;
+} lf_float8_weight_gradient_desc;
+LF_API uint64_t lf_float8_weight_gradient_workspace(const lf_context* ctx, int64_t rows, int32_t channels, int32_t out_channels);
+LF_API lf_status lf_float8_weight_gradient_run(lf_context* ctx, const lf_float8_weight_gradient_desc* d, lf_result* r);
+
 #ifdef __cplusplus
 }
 #endif

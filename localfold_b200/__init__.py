@@ -12,3 +12,6 @@ from .operators import (  # noqa: F401
 )
 from .pipeline import PairStackPipeline  # noqa: F401
 from .stack import Af3MsaBlockGpu, Af3MsaStackGpu, Af3PairformerStackGpu, EvoformerBlockGpu, EvoformerStackGpu, ExtraMsaBlockGpu, ExtraMsaStackGpu, PairStackGpu, PreparedMsaBlock, PreparedPairBlock  # noqa: F401
+from .training import (  # noqa: F401
+    Float8LinearGpu, Float8LinearWeights, Float8Tensor, LayerNormGpu, float8_decode, float8_encode, prepare_float8_linear_weights,
+)

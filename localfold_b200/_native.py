@@ -139,6 +139,44 @@ class ShardPeers(ctypes.Structure):
                 ("x", c_void_p * 16), ("bias", c_void_p * 16)]
 
 
+class Float8Matrix(ctypes.Structure):
+    _fields_ = [("rows", c_int64), ("channels", c_int32), ("format", c_int32), ("codes", c_void_p), ("exponents", c_void_p)]
+
+
+class Float8EncodeDesc(ctypes.Structure):
+    _fields_ = [("out", Float8Matrix), ("transposed", Float8Matrix), ("dtype", c_int32), ("block_rows", c_int32), ("source", c_void_p)]
+
+
+class Float8DecodeDesc(ctypes.Structure):
+    _fields_ = [("source", Float8Matrix), ("dtype", c_int32), ("reserved", c_int32), ("out", c_void_p)]
+
+
+class LayerNormDesc(ctypes.Structure):
+    _fields_ = [("rows", c_int64), ("channels", c_int32), ("variance", c_int32), ("act_dtype", c_int32), ("epsilon", c_float),
+                ("activations", c_void_p), ("scale", c_void_p), ("offset", c_void_p), ("out", c_void_p), ("mean", c_void_p),
+                ("inverse_deviation", c_void_p), ("checkpoint", Float8Matrix), ("encoded", Float8Matrix)]
+
+
+class LayerNormBackwardDesc(ctypes.Structure):
+    _fields_ = [("rows", c_int64), ("channels", c_int32), ("act_dtype", c_int32), ("gradient", c_void_p), ("activations", c_void_p),
+                ("checkpoint", Float8Matrix), ("mean", c_void_p), ("inverse_deviation", c_void_p), ("scale", c_void_p),
+                ("out", c_void_p), ("scale_gradient", c_void_p), ("offset_gradient", c_void_p), ("workspace", c_void_p),
+                ("workspace_bytes", ctypes.c_uint64)]
+
+
+class Float8LinearDesc(ctypes.Structure):
+    _fields_ = [("activations", Float8Matrix), ("weights", Float8Matrix), ("bias", c_void_p), ("out_dtype", c_int32),
+                ("reserved", c_int32), ("out", c_void_p)]
+
+
+class Float8WeightGradientDesc(ctypes.Structure):
+    _fields_ = [("activations", Float8Matrix), ("gradient", c_void_p), ("encoded_gradient", Float8Matrix), ("out_channels", c_int32),
+                ("reserved", c_int32), ("weight_gradient", c_void_p), ("bias_gradient", c_void_p), ("workspace", c_void_p),
+                ("workspace_bytes", ctypes.c_uint64)]
+
+
+FLOAT8_E4M3, FLOAT8_E5M2 = 0, 1
+
 EXPORTS = (
     "lf_version", "lf_context_create", "lf_context_create_on_stream", "lf_context_stream", "lf_context_await", "lf_context_destroy", "lf_last_error", "lf_context_synchronize",
     "lf_context_launch_count", "lf_context_profile", "lf_context_profile_read", "lf_context_reserve", "lf_context_release_scratch", "lf_context_limit_scratch", "lf_weights_create", "lf_weights_create_encoded",
@@ -148,6 +186,9 @@ EXPORTS = (
     "lf_global_column_attention_run", "lf_distogram_logits_run", "lf_pair_stack_run", "lf_pair_stack_run_from",
     "lf_pair_shard_step", "lf_pair_shard_exchange_step", "lf_pair_planes_scatter", "lf_peer_buffer_create", "lf_peer_buffer_open", "lf_peer_buffer_close",
     "lf_peer_buffer_destroy", "lf_pair_transpose_scatter",
+    "lf_float8_code_bytes", "lf_float8_exponent_bytes", "lf_float8_encode", "lf_float8_decode", "lf_layer_norm_run",
+    "lf_layer_norm_backward_workspace", "lf_layer_norm_backward_run", "lf_float8_linear_run",
+    "lf_float8_weight_gradient_workspace", "lf_float8_weight_gradient_run",
 )
 
 _lib = None
@@ -196,7 +237,10 @@ def load():
                        ("lf_single_attention_run", SingleAttentionDesc), ("lf_msa_attention_run", MsaAttentionDesc),
                        ("lf_global_column_attention_run", GlobalAttentionDesc),
                        ("lf_distogram_logits_run", DistogramDesc), ("lf_pair_stack_run", PairStackDesc),
-                       ("lf_pair_shard_step", ShardStepDesc)):
+                       ("lf_pair_shard_step", ShardStepDesc), ("lf_float8_encode", Float8EncodeDesc),
+                       ("lf_float8_decode", Float8DecodeDesc), ("lf_layer_norm_run", LayerNormDesc),
+                       ("lf_layer_norm_backward_run", LayerNormBackwardDesc), ("lf_float8_linear_run", Float8LinearDesc),
+                       ("lf_float8_weight_gradient_run", Float8WeightGradientDesc)):
         getattr(lib, name).argtypes = [c_void_p, ctypes.POINTER(desc), ctypes.POINTER(Result)]
     lib.lf_pair_stack_run_from.argtypes = [c_void_p, ctypes.POINTER(PairStackDesc), c_void_p, ctypes.POINTER(Result)]
     lib.lf_pair_shard_exchange_step.argtypes = [c_void_p, ctypes.POINTER(ShardStepDesc), ctypes.POINTER(ShardPeers),
@@ -208,6 +252,11 @@ def load():
     lib.lf_peer_buffer_destroy.argtypes = [c_void_p, c_void_p]
     lib.lf_pair_transpose_scatter.argtypes = [c_void_p, c_void_p, c_int32, c_int32, c_int32, c_int32, c_int32,
                                               ctypes.POINTER(c_void_p)]
+    for name, args in (("lf_float8_code_bytes", [c_int64, c_int32]), ("lf_float8_exponent_bytes", [c_int64, c_int32]),
+                       ("lf_layer_norm_backward_workspace", [c_void_p, c_int64, c_int32]),
+                       ("lf_float8_weight_gradient_workspace", [c_void_p, c_int64, c_int32, c_int32])):
+        getattr(lib, name).argtypes = args
+        getattr(lib, name).restype = ctypes.c_uint64
     _lib = lib
     return lib
 

@@ -1,0 +1,228 @@
+// To and from the 8-bit form of a matrix (float8.cuh): activations with an exponent for every 128 channels of a row, weights with one
+// for every 128 x 128 elements, both orientations in one pass.
+//
+// Each element is read and written once and needs a handful of instructions: memory bounds these kernels.  Sixteen lanes hold a
+// block of 128 channels, eight neighbours each (narrow rows: eight lanes for at most 64 channels), so that the block's largest magnitude takes
+// four shuffles and codes leave as eight bytes a lane; every lane keeps kUnits blocks in flight.
+#include "float8.cuh"
+
+namespace f8 {
+
+constexpr int kThreads = 256, kUnits = 4;
+
+template <typename T, int LANES>
+__global__ void __launch_bounds__(kThreads)
+encode_kernel(const T* x, const Matrix m, uint32_t units, uint32_t per_row, int vector) {
+  const int lane = threadIdx.x % LANES;
+  const uint32_t base = blockIdx.x * (uint32_t)(kThreads / LANES * kUnits) + threadIdx.x / LANES;
+  lf_chain();
+  float v[kUnits][8];
+  uint32_t row[kUnits], first[kUnits];
+#pragma unroll
+  for (int u = 0; u < kUnits; ++u) {
+    const uint32_t unit = base + u * (kThreads / LANES);
+    row[u] = per_row == 1 ? unit : unit / per_row;
+    first[u] = (unit - row[u] * per_row) * kBlock + lane * 8;
+    load8(x + (int64_t)row[u] * m.channels + first[u], unit < units ? m.channels - (int)first[u] : 0, vector, v[u]);
+  }
+#pragma unroll
+  for (int u = 0; u < kUnits; ++u) {
+    uint2 codes;
+    const int s = encode8<LANES>(v[u], m.format, codes);
+    if (base + u * (kThreads / LANES) < units) put8(m, row[u], first[u], codes, s, lane == 0);
+  }
+}
+
+template <typename T, int LANES>
+__global__ void __launch_bounds__(kThreads)
+decode_kernel(const Matrix m, T* out, uint32_t units, uint32_t per_row, int vector) {
+  const int lane = threadIdx.x % LANES;
+  const uint32_t base = blockIdx.x * (uint32_t)(kThreads / LANES * kUnits) + threadIdx.x / LANES;
+  lf_chain();
+  uint2 codes[kUnits];
+  int s[kUnits];
+  uint32_t row[kUnits], first[kUnits];
+#pragma unroll
+  for (int u = 0; u < kUnits; ++u) {
+    const uint32_t unit = base + u * (kThreads / LANES);
+    row[u] = per_row == 1 ? unit : unit / per_row;
+    const uint32_t block = unit - row[u] * per_row;
+    first[u] = block * kBlock + lane * 8;
+    if (unit >= units) first[u] = (uint32_t)m.channels;      // nothing left to write
+    codes[u] = make_uint2(0, 0);
+    s[u] = 1;
+    if (first[u] < (uint32_t)m.channels) {
+      codes[u] = *reinterpret_cast<const uint2*>(m.codes + row[u] * m.pitch + first[u]);
+      s[u] = m.exponents[exponent_at(row[u], block, m.tiles)];
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < kUnits; ++u) {
+    if (first[u] >= (uint32_t)m.channels) continue;
+    float v[8];
+    decode8(codes[u], up(s[u]), m.format, v);
+    store8(out + (int64_t)row[u] * m.channels + first[u], m.channels - (int)first[u], vector, v);
+  }
+}
+
+// One 128 x 128 block a block of threads: its largest magnitude, its codes in rows, and (t.codes set) the same codes with rows and
+// channels exchanged - the exponent is the block's, so the transposed matrix stands for the same values.
+template <typename T>
+__global__ void __launch_bounds__(kThreads)
+encode_square_kernel(const T* x, const Matrix m, const Matrix t, int vector) {
+  __shared__ uint32_t most_s[2][kThreads / 32];
+  __shared__ uint8_t turned[kBlock][kBlock + 8];
+  const int lane = threadIdx.x & 15, strand = threadIdx.x >> 4;
+  const int64_t row0 = (int64_t)blockIdx.y * kBlock;
+  const int first = blockIdx.x * kBlock + lane * 8;
+  lf_chain();
+  float v[8][8];
+  uint32_t most = 0, finite = 0;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    const int64_t row = row0 + strand + 16 * k;
+    load8(x + row * m.channels + first, row < m.rows ? m.channels - first : 0, vector, v[k]);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      most = max(most, magnitude(v[k][i]));
+      finite = max(finite, magnitude(v[k][i]) < kInfinity ? magnitude(v[k][i]) : 0u);
+    }
+  }
+  most = __reduce_max_sync(0xffffffffu, most);
+  finite = __reduce_max_sync(0xffffffffu, finite);
+  if ((threadIdx.x & 31) == 0) { most_s[0][threadIdx.x >> 5] = most; most_s[1][threadIdx.x >> 5] = finite; }
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; ++w) { most = max(most, most_s[0][w]); finite = max(finite, most_s[1][w]); }
+  const int s = exponent_byte(finite, m.format);
+  const float f = down(s);
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    const int64_t row = row0 + strand + 16 * k;
+    uint32_t w[2] = {0, 0};
+    if (most < kInfinity) {
+#pragma unroll
+      for (int i = 0; i < 8; i += 2) w[i >> 2] |= code2(v[k][i] * f, v[k][i + 1] * f, m.format) << (8 * (i & 3));
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[i >> 2] |= code_special(v[k][i] * f, m.format) << (8 * (i & 3));
+    }
+    if (row < m.rows && first < m.pitch) *reinterpret_cast<uint2*>(m.codes + row * m.pitch + first) = make_uint2(w[0], w[1]);
+    if (t.codes) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) turned[lane * 8 + i][strand + 16 * k] = (uint8_t)(w[i >> 2] >> (8 * (i & 3)));
+    }
+  }
+  if (threadIdx.x < kBlock) m.exponents[exponent_at(row0 + threadIdx.x, blockIdx.x, m.tiles)] = (uint8_t)s;
+  if (!t.codes) return;
+  __syncthreads();
+  const int64_t trow0 = (int64_t)blockIdx.x * kBlock;
+  const int tfirst = blockIdx.y * kBlock + lane * 8;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    const int64_t row = trow0 + strand + 16 * k;
+    if (row < t.rows && tfirst < t.pitch)
+      *reinterpret_cast<uint2*>(t.codes + row * t.pitch + tfirst) = *reinterpret_cast<const uint2*>(&turned[strand + 16 * k][lane * 8]);
+  }
+  if (threadIdx.x < kBlock) t.exponents[exponent_at(trow0 + threadIdx.x, blockIdx.y, t.tiles)] = (uint8_t)s;
+}
+
+static int vector_rows(const void* p, int c, int dtype) { return lf_aligned16(p) && c % (dtype == LF_DTYPE_BF16 ? 8 : 4) == 0; }
+
+}  // namespace f8
+
+using namespace f8;
+
+lf_status lf_float8_check_rows(lf_context* ctx, const char* what, int64_t rows, int channels, int dtype) {
+  if (rows <= 0 || channels <= 0) return lf_fail(ctx, LF_ERR_SHAPE, "%s: rows and channels must be positive safe integers", what);
+  if (rows > 0x7fffffff || channels > (1 << 24) || (uint64_t)rows * blocks(channels) > 0x7fffffffull)
+    return lf_fail(ctx, LF_ERR_UNSUPPORTED, "%s: %lld rows of %d channels are too many", what, (long long)rows, channels);
+  if (dtype != LF_DTYPE_F32 && dtype != LF_DTYPE_BF16) return lf_fail(ctx, LF_ERR_ARGUMENT, "unknown activation dtype %d", dtype);
+  return LF_OK;
+}
+
+lf_status lf_float8_check(lf_context* ctx, const char* what, const lf_float8_matrix& m, int64_t rows, int channels) {
+  if (!m.codes || !m.exponents) return lf_fail(ctx, LF_ERR_ARGUMENT, "%s: null codes or exponents", what);
+  if (m.rows != rows || m.channels != channels)
+    return lf_fail(ctx, LF_ERR_SHAPE, "%s: an 8-bit matrix of %lld x %d; expected %lld x %d", what, (long long)m.rows, m.channels, (long long)rows, channels);
+  if (m.format != LF_FLOAT8_E4M3 && m.format != LF_FLOAT8_E5M2) return lf_fail(ctx, LF_ERR_ARGUMENT, "%s: unknown 8-bit format %d", what, m.format);
+  if (!lf_aligned16(m.codes) || !lf_aligned16(m.exponents))
+    return lf_fail(ctx, LF_ERR_ARGUMENT, "%s: codes and exponents must start on 16-byte boundaries", what);
+  return LF_OK;
+}
+
+lf_status lf_float8_done(lf_context* ctx, lf_result* r, int launches) {
+  LF_CUDA(ctx, cudaGetLastError());
+  if (r) { r->elapsed_ms = 0.f; r->peak_bytes = ctx->arena_peak; r->launches = (uint32_t)launches; }
+  return LF_OK;
+}
+
+extern "C" {
+
+uint64_t lf_float8_code_bytes(int64_t rows, int32_t channels) { return rows > 0 && channels > 0 ? (uint64_t)(rows * pitch(channels)) : 0; }
+uint64_t lf_float8_exponent_bytes(int64_t rows, int32_t channels) { return rows > 0 && channels > 0 ? (uint64_t)exponent_bytes(rows, channels) : 0; }
+
+lf_status lf_float8_encode(lf_context* ctx, const lf_float8_encode_desc* d, lf_result* r) {
+  if (!ctx) return LF_ERR_ARGUMENT;
+  if (!d || !d->source) return lf_fail(ctx, LF_ERR_ARGUMENT, "float8 encode: null argument");
+  const lf_float8_matrix& o = d->out;
+  LF_TRY(lf_float8_check_rows(ctx, "float8 encode", o.rows, o.channels, d->dtype));
+  LF_TRY(lf_float8_check(ctx, "float8 encode", o, o.rows, o.channels));
+  if (d->block_rows != 1 && d->block_rows != kBlock) return lf_fail(ctx, LF_ERR_ARGUMENT, "float8 encode: an exponent covers 1 or 128 rows; received %d", d->block_rows);
+  const bool turned = d->transposed.codes != nullptr;
+  if (turned && d->block_rows != kBlock) return lf_fail(ctx, LF_ERR_ARGUMENT, "float8 encode: only blocks of 128 rows have a transposed form");
+  if (turned) {
+    if (o.rows > (1 << 24)) return lf_fail(ctx, LF_ERR_UNSUPPORTED, "float8 encode: %lld rows are too many for a transposed form", (long long)o.rows);
+    LF_TRY(lf_float8_check(ctx, "float8 encode, transposed", d->transposed, o.channels, (int)o.rows));
+    if (d->transposed.format != o.format) return lf_fail(ctx, LF_ERR_ARGUMENT, "float8 encode: both forms have one format");
+  }
+  if (d->block_rows == kBlock && row_tiles(o.rows) > 65535) return lf_fail(ctx, LF_ERR_UNSUPPORTED, "float8 encode: %lld rows are too many for blocks of 128 rows", (long long)o.rows);
+  LF_CUDA(ctx, cudaSetDevice(ctx->device));
+  const Matrix m = matrix(o);
+  const int vector = vector_rows(d->source, o.channels, d->dtype);
+  lf_prof_begin(ctx, LF_KERNEL_ELEMENTWISE);
+  if (d->block_rows == kBlock) {
+    Matrix t{};
+    if (turned) t = matrix(d->transposed);
+    const dim3 grid(blocks(o.channels), (unsigned)row_tiles(o.rows));
+    if (d->dtype == LF_DTYPE_BF16) lf_launch(ctx, encode_square_kernel<bf16>, grid, kThreads, 0, (const bf16*)d->source, m, t, vector);
+    else lf_launch(ctx, encode_square_kernel<float>, grid, kThreads, 0, (const float*)d->source, m, t, vector);
+  } else {
+    const uint32_t per_row = blocks(o.channels), units = (uint32_t)(o.rows * per_row);
+    auto run = [&](auto lanes) {
+      constexpr int L = decltype(lanes)::value;
+      const int grid = lf_ceil_div(units, kThreads / L * kUnits);
+      if (d->dtype == LF_DTYPE_BF16) lf_launch(ctx, encode_kernel<bf16, L>, grid, kThreads, 0, (const bf16*)d->source, m, units, per_row, vector);
+      else lf_launch(ctx, encode_kernel<float, L>, grid, kThreads, 0, (const float*)d->source, m, units, per_row, vector);
+    };
+    if (o.channels <= 64) run(std::integral_constant<int, 8>{}); else run(std::integral_constant<int, 16>{});
+  }
+  lf_prof_end(ctx);
+  ctx->launches++;
+  return lf_float8_done(ctx, r, 1);
+}
+
+lf_status lf_float8_decode(lf_context* ctx, const lf_float8_decode_desc* d, lf_result* r) {
+  if (!ctx) return LF_ERR_ARGUMENT;
+  if (!d || !d->out) return lf_fail(ctx, LF_ERR_ARGUMENT, "float8 decode: null argument");
+  const lf_float8_matrix& o = d->source;
+  LF_TRY(lf_float8_check_rows(ctx, "float8 decode", o.rows, o.channels, d->dtype));
+  LF_TRY(lf_float8_check(ctx, "float8 decode", o, o.rows, o.channels));
+  LF_CUDA(ctx, cudaSetDevice(ctx->device));
+  const Matrix m = matrix(o);
+  const int vector = vector_rows(d->out, o.channels, d->dtype);
+  const uint32_t per_row = blocks(o.channels), units = (uint32_t)(o.rows * per_row);
+  lf_prof_begin(ctx, LF_KERNEL_ELEMENTWISE);
+  auto run = [&](auto lanes) {
+    constexpr int L = decltype(lanes)::value;
+    const int grid = lf_ceil_div(units, kThreads / L * kUnits);
+    if (d->dtype == LF_DTYPE_BF16) lf_launch(ctx, decode_kernel<bf16, L>, grid, kThreads, 0, m, (bf16*)d->out, units, per_row, vector);
+    else lf_launch(ctx, decode_kernel<float, L>, grid, kThreads, 0, m, (float*)d->out, units, per_row, vector);
+  };
+  if (o.channels <= 64) run(std::integral_constant<int, 8>{}); else run(std::integral_constant<int, 16>{});
+  lf_prof_end(ctx);
+  ctx->launches++;
+  return lf_float8_done(ctx, r, 1);
+}
+
+}  // extern "C"

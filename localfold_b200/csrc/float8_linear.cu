@@ -1,0 +1,313 @@
+// The projection on 8-bit operands (float8.cuh): out[m][n] = sum_k x[m][k] w[n][k] (+ bias[n]), float32 sums, float32 or bf16 rows.
+//
+// tcgen05.mma of kind mxf8f6f4 multiplies 32 channels at a time and takes a power of two per row and 32 channels from tensor memory: the
+// exponent bytes as they lie in the matrices, one byte for four instructions (a block of 128 channels).  No product is scaled by an
+// instruction of ours, and partial sums of different blocks meet in one float32 accumulator.
+#include <cuda.h>
+
+#include "float8.cuh"
+#include "tc05.cuh"
+#include "tc_kernels.cuh"
+
+namespace tc {
+
+using namespace tc05;
+
+lf_status make_map_bytes(lf_context* ctx, CUtensorMap* map, const void* base, uint64_t width, uint64_t rows, uint64_t pitch, uint32_t box_rows);
+lf_status make_map_rows(lf_context* ctx, CUtensorMap* map, const void* base, bool f32, uint64_t width, uint64_t rows, uint32_t box_rows);
+
+constexpr int F8_BM = 128, F8_BK = 128;      // a k step is a block of the format, and a row of it 128 bytes of shared memory
+constexpr int F8_A_BYTES = F8_BM * F8_BK;
+
+struct Float8Params {
+  int m, n, k;
+  int vector_out;              // rows start on 16-byte boundaries: they leave by TMA
+  const float* bias;           // [n] or null
+  const uint8_t *ex, *ew;      // exponents
+  int64_t ex_tiles, ew_tiles;  // 128-row tiles of each
+  int formats;                 // bit 0: x is e5m2, bit 1: w
+  void* out;
+  Status* status;
+};
+
+// kind::mxf8f6f4, scales 2^(byte - 127): formats of A and B (0 e4m3, 1 e5m2), both K-major; `id`: which byte of a scale word
+__device__ __forceinline__ uint32_t make_idesc_f8(int M, int N, int a_format, int b_format, int id) {
+  return ((uint32_t)id << 4) | ((uint32_t)a_format << 7) | ((uint32_t)b_format << 10) | ((uint32_t)(N >> 3) << 17) | (1u << 23) |
+         ((uint32_t)(M >> 4) << 24) | ((uint32_t)id << 29);
+}
+__device__ __forceinline__ void umma_f8_scaled(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t a_scale, uint32_t b_scale,
+                                               uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(a_scale), "r"(b_scale), "r"(accumulate)
+      : "memory");
+}
+// 32 rows of 16 bytes of shared memory -> four columns of tensor memory, the same for each quarter of the lanes
+__device__ __forceinline__ void tmem_copy_scales(uint32_t taddr, uint64_t desc) {
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+
+// One 128 x BN tile per work item, k stepped by 128 through a TMA ring.  A step that opens a group of four brings the group's exponent tiles
+// with it; the MMA thread copies them to tensor memory (four slots in turn) in front of the step's products.  An accumulator
+// of 256 columns has no second one beside it and the scales (512 columns in all): the epilogue's warps take their shares into registers with
+// one wait and hand it back, so that the next tile's products run under the stores.  Narrower tiles have two.
+// Warp roles: 0 = TMA producer, 1 = MMA issuer (owns TMEM), 2.. = epilogue, 64 columns of a lane quadrant each.
+template <int BN>
+struct Float8Shape {
+  static constexpr int stages = BN == 256 ? 3 : BN == 128 ? 5 : 6;
+  static constexpr int b_bytes = BN * F8_BK, stage = F8_A_BYTES + b_bytes;
+  static constexpr int b_tiles = (BN + 127) / 128, scales = 512 * (1 + b_tiles);
+  static constexpr int accumulators = BN == 256 ? 1 : 2;
+  static constexpr int parts = BN / 64, epi = 4 * parts;
+  static constexpr int threads = 64 + 32 * epi;
+  static constexpr int smem = stages * (stage + scales) + epi * (4096 + 256) + 256 + 1024;
+};
+
+template <int BN, bool F32>
+__global__ void __launch_bounds__(Float8Shape<BN>::threads, 1)
+float8_linear_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant__ CUtensorMap mapB, const __grid_constant__ CUtensorMap mapO,
+                     const Float8Params p) {
+  using S = Float8Shape<BN>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = align_shared(smem_raw);
+  uint8_t* out_stage = smem + S::stages * S::stage;
+  uint8_t* scale_s = out_stage + S::epi * 4096;
+  float* bias_s = reinterpret_cast<float*>(scale_s + S::stages * S::scales);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(bias_s + S::epi * 64);
+  uint64_t* full = bars;
+  uint64_t* empty = full + S::stages;
+  uint64_t* tmem_full = empty + S::stages;
+  uint64_t* tmem_empty = tmem_full + S::accumulators;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tmem_empty + S::accumulators);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int tiles_m = (p.m + F8_BM - 1) / F8_BM, tiles_n = (p.n + BN - 1) / BN;
+  const int total = tiles_m * tiles_n;
+  const int kblocks = (p.k + F8_BK - 1) / F8_BK;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S::stages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+    for (int b = 0; b < S::accumulators; ++b) { mbar_init(&tmem_full[b], 1); mbar_init(&tmem_empty[b], S::epi); }
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 1) { tmem_alloc(tmem_slot, 512); tmem_relinquish(); }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  lf_chain();
+
+  if (warp == 0) {
+    if (lane == 0) {
+      prefetch_tensormap(&mapA);
+      prefetch_tensormap(&mapB);
+      int stage = 0; uint32_t phase = 0;
+      bool ok = true;
+      for (int t = blockIdx.x; t < total && ok; t += gridDim.x) {
+        const int mi = t / tiles_n, nj = t - mi * tiles_n;
+        // exponent tiles of the second 128 columns may not exist
+        const int b_tiles = min((int64_t)S::b_tiles, p.ew_tiles - (int64_t)nj * BN / 128);
+        for (int kb = 0; kb < kblocks; ++kb) {
+          if (!mbar_wait(&empty[stage], phase ^ 1, abort_flag, p.status, 121)) { ok = false; break; }
+          uint8_t* sA = smem + stage * S::stage;
+          const bool opens = (kb & 3) == 0;
+          mbar_expect_tx(&full[stage], S::stage + (opens ? 512 * (1 + b_tiles) : 0));
+          tma_load_3d(sA, &mapA, &full[stage], kb * F8_BK, mi * F8_BM, 0);
+          tma_load_3d(sA + F8_A_BYTES, &mapB, &full[stage], kb * F8_BK, nj * BN, 0);
+          if (opens) {
+            uint8_t* sc = scale_s + stage * S::scales;
+            bulk_load(sc, p.ex + ((int64_t)(kb >> 2) * p.ex_tiles + mi) * 512, 512, &full[stage]);
+            bulk_load(sc + 512, p.ew + ((int64_t)(kb >> 2) * p.ew_tiles + (int64_t)nj * BN / 128) * 512, 512 * b_tiles, &full[stage]);
+          }
+          if (++stage == S::stages) { stage = 0; phase ^= 1; }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      int stage = 0; uint32_t phase = 0, it = 0, group = 0;
+      bool ok = true;
+      for (int t = blockIdx.x; t < total && ok; t += gridDim.x, ++it) {
+        const int nj = t % tiles_n;
+        const int left = p.n - nj * BN, columns = left >= BN ? BN : (left + 15) / 16 * 16;
+        const uint32_t acc = it % S::accumulators;
+        if (!mbar_wait(&tmem_empty[acc], ((it / S::accumulators) & 1) ^ 1, abort_flag, p.status, 122)) break;
+        tc_fence_after();
+        const uint32_t d = tmem_base + acc * BN;
+        uint32_t scales = 0;
+        for (int kb = 0; kb < kblocks; ++kb) {
+          if (!mbar_wait(&full[stage], phase, abort_flag, p.status, 123)) { ok = false; break; }
+          tc_fence_after();
+          const uint32_t a0 = smem_u32(smem + stage * S::stage), b0 = a0 + F8_A_BYTES;
+          if ((kb & 3) == 0) {
+            // Four slots in turn: when a group's first step is here, the step `stages` <= 6 before it is complete, and with it
+            // the group before last; the slot's last reader is four groups back.
+            scales = tmem_base + 256 + (group++ & 3) * 16;
+            const uint32_t sc = smem_u32(scale_s + stage * S::scales);
+            tmem_copy_scales(scales, make_smem_desc_plain(sc, 0, 128));
+            tmem_copy_scales(scales + 8, make_smem_desc_plain(sc + 512, 0, 128));
+            if (BN == 256 && columns > 128) tmem_copy_scales(scales + 12, make_smem_desc_plain(sc + 1024, 0, 128));
+          }
+          const uint32_t idesc = make_idesc_f8(F8_BM, columns, p.formats & 1, p.formats >> 1, kb & 3);
+#pragma unroll
+          for (int kk = 0; kk < F8_BK / 32; ++kk)
+            umma_f8_scaled(d, make_smem_desc(a0 + kk * 32, 16, 1024), make_smem_desc(b0 + kk * 32, 16, 1024), idesc, scales,
+                           scales + 8 + (BN == 64 ? 2u * (nj & 1) : 0u), (kb | kk) != 0 ? 1u : 0u);
+          umma_commit(&empty[stage]);
+          if (++stage == S::stages) { stage = 0; phase ^= 1; }
+        }
+        if (ok) umma_commit(&tmem_full[acc]);
+      }
+    }
+  } else {
+    const int q = warp & 3, part = (warp - 2) >> 2;      // TMEM lane quadrant, 64 of the tile's columns
+    uint8_t* stage = out_stage + (warp - 2) * 4096;
+    float* bias = bias_s + (warp - 2) * 64;
+    uint32_t it = 0;
+    int held = -1;      // first column of the bias share in shared memory
+    if (lane == 0 && p.vector_out) prefetch_tensormap(&mapO);
+    for (int t = blockIdx.x; t < total; t += gridDim.x, ++it) {
+      const int mi = t / tiles_n, nj = t - mi * tiles_n;
+      const int col0 = nj * BN + part * 64, row0 = mi * F8_BM + q * 32;
+      const bool mine = col0 < p.n && row0 < p.m;
+      if (mine && held != col0) {
+        held = col0;
+        __syncwarp();
+#pragma unroll
+        for (int e = 0; e < 64; e += 32) bias[e + lane] = p.bias && col0 + e + lane < p.n ? p.bias[col0 + e + lane] : 0.f;
+        __syncwarp();
+      }
+      const uint32_t acc = it % S::accumulators;
+      if (!mbar_wait(&tmem_full[acc], (it / S::accumulators) & 1, abort_flag, p.status, 124)) break;
+      tc_fence_after();
+      uint32_t r[2][32];
+      if (mine) {
+        const uint32_t d = tmem_base + ((uint32_t)(q * 32) << 16) + acc * BN + part * 64;
+        tmem_ld32(d, r[0]);
+        tmem_ld32(d + 32, r[1]);
+        tmem_ld_wait();
+        tie32(r[0]);
+        tie32(r[1]);
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&tmem_empty[acc]);      // the share is in registers: the accumulator may be overwritten
+      if (!mine) continue;
+#pragma unroll
+      for (int half = 0; half < (F32 ? 2 : 1); ++half) {
+        const int c0 = col0 + half * 32;
+        if (F32 && c0 >= p.n) break;
+        if (lane == 0) bulk_wait_read();      // the previous copy has read the staging rows
+        __syncwarp();
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {      // 16-byte pieces of the 128-byte rows
+          uint4 w;
+          if (F32) {
+            const float4 b = *reinterpret_cast<const float4*>(bias + half * 32 + c * 4);
+            w = make_uint4(__float_as_uint(__uint_as_float(r[half][c * 4]) + b.x), __float_as_uint(__uint_as_float(r[half][c * 4 + 1]) + b.y),
+                           __float_as_uint(__uint_as_float(r[half][c * 4 + 2]) + b.z), __float_as_uint(__uint_as_float(r[half][c * 4 + 3]) + b.w));
+          } else {
+            uint32_t u[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float2 b = *reinterpret_cast<const float2*>(bias + c * 8 + e * 2);
+              const __nv_bfloat162 two = __floats2bfloat162_rn(__uint_as_float(r[c >> 2][(c & 3) * 8 + e * 2]) + b.x,
+                                                               __uint_as_float(r[c >> 2][(c & 3) * 8 + e * 2 + 1]) + b.y);
+              u[e] = *reinterpret_cast<const uint32_t*>(&two);
+            }
+            w = make_uint4(u[0], u[1], u[2], u[3]);
+          }
+          *reinterpret_cast<uint4*>(stage + lane * 128 + ((c ^ (lane & 7)) << 4)) = w;
+        }
+        if (p.vector_out) {
+          fence_async_smem();
+          __syncwarp();
+          if (lane == 0) { tma_store_3d(&mapO, stage, c0, row0, 0); bulk_commit(); }
+        } else {      // rows that no 16-byte access divides: a row of the staging tile after the other
+          __syncwarp();
+          const int rows = min(32, p.m - row0);
+          for (int row = 0; row < rows; ++row) {
+            const int64_t at = (int64_t)(row0 + row) * p.n;
+            if (F32) {
+              if (c0 + lane < p.n)
+                static_cast<float*>(p.out)[at + c0 + lane] = *reinterpret_cast<const float*>(stage + row * 128 + (((lane >> 2) ^ (row & 7)) << 4) + (lane & 3) * 4);
+            } else {
+#pragma unroll
+              for (int e = 0; e < 64; e += 32)
+                if (c0 + e + lane < p.n)
+                  static_cast<bf16*>(p.out)[at + c0 + e + lane] =
+                      *reinterpret_cast<const bf16*>(stage + row * 128 + ((((e + lane) >> 3) ^ (row & 7)) << 4) + (lane & 7) * 2);
+            }
+          }
+          __syncwarp();
+        }
+      }
+    }
+    if (lane == 0) bulk_wait_all();      // this thread's stores have landed
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (*abort_flag) drain_after_abort();
+  if (warp == 1) { tc_fence_after(); tmem_dealloc(tmem_base, 512); }
+}
+
+void configure_float8_linear() {
+  cudaFuncSetAttribute(float8_linear_kernel<256, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, Float8Shape<256>::smem);
+  cudaFuncSetAttribute(float8_linear_kernel<256, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, Float8Shape<256>::smem);
+  cudaFuncSetAttribute(float8_linear_kernel<128, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, Float8Shape<128>::smem);
+  cudaFuncSetAttribute(float8_linear_kernel<128, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, Float8Shape<128>::smem);
+  cudaFuncSetAttribute(float8_linear_kernel<64, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, Float8Shape<64>::smem);
+  cudaFuncSetAttribute(float8_linear_kernel<64, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, Float8Shape<64>::smem);
+}
+
+template <int BN, bool F32>
+static lf_status launch_float8(lf_context* ctx, const f8::Matrix& x, const f8::Matrix& w, Float8Params p) {
+  using S = Float8Shape<BN>;
+  CUtensorMap ma, mb, mo{};
+  LF_TRY(make_map_bytes(ctx, &ma, x.codes, x.channels, x.rows, x.pitch, F8_BM));
+  LF_TRY(make_map_bytes(ctx, &mb, w.codes, w.channels, w.rows, w.pitch, BN));
+  if (p.vector_out) LF_TRY(make_map_rows(ctx, &mo, p.out, F32, p.n, p.m, 32));
+  const int64_t tiles = (int64_t)((p.m + F8_BM - 1) / F8_BM) * ((p.n + BN - 1) / BN);
+  lf_prof_begin(ctx, LF_KERNEL_LN_GEMM);
+  lf_launch(ctx, float8_linear_kernel<BN, F32>, (int)(tiles < ctx->sm_count ? tiles : ctx->sm_count), S::threads, S::smem, ma, mb, mo, p);
+  lf_prof_end(ctx);
+  ctx->launches++;
+  return LF_OK;
+}
+
+}  // namespace tc
+
+using namespace f8;
+
+extern "C" lf_status lf_float8_linear_run(lf_context* ctx, const lf_float8_linear_desc* d, lf_result* r) {
+  if (!ctx) return LF_ERR_ARGUMENT;
+  if (!d || !d->out) return lf_fail(ctx, LF_ERR_ARGUMENT, "float8 linear: null argument");
+  const lf_float8_matrix &x = d->activations, &w = d->weights;
+  LF_TRY(lf_float8_check_rows(ctx, "float8 linear", x.rows, x.channels, d->out_dtype));
+  LF_TRY(lf_float8_check_rows(ctx, "float8 linear", w.rows, x.channels, d->out_dtype));
+  LF_TRY(lf_float8_check(ctx, "float8 linear, activations", x, x.rows, x.channels));
+  LF_TRY(lf_float8_check(ctx, "float8 linear, weights", w, w.rows, x.channels));
+  if (w.rows > (1 << 24)) return lf_fail(ctx, LF_ERR_UNSUPPORTED, "float8 linear: %lld output channels are too many", (long long)w.rows);
+  if (row_tiles(x.rows) * ((w.rows + 63) / 64) > 0x7fffffffll) return lf_fail(ctx, LF_ERR_UNSUPPORTED, "float8 linear: %lld x %lld outputs are too many", (long long)x.rows, (long long)w.rows);
+  LF_CUDA(ctx, cudaSetDevice(ctx->device));
+  const Matrix mx = matrix(x), mw = matrix(w);
+  const bool f32 = d->out_dtype == LF_DTYPE_F32;
+  tc::Float8Params p{};
+  p.m = (int)x.rows; p.n = (int)w.rows; p.k = x.channels;
+  p.vector_out = lf_aligned16(d->out) && p.n % (f32 ? 4 : 8) == 0;
+  p.bias = d->bias; p.ex = mx.exponents; p.ew = mw.exponents; p.ex_tiles = mx.tiles; p.ew_tiles = mw.tiles;
+  p.formats = (x.format == LF_FLOAT8_E5M2) | (w.format == LF_FLOAT8_E5M2) << 1;
+  p.out = d->out;
+  p.status = (tc05::Status*)ctx->tc_status;
+  const int64_t rows = mx.tiles;
+  const int bn = rows * ((p.n + 255) / 256) >= ctx->sm_count && p.n > 128 ? 256 : rows * ((p.n + 127) / 128) >= ctx->sm_count && p.n > 64 ? 128 : 64;
+  if (bn == 256) LF_TRY(f32 ? (tc::launch_float8<256, true>(ctx, mx, mw, p)) : (tc::launch_float8<256, false>(ctx, mx, mw, p)));
+  else if (bn == 128) LF_TRY(f32 ? (tc::launch_float8<128, true>(ctx, mx, mw, p)) : (tc::launch_float8<128, false>(ctx, mx, mw, p)));
+  else LF_TRY(f32 ? (tc::launch_float8<64, true>(ctx, mx, mw, p)) : (tc::launch_float8<64, false>(ctx, mx, mw, p)));
+  return lf_float8_done(ctx, r, 1);
+}

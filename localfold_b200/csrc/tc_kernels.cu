@@ -153,6 +153,29 @@ lf_status make_map_grouped(lf_context* ctx, CUtensorMap* map, const void* base, 
   return LF_OK;
 }
 
+// bytes [rows][pitch] of which `width` count (zeros behind them), 128-byte swizzled boxes of 128 bytes x `box_rows` rows
+lf_status make_map_bytes(lf_context* ctx, CUtensorMap* map, const void* base, uint64_t width, uint64_t rows, uint64_t pitch, uint32_t box_rows) {
+  if (!g_encode) return lf_fail(ctx, LF_ERR_CUDA, "cuTensorMapEncodeTiled is not available from this driver");
+  cuuint64_t dims[3] = {width, rows, 1}, strides[2] = {pitch, pitch * rows};
+  cuuint32_t box[3] = {128, box_rows, 1}, estr[3] = {1, 1, 1};
+  CUresult r = g_encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return lf_fail(ctx, LF_ERR_CUDA, "cuTensorMapEncodeTiled (bytes) failed with code %d", (int)r);
+  return LF_OK;
+}
+
+// float32 or bf16 rows (a multiple of 16 bytes), 128-byte swizzled boxes of 128 bytes x `box_rows` rows
+lf_status make_map_rows(lf_context* ctx, CUtensorMap* map, const void* base, bool f32, uint64_t width, uint64_t rows, uint32_t box_rows) {
+  if (!g_encode) return lf_fail(ctx, LF_ERR_CUDA, "cuTensorMapEncodeTiled is not available from this driver");
+  const uint64_t pitch = width * (f32 ? 4 : 2);
+  cuuint64_t dims[3] = {width, rows, 1}, strides[2] = {pitch, pitch * rows};
+  cuuint32_t box[3] = {f32 ? 32u : 64u, box_rows, 1}, estr[3] = {1, 1, 1};
+  CUresult r = g_encode(map, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, estr,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return lf_fail(ctx, LF_ERR_CUDA, "cuTensorMapEncodeTiled (rows) failed with code %d", (int)r);
+  return LF_OK;
+}
+
 // fp16 operand planes [planes][plane_rows][ld] seen as (k, i, plane); boxes of 32 k (64 bytes, 64-byte swizzle) x 1 x box_h
 // planes: what an epilogue warp of the triangle projection stores per pass
 lf_status make_map_plane_runs(lf_context* ctx, CUtensorMap* map, const void* base, uint64_t n, uint64_t plane_rows, uint64_t planes,
@@ -444,6 +467,8 @@ void configure_once() {
     configure_transition();
     configure_gemm3();
     configure_gemm();
+    configure_float8_linear();
+    configure_float8_gradient();
     cudaGetLastError();
   });
 }

@@ -74,6 +74,8 @@ lf_status contract_rect(lf_context* ctx, ArenaCursor& cur, const op16* a, const 
 
 // Plain fp16 GEMMs (tc_gemm.cu), weights [n_out][k]:
 void configure_gemm();
+void configure_float8_linear();        // float8_linear.cu
+void configure_float8_gradient();      // float8_gradient.cu
 // q | k | v | gate of rows (b, q) as the attention core reads them: [q, k, v, gate][width / 128][batch][ldq * 128] in 8 x 8 pieces (see
 // attention_project), value (acc + bias) * (qscale for q), gate through a sigmoid; rows Q .. ldq hold finite values
 lf_status gemm_pieces(lf_context* ctx, ArenaCursor& cur, const op16* a, const op16* w, op16* out, int batch, int Q, int ldq, int k_len, int width,

@@ -1,0 +1,376 @@
+"""Operators for training and for 8-bit operands around the pair stack: LayerNorm with its gradients, activations kept in 8 bits, and the
+projection on 8-bit operands with its gradients.  The reference runs the stack forward only: no counterpart there.
+
+They stand beside the operators of ``operators.py`` and are called alike (``run(input[, options])`` on a ``Device``), but take
+and return CUDA tensors only.  A call enqueues on the device's stream and returns.  Results and workspaces come from torch's
+allocator, so a call can be captured into a CUDA graph (on the stream that the ``Device`` was made on) and graphs share nothing.
+
+    norm, linear = lf.LayerNormGpu(dev), lf.Float8LinearGpu(dev)
+    weights = lf.prepare_float8_linear_weights(dev, weight, bias)                 # [out][in], encoded once (update() after a step)
+    a = norm.run({"rows": r, "channels": c, "activations": x, "scale": g, "offset": b}, {"checkpoint": "e4m3", "encode": "e4m3"})
+    shape = {"rows": r, "channels": c, "outChannels": n}
+    y = linear.run({**shape, "activations": a["output"], "weights": weights})["output"]
+    back = linear.input_gradient({**shape, "gradient": dy, "weights": weights})
+    grads = linear.weight_gradient({**shape, "gradient": dy, "activations": a["output"]})         # "weight", "bias"
+    dx = norm.backward({"rows": r, "channels": c, "gradient": back["output"], "activations": a["checkpoint"], "mean": a["mean"],
+                        "inverseDeviation": a["inverseDeviation"], "scale": g})                   # "activations", "scale", "offset"
+"""
+from __future__ import annotations
+
+import math
+
+import numpy as np
+
+from . import _native as nat
+from ._native import RangeError
+from .operators import Device, EncodedTensor, _device, _positive, _result, _torch_stream, _variance
+
+_FORMAT = {"e4m3": nat.FLOAT8_E4M3, "e5m2": nat.FLOAT8_E5M2}
+_DTYPE = {"f32": nat.DTYPE_F32, "bf16": nat.DTYPE_BF16}
+_NO_MATRIX = nat.Float8Matrix()
+
+
+def _format(value, name="format"):
+    if value not in _FORMAT:
+        raise ValueError(f'{name} must be "e4m3" or "e5m2"; received {value!r}')
+    return value
+
+
+def _shape(inp, *names):
+    values = tuple(inp[name] for name in names)
+    for name, value in zip(names, values):
+        _positive(name, value)
+    return tuple(int(value) for value in values)
+
+
+def _tensor(device, name, value, count, only=None):
+    """A tensor argument: on the device's GPU, contiguous, float32 or bfloat16 (``only``: one of them), of ``count`` values.
+    Returns the library's dtype."""
+    if not getattr(value, "is_cuda", False):
+        raise ValueError(f"{name} must be a CUDA tensor")
+    if value.device.index != device.ordinal:
+        raise ValueError(f"{name} is on {value.device}, the device's GPU is cuda:{device.ordinal}")
+    dtype = str(value.dtype)
+    dtype = "f32" if dtype == "torch.float32" else "bf16" if dtype == "torch.bfloat16" else dtype
+    if dtype not in _DTYPE or only not in (None, dtype):
+        raise ValueError(f"{name} must be {only or 'f32 or bf16'}; received {value.dtype}")
+    if not value.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+    if value.numel() != count:
+        raise RangeError(f"{name} has {value.numel()} values; expected {count}")
+    return dtype
+
+
+def _torch_dtype(name):
+    import torch
+    return torch.float32 if name == "f32" else torch.bfloat16
+
+
+def _call(device, function, desc, tensors):
+    """The call; its tensors' memory stays theirs until the device's stream is done, whatever stream torch allocates for."""
+    res = device.call(function, desc, True)
+    if _torch_stream(device.ordinal) != device.stream:
+        import torch
+        stream = torch.cuda.ExternalStream(device.stream, device=f"cuda:{device.ordinal}")
+        for t in tensors:
+            if isinstance(t, Float8Tensor):
+                t = t.memory
+            if t is not None:
+                t.record_stream(stream)
+    return res
+
+
+class Float8Tensor:
+    """A float matrix ``[rows][channels]`` in 8 bits: codes in e4m3 or e5m2 and a power of two for every 128 consecutive channels of a
+    row (of a weight: 128 x 128 elements), the least that brings the block's largest finite magnitude to the format's largest code.
+    NaN stays NaN; an infinity becomes NaN in e4m3 and stays one in e5m2.  Made by ``float8_encode`` and by the operators; takes about
+    ``rows * channels`` bytes (``nbytes``)."""
+
+    def __init__(self, rows: int, channels: int, format: str, memory):
+        """``memory``: contiguous uint8 CUDA tensor with the codes, then the exponents, 16-byte aligned (``lf_float8_matrix``)."""
+        self.rows, self.channels, self.format, self.memory = rows, channels, format, memory
+        lib = nat.load()
+        self._codes = int(lib.lf_float8_code_bytes(rows, channels))
+        if memory.numel() != self._codes + int(lib.lf_float8_exponent_bytes(rows, channels)):
+            raise RangeError(f"memory has {memory.numel()} values; expected {self._codes + int(lib.lf_float8_exponent_bytes(rows, channels))}")
+        base = memory.data_ptr()
+        self.desc = nat.Float8Matrix(rows, channels, _FORMAT[format], base, base + self._codes)
+
+    @classmethod
+    def empty(cls, rows, channels, format, like):
+        lib = nat.load()
+        nbytes = int(lib.lf_float8_code_bytes(rows, channels)) + int(lib.lf_float8_exponent_bytes(rows, channels))
+        import torch
+        return cls(rows, channels, format, torch.empty(nbytes, dtype=torch.uint8, device=like.device))
+
+    @property
+    def nbytes(self):
+        return self.memory.numel()
+
+    @property
+    def codes(self):
+        """``[rows][channels rounded up to 16]`` bytes."""
+        return self.memory[:self._codes].view(self.rows, -1)
+
+    @property
+    def exponents(self):
+        """``[ceil(channels / 512)][ceil(rows / 128)][row % 32][row % 128 / 32][block % 4]`` bytes, 127 more than the powers."""
+        return self.memory[self._codes:].view(-1, (self.rows + 127) // 128, 32, 4, 4)
+
+
+def _matrix(device, name, value, rows, channels):
+    if not isinstance(value, Float8Tensor):
+        raise ValueError(f"{name} must be a Float8Tensor")
+    if value.memory.device.index != device.ordinal:
+        raise ValueError(f"{name} is on {value.memory.device}, the device's GPU is cuda:{device.ordinal}")
+    if (value.rows, value.channels) != (rows, channels):
+        raise RangeError(f"{name} is {value.rows} x {value.channels}; expected {rows} x {channels}")
+    return value
+
+
+def _encode(device, source, dtype, out, block_rows=1, transposed=None):
+    desc = nat.Float8EncodeDesc(out.desc, transposed.desc if transposed is not None else _NO_MATRIX, _DTYPE[dtype], block_rows, source.data_ptr())
+    return _call(device, device.lib.lf_float8_encode, desc, (source, out, transposed))
+
+
+def float8_encode(device, activations, rows, channels, options=None):
+    """The 8-bit form of ``activations`` ``[rows][channels]`` (float32 or bfloat16).  ``options``: format "e4m3" (default) or "e5m2"
+    (more range, less precision: gradients)."""
+    dev = _device(device)
+    rows, channels = _shape({"rows": rows, "channels": channels}, "rows", "channels")
+    format = _format((options or {}).get("format", "e4m3"))
+    dtype = _tensor(dev, "activations", activations, rows * channels)
+    out = Float8Tensor.empty(rows, channels, format, activations)
+    _encode(dev, activations, dtype, out)
+    return out
+
+
+def float8_decode(device, encoded, options=None, out=None):
+    """The values of a ``Float8Tensor`` as a tensor ``[rows][channels]``.  ``options``: output "bf16" (default) or "f32"; both hold them
+    exactly."""
+    dev = _device(device)
+    if not isinstance(encoded, Float8Tensor):
+        raise ValueError("encoded must be a Float8Tensor")
+    _matrix(dev, "encoded", encoded, encoded.rows, encoded.channels)
+    dtype = _output(options, "bf16")
+    if out is None:
+        out = encoded.memory.new_empty((encoded.rows, encoded.channels), dtype=_torch_dtype(dtype))
+    else:
+        _tensor(dev, "out", out, encoded.rows * encoded.channels, dtype)
+    _call(dev, dev.lib.lf_float8_decode, nat.Float8DecodeDesc(encoded.desc, _DTYPE[dtype], 0, out.data_ptr()), (encoded, out))
+    return out
+
+
+def _output(options, default):
+    value = (options or {}).get("output") or default
+    if value not in _DTYPE:
+        raise ValueError(f'output must be "f32" or "bf16"; received {value!r}')
+    return value
+
+
+class LayerNormGpu:
+    """LayerNorm over the channels of each row (at most 8192), and its gradients.  Statistics and sums are float32."""
+
+    def __init__(self, device: Device | None = None):
+        self.device = _device(device)
+
+    def run(self, input, options=None, out=None):
+        """``input``: rows, channels, activations ``[rows][channels]`` (float32 or bfloat16, as is the output), scale and offset
+        ``[channels]`` (float32), epsilon (default 1e-5).  ``options``: statistics - also return ``mean`` and ``inverseDeviation``
+        ``[rows]`` for ``backward``; checkpoint "e4m3" | "e5m2" - those and the input's 8-bit form as ``checkpoint``; encode "e4m3" |
+        "e5m2" - the output is a ``Float8Tensor``, the operand of a ``Float8LinearGpu``; variance "two-pass" | "fast" (two passes
+        either way).  ``out`` may be the activations."""
+        dev, opts = self.device, options or {}
+        rows, c = _shape(input, "rows", "channels")
+        x, scale, offset = input["activations"], input["scale"], input["offset"]
+        epsilon = input.get("epsilon", 1e-5)
+        if not epsilon > 0 or not math.isfinite(epsilon):
+            raise RangeError(f"epsilon must be finite and positive; received {epsilon}")
+        variance = _variance(opts, "two-pass")
+        kept, encode = opts.get("checkpoint"), opts.get("encode")
+        kept = None if kept is None else _format(kept, "checkpoint")
+        encode = None if encode is None else _format(encode, "encode")
+        dtype = _tensor(dev, "activations", x, rows * c)
+        _tensor(dev, "scale", scale, c, "f32")
+        _tensor(dev, "offset", offset, c, "f32")
+        if encode and out is not None:
+            raise ValueError("an encoded output is a new Float8Tensor; out is for the other kind")
+        if out is not None:
+            _tensor(dev, "out", out, rows * c, dtype)
+        elif not encode:
+            out = x.new_empty(x.shape)
+        checkpoint = Float8Tensor.empty(rows, c, kept, x) if kept else None
+        encoded = Float8Tensor.empty(rows, c, encode, x) if encode else None
+        statistics = scale.new_empty((2, rows)) if kept or opts.get("statistics") else None
+        mean = statistics.data_ptr() if statistics is not None else None
+        desc = nat.LayerNormDesc(rows, c, variance, _DTYPE[dtype], epsilon, x.data_ptr(), scale.data_ptr(), offset.data_ptr(),
+                                 out.data_ptr() if out is not None else None, mean, mean and mean + 4 * rows,
+                                 checkpoint.desc if kept else _NO_MATRIX, encoded.desc if encode else _NO_MATRIX)
+        res = _call(dev, dev.lib.lf_layer_norm_run, desc, (x, scale, offset, out, statistics, checkpoint, encoded))
+        result = _result(dev, res, encoded if encode else out)
+        if statistics is not None:
+            result["mean"], result["inverseDeviation"] = statistics[0], statistics[1]
+        if kept:
+            result["checkpoint"] = checkpoint
+        return result
+
+    def backward(self, input, options=None, out=None):
+        """``input``: rows, channels, gradient (of the output, ``[rows][channels]``), activations (the forward pass' input: a tensor of
+        the gradient's type, or its checkpoint), mean, inverseDeviation, scale.  Returns the gradients of ``activations`` (of the
+        gradient's type; ``out`` may be the gradient itself), ``scale`` and ``offset`` (float32).  The sums over the rows have a
+        fixed order: the same call gives the same bits."""
+        dev = self.device
+        rows, c = _shape(input, "rows", "channels")
+        dy, x, scale = input["gradient"], input["activations"], input["scale"]
+        dtype = _tensor(dev, "gradient", dy, rows * c)
+        encoded = isinstance(x, Float8Tensor)
+        if encoded:
+            _matrix(dev, "activations", x, rows, c)
+        else:
+            _tensor(dev, "activations", x, rows * c, dtype)
+        _tensor(dev, "mean", input["mean"], rows, "f32")
+        _tensor(dev, "inverseDeviation", input["inverseDeviation"], rows, "f32")
+        _tensor(dev, "scale", scale, c, "f32")
+        if out is not None:
+            _tensor(dev, "out", out, rows * c, dtype)
+        else:
+            out = dy.new_empty(dy.shape)
+        nbytes = int(dev.lib.lf_layer_norm_backward_workspace(dev.handle, rows, c))
+        # the two weights' gradients, then the workspace on a 16-byte boundary
+        ahead = (2 * c + 3) // 4 * 4
+        memory = scale.new_empty(ahead + nbytes // 4)
+        base = memory.data_ptr()
+        desc = nat.LayerNormBackwardDesc(rows, c, _DTYPE[dtype], dy.data_ptr(), None if encoded else x.data_ptr(),
+                                         x.desc if encoded else _NO_MATRIX, input["mean"].data_ptr(), input["inverseDeviation"].data_ptr(),
+                                         scale.data_ptr(), out.data_ptr(), base, base + 4 * c, base + 4 * ahead, nbytes)
+        res = _call(dev, dev.lib.lf_layer_norm_backward_run, desc, (dy, x, input["mean"], input["inverseDeviation"], scale, out, memory))
+        result = _result(dev, res, out)
+        result["activations"] = result.pop("output")
+        result["scale"], result["offset"] = memory[:c], memory[c:2 * c]
+        return result
+
+
+class Float8LinearWeights:
+    """A projection's weight ``[outChannels][channels]`` on the device in e4m3, one power of two for every 128 x 128 elements, in both
+    orientations (the transposed one multiplies gradients), and its bias.  ``update`` encodes new values into the same memory, as
+    a training step does; calls enqueued before it have read the old ones."""
+
+    def __init__(self, device: Device, weight, bias=None):
+        self.device = device
+        shape = tuple(getattr(weight, "shape", ()))
+        if len(shape) != 2:
+            raise RangeError(f"weight must be [outChannels][channels]; received shape {shape}")
+        self.out_channels, self.channels = int(shape[0]), int(shape[1])
+        _positive("outChannels", self.out_channels)
+        _positive("channels", self.channels)
+        weight, bias = self._on_device(weight), self._on_device(bias)
+        _tensor(device, "weight", weight, self.out_channels * self.channels)
+        self.forward = Float8Tensor.empty(self.out_channels, self.channels, "e4m3", weight)
+        self.transposed = Float8Tensor.empty(self.channels, self.out_channels, "e4m3", weight)
+        self.update(weight, bias)
+
+    def _on_device(self, value):
+        if value is None or getattr(value, "is_cuda", False):
+            return value
+        import torch
+        host = value.decode() if isinstance(value, EncodedTensor) else np.ascontiguousarray(np.asarray(value, np.float32))
+        return torch.as_tensor(host).to(f"cuda:{self.device.ordinal}")
+
+    def update(self, weight, bias=None):
+        """New values (float32 or bfloat16 CUDA tensors or host arrays).  The bias tensor is used as it is at every call."""
+        weight, bias = self._on_device(weight), self._on_device(bias)
+        if tuple(weight.shape) != (self.out_channels, self.channels):
+            raise RangeError(f"weight is {tuple(weight.shape)}; expected {(self.out_channels, self.channels)}")
+        dtype = _tensor(self.device, "weight", weight, self.out_channels * self.channels)
+        if bias is not None:
+            _tensor(self.device, "bias", bias, self.out_channels, "f32")
+        self.bias = bias
+        _encode(self.device, weight, dtype, self.forward, 128, self.transposed)
+
+
+def prepare_float8_linear_weights(device, weight, bias=None):
+    """``Float8LinearWeights`` of a ``[outChannels][channels]`` weight: a CUDA tensor, a host array or an ``EncodedTensor`` of a bundle."""
+    return Float8LinearWeights(_device(device), weight, bias)
+
+
+class Float8LinearGpu:
+    """The projection ``y = x . weight^T + bias`` on 8-bit operands with float32 sums, and its gradients.
+
+    ``run`` and ``input_gradient`` encode a float32 or bfloat16 operand in the call (``options``: format "e4m3" (default) | "e5m2") or take
+    a ``Float8Tensor``; with the option checkpoint the encoded operand is returned as ``checkpoint``.  Option output "f32" | "bf16":
+    the result's type, by default the operand's (bf16 for a ``Float8Tensor``)."""
+
+    def __init__(self, device: Device | None = None):
+        self.device = _device(device)
+
+    def _product(self, name, value, rows, channels, weights, bias, options, out):
+        dev, opts = self.device, options or {}
+        format = _format(opts.get("format", "e4m3"))
+        res = None
+        if isinstance(value, Float8Tensor):
+            operand, dtype = _matrix(dev, name, value, rows, channels), _output(opts, "bf16")
+        else:
+            source = _tensor(dev, name, value, rows * channels)
+            dtype = _output(opts, source)
+        if out is not None:
+            _tensor(dev, "out", out, rows * weights.rows, dtype)
+        if not isinstance(value, Float8Tensor):
+            operand = Float8Tensor.empty(rows, channels, format, value)
+            res = _encode(dev, value, source, operand)
+        if out is None:
+            out = operand.memory.new_empty((rows, weights.rows), dtype=_torch_dtype(dtype))
+        desc = nat.Float8LinearDesc(operand.desc, weights.desc, bias.data_ptr() if bias is not None else None, _DTYPE[dtype], 0, out.data_ptr())
+        done = _call(dev, dev.lib.lf_float8_linear_run, desc, (operand, weights, bias, out))
+        result = _result(dev, done, out)
+        if res is not None:
+            result["launches"] += int(res.launches)
+        if opts.get("checkpoint"):
+            result["checkpoint"] = operand
+        return result
+
+    def _weights(self, input):
+        rows, channels, n = _shape(input, "rows", "channels", "outChannels")
+        weights = input["weights"]
+        if not isinstance(weights, Float8LinearWeights):
+            raise ValueError("weights must come from prepare_float8_linear_weights")
+        if weights.device.ordinal != self.device.ordinal:
+            raise ValueError(f"weights are on cuda:{weights.device.ordinal}, the device's GPU is cuda:{self.device.ordinal}")
+        if (weights.out_channels, weights.channels) != (n, channels):
+            raise RangeError(f"weights are {weights.out_channels} x {weights.channels}; expected {n} x {channels}")
+        return rows, channels, n, weights
+
+    def run(self, input, options=None, out=None):
+        """``input``: rows, channels, outChannels, activations ``[rows][channels]``, weights -> ``output`` ``[rows][outChannels]``."""
+        rows, channels, _, weights = self._weights(input)
+        return self._product("activations", input["activations"], rows, channels, weights.forward, weights.bias, options, out)
+
+    def input_gradient(self, input, options=None, out=None):
+        """``input``: rows, channels, outChannels, gradient ``[rows][outChannels]``, weights -> ``output`` ``[rows][channels]``, the
+        gradient of the activations."""
+        rows, _, n, weights = self._weights(input)
+        return self._product("gradient", input["gradient"], rows, n, weights.transposed, None, options, out)
+
+    def weight_gradient(self, input, options=None):
+        """``input``: rows, channels, outChannels, gradient ``[rows][outChannels]`` (bfloat16 or a ``Float8Tensor``; a float32 gradient is
+        encoded first, ``float8_encode``), activations (the ``Float8Tensor`` that the forward pass multiplied with) -> ``weight``
+        ``[outChannels][channels]`` and ``bias`` ``[outChannels]``, float32, the same bits at every call."""
+        dev = self.device
+        rows, channels, n = _shape(input, "rows", "channels", "outChannels")
+        dy, x = input["gradient"], _matrix(dev, "activations", input["activations"], rows, channels)
+        encoded = isinstance(dy, Float8Tensor)
+        if encoded:
+            _matrix(dev, "gradient", dy, rows, n)
+        else:
+            _tensor(dev, "gradient", dy, rows * n, "bf16")
+        nbytes = int(dev.lib.lf_float8_weight_gradient_workspace(dev.handle, rows, channels, n))
+        import torch
+        weight = torch.empty((n, channels), dtype=torch.float32, device=x.memory.device)
+        bias = torch.empty(n, dtype=torch.float32, device=x.memory.device)
+        workspace = torch.empty(nbytes, dtype=torch.uint8, device=x.memory.device) if nbytes else None
+        desc = nat.Float8WeightGradientDesc(x.desc, None if encoded else dy.data_ptr(), dy.desc if encoded else _NO_MATRIX, n, 0, weight.data_ptr(),
+                                            bias.data_ptr(), workspace.data_ptr() if nbytes else None, nbytes)
+        res = _call(dev, dev.lib.lf_float8_weight_gradient_run, desc, (dy, x, weight, bias, workspace))
+        result = _result(dev, res, weight)
+        result["weight"] = result.pop("output")
+        result["bias"] = bias
+        return result

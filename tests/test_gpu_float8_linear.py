@@ -1,0 +1,83 @@
+"""The projection on 8-bit operands and its gradients against 64 bits.
+
+Products of two codes and their powers of two are exact in float32, and so are values of 8-bit forms in bf16; what is off is the sum.  A float32 sum of K
+terms is off by at most K 2^-23 sum|terms| to first order (2^-23: additions may truncate), however they are grouped; the
+weight's gradient adds products in sixteens (one instruction) and splits, whose chain is rows / 16 and at most 148 splits."""
+import numpy as np
+import pytest
+import torch
+
+import training_reference as ref
+
+pytestmark = pytest.mark.gpu
+TYPES = {"f32": torch.float32, "bf16": torch.bfloat16}
+STEP = 2.0 ** -23
+# rows, channels, outputs: single tokens, partial tiles, all tile widths (64, 128, 256 columns), several groups of 512 channels, odd everything
+SHAPES = [(1, 1, 1), (1, 16, 8), (3, 128, 64), (4, 1536, 384), (16, 384, 1536), (17, 130, 72), (33, 5, 500), (64, 640, 24), (127, 129, 65), (128, 128, 128), (129, 512, 257),
+          (200, 513, 100), (300, 1030, 333), (1000, 64, 1), (2500, 128, 512), (5000, 256, 1000), (20001, 72, 136), (4099, 1200, 640)]
+
+
+@pytest.fixture(scope="module")
+def dev():
+    import localfold_b200 as lf
+    d = lf.Device(0)
+    yield d
+    d.close()
+
+
+def host(t):
+    return t.double().cpu().numpy()
+
+
+def operands(seed, rows, c, n, dtype):
+    """Blocks of very different size, so that a scale taken from the wrong block shows."""
+    rng = np.random.default_rng(seed)
+    blocks = -(-c // 128)
+    x = rng.standard_normal((rows, c)) * np.exp2(rng.integers(-6, 6, (rows, blocks))).repeat(128, 1)[:, :c]
+    w = rng.standard_normal((n, c)) * np.exp2(rng.integers(-5, 5, (-(-n // 128), blocks))).repeat(128, 0)[:n].repeat(128, 1)[:, :c]
+    dy = rng.standard_normal((rows, n)) * np.exp2(rng.integers(-6, 6, (rows, 1))) * 1e-3
+    dy[rows - rows // 20:] = 0
+    bias = rng.standard_normal(n)
+    return [torch.as_tensor(t).to(TYPES[dtype]).cuda() for t in (x, w, dy)] + [torch.as_tensor(bias).float().cuda()]
+
+
+@pytest.mark.parametrize("name,dtype", [("e4m3", "f32"), ("e4m3", "bf16"), ("e5m2", "f32"), ("e5m2", "bf16")])
+@pytest.mark.parametrize("rows,c,n", SHAPES)
+def test_product(dev, rows, c, n, name, dtype):
+    import localfold_b200 as lf
+    x, w, _, bias = operands(rows + c + n, rows, c, n, dtype)
+    weights = lf.prepare_float8_linear_weights(dev, w, bias)
+    shape = {"rows": rows, "channels": c, "outChannels": n, "weights": weights}
+    linear = lf.Float8LinearGpu(dev)
+    got = linear.run({**shape, "activations": x}, {"format": name, "checkpoint": True})
+    weights.bias = None
+    again = linear.run({**shape, "activations": got["checkpoint"]}, {"output": "f32"})
+    dev.synchronize()
+    assert got["output"].dtype == TYPES[dtype] and again["output"].dtype == torch.float32
+    x8, w8 = ref.decoded(host(x), name), ref.decoded(host(w), "e4m3", 128)
+    want, size = x8 @ w8.T, np.abs(x8) @ np.abs(w8).T
+    ref.close(again["output"], want, c * STEP * size, "without a bias, float32")
+    want = want + host(bias)
+    ref.close(got["output"], want, c * STEP * size + (STEP + ref.half_step(dtype)) * (np.abs(want) + c * STEP * size), dtype)
+
+
+@pytest.mark.parametrize("name,dtype", [("e4m3", "bf16"), ("e5m2", "f32")])
+@pytest.mark.parametrize("rows,c,n", SHAPES)
+def test_gradients(dev, rows, c, n, name, dtype):
+    import localfold_b200 as lf
+    x, w, dy, bias = operands(rows + c + n, rows, c, n, dtype)
+    linear, weights = lf.Float8LinearGpu(dev), lf.prepare_float8_linear_weights(dev, w, bias)
+    shape = {"rows": rows, "channels": c, "outChannels": n}
+    x8 = lf.float8_encode(dev, x, rows, c)
+    dx = linear.input_gradient({**shape, "gradient": dy, "weights": weights}, {"format": name, "checkpoint": True, "output": "f32"})
+    operand = dx["checkpoint"] if dtype == "f32" else dy
+    grads = linear.weight_gradient({**shape, "gradient": operand, "activations": x8})
+    same = linear.weight_gradient({**shape, "gradient": operand, "activations": x8})
+    dev.synchronize()
+    assert torch.equal(grads["weight"], same["weight"]) and torch.equal(grads["bias"], same["bias"])
+    xv, wv, dyv = ref.decoded(host(x), "e4m3"), ref.decoded(host(w), "e4m3", 128), ref.decoded(host(dy), name)
+    ref.close(dx["output"], dyv @ wv, n * STEP * (np.abs(dyv) @ np.abs(wv)), "input")
+    dv = dyv if dtype == "f32" else host(dy)
+    chain = (rows / 16 + 16 + 148) * STEP
+    ref.close(grads["weight"], dv.T @ xv, chain * (np.abs(dv).T @ np.abs(xv)), "weight")
+    ref.close(grads["bias"], dv.sum(0), chain * np.abs(dv).sum(0), "bias")
