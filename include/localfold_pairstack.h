@@ -645,14 +645,16 @@ typedef struct lf_layer_norm_backward_desc {
 LF_API uint64_t lf_layer_norm_backward_workspace(const lf_context* ctx, int64_t rows, int32_t channels);
 LF_API lf_status lf_layer_norm_backward_run(lf_context* ctx, const lf_layer_norm_backward_desc* d, lf_result* r);
 
-/* out[m][n] = sum_k activations[m][k] weights[n][k] (+ bias[n]), float32 sums, out_dtype rows.  The
- * gradient of a projection's input is the same call on the encoded gradient and the transposed
- * weights. */
+/* out[m][n] = sum_k activations[m][k] weights[n][k] (+ bias[n]), float32 sums, out_dtype rows.  With
+ * `source` [rows][channels] of source_dtype its 8-bit form is made first, into the buffers of
+ * `activations`.  The gradient of a projection's input is the same call on the encoded gradient and
+ * the transposed weights. */
 typedef struct lf_float8_linear_desc {
   lf_float8_matrix activations;   /* [rows][channels] */
   lf_float8_matrix weights;       /* [out channels][channels] */
   const float* bias;              /* [out channels] or null */
-  int32_t out_dtype, reserved;
+  int32_t out_dtype, source_dtype;
+  const void* source;             /* or null: activations are encoded already */
   void* out;
 } lf_float8_linear_desc;
 LF_API lf_status lf_float8_linear_run(lf_context* ctx, const lf_float8_linear_desc* d, lf_result* r);

@@ -166,7 +166,7 @@ class LayerNormBackwardDesc(ctypes.Structure):
 
 class Float8LinearDesc(ctypes.Structure):
     _fields_ = [("activations", Float8Matrix), ("weights", Float8Matrix), ("bias", c_void_p), ("out_dtype", c_int32),
-                ("reserved", c_int32), ("out", c_void_p)]
+                ("source_dtype", c_int32), ("source", c_void_p), ("out", c_void_p)]
 
 
 class Float8WeightGradientDesc(ctypes.Structure):

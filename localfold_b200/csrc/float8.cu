@@ -1,45 +1,46 @@
 // To and from the 8-bit form of a matrix (float8.cuh): activations with an exponent for every 128 channels of a row, weights with one
 // for every 128 x 128 elements, both orientations in one pass.
 //
-// Each element is read and written once and needs a handful of instructions: memory bounds these kernels.  Sixteen lanes hold a
-// block of 128 channels, eight neighbours each (narrow rows: eight lanes for at most 64 channels), so that the block's largest magnitude takes
-// four shuffles and codes leave as eight bytes a lane; every lane keeps kUnits blocks in flight.
+// Each element is read and written once and needs a handful of instructions: memory bounds these kernels.  A lane has sixteen neighbouring
+// channels, eight lanes a block of 128 (narrow rows: four lanes for at most 64 channels), so that the block's largest magnitude takes
+// three shuffles and all accesses are 16 or 32 bytes; every lane keeps kUnits blocks in flight.
 #include "float8.cuh"
 
 namespace f8 {
 
-constexpr int kThreads = 256, kUnits = 4;
+constexpr int kThreads = 256, kUnits = 2;
 
 template <typename T, int LANES>
 __global__ void __launch_bounds__(kThreads)
-encode_kernel(const T* x, const Matrix m, uint32_t units, uint32_t per_row, int vector) {
+encode_kernel(const T* x, const Matrix m, uint32_t units, uint32_t per_row, int access) {
   const int lane = threadIdx.x % LANES;
   const uint32_t base = blockIdx.x * (uint32_t)(kThreads / LANES * kUnits) + threadIdx.x / LANES;
   lf_chain();
-  float v[kUnits][8];
+  Raw<T> raw[kUnits];
   uint32_t row[kUnits], first[kUnits];
 #pragma unroll
   for (int u = 0; u < kUnits; ++u) {
     const uint32_t unit = base + u * (kThreads / LANES);
     row[u] = per_row == 1 ? unit : unit / per_row;
-    first[u] = (unit - row[u] * per_row) * kBlock + lane * 8;
-    load8(x + (int64_t)row[u] * m.channels + first[u], unit < units ? m.channels - (int)first[u] : 0, vector, v[u]);
+    first[u] = (unit - row[u] * per_row) * kBlock + lane * kShare;
+    if (unit >= units) first[u] = (uint32_t)m.channels;      // nothing to read or write
+    load16(raw[u], x + (int64_t)row[u] * m.channels + first[u], m.channels - (int)first[u], access);
   }
 #pragma unroll
   for (int u = 0; u < kUnits; ++u) {
-    uint2 codes;
-    const int s = encode8<LANES>(v[u], m.format, codes);
-    if (base + u * (kThreads / LANES) < units) put8(m, row[u], first[u], codes, s, lane == 0);
+    uint4 codes;
+    const int s = encode16<LANES>(unpack(raw[u]), m.format, codes);
+    put16(m, row[u], first[u], codes, s);
   }
 }
 
 template <typename T, int LANES>
 __global__ void __launch_bounds__(kThreads)
-decode_kernel(const Matrix m, T* out, uint32_t units, uint32_t per_row, int vector) {
+decode_kernel(const Matrix m, T* out, uint32_t units, uint32_t per_row, int access) {
   const int lane = threadIdx.x % LANES;
   const uint32_t base = blockIdx.x * (uint32_t)(kThreads / LANES * kUnits) + threadIdx.x / LANES;
   lf_chain();
-  uint2 codes[kUnits];
+  uint4 codes[kUnits];
   int s[kUnits];
   uint32_t row[kUnits], first[kUnits];
 #pragma unroll
@@ -47,21 +48,23 @@ decode_kernel(const Matrix m, T* out, uint32_t units, uint32_t per_row, int vect
     const uint32_t unit = base + u * (kThreads / LANES);
     row[u] = per_row == 1 ? unit : unit / per_row;
     const uint32_t block = unit - row[u] * per_row;
-    first[u] = block * kBlock + lane * 8;
-    if (unit >= units) first[u] = (uint32_t)m.channels;      // nothing left to write
-    codes[u] = make_uint2(0, 0);
+    first[u] = block * kBlock + lane * kShare;
+    if (unit >= units) first[u] = (uint32_t)m.channels;      // nothing to read or write
+    codes[u] = make_uint4(0, 0, 0, 0);
     s[u] = 1;
     if (first[u] < (uint32_t)m.channels) {
-      codes[u] = *reinterpret_cast<const uint2*>(m.codes + row[u] * m.pitch + first[u]);
+      codes[u] = *reinterpret_cast<const uint4*>(m.codes + row[u] * m.pitch + first[u]);
       s[u] = m.exponents[exponent_at(row[u], block, m.tiles)];
     }
   }
 #pragma unroll
   for (int u = 0; u < kUnits; ++u) {
     if (first[u] >= (uint32_t)m.channels) continue;
-    float v[8];
-    decode8(codes[u], up(s[u]), m.format, v);
-    store8(out + (int64_t)row[u] * m.channels + first[u], m.channels - (int)first[u], vector, v);
+    Share v = decode16(codes[u], m.format);
+    const float2 factor = both(up(s[u]));
+#pragma unroll
+    for (int i = 0; i < kShare / 2; ++i) v.v[i] = mul2(v.v[i], factor);
+    store16(out + (int64_t)row[u] * m.channels + first[u], m.channels - (int)first[u], access, v);
   }
 }
 
@@ -69,65 +72,71 @@ decode_kernel(const Matrix m, T* out, uint32_t units, uint32_t per_row, int vect
 // channels exchanged - the exponent is the block's, so the transposed matrix stands for the same values.
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
-encode_square_kernel(const T* x, const Matrix m, const Matrix t, int vector) {
-  __shared__ uint32_t most_s[2][kThreads / 32];
-  __shared__ uint8_t turned[kBlock][kBlock + 8];
-  const int lane = threadIdx.x & 15, strand = threadIdx.x >> 4;
+encode_square_kernel(const T* x, const Matrix m, const Matrix t, int access) {
+  __shared__ float most_s[2][kThreads / 32];
+  __shared__ __align__(16) uint8_t turned[kBlock][kBlock + 16];
+  constexpr int kRows = kBlock * 8 / kThreads;      // of a thread
+  const int lane = threadIdx.x & 7, strand = threadIdx.x >> 3;
   const int64_t row0 = (int64_t)blockIdx.y * kBlock;
-  const int first = blockIdx.x * kBlock + lane * 8;
+  const int first = blockIdx.x * kBlock + lane * kShare;
   lf_chain();
-  float v[8][8];
-  uint32_t most = 0, finite = 0;
+  Raw<T> raw[kRows];
 #pragma unroll
-  for (int k = 0; k < 8; ++k) {
-    const int64_t row = row0 + strand + 16 * k;
-    load8(x + row * m.channels + first, row < m.rows ? m.channels - first : 0, vector, v[k]);
+  for (int k = 0; k < kRows; ++k) {
+    const int64_t row = row0 + strand + kThreads / 8 * k;
+    load16(raw[k], x + row * m.channels + first, row < m.rows ? m.channels - first : 0, access);
+  }
+  float most = 0.f, finite = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      most = max(most, magnitude(v[k][i]));
-      finite = max(finite, magnitude(v[k][i]) < kInfinity ? magnitude(v[k][i]) : 0u);
+  for (int k = 0; k < kRows; ++k) {
+    const Share v = unpack(raw[k]);
+#pragma unroll
+    for (int i = 0; i < kShare; ++i) {
+      const float a = fabsf(i & 1 ? v.v[i / 2].y : v.v[i / 2].x);
+      most = fmaxf(most, a);
+      if (a < kInfinity) finite = fmaxf(finite, a);
     }
   }
-  most = __reduce_max_sync(0xffffffffu, most);
-  finite = __reduce_max_sync(0xffffffffu, finite);
+#pragma unroll
+  for (int o = 16; o; o >>= 1) { most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o)); finite = fmaxf(finite, __shfl_xor_sync(0xffffffffu, finite, o)); }
   if ((threadIdx.x & 31) == 0) { most_s[0][threadIdx.x >> 5] = most; most_s[1][threadIdx.x >> 5] = finite; }
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < kThreads / 32; ++w) { most = max(most, most_s[0][w]); finite = max(finite, most_s[1][w]); }
-  const int s = exponent_byte(finite, m.format);
+  for (int w = 0; w < kThreads / 32; ++w) { most = fmaxf(most, most_s[0][w]); finite = fmaxf(finite, most_s[1][w]); }
+  const int s = exponent_byte(__float_as_uint(finite), m.format);
   const float f = down(s);
 #pragma unroll
-  for (int k = 0; k < 8; ++k) {
-    const int64_t row = row0 + strand + 16 * k;
-    uint32_t w[2] = {0, 0};
+  for (int k = 0; k < kRows; ++k) {
+    const int64_t row = row0 + strand + kThreads / 8 * k;
+    const Share v = unpack(raw[k]);
+    uint32_t w[4] = {0, 0, 0, 0};
     if (most < kInfinity) {
 #pragma unroll
-      for (int i = 0; i < 8; i += 2) w[i >> 2] |= code2(v[k][i] * f, v[k][i + 1] * f, m.format) << (8 * (i & 3));
+      for (int i = 0; i < kShare / 2; ++i) w[i >> 1] |= code2(v.v[i].x * f, v.v[i].y * f, m.format) << (16 * (i & 1));
     } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) w[i >> 2] |= code_special(v[k][i] * f, m.format) << (8 * (i & 3));
+      for (int i = 0; i < kShare / 2; ++i)
+        w[i >> 1] |= (code_special(v.v[i].x * f, m.format) | code_special(v.v[i].y * f, m.format) << 8) << (16 * (i & 1));
     }
-    if (row < m.rows && first < m.pitch) *reinterpret_cast<uint2*>(m.codes + row * m.pitch + first) = make_uint2(w[0], w[1]);
+    if (row < m.rows && first < m.channels) *reinterpret_cast<uint4*>(m.codes + row * m.pitch + first) = make_uint4(w[0], w[1], w[2], w[3]);
     if (t.codes) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) turned[lane * 8 + i][strand + 16 * k] = (uint8_t)(w[i >> 2] >> (8 * (i & 3)));
+      for (int i = 0; i < kShare; ++i) turned[lane * kShare + i][strand + kThreads / 8 * k] = (uint8_t)(w[i >> 2] >> (8 * (i & 3)));
     }
   }
   if (threadIdx.x < kBlock) m.exponents[exponent_at(row0 + threadIdx.x, blockIdx.x, m.tiles)] = (uint8_t)s;
   if (!t.codes) return;
   __syncthreads();
   const int64_t trow0 = (int64_t)blockIdx.x * kBlock;
-  const int tfirst = blockIdx.y * kBlock + lane * 8;
+  const int tfirst = blockIdx.y * kBlock + lane * kShare;
 #pragma unroll
-  for (int k = 0; k < 8; ++k) {
-    const int64_t row = trow0 + strand + 16 * k;
-    if (row < t.rows && tfirst < t.pitch)
-      *reinterpret_cast<uint2*>(t.codes + row * t.pitch + tfirst) = *reinterpret_cast<const uint2*>(&turned[strand + 16 * k][lane * 8]);
+  for (int k = 0; k < kRows; ++k) {
+    const int64_t row = trow0 + strand + kThreads / 8 * k;
+    if (row < t.rows && tfirst < t.channels)
+      *reinterpret_cast<uint4*>(t.codes + row * t.pitch + tfirst) = *reinterpret_cast<const uint4*>(&turned[strand + kThreads / 8 * k][lane * kShare]);
   }
   if (threadIdx.x < kBlock) t.exponents[exponent_at(trow0 + threadIdx.x, blockIdx.y, t.tiles)] = (uint8_t)s;
 }
-
-static int vector_rows(const void* p, int c, int dtype) { return lf_aligned16(p) && c % (dtype == LF_DTYPE_BF16 ? 8 : 4) == 0; }
 
 }  // namespace f8
 
@@ -179,23 +188,23 @@ lf_status lf_float8_encode(lf_context* ctx, const lf_float8_encode_desc* d, lf_r
   if (d->block_rows == kBlock && row_tiles(o.rows) > 65535) return lf_fail(ctx, LF_ERR_UNSUPPORTED, "float8 encode: %lld rows are too many for blocks of 128 rows", (long long)o.rows);
   LF_CUDA(ctx, cudaSetDevice(ctx->device));
   const Matrix m = matrix(o);
-  const int vector = vector_rows(d->source, o.channels, d->dtype);
+  const int access = row_access(d->source, o.channels, d->dtype);
   lf_prof_begin(ctx, LF_KERNEL_ELEMENTWISE);
   if (d->block_rows == kBlock) {
     Matrix t{};
     if (turned) t = matrix(d->transposed);
     const dim3 grid(blocks(o.channels), (unsigned)row_tiles(o.rows));
-    if (d->dtype == LF_DTYPE_BF16) lf_launch(ctx, encode_square_kernel<bf16>, grid, kThreads, 0, (const bf16*)d->source, m, t, vector);
-    else lf_launch(ctx, encode_square_kernel<float>, grid, kThreads, 0, (const float*)d->source, m, t, vector);
+    if (d->dtype == LF_DTYPE_BF16) lf_launch(ctx, encode_square_kernel<bf16>, grid, kThreads, 0, (const bf16*)d->source, m, t, access);
+    else lf_launch(ctx, encode_square_kernel<float>, grid, kThreads, 0, (const float*)d->source, m, t, access);
   } else {
     const uint32_t per_row = blocks(o.channels), units = (uint32_t)(o.rows * per_row);
     auto run = [&](auto lanes) {
       constexpr int L = decltype(lanes)::value;
       const int grid = lf_ceil_div(units, kThreads / L * kUnits);
-      if (d->dtype == LF_DTYPE_BF16) lf_launch(ctx, encode_kernel<bf16, L>, grid, kThreads, 0, (const bf16*)d->source, m, units, per_row, vector);
-      else lf_launch(ctx, encode_kernel<float, L>, grid, kThreads, 0, (const float*)d->source, m, units, per_row, vector);
+      if (d->dtype == LF_DTYPE_BF16) lf_launch(ctx, encode_kernel<bf16, L>, grid, kThreads, 0, (const bf16*)d->source, m, units, per_row, access);
+      else lf_launch(ctx, encode_kernel<float, L>, grid, kThreads, 0, (const float*)d->source, m, units, per_row, access);
     };
-    if (o.channels <= 64) run(std::integral_constant<int, 8>{}); else run(std::integral_constant<int, 16>{});
+    if (o.channels <= 64) run(std::integral_constant<int, 4>{}); else run(std::integral_constant<int, 8>{});
   }
   lf_prof_end(ctx);
   ctx->launches++;
@@ -210,16 +219,16 @@ lf_status lf_float8_decode(lf_context* ctx, const lf_float8_decode_desc* d, lf_r
   LF_TRY(lf_float8_check(ctx, "float8 decode", o, o.rows, o.channels));
   LF_CUDA(ctx, cudaSetDevice(ctx->device));
   const Matrix m = matrix(o);
-  const int vector = vector_rows(d->out, o.channels, d->dtype);
+  const int access = row_access(d->out, o.channels, d->dtype);
   const uint32_t per_row = blocks(o.channels), units = (uint32_t)(o.rows * per_row);
   lf_prof_begin(ctx, LF_KERNEL_ELEMENTWISE);
   auto run = [&](auto lanes) {
     constexpr int L = decltype(lanes)::value;
     const int grid = lf_ceil_div(units, kThreads / L * kUnits);
-    if (d->dtype == LF_DTYPE_BF16) lf_launch(ctx, decode_kernel<bf16, L>, grid, kThreads, 0, m, (bf16*)d->out, units, per_row, vector);
-    else lf_launch(ctx, decode_kernel<float, L>, grid, kThreads, 0, m, (float*)d->out, units, per_row, vector);
+    if (d->dtype == LF_DTYPE_BF16) lf_launch(ctx, decode_kernel<bf16, L>, grid, kThreads, 0, m, (bf16*)d->out, units, per_row, access);
+    else lf_launch(ctx, decode_kernel<float, L>, grid, kThreads, 0, m, (float*)d->out, units, per_row, access);
   };
-  if (o.channels <= 64) run(std::integral_constant<int, 8>{}); else run(std::integral_constant<int, 16>{});
+  if (o.channels <= 64) run(std::integral_constant<int, 4>{}); else run(std::integral_constant<int, 8>{});
   lf_prof_end(ctx);
   ctx->launches++;
   return lf_float8_done(ctx, r, 1);

@@ -46,8 +46,7 @@ __device__ __forceinline__ int exponent_byte(uint32_t amax, int format) {
 __device__ __forceinline__ float down(int s) { return __int_as_float((254 - s) << 23); }
 __device__ __forceinline__ float up(int s) { return __int_as_float(s << 23); }
 
-__device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
-constexpr uint32_t kInfinity = 0x7f800000u;
+constexpr float kInfinity = __builtin_huge_valf();
 
 // Two codes, x in the low byte.  `scaled` values are within the format's range (or not finite: see code_special).
 __device__ __forceinline__ uint32_t code2(float x, float y, int format) {
@@ -55,107 +54,162 @@ __device__ __forceinline__ uint32_t code2(float x, float y, int format) {
 }
 // One code of a value that may be infinite: e4m3 has no infinity, so that it becomes NaN and is not lost in a finite code.
 __device__ __forceinline__ uint32_t code_special(float v, int format) {
-  const uint32_t sign = __float_as_uint(v) >> 24 & 0x80u;
-  if (magnitude(v) > kInfinity) return format == LF_FLOAT8_E4M3 ? 0x7fu : 0x7eu;
-  if (magnitude(v) == kInfinity) return sign | (format == LF_FLOAT8_E4M3 ? 0x7fu : 0x7cu);
+  if (fabsf(v) == kInfinity) return (__float_as_uint(v) >> 24 & 0x80u) | (format == LF_FLOAT8_E4M3 ? 0x7fu : 0x7cu);
   return code2(v, 0.f, format) & 0xffu;
 }
 __device__ __forceinline__ float2 decode2(uint32_t two, int format) {
   const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)two, format == LF_FLOAT8_E4M3 ? __NV_E4M3 : __NV_E5M2);
   return __half22float2(*reinterpret_cast<const __half2*>(&h));
 }
-// Eight codes -> eight values times `factor`
-__device__ __forceinline__ void decode8(uint2 codes, float factor, int format, float (&v)[8]) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 d = decode2((i < 2 ? codes.x : codes.y) >> (16 * (i & 1)) & 0xffffu, format);
-    v[2 * i] = d.x * factor;
-    v[2 * i + 1] = d.y * factor;
-  }
+
+// A lane's share of a row is sixteen neighbouring channels, as eight pairs for the two-at-once float32 instructions: eight lanes hold a
+// block.  (Eight channels a lane: the shuffles of a block's maximum and of a row's sums cost twice as much an element, and codes leave
+// in pieces of eight bytes; LayerNorm + checkpoint of 147456 x 128 took 42 us then, its backward pass 48, encoding 1 Mi x 128 121.)
+constexpr int kShare = 16;
+struct Share { float2 v[kShare / 2]; };
+
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 y;
+  asm("{\n\t.reg .b64 a, b;\n\t"
+      "mov.b64 a, {%2, %3};\n\t"
+      "mov.b64 b, {%4, %5};\n\t"
+      "mul.rn.f32x2 a, a, b;\n\t"
+      "mov.b64 {%0, %1}, a;\n\t}"
+      : "=f"(y.x), "=f"(y.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return y;
+}
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+
+// What a lane loads of a row, still as it lies in memory.
+template <typename T>
+struct Raw { uint32_t w[kShare * sizeof(T) / 4]; };
+
+// How rows can be accessed: 32 bytes at a time, 16, or element by element.
+enum { kElements = 0, kSixteen = 1, kThirtyTwo = 2 };
+static inline int row_access(const void* p, int c, int dtype) {
+  const int64_t bytes = (int64_t)c * (dtype == LF_DTYPE_BF16 ? 2 : 4);
+  return ((uintptr_t)p & 31) == 0 && bytes % 32 == 0 ? kThirtyTwo : ((uintptr_t)p & 15) == 0 && bytes % 16 == 0 ? kSixteen : kElements;
 }
 
-// Eight neighbouring values of a row as one lane of a group of LANES <= 16 (a whole block's, or all of a narrower row's) holds them: the
-// block's exponent byte, and the lane's codes.  All lanes of the warp call it.
-template <int LANES>
-__device__ __forceinline__ int encode8(const float (&v)[8], int format, uint2& codes) {
-  uint32_t most = 0;
+// `count` channels of the row are left from p on; what lies behind them reads as zero.
+template <typename T>
+__device__ __forceinline__ void load16(Raw<T>& r, const T* p, int count, int access) {
+  constexpr int kWords = kShare * sizeof(T) / 4;
+  if (count >= kShare && access == kThirtyTwo) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) most = max(most, magnitude(v[i]));
+    for (int i = 0; i < kWords; i += 8)
+      asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                   : "=r"(r.w[i]), "=r"(r.w[i + 1]), "=r"(r.w[i + 2]), "=r"(r.w[i + 3]), "=r"(r.w[i + 4]), "=r"(r.w[i + 5]), "=r"(r.w[i + 6]), "=r"(r.w[i + 7])
+                   : "l"(reinterpret_cast<const uint32_t*>(p) + i)
+                   : "memory");
+  } else if (count >= kShare && access == kSixteen) {
 #pragma unroll
-  for (int o = LANES / 2; o; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
-  if (__any_sync(0xffffffffu, most >= kInfinity)) {      // values that are not finite have no say in the scale
-    uint32_t finite = 0;
+    for (int i = 0; i < kWords; i += 4) {
+      const uint4 u = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint32_t*>(p) + i);
+      r.w[i] = u.x; r.w[i + 1] = u.y; r.w[i + 2] = u.z; r.w[i + 3] = u.w;
+    }
+  } else if (sizeof(T) == 4) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) finite = max(finite, magnitude(v[i]) < kInfinity ? magnitude(v[i]) : 0u);
+    for (int i = 0; i < kShare; ++i) r.w[i] = i < count ? reinterpret_cast<const uint32_t*>(p)[i] : 0u;
+  } else {
 #pragma unroll
-    for (int o = LANES / 2; o; o >>= 1) finite = max(finite, __shfl_xor_sync(0xffffffffu, finite, o));
-    const int s = exponent_byte(finite, format);
-    const float f = down(s);
-    uint32_t w[2] = {0, 0};
-#pragma unroll
-    for (int i = 0; i < 8; ++i) w[i >> 2] |= code_special(v[i] * f, format) << (8 * (i & 3));
-    codes = make_uint2(w[0], w[1]);
-    return s;
+    for (int i = 0; i < kShare; i += 2)
+      r.w[i / 2] = (i < count ? (uint32_t)reinterpret_cast<const uint16_t*>(p)[i] : 0u) |
+                   (i + 1 < count ? (uint32_t)reinterpret_cast<const uint16_t*>(p)[i + 1] << 16 : 0u);
   }
-  const int s = exponent_byte(most, format);
-  const float f = down(s);
-  codes.x = code2(v[0] * f, v[1] * f, format) | code2(v[2] * f, v[3] * f, format) << 16;
-  codes.y = code2(v[4] * f, v[5] * f, format) | code2(v[6] * f, v[7] * f, format) << 16;
+}
+template <typename T>
+__device__ __forceinline__ Share unpack(const Raw<T>& r) {
+  Share s;
+#pragma unroll
+  for (int i = 0; i < kShare / 2; ++i) {
+    if (sizeof(T) == 4) s.v[i] = make_float2(__uint_as_float(r.w[(2 * i) % (kShare * sizeof(T) / 4)]), __uint_as_float(r.w[(2 * i + 1) % (kShare * sizeof(T) / 4)]));
+    else s.v[i] = make_float2(__uint_as_float(r.w[i] << 16), __uint_as_float(r.w[i] & 0xffff0000u));
+  }
+  return s;
+}
+template <typename T>
+__device__ __forceinline__ void store16(T* p, int count, int access, const Share& s) {
+  constexpr int kWords = kShare * sizeof(T) / 4;
+  uint32_t w[kWords];
+#pragma unroll
+  for (int i = 0; i < kShare / 2; ++i) {
+    if (sizeof(T) == 4) { w[(2 * i) % kWords] = __float_as_uint(s.v[i].x); w[(2 * i + 1) % kWords] = __float_as_uint(s.v[i].y); }
+    else {
+      const __nv_bfloat162 t = __floats2bfloat162_rn(s.v[i].x, s.v[i].y);
+      w[i] = *reinterpret_cast<const uint32_t*>(&t);
+    }
+  }
+  if (count >= kShare && access == kThirtyTwo) {
+#pragma unroll
+    for (int i = 0; i < kWords; i += 8)
+      asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(reinterpret_cast<uint32_t*>(p) + i), "r"(w[i]), "r"(w[i + 1]), "r"(w[i + 2]),
+                   "r"(w[i + 3]), "r"(w[i + 4]), "r"(w[i + 5]), "r"(w[i + 6]), "r"(w[i + 7])
+                   : "memory");
+  } else if (count >= kShare && access == kSixteen) {
+#pragma unroll
+    for (int i = 0; i < kWords; i += 4) *reinterpret_cast<uint4*>(reinterpret_cast<uint32_t*>(p) + i) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kShare; ++i) {
+      if (sizeof(T) == 4) { if (i < count) reinterpret_cast<uint32_t*>(p)[i] = w[i % kWords]; }
+      else if (i < count) reinterpret_cast<uint16_t*>(p)[i] = (uint16_t)(w[i / 2] >> (16 * (i & 1)));
+    }
+  }
+}
+__device__ __forceinline__ Share load_weights(const float* p, int count) {
+  Raw<float> r;
+  load16(r, p, count, kElements);
+  return unpack(r);
+}
+
+// A lane's sixteen codes -> values times `factor`
+__device__ __forceinline__ Share decode16(uint4 codes, int format) {
+  const uint32_t w[4] = {codes.x, codes.y, codes.z, codes.w};
+  Share s;
+#pragma unroll
+  for (int i = 0; i < kShare / 2; ++i) s.v[i] = decode2(w[i >> 1] >> (16 * (i & 1)) & 0xffffu, format);
   return s;
 }
 
-// Eight neighbouring elements of a row: `vector` - the address is a multiple of their bytes (or of 16) and all eight exist; else the
-// first `count`, zeros behind them.
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, int count, bool vector, float (&v)[8]);
-template <>
-__device__ __forceinline__ void load8<float>(const float* p, int count, bool vector, float (&v)[8]) {
-  if (vector && count >= 8) {
-    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-  } else {
+// The exponent byte of the block that LANES neighbouring lanes hold (eight lanes, or all of a narrower row's), and the lane's codes.  All lanes of
+// the warp call it.  NaN has no say in a maximum; infinities must not have one either.
+template <int LANES>
+__device__ __forceinline__ int encode16(const Share& x, int format, uint4& codes) {
+  float most = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = i < count ? p[i] : 0.f;
-  }
-}
-template <>
-__device__ __forceinline__ void load8<bf16>(const bf16* p, int count, bool vector, float (&v)[8]) {
-  if (vector && count >= 8) {
-    const uint4 w = *reinterpret_cast<const uint4*>(p);
-    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+  for (int i = 0; i < kShare / 2; ++i) most = fmaxf(most, fmaxf(fabsf(x.v[i].x), fabsf(x.v[i].y)));
 #pragma unroll
-    for (int i = 0; i < 4; ++i) { v[2 * i] = __uint_as_float(u[i] << 16); v[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u); }
-  } else {
+  for (int o = LANES / 2; o; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+  uint32_t w[4];
+  if (__any_sync(0xffffffffu, most == kInfinity)) {
+    most = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = i < count ? __bfloat162float(p[i]) : 0.f;
-  }
-}
-template <typename T>
-__device__ __forceinline__ void store8(T* p, int count, bool vector, const float (&v)[8]);
-template <>
-__device__ __forceinline__ void store8<float>(float* p, int count, bool vector, const float (&v)[8]) {
-  if (vector && count >= 8) {
-    reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
-    reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) if (i < count) p[i] = v[i];
-  }
-}
-template <>
-__device__ __forceinline__ void store8<bf16>(bf16* p, int count, bool vector, const float (&v)[8]) {
-  if (vector && count >= 8) {
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const __nv_bfloat162 t = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
-      w[i] = *reinterpret_cast<const uint32_t*>(&t);
+    for (int i = 0; i < kShare / 2; ++i) {
+      if (fabsf(x.v[i].x) < kInfinity) most = fmaxf(most, fabsf(x.v[i].x));
+      if (fabsf(x.v[i].y) < kInfinity) most = fmaxf(most, fabsf(x.v[i].y));
     }
-    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
-  } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) if (i < count) p[i] = __float2bfloat16_rn(v[i]);
+    for (int o = LANES / 2; o; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+    const int s = exponent_byte(__float_as_uint(most), format);
+    const float f = down(s);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      w[i] = code_special(x.v[2 * i].x * f, format) | code_special(x.v[2 * i].y * f, format) << 8 | code_special(x.v[2 * i + 1].x * f, format) << 16 |
+             code_special(x.v[2 * i + 1].y * f, format) << 24;
+    codes = make_uint4(w[0], w[1], w[2], w[3]);
+    return s;
   }
+  const int s = exponent_byte(__float_as_uint(most), format);
+  const float2 f = both(down(s));
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 a = mul2(x.v[2 * i], f), b = mul2(x.v[2 * i + 1], f);
+    w[i] = code2(a.x, a.y, format) | code2(b.x, b.y, format) << 16;
+  }
+  codes = make_uint4(w[0], w[1], w[2], w[3]);
+  return s;
 }
 
 // A matrix as the kernels take it.
@@ -168,13 +222,13 @@ struct Matrix {
 static inline Matrix matrix(const lf_float8_matrix& m) {
   return {(uint8_t*)m.codes, (uint8_t*)m.exponents, m.rows, row_tiles(m.rows), pitch(m.channels), m.channels, m.format};
 }
-// Codes and exponent of eight channels from `first`, all of which lie in the row's pitch; lanes whose `lead` is set write the exponent.
-__device__ __forceinline__ void put8(const Matrix& m, int64_t row, int first, uint2 codes, int s, bool lead) {
-  if (first < m.pitch) *reinterpret_cast<uint2*>(m.codes + row * m.pitch + first) = codes;
-  if (lead) {
-    // a row of one block writes its whole word: the words of a tile fill its sectors
+// A lane's codes (its channels from `first` on) and, from the lane that leads its block, the exponent.
+__device__ __forceinline__ void put16(const Matrix& m, int64_t row, int first, uint4 codes, int s) {
+  if (first >= m.channels) return;
+  *reinterpret_cast<uint4*>(m.codes + row * m.pitch + first) = codes;
+  if ((first & (kBlock - 1)) == 0) {
     uint8_t* e = m.exponents + exponent_at(row, first / kBlock, m.tiles);
-    if (m.channels <= kBlock) *reinterpret_cast<uint32_t*>(e) = 0x01010100u | (uint32_t)s;
+    if (m.channels <= kBlock) *reinterpret_cast<uint32_t*>(e) = 0x01010100u | (uint32_t)s;      // the only block of the row: its whole word
     else *e = (uint8_t)s;
   }
 }

@@ -294,6 +294,13 @@ extern "C" lf_status lf_float8_linear_run(lf_context* ctx, const lf_float8_linea
   LF_TRY(lf_float8_check(ctx, "float8 linear, weights", w, w.rows, x.channels));
   if (w.rows > (1 << 24)) return lf_fail(ctx, LF_ERR_UNSUPPORTED, "float8 linear: %lld output channels are too many", (long long)w.rows);
   if (row_tiles(x.rows) * ((w.rows + 63) / 64) > 0x7fffffffll) return lf_fail(ctx, LF_ERR_UNSUPPORTED, "float8 linear: %lld x %lld outputs are too many", (long long)x.rows, (long long)w.rows);
+  int launches = 1;
+  if (d->source) {
+    lf_float8_encode_desc e{};
+    e.out = x; e.dtype = d->source_dtype; e.block_rows = 1; e.source = d->source;
+    LF_TRY(lf_float8_encode(ctx, &e, nullptr));
+    ++launches;
+  }
   LF_CUDA(ctx, cudaSetDevice(ctx->device));
   const Matrix mx = matrix(x), mw = matrix(w);
   const bool f32 = d->out_dtype == LF_DTYPE_F32;
@@ -309,5 +316,5 @@ extern "C" lf_status lf_float8_linear_run(lf_context* ctx, const lf_float8_linea
   if (bn == 256) LF_TRY(f32 ? (tc::launch_float8<256, true>(ctx, mx, mw, p)) : (tc::launch_float8<256, false>(ctx, mx, mw, p)));
   else if (bn == 128) LF_TRY(f32 ? (tc::launch_float8<128, true>(ctx, mx, mw, p)) : (tc::launch_float8<128, false>(ctx, mx, mw, p)));
   else LF_TRY(f32 ? (tc::launch_float8<64, true>(ctx, mx, mw, p)) : (tc::launch_float8<64, false>(ctx, mx, mw, p)));
-  return lf_float8_done(ctx, r, 1);
+  return lf_float8_done(ctx, r, launches);
 }

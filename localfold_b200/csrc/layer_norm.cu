@@ -3,21 +3,24 @@
 //   forward   y = (x - mean) rstd g + b, mean and rstd over the c channels of a row in float32, in two passes over registers
 //   backward  u = (x - mean) rstd, h = dy g:  dx = rstd (h - mean(h) - u mean(h u)), dg = sum over rows of dy u, db = sum of dy
 //
-// Both read and write each element once, so memory bounds them.  A group of G lanes holds a row in registers, eight neighbouring
-// channels a lane and step: 16 lanes a block of 128 channels, so that the row can leave in its 8-bit form (float8.cuh) or come back
-// from it in the same pass.  Blocks stay and walk over the rows, the weights in registers; a lane always has the same channels, so
-// dg and db add up in its registers and every block leaves one row of sums, which a second, small kernel adds in a fixed order.
+// Both read and write each element once, so memory bounds them - as long as the instructions an element costs stay few: a lane has sixteen
+// neighbouring channels of a row, so that the shuffles of the sums are shared by sixteen elements, arithmetic goes two float32 at a time,
+// and eight lanes are a block of the 8-bit form (float8.cuh), which leaves or comes back in the same pass.  G lanes hold a row in registers.
+// Blocks stay and walk over the rows, the next row's loads in flight under the present one's arithmetic and the weights in registers; a lane always
+// has the same channels, so dg and db add up in its registers and every block leaves one row of sums, which a second, small kernel
+// adds in a fixed order.
 #include "float8.cuh"
+#include "tc05.cuh"
 
 namespace lnorm {
 
 using namespace f8;
-
-constexpr int kThreads = 256;
+using tc05::add2;
+using tc05::fma2;
 
 struct Forward {
   int64_t rows;
-  int c, vector_in, vector_out;
+  int c, access_in, access_out;
   float epsilon;
   const void* x;
   const float *scale, *offset;
@@ -28,7 +31,7 @@ struct Forward {
 
 struct Backward {
   int64_t rows;
-  int c, vector_dy, vector_x, vector_dx;
+  int c, access_dy, access_x, access_dx;
   const void *dy, *x;            // x null: `kept`
   Matrix kept;
   const float *mean, *inverse, *scale;
@@ -36,213 +39,193 @@ struct Backward {
   float* partial;                // [blocks][2][c]
 };
 
-// Sum over the G lanes of a row; G = kThreads: the whole block, through two rows of slots in turn.
+__host__ __device__ constexpr int threads_of(int G) { return G <= 256 ? 256 : G; }
+__host__ __device__ constexpr int blocks_of(int G) { return 512 / threads_of(G); }      // a multiprocessor's
+
+// Two sums over the G lanes of a row.  Wider than a warp: through two sets of slots in turn, with a barrier for the group's warps alone (which
+// all make the same number of calls).
 template <int G>
-__device__ __forceinline__ float group_sum(float v, float* slots, int& turn) {
+__device__ __forceinline__ float2 group_sum(float2 v, float2* slots, int& turn) {
 #pragma unroll
-  for (int o = (G < 32 ? G : 32) / 2; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  for (int o = (G < 32 ? G : 32) / 2; o; o >>= 1) {
+    v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
+    v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
+  }
   if (G > 32) {
-    float* s = slots + (turn++ & 1) * (kThreads / 32);
-    if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = 0.f;
+    constexpr int kWarps = threads_of(G) / 32, kOwn = G > 32 ? G / 32 : 1;
+    const int warp = threadIdx.x >> 5, group = warp / kOwn;
+    float2* s = slots + (turn++ & 1) * kWarps;
+    if ((threadIdx.x & 31) == 0) s[warp] = v;
+    asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "n"(G > 32 ? G : 32) : "memory");
+    v = make_float2(0.f, 0.f);
 #pragma unroll
-    for (int w = 0; w < kThreads / 32; ++w) v += s[w];
+    for (int w = 0; w < kOwn; ++w) { v.x += s[group * kOwn + w].x; v.y += s[group * kOwn + w].y; }
   }
   return v;
 }
 
-template <typename T, int G, int NV, int R>
-__global__ void __launch_bounds__(kThreads)
+template <typename T, int G>
+__global__ void __launch_bounds__(threads_of(G), blocks_of(G))
 forward_kernel(const Forward a) {
-  __shared__ float slots[2 * kThreads / 32];
-  constexpr int kGroups = kThreads / G;
-  const int lane = threadIdx.x % G, group = threadIdx.x / G;
+  constexpr int kGroups = threads_of(G) / G, kLanes = G < 8 ? G : 8;
+  __shared__ float2 slots[2 * threads_of(G) / 32];
+  const int lane = threadIdx.x % G, group = threadIdx.x / G, first = lane * kShare, left = a.c - first;
   int turn = 0;
   lf_chain();
-  float scale[NV][8], offset[NV][8];
-#pragma unroll
-  for (int v = 0; v < NV; ++v) {
-    const int first = (v * G + lane) * 8;
-    load8(a.scale + first, a.c - first, false, scale[v]);
-    load8(a.offset + first, a.c - first, false, offset[v]);
-  }
+  const int64_t step = (int64_t)gridDim.x * kGroups;
+  int64_t row = (int64_t)blockIdx.x * kGroups + group;
+  Raw<T> raw;
+  load16(raw, static_cast<const T*>(a.x) + row * a.c + first, row < a.rows ? left : 0, a.access_in);
+  const Share scale = load_weights(a.scale + first, left), offset = load_weights(a.offset + first, left);
   const float over = 1.0f / (float)a.c;
   // (the trip count is the same for every lane of a block)
-  for (int64_t base = (int64_t)blockIdx.x * kGroups * R; base < a.rows; base += (int64_t)gridDim.x * kGroups * R) {
-    float x[R][NV][8];
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const int64_t row = base + r * kGroups + group;
-#pragma unroll
-      for (int v = 0; v < NV; ++v) {
-        const int first = (v * G + lane) * 8;
-        load8(static_cast<const T*>(a.x) + row * a.c + first, row < a.rows ? a.c - first : 0, a.vector_in, x[r][v]);
-      }
+  for (int64_t base = (int64_t)blockIdx.x * kGroups; base < a.rows; base += step, row += step) {
+    const bool live = row < a.rows;
+    Share x = unpack(raw);
+    load16(raw, static_cast<const T*>(a.x) + (row + step) * a.c + first, row + step < a.rows ? left : 0, a.access_in);
+    if (a.kept.codes) {
+      uint4 codes;
+      const int s = encode16<kLanes>(x, a.kept.format, codes);
+      if (live) put16(a.kept, row, first, codes, s);
     }
+    float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const int64_t row = base + r * kGroups + group;
-      const bool live = row < a.rows;
-      if (a.kept.codes) {
+    for (int i = 0; i < kShare / 2; ++i) sum = add2(sum, x.v[i]);
+    const float mean = group_sum<G>(make_float2(sum.x + sum.y, 0.f), slots, turn).x * over;
+    sum = make_float2(0.f, 0.f);
 #pragma unroll
-        for (int v = 0; v < NV; ++v) {
-          const int first = (v * G + lane) * 8;
-          uint2 codes;
-          const int s = encode8<(G < 16 ? G : 16)>(x[r][v], a.kept.format, codes);
-          if (live) put8(a.kept, row, first, codes, s, (first & 127) == 0 && first < a.c);
+    for (int i = 0; i < kShare / 2; ++i) {
+      x.v[i] = add2(x.v[i], both(-mean));
+      if (left < kShare) {      // channels behind the last have no deviation
+        if (2 * i >= left) x.v[i].x = 0.f;
+        if (2 * i + 1 >= left) x.v[i].y = 0.f;
+      }
+      sum = fma2(x.v[i], x.v[i], sum);
+    }
+    const float inverse = 1.0f / sqrtf(fmaf(group_sum<G>(make_float2(sum.x + sum.y, 0.f), slots, turn).x, over, a.epsilon));
+    if (a.mean && live && lane == 0) { a.mean[row] = mean; a.inverse[row] = inverse; }
+#pragma unroll
+    for (int i = 0; i < kShare / 2; ++i) x.v[i] = fma2(mul2(x.v[i], both(inverse)), scale.v[i], offset.v[i]);
+    if (a.y && live) store16(static_cast<T*>(a.y) + row * a.c + first, left, a.access_out, x);
+    if (a.encoded.codes) {
+      if (left < kShare) {      // (0 * inverse is no zero in a row whose statistics are no numbers)
+#pragma unroll
+        for (int i = 0; i < kShare / 2; ++i) {
+          if (2 * i >= left) x.v[i].x = 0.f;
+          if (2 * i + 1 >= left) x.v[i].y = 0.f;
         }
       }
-      float sum = 0.f;
-#pragma unroll
-      for (int v = 0; v < NV; ++v)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) sum += x[r][v][i];
-      const float mean = group_sum<G>(sum, slots, turn) * over;
-      sum = 0.f;
-#pragma unroll
-      for (int v = 0; v < NV; ++v)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          x[r][v][i] -= mean;
-          if ((v * G + lane) * 8 + i < a.c) sum = fmaf(x[r][v][i], x[r][v][i], sum);
-        }
-      const float inverse = 1.0f / sqrtf(fmaf(group_sum<G>(sum, slots, turn), over, a.epsilon));
-      if (a.mean && live && lane == 0) { a.mean[row] = mean; a.inverse[row] = inverse; }
-#pragma unroll
-      for (int v = 0; v < NV; ++v) {
-        const int first = (v * G + lane) * 8;
-        float y[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = fmaf(x[r][v][i] * inverse, scale[v][i], offset[v][i]);
-        if (a.y && live) store8(static_cast<T*>(a.y) + row * a.c + first, a.c - first, a.vector_out, y);
-        if (a.encoded.codes) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) if (first + i >= a.c) y[i] = 0.f;
-          uint2 codes;
-          const int s = encode8<(G < 16 ? G : 16)>(y, a.encoded.format, codes);
-          if (live) put8(a.encoded, row, first, codes, s, (first & 127) == 0 && first < a.c);
-        }
-      }
+      uint4 codes;
+      const int s = encode16<kLanes>(x, a.encoded.format, codes);
+      if (live) put16(a.encoded, row, first, codes, s);
     }
   }
 }
 
-template <typename T, int G, int NV, int R>
-__global__ void __launch_bounds__(kThreads)
+template <typename T, int G, bool KEPT>
+__global__ void __launch_bounds__(threads_of(G), blocks_of(G))
 backward_kernel(const Backward a) {
-  constexpr int kGroups = kThreads / G;
-  __shared__ float slots[2 * kThreads / 32];
-  __shared__ float sums[kGroups > 1 ? kThreads * NV * 8 : 1];
-  const int lane = threadIdx.x % G, group = threadIdx.x / G;
+  constexpr int kThreads = threads_of(G), kGroups = kThreads / G;
+  __shared__ float2 slots[2 * kThreads / 32];
+  __shared__ float sums[kGroups > 1 ? kThreads * kShare : 1];
+  const int lane = threadIdx.x % G, group = threadIdx.x / G, first = lane * kShare, left = a.c - first;
   int turn = 0;
   lf_chain();
-  float scale[NV][8], dg[NV][8], db[NV][8];
-#pragma unroll
-  for (int v = 0; v < NV; ++v) {
-    const int first = (v * G + lane) * 8;
-    load8(a.scale + first, a.c - first, false, scale[v]);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) dg[v][i] = db[v][i] = 0.f;
-  }
-  const float over = 1.0f / (float)a.c;
-  for (int64_t base = (int64_t)blockIdx.x * kGroups * R; base < a.rows; base += (int64_t)gridDim.x * kGroups * R) {
-    float dy[R][NV][8], u[R][NV][8], mean[R], inverse[R];
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const int64_t row = base + r * kGroups + group;
-      const bool live = row < a.rows;
-      mean[r] = live ? a.mean[row] : 0.f;
-      inverse[r] = live ? a.inverse[row] : 0.f;
-#pragma unroll
-      for (int v = 0; v < NV; ++v) {
-        const int first = (v * G + lane) * 8, count = live ? a.c - first : 0;
-        load8(static_cast<const T*>(a.dy) + row * a.c + first, count, a.vector_dy, dy[r][v]);
-        if (a.x) load8(static_cast<const T*>(a.x) + row * a.c + first, count, a.vector_x, u[r][v]);
-        else {
-          uint2 codes = make_uint2(0, 0);
-          float factor = 0.f;
-          if (count > 0) {
-            codes = *reinterpret_cast<const uint2*>(a.kept.codes + row * a.kept.pitch + first);
-            factor = up(a.kept.exponents[exponent_at(row, first / kBlock, a.kept.tiles)]);
-          }
-          decode8(codes, factor, a.kept.format, u[r][v]);
-        }
-      }
+  const int64_t step = (int64_t)gridDim.x * kGroups;
+  int64_t row = (int64_t)blockIdx.x * kGroups + group;
+  Raw<T> raw_dy, raw_x;
+  uint4 codes;
+  float factor, mean, inverse;
+  auto fetch = [&](int64_t r) {      // (a row that does not exist is all zeros)
+    const bool live = r < a.rows;
+    const int count = live ? left : 0;
+    load16(raw_dy, static_cast<const T*>(a.dy) + r * a.c + first, count, a.access_dy);
+    codes = make_uint4(0, 0, 0, 0);
+    factor = 0.f;
+    if (!KEPT) load16(raw_x, static_cast<const T*>(a.x) + r * a.c + first, count, a.access_x);
+    else if (count > 0) {
+      codes = *reinterpret_cast<const uint4*>(a.kept.codes + r * a.kept.pitch + first);
+      factor = up(a.kept.exponents[exponent_at(r, first / kBlock, a.kept.tiles)]);
     }
+    mean = live ? a.mean[r] : 0.f;
+    inverse = live ? a.inverse[r] : 0.f;
+  };
+  fetch(row);
+  const Share scale = load_weights(a.scale + first, left);
+  Share dg, db;
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const int64_t row = base + r * kGroups + group;
-      float s1 = 0.f, s2 = 0.f;
+  for (int i = 0; i < kShare / 2; ++i) dg.v[i] = db.v[i] = make_float2(0.f, 0.f);
+  const float over = 1.0f / (float)a.c;
+  for (int64_t base = (int64_t)blockIdx.x * kGroups; base < a.rows; base += step, row += step) {
+    const Share dy = unpack(raw_dy);
+    Share u = KEPT ? decode16(codes, a.kept.format) : unpack(raw_x);
+    const float inv = inverse;
+    // (x - mean) rstd; of codes by one multiply-add, their power of two with rstd
+    const float2 by = both(KEPT ? factor * inv : inv), from = both(KEPT ? -mean * inv : -mean);
 #pragma unroll
-      for (int v = 0; v < NV; ++v)
+    for (int i = 0; i < kShare / 2; ++i) u.v[i] = KEPT ? fma2(u.v[i], by, from) : mul2(add2(u.v[i], from), by);
+    fetch(row + step);
+    float2 s1 = make_float2(0.f, 0.f), s2 = s1;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          u[r][v][i] = (u[r][v][i] - mean[r]) * inverse[r];
-          const float h = dy[r][v][i] * scale[v][i];
-          dg[v][i] = fmaf(dy[r][v][i], u[r][v][i], dg[v][i]);
-          db[v][i] += dy[r][v][i];
-          s1 += h;
-          s2 = fmaf(h, u[r][v][i], s2);
-        }
-      s1 = group_sum<G>(s1, slots, turn) * over;
-      s2 = group_sum<G>(s2, slots, turn) * over;
-      if (row < a.rows) {
+    for (int i = 0; i < kShare / 2; ++i) {
+      const float2 h = mul2(dy.v[i], scale.v[i]);
+      dg.v[i] = fma2(dy.v[i], u.v[i], dg.v[i]);
+      db.v[i] = add2(db.v[i], dy.v[i]);
+      s1 = add2(s1, h);
+      s2 = fma2(h, u.v[i], s2);
+    }
+    const float2 s = group_sum<G>(make_float2(s1.x + s1.y, s2.x + s2.y), slots, turn);
+    if (row < a.rows) {
+      const float2 t1 = both(-s.x * over * inv), t2 = both(-s.y * over * inv);
 #pragma unroll
-        for (int v = 0; v < NV; ++v) {
-          const int first = (v * G + lane) * 8;
-          float dx[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) dx[i] = inverse[r] * (fmaf(dy[r][v][i], scale[v][i], -s1) - u[r][v][i] * s2);
-          store8(static_cast<T*>(a.dx) + row * a.c + first, a.c - first, a.vector_dx, dx);
-        }
-      }
+      for (int i = 0; i < kShare / 2; ++i) u.v[i] = fma2(u.v[i], t2, fma2(mul2(dy.v[i], scale.v[i]), both(inv), t1));
+      store16(static_cast<T*>(a.dx) + row * a.c + first, left, a.access_dx, u);
     }
   }
   // this block's row of sums
 #pragma unroll
   for (int which = 0; which < 2; ++which) {
     float* out = a.partial + ((int64_t)blockIdx.x * 2 + which) * a.c;
-    if (kGroups == 1) {
-#pragma unroll
-      for (int v = 0; v < NV; ++v) {
-        const int first = (v * G + lane) * 8;
-        store8(out + first, a.c - first, false, which ? db[v] : dg[v]);
-      }
-    } else {
+    if (kGroups == 1) store16(out + first, left, kElements, which ? db : dg);
+    else {
       __syncthreads();
 #pragma unroll
-      for (int v = 0; v < NV; ++v)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) sums[group * (G * NV * 8) + (v * G + lane) * 8 + i] = which ? db[v][i] : dg[v][i];
+      for (int i = 0; i < kShare / 2; ++i) *reinterpret_cast<float2*>(&sums[threadIdx.x * kShare + 2 * i]) = which ? db.v[i] : dg.v[i];
       __syncthreads();
       for (int col = threadIdx.x; col < a.c; col += kThreads) {
         float t = 0.f;
-#pragma unroll 8
-        for (int g = 0; g < kGroups; ++g) t += sums[g * (G * NV * 8) + col];
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g) t += sums[g * (G * kShare) + col];
         out[col] = t;
       }
     }
   }
 }
 
-// Column sums of the blocks' rows, in the same order every time: 32 columns a block, 16 strands of rows, then the strands.
-__global__ void __launch_bounds__(512)
+// Column sums of the blocks' rows, in the same order every time: 32 columns a block, 32 strands of rows with eight loads in flight each, then
+// the strands.
+__global__ void __launch_bounds__(1024)
 join_kernel(const float* partial, int count, int c, float* dg, float* db) {
-  __shared__ float s[16][33];
+  __shared__ float s[32][33];
   const int lane = threadIdx.x & 31, strand = threadIdx.x >> 5, col = blockIdx.x * 32 + lane;
   lf_chain();
   float t = 0.f;
-  if (col < c)
-    for (int i = strand; i < count; i += 16) t += partial[((int64_t)i * 2 + blockIdx.y) * c + col];
+  if (col < c) {
+    const float* from = partial + (int64_t)blockIdx.y * c + col;
+    for (int i = strand; i < count; i += 256) {
+      float v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = i + 32 * k < count ? from[(int64_t)(i + 32 * k) * 2 * c] : 0.f;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) t += v[k];
+    }
+  }
   s[strand][lane] = t;
   __syncthreads();
-  if (strand == 0 && col < c) {
-    t = 0.f;
+  t = s[lane][strand];      // (a column's strands are a warp's lanes)
 #pragma unroll
-    for (int i = 0; i < 16; ++i) t += s[i][lane];
-    (blockIdx.y ? db : dg)[col] = t;
-  }
+  for (int o = 16; o; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+  if (lane == 0 && blockIdx.x * 32 + strand < c) (blockIdx.y ? db : dg)[blockIdx.x * 32 + strand] = t;
 }
 
 // Blocks that stay on the GPU, and no more than there are rows for.
@@ -251,44 +234,41 @@ static int grid_of(const lf_context* ctx, int64_t rows, int per_block, int per_s
   return (int)(need < most ? need : most);
 }
 
-// Lanes of a row, steps of eight channels a lane, rows in flight: by the width alone.
-//   f(G, NV, R) with the constants as types
+constexpr int kMostChannels = 8192;
+
+// f(lanes of a row as a type), by the width alone
 template <typename F>
 static auto by_width(int c, F f) {
-#define LF_NORM_FORM(G, NV, R) f(std::integral_constant<int, G>{}, std::integral_constant<int, NV>{}, std::integral_constant<int, R>{})
-  if (c <= 64) return LF_NORM_FORM(8, 1, 2);
-  if (c <= 128) return LF_NORM_FORM(16, 1, 2);
-  if (c <= 256) return LF_NORM_FORM(32, 1, 2);
-  if (c <= 512) return LF_NORM_FORM(32, 2, 1);
-  if (c <= 1024) return LF_NORM_FORM(32, 4, 1);
-  if (c <= 2048) return LF_NORM_FORM(kThreads, 1, 1);
-  if (c <= 4096) return LF_NORM_FORM(kThreads, 2, 1);
-  return LF_NORM_FORM(kThreads, 4, 1);
-#undef LF_NORM_FORM
-}
-
-constexpr int kMostChannels = 8192, kPerSm = 4;
-
-template <typename T>
-static void launch_forward(lf_context* ctx, const Forward& a) {
-  by_width(a.c, [&](auto g, auto nv, auto r) {
-    constexpr int G = decltype(g)::value, NV = decltype(nv)::value, R = decltype(r)::value;
-    lf_launch(ctx, forward_kernel<T, G, NV, R>, grid_of(ctx, a.rows, kThreads / G * R, kPerSm), kThreads, 0, a);
-  });
+  if (c <= 64) return f(std::integral_constant<int, 4>{});
+  if (c <= 128) return f(std::integral_constant<int, 8>{});
+  if (c <= 256) return f(std::integral_constant<int, 16>{});
+  if (c <= 512) return f(std::integral_constant<int, 32>{});
+  if (c <= 1024) return f(std::integral_constant<int, 64>{});
+  if (c <= 2048) return f(std::integral_constant<int, 128>{});
+  if (c <= 4096) return f(std::integral_constant<int, 256>{});
+  return f(std::integral_constant<int, 512>{});
 }
 
 static int backward_blocks(const lf_context* ctx, int64_t rows, int c) {
-  return by_width(c, [&](auto g, auto, auto r) { return grid_of(ctx, rows, kThreads / decltype(g)::value * decltype(r)::value, kPerSm); });
+  return by_width(c, [&](auto g) { constexpr int G = decltype(g)::value; return grid_of(ctx, rows, threads_of(G) / G, blocks_of(G)); });
+}
+
+template <typename T>
+static void launch_forward(lf_context* ctx, const Forward& a) {
+  by_width(a.c, [&](auto g) {
+    constexpr int G = decltype(g)::value;
+    lf_launch(ctx, forward_kernel<T, G>, grid_of(ctx, a.rows, threads_of(G) / G, blocks_of(G)), threads_of(G), 0, a);
+  });
 }
 
 template <typename T>
 static void launch_backward(lf_context* ctx, const Backward& a, int blocks) {
-  by_width(a.c, [&](auto g, auto nv, auto r) {
-    lf_launch(ctx, backward_kernel<T, decltype(g)::value, decltype(nv)::value, decltype(r)::value>, blocks, kThreads, 0, a);
+  by_width(a.c, [&](auto g) {
+    constexpr int G = decltype(g)::value;
+    if (a.x) lf_launch(ctx, backward_kernel<T, G, false>, blocks, threads_of(G), 0, a);
+    else lf_launch(ctx, backward_kernel<T, G, true>, blocks, threads_of(G), 0, a);
   });
 }
-
-static bool vector_rows(const void* p, int c, int dtype) { return lf_aligned16(p) && c % (dtype == LF_DTYPE_BF16 ? 8 : 4) == 0; }
 
 }  // namespace lnorm
 
@@ -310,8 +290,8 @@ lf_status lf_layer_norm_run(lf_context* ctx, const lf_layer_norm_desc* d, lf_res
   LF_CUDA(ctx, cudaSetDevice(ctx->device));
   Forward a{};
   a.rows = d->rows; a.c = d->channels; a.epsilon = d->epsilon;
-  a.vector_in = vector_rows(d->activations, a.c, d->act_dtype);
-  a.vector_out = vector_rows(d->out, a.c, d->act_dtype);
+  a.access_in = row_access(d->activations, a.c, d->act_dtype);
+  a.access_out = row_access(d->out, a.c, d->act_dtype);
   a.x = d->activations; a.scale = d->scale; a.offset = d->offset; a.y = d->out; a.mean = d->mean; a.inverse = d->inverse_deviation;
   if (d->checkpoint.codes) a.kept = matrix(d->checkpoint);
   if (d->encoded.codes) a.encoded = matrix(d->encoded);
@@ -342,9 +322,9 @@ lf_status lf_layer_norm_backward_run(lf_context* ctx, const lf_layer_norm_backwa
   LF_CUDA(ctx, cudaSetDevice(ctx->device));
   Backward a{};
   a.rows = d->rows; a.c = d->channels;
-  a.vector_dy = vector_rows(d->gradient, a.c, d->act_dtype);
-  a.vector_x = vector_rows(d->activations, a.c, d->act_dtype);
-  a.vector_dx = vector_rows(d->out, a.c, d->act_dtype);
+  a.access_dy = row_access(d->gradient, a.c, d->act_dtype);
+  a.access_x = row_access(d->activations, a.c, d->act_dtype);
+  a.access_dx = row_access(d->out, a.c, d->act_dtype);
   a.dy = d->gradient; a.x = d->activations; a.mean = d->mean; a.inverse = d->inverse_deviation; a.scale = d->scale; a.dx = d->out;
   if (d->checkpoint.codes) a.kept = matrix(d->checkpoint);
   a.partial = (float*)d->workspace;
@@ -353,7 +333,7 @@ lf_status lf_layer_norm_backward_run(lf_context* ctx, const lf_layer_norm_backwa
   if (d->act_dtype == LF_DTYPE_BF16) launch_backward<bf16>(ctx, a, blocks); else launch_backward<float>(ctx, a, blocks);
   lf_prof_end(ctx);
   lf_prof_begin(ctx, LF_KERNEL_ELEMENTWISE);
-  lf_launch(ctx, join_kernel, dim3(lf_ceil_div(a.c, 32), 2), 512, 0, a.partial, blocks, a.c, d->scale_gradient, d->offset_gradient);
+  lf_launch(ctx, join_kernel, dim3(lf_ceil_div(a.c, 32), 2), 1024, 0, a.partial, blocks, a.c, d->scale_gradient, d->offset_gradient);
   lf_prof_end(ctx);
   ctx->launches += 2;
   return lf_float8_done(ctx, r, 2);

@@ -23,7 +23,7 @@ import numpy as np
 
 from . import _native as nat
 from ._native import RangeError
-from .operators import Device, EncodedTensor, _device, _positive, _result, _torch_stream, _variance
+from .operators import Device, EncodedTensor, _device, _positive, _torch_stream, _variance
 
 _FORMAT = {"e4m3": nat.FLOAT8_E4M3, "e5m2": nat.FLOAT8_E5M2}
 _DTYPE = {"f32": nat.DTYPE_F32, "bf16": nat.DTYPE_BF16}
@@ -37,22 +37,32 @@ def _format(value, name="format"):
 
 
 def _shape(inp, *names):
-    values = tuple(inp[name] for name in names)
+    values = [inp[name] for name in names]
     for name, value in zip(names, values):
-        _positive(name, value)
-    return tuple(int(value) for value in values)
+        if type(value) is not int or value <= 0:
+            _positive(name, value)
+    return [int(value) for value in values]
+
+
+_names = {}      # torch dtype -> "f32" | "bf16"
+
+
+def _torch():
+    import torch
+    if not _names:
+        _names.update({torch.float32: "f32", torch.bfloat16: "bf16"})
+    return torch
 
 
 def _tensor(device, name, value, count, only=None):
     """A tensor argument: on the device's GPU, contiguous, float32 or bfloat16 (``only``: one of them), of ``count`` values.
-    Returns the library's dtype."""
+    Returns "f32" or "bf16"."""
     if not getattr(value, "is_cuda", False):
         raise ValueError(f"{name} must be a CUDA tensor")
-    if value.device.index != device.ordinal:
+    if value.get_device() != device.ordinal:
         raise ValueError(f"{name} is on {value.device}, the device's GPU is cuda:{device.ordinal}")
-    dtype = str(value.dtype)
-    dtype = "f32" if dtype == "torch.float32" else "bf16" if dtype == "torch.bfloat16" else dtype
-    if dtype not in _DTYPE or only not in (None, dtype):
+    dtype = _names.get(value.dtype) or _names.get(value.dtype if _torch() else None)
+    if dtype is None or (only is not None and dtype != only):
         raise ValueError(f"{name} must be {only or 'f32 or bf16'}; received {value.dtype}")
     if not value.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
@@ -62,22 +72,33 @@ def _tensor(device, name, value, count, only=None):
 
 
 def _torch_dtype(name):
-    import torch
+    torch = _torch()
     return torch.float32 if name == "f32" else torch.bfloat16
 
 
-def _call(device, function, desc, tensors):
-    """The call; its tensors' memory stays theirs until the device's stream is done, whatever stream torch allocates for."""
-    res = device.call(function, desc, True)
-    if _torch_stream(device.ordinal) != device.stream:
-        import torch
+def _call(device, function, desc, tensors, output=None):
+    """One library call and its result object.  Where torch's current stream is not the device's: the tensors' memory stays theirs until
+    the device's stream is done with it, and a device with a stream of its own waits for torch's work first."""
+    current = _torch_stream(device.ordinal)
+    if current != device.stream and device._own_stream:
+        device.check(device.lib.lf_context_await(device.handle, current))
+    res = nat.Result()
+    status = function(device.handle, desc, res)
+    if status != nat.LF_OK:
+        device.check(status)
+    if current != device.stream:
+        torch = _torch()
         stream = torch.cuda.ExternalStream(device.stream, device=f"cuda:{device.ordinal}")
         for t in tensors:
-            if isinstance(t, Float8Tensor):
-                t = t.memory
+            t = t.memory if isinstance(t, Float8Tensor) else t
             if t is not None:
                 t.record_stream(stream)
-    return res
+    return {"output": output, "elapsedMilliseconds": 0.0, "memory": {"peakBytes": res.peak_bytes}, "launches": res.launches}
+
+
+def _sizes(rows, channels):
+    """Bytes of the codes and of the exponents (``lf_float8_code_bytes``, ``lf_float8_exponent_bytes``)."""
+    return rows * ((channels + 15) // 16 * 16), (channels + 511) // 512 * ((rows + 127) // 128) * 512
 
 
 class Float8Tensor:
@@ -89,19 +110,15 @@ class Float8Tensor:
     def __init__(self, rows: int, channels: int, format: str, memory):
         """``memory``: contiguous uint8 CUDA tensor with the codes, then the exponents, 16-byte aligned (``lf_float8_matrix``)."""
         self.rows, self.channels, self.format, self.memory = rows, channels, format, memory
-        lib = nat.load()
-        self._codes = int(lib.lf_float8_code_bytes(rows, channels))
-        if memory.numel() != self._codes + int(lib.lf_float8_exponent_bytes(rows, channels)):
-            raise RangeError(f"memory has {memory.numel()} values; expected {self._codes + int(lib.lf_float8_exponent_bytes(rows, channels))}")
+        self._codes, exponents = _sizes(rows, channels)
+        if memory.numel() != self._codes + exponents:
+            raise RangeError(f"memory has {memory.numel()} values; expected {self._codes + exponents}")
         base = memory.data_ptr()
         self.desc = nat.Float8Matrix(rows, channels, _FORMAT[format], base, base + self._codes)
 
     @classmethod
     def empty(cls, rows, channels, format, like):
-        lib = nat.load()
-        nbytes = int(lib.lf_float8_code_bytes(rows, channels)) + int(lib.lf_float8_exponent_bytes(rows, channels))
-        import torch
-        return cls(rows, channels, format, torch.empty(nbytes, dtype=torch.uint8, device=like.device))
+        return cls(rows, channels, format, like.new_empty(sum(_sizes(rows, channels)), dtype=_torch().uint8))
 
     @property
     def nbytes(self):
@@ -121,7 +138,7 @@ class Float8Tensor:
 def _matrix(device, name, value, rows, channels):
     if not isinstance(value, Float8Tensor):
         raise ValueError(f"{name} must be a Float8Tensor")
-    if value.memory.device.index != device.ordinal:
+    if value.memory.get_device() != device.ordinal:
         raise ValueError(f"{name} is on {value.memory.device}, the device's GPU is cuda:{device.ordinal}")
     if (value.rows, value.channels) != (rows, channels):
         raise RangeError(f"{name} is {value.rows} x {value.channels}; expected {rows} x {channels}")
@@ -130,7 +147,7 @@ def _matrix(device, name, value, rows, channels):
 
 def _encode(device, source, dtype, out, block_rows=1, transposed=None):
     desc = nat.Float8EncodeDesc(out.desc, transposed.desc if transposed is not None else _NO_MATRIX, _DTYPE[dtype], block_rows, source.data_ptr())
-    return _call(device, device.lib.lf_float8_encode, desc, (source, out, transposed))
+    _call(device, device.lib.lf_float8_encode, desc, (source, out, transposed))
 
 
 def float8_encode(device, activations, rows, channels, options=None):
@@ -206,10 +223,9 @@ class LayerNormGpu:
         desc = nat.LayerNormDesc(rows, c, variance, _DTYPE[dtype], epsilon, x.data_ptr(), scale.data_ptr(), offset.data_ptr(),
                                  out.data_ptr() if out is not None else None, mean, mean and mean + 4 * rows,
                                  checkpoint.desc if kept else _NO_MATRIX, encoded.desc if encode else _NO_MATRIX)
-        res = _call(dev, dev.lib.lf_layer_norm_run, desc, (x, scale, offset, out, statistics, checkpoint, encoded))
-        result = _result(dev, res, encoded if encode else out)
+        result = _call(dev, dev.lib.lf_layer_norm_run, desc, (x, scale, offset, out, statistics, checkpoint, encoded), encoded if encode else out)
         if statistics is not None:
-            result["mean"], result["inverseDeviation"] = statistics[0], statistics[1]
+            result["mean"], result["inverseDeviation"] = statistics.unbind(0)
         if kept:
             result["checkpoint"] = checkpoint
         return result
@@ -235,7 +251,7 @@ class LayerNormGpu:
             _tensor(dev, "out", out, rows * c, dtype)
         else:
             out = dy.new_empty(dy.shape)
-        nbytes = int(dev.lib.lf_layer_norm_backward_workspace(dev.handle, rows, c))
+        nbytes = dev.lib.lf_layer_norm_backward_workspace(dev.handle, rows, c)
         # the two weights' gradients, then the workspace on a 16-byte boundary
         ahead = (2 * c + 3) // 4 * 4
         memory = scale.new_empty(ahead + nbytes // 4)
@@ -243,8 +259,7 @@ class LayerNormGpu:
         desc = nat.LayerNormBackwardDesc(rows, c, _DTYPE[dtype], dy.data_ptr(), None if encoded else x.data_ptr(),
                                          x.desc if encoded else _NO_MATRIX, input["mean"].data_ptr(), input["inverseDeviation"].data_ptr(),
                                          scale.data_ptr(), out.data_ptr(), base, base + 4 * c, base + 4 * ahead, nbytes)
-        res = _call(dev, dev.lib.lf_layer_norm_backward_run, desc, (dy, x, input["mean"], input["inverseDeviation"], scale, out, memory))
-        result = _result(dev, res, out)
+        result = _call(dev, dev.lib.lf_layer_norm_backward_run, desc, (dy, x, input["mean"], input["inverseDeviation"], scale, out, memory), out)
         result["activations"] = result.pop("output")
         result["scale"], result["offset"] = memory[:c], memory[c:2 * c]
         return result
@@ -306,24 +321,20 @@ class Float8LinearGpu:
     def _product(self, name, value, rows, channels, weights, bias, options, out):
         dev, opts = self.device, options or {}
         format = _format(opts.get("format", "e4m3"))
-        res = None
+        source = None
         if isinstance(value, Float8Tensor):
             operand, dtype = _matrix(dev, name, value, rows, channels), _output(opts, "bf16")
         else:
             source = _tensor(dev, name, value, rows * channels)
             dtype = _output(opts, source)
+            operand = Float8Tensor.empty(rows, channels, format, value)
         if out is not None:
             _tensor(dev, "out", out, rows * weights.rows, dtype)
-        if not isinstance(value, Float8Tensor):
-            operand = Float8Tensor.empty(rows, channels, format, value)
-            res = _encode(dev, value, source, operand)
-        if out is None:
-            out = operand.memory.new_empty((rows, weights.rows), dtype=_torch_dtype(dtype))
-        desc = nat.Float8LinearDesc(operand.desc, weights.desc, bias.data_ptr() if bias is not None else None, _DTYPE[dtype], 0, out.data_ptr())
-        done = _call(dev, dev.lib.lf_float8_linear_run, desc, (operand, weights, bias, out))
-        result = _result(dev, done, out)
-        if res is not None:
-            result["launches"] += int(res.launches)
+        else:
+            out = weights.memory.new_empty((rows, weights.rows), dtype=_torch_dtype(dtype))
+        desc = nat.Float8LinearDesc(operand.desc, weights.desc, bias.data_ptr() if bias is not None else None, _DTYPE[dtype],
+                                    _DTYPE[source or "f32"], value.data_ptr() if source else None, out.data_ptr())
+        result = _call(dev, dev.lib.lf_float8_linear_run, desc, (value, operand, weights, bias, out), out)
         if opts.get("checkpoint"):
             result["checkpoint"] = operand
         return result
@@ -362,15 +373,15 @@ class Float8LinearGpu:
             _matrix(dev, "gradient", dy, rows, n)
         else:
             _tensor(dev, "gradient", dy, rows * n, "bf16")
-        nbytes = int(dev.lib.lf_float8_weight_gradient_workspace(dev.handle, rows, channels, n))
-        import torch
-        weight = torch.empty((n, channels), dtype=torch.float32, device=x.memory.device)
-        bias = torch.empty(n, dtype=torch.float32, device=x.memory.device)
-        workspace = torch.empty(nbytes, dtype=torch.uint8, device=x.memory.device) if nbytes else None
-        desc = nat.Float8WeightGradientDesc(x.desc, None if encoded else dy.data_ptr(), dy.desc if encoded else _NO_MATRIX, n, 0, weight.data_ptr(),
-                                            bias.data_ptr(), workspace.data_ptr() if nbytes else None, nbytes)
-        res = _call(dev, dev.lib.lf_float8_weight_gradient_run, desc, (dy, x, weight, bias, workspace))
-        result = _result(dev, res, weight)
+        nbytes = dev.lib.lf_float8_weight_gradient_workspace(dev.handle, rows, channels, n)
+        weight = x.memory.new_empty((n, channels), dtype=_torch().float32)
+        # the bias' gradient, then the workspace on a 16-byte boundary
+        ahead = (n + 3) // 4 * 4
+        memory = weight.new_empty(ahead + nbytes // 4)
+        base = memory.data_ptr()
+        desc = nat.Float8WeightGradientDesc(x.desc, None if encoded else dy.data_ptr(), dy.desc if encoded else _NO_MATRIX, n, 0, weight.data_ptr(), base,
+                                            base + 4 * ahead, nbytes)
+        result = _call(dev, dev.lib.lf_float8_weight_gradient_run, desc, (dy, x, weight, memory), weight)
         result["weight"] = result.pop("output")
-        result["bias"] = bias
+        result["bias"] = memory[:n]
         return result
