@@ -15,6 +15,8 @@ __global__ void __launch_bounds__(kThreads)
 encode_kernel(const T* x, const Matrix m, uint32_t units, uint32_t per_row, int access) {
   const int lane = threadIdx.x % LANES;
   const uint32_t base = blockIdx.x * (uint32_t)(kThreads / LANES * kUnits) + threadIdx.x / LANES;
+  __shared__ __align__(16) float rooms[kThreads / 32][kRoom];
+  float* room = rooms[threadIdx.x >> 5];
   lf_chain();
   Raw<T> raw[kUnits];
   uint32_t row[kUnits], first[kUnits];
@@ -23,14 +25,13 @@ encode_kernel(const T* x, const Matrix m, uint32_t units, uint32_t per_row, int 
     const uint32_t unit = base + u * (kThreads / LANES);
     row[u] = per_row == 1 ? unit : unit / per_row;
     first[u] = (unit - row[u] * per_row) * kBlock + lane * kShare;
-    if (unit >= units) first[u] = (uint32_t)m.channels;      // nothing to read or write
-    load16(raw[u], x + (int64_t)row[u] * m.channels + first[u], m.channels - (int)first[u], access);
+    load16<T, LANES>(raw[u], x + (int64_t)row[u] * m.channels + first[u], m.channels - (int)first[u], unit < units, access);
   }
 #pragma unroll
   for (int u = 0; u < kUnits; ++u) {
     uint4 codes;
-    const int s = encode16<LANES>(unpack(raw[u]), m.format, codes);
-    put16(m, row[u], first[u], codes, s);
+    const int s = encode16<LANES>(unpack<T, LANES>(raw[u], access, room), m.format, codes);
+    if (base + u * (kThreads / LANES) < units) put16(m, row[u], first[u], codes, s);
   }
 }
 
@@ -39,6 +40,8 @@ __global__ void __launch_bounds__(kThreads)
 decode_kernel(const Matrix m, T* out, uint32_t units, uint32_t per_row, int access) {
   const int lane = threadIdx.x % LANES;
   const uint32_t base = blockIdx.x * (uint32_t)(kThreads / LANES * kUnits) + threadIdx.x / LANES;
+  __shared__ __align__(16) float rooms[kThreads / 32][kRoom];
+  float* room = rooms[threadIdx.x >> 5];
   lf_chain();
   uint4 codes[kUnits];
   int s[kUnits];
@@ -49,22 +52,20 @@ decode_kernel(const Matrix m, T* out, uint32_t units, uint32_t per_row, int acce
     row[u] = per_row == 1 ? unit : unit / per_row;
     const uint32_t block = unit - row[u] * per_row;
     first[u] = block * kBlock + lane * kShare;
-    if (unit >= units) first[u] = (uint32_t)m.channels;      // nothing to read or write
     codes[u] = make_uint4(0, 0, 0, 0);
     s[u] = 1;
-    if (first[u] < (uint32_t)m.channels) {
+    if (unit < units && first[u] < (uint32_t)m.channels) {
       codes[u] = *reinterpret_cast<const uint4*>(m.codes + row[u] * m.pitch + first[u]);
       s[u] = m.exponents[exponent_at(row[u], block, m.tiles)];
     }
   }
 #pragma unroll
   for (int u = 0; u < kUnits; ++u) {
-    if (first[u] >= (uint32_t)m.channels) continue;
     Share v = decode16(codes[u], m.format);
     const float2 factor = both(up(s[u]));
 #pragma unroll
     for (int i = 0; i < kShare / 2; ++i) v.v[i] = mul2(v.v[i], factor);
-    store16(out + (int64_t)row[u] * m.channels + first[u], m.channels - (int)first[u], access, v);
+    store16<T, LANES>(out + (int64_t)row[u] * m.channels + first[u], m.channels - (int)first[u], base + u * (kThreads / LANES) < units, access, v, room);
   }
 }
 
@@ -76,6 +77,8 @@ encode_square_kernel(const T* x, const Matrix m, const Matrix t, int access) {
   __shared__ float most_s[2][kThreads / 32];
   __shared__ __align__(16) uint8_t turned[kBlock][kBlock + 16];
   constexpr int kRows = kBlock * 8 / kThreads;      // of a thread
+  __shared__ __align__(16) float rooms[kThreads / 32][kRoom];
+  float* room = rooms[threadIdx.x >> 5];
   const int lane = threadIdx.x & 7, strand = threadIdx.x >> 3;
   const int64_t row0 = (int64_t)blockIdx.y * kBlock;
   const int first = blockIdx.x * kBlock + lane * kShare;
@@ -84,12 +87,13 @@ encode_square_kernel(const T* x, const Matrix m, const Matrix t, int access) {
 #pragma unroll
   for (int k = 0; k < kRows; ++k) {
     const int64_t row = row0 + strand + kThreads / 8 * k;
-    load16(raw[k], x + row * m.channels + first, row < m.rows ? m.channels - first : 0, access);
+    load16<T, 8>(raw[k], x + row * m.channels + first, m.channels - first, row < m.rows, access);
   }
   float most = 0.f, finite = 0.f;
+  Share all[kRows];
 #pragma unroll
   for (int k = 0; k < kRows; ++k) {
-    const Share v = unpack(raw[k]);
+    const Share v = all[k] = unpack<T, 8>(raw[k], access, room);
 #pragma unroll
     for (int i = 0; i < kShare; ++i) {
       const float a = fabsf(i & 1 ? v.v[i / 2].y : v.v[i / 2].x);
@@ -108,7 +112,7 @@ encode_square_kernel(const T* x, const Matrix m, const Matrix t, int access) {
 #pragma unroll
   for (int k = 0; k < kRows; ++k) {
     const int64_t row = row0 + strand + kThreads / 8 * k;
-    const Share v = unpack(raw[k]);
+    const Share& v = all[k];
     uint32_t w[4] = {0, 0, 0, 0};
     if (most < kInfinity) {
 #pragma unroll

@@ -92,46 +92,99 @@ static inline int row_access(const void* p, int c, int dtype) {
   return ((uintptr_t)p & 31) == 0 && bytes % 32 == 0 ? kThirtyTwo : ((uintptr_t)p & 15) == 0 && bytes % 16 == 0 ? kSixteen : kElements;
 }
 
-// `count` channels of the row are left from p on; what lies behind them reads as zero.
-template <typename T>
-__device__ __forceinline__ void load16(Raw<T>& r, const T* p, int count, int access) {
+// Rows that no 16-byte access divides go through shared memory: neighbouring lanes load neighbouring elements, and each takes its sixteen from there when
+// it needs them (lane by lane, sixteen elements each, a warp's load touches sixteen lines instead of one).  A warp's room, in float32; every
+// 32 elements are followed by four of padding, so that eight lanes' 16-byte pieces lie in different banks.
+constexpr int kRoom = 32 * kShare / 32 * 36;
+__device__ __forceinline__ int room_at(int e) { return e + (e >> 5) * 4; }
+
+// The lane's part of a row (p: its first channel, `left` channels from there to the row's end; channels behind it read as zero, as
+// does a row that is not `live`).  LANES neighbouring lanes have neighbouring parts.  All lanes of a warp call these three.
+template <typename T, int LANES>
+__device__ __forceinline__ void load16(Raw<T>& r, const T* p, int left, bool live, int access) {
   constexpr int kWords = kShare * sizeof(T) / 4;
-  if (count >= kShare && access == kThirtyTwo) {
+  const int count = live ? left : 0;
+  if (access == kElements) {      // element j * LANES + lane of the group's
+    const int lane = threadIdx.x % LANES, all = live ? left + lane * kShare : 0;
+    const T* from = p - lane * kShare;
+    if (sizeof(T) == 4) {
+#pragma unroll
+      for (int j = 0; j < kShare; ++j) r.w[j % kWords] = j * LANES + lane < all ? reinterpret_cast<const uint32_t*>(from)[j * LANES + lane] : 0u;
+    } else {
+#pragma unroll
+      for (int j = 0; j < kShare; j += 2)
+        r.w[j / 2] = (j * LANES + lane < all ? (uint32_t)reinterpret_cast<const uint16_t*>(from)[j * LANES + lane] : 0u) |
+                     ((j + 1) * LANES + lane < all ? (uint32_t)reinterpret_cast<const uint16_t*>(from)[(j + 1) * LANES + lane] << 16 : 0u);
+    }
+  } else if (count >= kShare && access == kThirtyTwo) {
 #pragma unroll
     for (int i = 0; i < kWords; i += 8)
       asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
                    : "=r"(r.w[i]), "=r"(r.w[i + 1]), "=r"(r.w[i + 2]), "=r"(r.w[i + 3]), "=r"(r.w[i + 4]), "=r"(r.w[i + 5]), "=r"(r.w[i + 6]), "=r"(r.w[i + 7])
                    : "l"(reinterpret_cast<const uint32_t*>(p) + i)
                    : "memory");
-  } else if (count >= kShare && access == kSixteen) {
+  } else {      // rows are whole 16-byte pieces
+    constexpr int kPiece = 16 / sizeof(T);
 #pragma unroll
     for (int i = 0; i < kWords; i += 4) {
-      const uint4 u = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint32_t*>(p) + i);
+      uint4 u = make_uint4(0, 0, 0, 0);
+      if (i / 4 * kPiece < count) u = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint32_t*>(p) + i);
       r.w[i] = u.x; r.w[i + 1] = u.y; r.w[i + 2] = u.z; r.w[i + 3] = u.w;
     }
-  } else if (sizeof(T) == 4) {
-#pragma unroll
-    for (int i = 0; i < kShare; ++i) r.w[i] = i < count ? reinterpret_cast<const uint32_t*>(p)[i] : 0u;
-  } else {
-#pragma unroll
-    for (int i = 0; i < kShare; i += 2)
-      r.w[i / 2] = (i < count ? (uint32_t)reinterpret_cast<const uint16_t*>(p)[i] : 0u) |
-                   (i + 1 < count ? (uint32_t)reinterpret_cast<const uint16_t*>(p)[i + 1] << 16 : 0u);
   }
 }
 template <typename T>
-__device__ __forceinline__ Share unpack(const Raw<T>& r) {
+__device__ __forceinline__ Share unpack_in_order(const Raw<T>& r) {
+  constexpr int kWords = kShare * sizeof(T) / 4;
   Share s;
 #pragma unroll
   for (int i = 0; i < kShare / 2; ++i) {
-    if (sizeof(T) == 4) s.v[i] = make_float2(__uint_as_float(r.w[(2 * i) % (kShare * sizeof(T) / 4)]), __uint_as_float(r.w[(2 * i + 1) % (kShare * sizeof(T) / 4)]));
+    if (sizeof(T) == 4) s.v[i] = make_float2(__uint_as_float(r.w[(2 * i) % kWords]), __uint_as_float(r.w[(2 * i + 1) % kWords]));
     else s.v[i] = make_float2(__uint_as_float(r.w[i] << 16), __uint_as_float(r.w[i] & 0xffff0000u));
   }
   return s;
 }
-template <typename T>
-__device__ __forceinline__ void store16(T* p, int count, int access, const Share& s) {
+template <typename T, int LANES>
+__device__ __forceinline__ Share unpack(const Raw<T>& r, int access, float* room) {
+  const Share s = unpack_in_order(r);
+  if (access != kElements) return s;
+  // (LANES <= 32 divides 32, and so do the groups' parts of the room)
+  const int lane = threadIdx.x % LANES, base = (threadIdx.x & 31) / LANES * LANES * kShare;
+  __syncwarp();
+#pragma unroll
+  for (int j = 0; j < kShare; ++j) room[room_at(base + j * LANES + lane)] = j & 1 ? s.v[j / 2].y : s.v[j / 2].x;
+  __syncwarp();
+  Share t;
+#pragma unroll
+  for (int i = 0; i < kShare; i += 4) {
+    const float4 f = *reinterpret_cast<const float4*>(&room[room_at(base + lane * kShare + i)]);
+    t.v[i / 2] = make_float2(f.x, f.y);
+    t.v[i / 2 + 1] = make_float2(f.z, f.w);
+  }
+  return t;
+}
+template <typename T, int LANES>
+__device__ __forceinline__ void store16(T* p, int left, bool live, int access, const Share& s, float* room) {
   constexpr int kWords = kShare * sizeof(T) / 4;
+  const int count = live ? left : 0;
+  if (access == kElements) {
+    const int lane = threadIdx.x % LANES, base = (threadIdx.x & 31) / LANES * LANES * kShare, all = live ? left + lane * kShare : 0;
+    T* to = p - lane * kShare;
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < kShare; i += 4)
+      *reinterpret_cast<float4*>(&room[room_at(base + lane * kShare + i)]) = make_float4(s.v[i / 2].x, s.v[i / 2].y, s.v[i / 2 + 1].x, s.v[i / 2 + 1].y);
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < kShare; ++j) {
+      const float v = room[room_at(base + j * LANES + lane)];
+      if (j * LANES + lane < all) {
+        if (sizeof(T) == 4) reinterpret_cast<float*>(to)[j * LANES + lane] = v;
+        else reinterpret_cast<bf16*>(to)[j * LANES + lane] = __float2bfloat16_rn(v);
+      }
+    }
+    return;
+  }
   uint32_t w[kWords];
 #pragma unroll
   for (int i = 0; i < kShare / 2; ++i) {
@@ -147,21 +200,12 @@ __device__ __forceinline__ void store16(T* p, int count, int access, const Share
       asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(reinterpret_cast<uint32_t*>(p) + i), "r"(w[i]), "r"(w[i + 1]), "r"(w[i + 2]),
                    "r"(w[i + 3]), "r"(w[i + 4]), "r"(w[i + 5]), "r"(w[i + 6]), "r"(w[i + 7])
                    : "memory");
-  } else if (count >= kShare && access == kSixteen) {
-#pragma unroll
-    for (int i = 0; i < kWords; i += 4) *reinterpret_cast<uint4*>(reinterpret_cast<uint32_t*>(p) + i) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
   } else {
+    constexpr int kPiece = 16 / sizeof(T);
 #pragma unroll
-    for (int i = 0; i < kShare; ++i) {
-      if (sizeof(T) == 4) { if (i < count) reinterpret_cast<uint32_t*>(p)[i] = w[i % kWords]; }
-      else if (i < count) reinterpret_cast<uint16_t*>(p)[i] = (uint16_t)(w[i / 2] >> (16 * (i & 1)));
-    }
+    for (int i = 0; i < kWords; i += 4)
+      if (i / 4 * kPiece < count) *reinterpret_cast<uint4*>(reinterpret_cast<uint32_t*>(p) + i) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
   }
-}
-__device__ __forceinline__ Share load_weights(const float* p, int count) {
-  Raw<float> r;
-  load16(r, p, count, kElements);
-  return unpack(r);
 }
 
 // A lane's sixteen codes -> values times `factor`

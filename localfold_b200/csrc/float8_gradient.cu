@@ -20,14 +20,20 @@ namespace tc {
 
 using namespace tc05;
 
+lf_status make_map_bytes(lf_context* ctx, CUtensorMap* map, const void* base, uint64_t width, uint64_t rows, uint64_t pitch, uint32_t box_rows);
 lf_status make_map_rows(lf_context* ctx, CUtensorMap* map, const void* base, bool f32, uint64_t width, uint64_t rows, uint32_t box_rows);
 lf_status make_map_f32_any(lf_context* ctx, CUtensorMap* map, const void* base, const uint64_t (&dims)[3], const uint64_t (&strides)[2], const uint32_t (&box)[3]);
 
 constexpr int WG_BN = 128, WG_BK = 256, WG_ROWS = 64;      // outputs, channels, rows of a step
-constexpr int WG_A_BYTES = WG_BN * WG_ROWS * 2, WG_B_BYTES = WG_BK * WG_ROWS * 2, WG_STAGE = WG_A_BYTES + WG_B_BYTES, WG_STAGES = 3;
+constexpr int WG_A_BYTES = WG_BN * WG_ROWS * 2, WG_B_BYTES = WG_BK * WG_ROWS * 2;
+constexpr int WG_CODES = WG_BK * WG_ROWS, WG_DY_CODES = WG_BN * WG_ROWS;
+constexpr int WG_RING = 4, WG_OPERANDS = 2;                // steps on their way from memory, converted ones
 constexpr int WG_CONVERT = 16;                             // warps that convert, and store the tile
 constexpr int WG_THREADS = 64 + 32 * WG_CONVERT;
-constexpr int WG_SMEM = WG_STAGES * WG_STAGE + WG_CONVERT * 4096 + 512 + 256 + 1024;
+// [ring of dy: four bf16 operands, or two that are converted and four times its codes][ring of x's codes][x's operands][exponents][ones]
+constexpr int WG_DY = WG_RING * WG_A_BYTES, WG_EXPONENTS = 2 * 512;
+constexpr int WG_SMEM = WG_DY + WG_RING * (WG_CODES + WG_EXPONENTS) + WG_OPERANDS * WG_B_BYTES + 512 + 256 + 1024;
+static_assert(WG_OPERANDS * WG_A_BYTES + WG_RING * WG_DY_CODES <= WG_DY && WG_CONVERT * 4096 <= WG_DY, "");
 
 struct GradientParams {
   int m, n, k;
@@ -64,15 +70,22 @@ __device__ __forceinline__ void convert16(uint4 codes, int s, int format, uint4 
 // The place of a piece of eight columns in an MN-major operand: blocks of 64 columns, rows of 128 bytes, 128-byte swizzle.
 __device__ __forceinline__ uint32_t piece_at(int row, int piece) { return (piece >> 3) * (WG_ROWS * 128) + row * 128 + (((piece & 7) ^ (row & 7)) << 4); }
 
+// Warp roles: 0 = loads (dy, x's codes, the exponents that belong to them), 1 = MMA issuer (owns TMEM), 2.. = conversion, then the tile's stores.
 __global__ void __launch_bounds__(WG_THREADS, 1)
-float8_gradient_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant__ CUtensorMap mapO, const GradientParams p) {
+float8_gradient_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant__ CUtensorMap mapX, const __grid_constant__ CUtensorMap mapO,
+                       const GradientParams p) {
   extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = align_shared(smem_raw);
-  uint8_t* out_stage = smem + WG_STAGES * WG_STAGE;
-  uint8_t* ones = out_stage + WG_CONVERT * 4096;
-  uint64_t* full = reinterpret_cast<uint64_t*>(ones + 512);
-  uint64_t* empty = full + WG_STAGES;
-  uint64_t* done = empty + WG_STAGES;
+  uint8_t* dy_s = align_shared(smem_raw);
+  uint8_t* dy_codes = dy_s + WG_OPERANDS * WG_A_BYTES;
+  uint8_t* x_codes = dy_s + WG_DY;
+  uint8_t* x_s = x_codes + WG_RING * WG_CODES;
+  uint8_t* exponents = x_s + WG_OPERANDS * WG_B_BYTES;
+  uint8_t* ones = exponents + WG_RING * WG_EXPONENTS;
+  uint64_t* loaded = reinterpret_cast<uint64_t*>(ones + 512);      // [RING] codes, exponents and a bf16 dy are here
+  uint64_t* taken = loaded + WG_RING;                              // [RING] their codes are read (and a bf16 dy multiplied)
+  uint64_t* full = taken + WG_RING;                                // [OPERANDS]
+  uint64_t* empty = full + WG_OPERANDS;
+  uint64_t* done = empty + WG_OPERANDS;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
@@ -84,7 +97,8 @@ float8_gradient_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_co
   const bool sums = blockIdx.x == 0;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < WG_STAGES; ++s) { mbar_init(&full[s], WG_CONVERT + (p.dy_mode == 0)); mbar_init(&empty[s], 1); }
+    for (int s = 0; s < WG_RING; ++s) { mbar_init(&loaded[s], 1); mbar_init(&taken[s], WG_CONVERT + (p.dy_mode == 0)); }
+    for (int s = 0; s < WG_OPERANDS; ++s) { mbar_init(&full[s], WG_CONVERT); mbar_init(&empty[s], 1); }
     mbar_init(done, 1);
     *abort_flag = 0;
     fence_barrier_init();
@@ -99,37 +113,54 @@ float8_gradient_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_co
   lf_chain();
 
   if (warp == 0) {
-    if (lane == 0 && p.dy_mode == 0) {
-      prefetch_tensormap(&mapA);
+    if (lane == 0) {
+      if (p.dy_mode != 1) prefetch_tensormap(&mapA);
+      prefetch_tensormap(&mapX);
+      const uint32_t x_boxes = columns > 128 ? 2 : 1;
+      const uint32_t bytes = x_boxes * (WG_CODES / 2) + 512 + (p.dy_mode == 0 ? WG_A_BYTES : p.dy_mode == 2 ? WG_DY_CODES + 512 : 0);
+      const uint8_t* ex = p.x.exponents + (int64_t)(k0 >> 9) * p.x.tiles * 512;
+      const uint8_t* ey = p.dy8.exponents + (int64_t)(n0 >> 9) * p.dy8.tiles * 512;
       int stage = 0; uint32_t phase = 0;
       for (int t = first; t < last; ++t) {
-        if (!mbar_wait(&empty[stage], phase ^ 1, abort_flag, p.status, 131)) break;
-        uint8_t* sA = smem + stage * WG_STAGE;
-        mbar_expect_tx(&full[stage], WG_A_BYTES);
-        tma_load_3d(sA, &mapA, &full[stage], n0, t * WG_ROWS, 0);
-        tma_load_3d(sA + WG_A_BYTES / 2, &mapA, &full[stage], n0 + 64, t * WG_ROWS, 0);
-        if (++stage == WG_STAGES) { stage = 0; phase ^= 1; }
+        if (!mbar_wait(&taken[stage], phase ^ 1, abort_flag, p.status, 131)) break;
+        uint64_t* bar = &loaded[stage];
+        mbar_expect_tx(bar, bytes);
+        for (uint32_t i = 0; i < x_boxes; ++i) tma_load_3d(x_codes + stage * WG_CODES + i * (WG_CODES / 2), &mapX, bar, k0 + i * 128, t * WG_ROWS, 0);
+        bulk_load(exponents + stage * WG_EXPONENTS, ex + (int64_t)(t >> 1) * 512, 512, bar);
+        if (p.dy_mode == 0) {
+          tma_load_3d(dy_s + stage * WG_A_BYTES, &mapA, bar, n0, t * WG_ROWS, 0);
+          tma_load_3d(dy_s + stage * WG_A_BYTES + WG_A_BYTES / 2, &mapA, bar, n0 + 64, t * WG_ROWS, 0);
+        } else if (p.dy_mode == 2) {
+          tma_load_3d(dy_codes + stage * WG_DY_CODES, &mapA, bar, n0, t * WG_ROWS, 0);
+          bulk_load(exponents + stage * WG_EXPONENTS + 512, ey + (int64_t)(t >> 1) * 512, 512, bar);
+        }
+        if (++stage == WG_RING) { stage = 0; phase ^= 1; }
       }
     }
   } else if (warp == 1) {
     if (lane == 0) {
-      int stage = 0; uint32_t phase = 0;
+      int slot = 0, stage = 0; uint32_t phase = 0, ring_phase = 0;
       bool ok = true;
       constexpr uint32_t both = (1u << 7) | (1u << 10);      // bf16 operands
       const uint32_t idesc = make_idesc_f16(WG_BN, groups * 64, 1, 1) | both, idesc_ones = make_idesc_f16(WG_BN, 16, 1, 0) | both;
       const uint64_t ones_desc = make_smem_desc_plain(smem_u32(ones), 128, 256);
       for (int t = first; t < last; ++t) {
-        if (!mbar_wait(&full[stage], phase, abort_flag, p.status, 132)) { ok = false; break; }
+        if (!mbar_wait(&full[slot], phase, abort_flag, p.status, 132) || (p.dy_mode == 0 && !mbar_wait(&loaded[stage], ring_phase, abort_flag, p.status, 136))) {
+          ok = false;
+          break;
+        }
         tc_fence_after();
-        const uint32_t a0 = smem_u32(smem + stage * WG_STAGE), b0 = a0 + WG_A_BYTES;
+        const uint32_t a0 = smem_u32(dy_s + (p.dy_mode == 0 ? stage : slot) * WG_A_BYTES), b0 = smem_u32(x_s + slot * WG_B_BYTES);
 #pragma unroll
         for (int kk = 0; kk < WG_ROWS / 16; ++kk) {
           const uint64_t a = make_smem_desc(a0 + kk * 2048, WG_ROWS * 128, 1024);
           umma_f16(tmem_base, a, make_smem_desc(b0 + kk * 2048, WG_ROWS * 128, 1024), idesc, (t != first || kk != 0) ? 1u : 0u);
           if (sums) umma_f16(tmem_base + WG_BK, a, ones_desc, idesc_ones, (t != first || kk != 0) ? 1u : 0u);
         }
-        umma_commit(&empty[stage]);
-        if (++stage == WG_STAGES) { stage = 0; phase ^= 1; }
+        umma_commit(&empty[slot]);
+        if (p.dy_mode == 0) umma_commit(&taken[stage]);
+        if (++slot == WG_OPERANDS) { slot = 0; phase ^= 1; }
+        if (++stage == WG_RING) { stage = 0; ring_phase ^= 1; }
       }
       if (ok) umma_commit(done);
     }
@@ -139,56 +170,48 @@ float8_gradient_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_co
     constexpr int kUnits = WG_ROWS * 16 / (32 * WG_CONVERT);      // of x a thread
     const int xp = thread & 15, xr = thread >> 4;                 // piece, first row (rows xr + 32 u)
     const int yp = thread & 7, yr = thread >> 3;                  // of dy, one unit a thread
-    const int xch = k0 + xp * 16, ych = n0 + yp * 16;
-    const bool x_any = xch < p.x.pitch && xp < groups * 4, y_any = ych < p.n;
-    const int64_t xblock = xch / f8::kBlock, yblock = ych / f8::kBlock;
-    uint4 xc[kUnits], yc[2];
-    int xs[kUnits], ys = 1;
+    const int ych = n0 + yp * 16;
+    const int x_block = (k0 >> 7 & 3) + (xp >> 3), y_block = n0 >> 7 & 3;
+    const bool x_any = xp < groups * 4, x_here = xp * 16 < (columns > 128 ? 256 : 128);
+    uint4 ahead[2];      // dy_mode 1: the next step's unit
     auto fetch = [&](int t) {
+      const int64_t row = (int64_t)t * WG_ROWS + yr;
+      const uint16_t* from = reinterpret_cast<const uint16_t*>(p.dy) + row * p.n + ych;
+      uint32_t o[8];
 #pragma unroll
-      for (int u = 0; u < kUnits; ++u) {
-        const int64_t row = (int64_t)t * WG_ROWS + xr + 32 * u;
-        xc[u] = make_uint4(0, 0, 0, 0);
-        xs[u] = 1;
-        if (x_any && row < p.m) {
-          xc[u] = *reinterpret_cast<const uint4*>(p.x.codes + row * p.x.pitch + xch);
-          xs[u] = p.x.exponents[f8::exponent_at(row, (int)xblock, p.x.tiles)];
-        }
-      }
-      if (p.dy_mode != 0) {
-        const int64_t row = (int64_t)t * WG_ROWS + yr;
-        yc[0] = yc[1] = make_uint4(0, 0, 0, 0);
-        if (y_any && row < p.m) {
-          if (p.dy_mode == 2) {
-            yc[0] = *reinterpret_cast<const uint4*>(p.dy8.codes + row * p.dy8.pitch + ych);
-            ys = p.dy8.exponents[f8::exponent_at(row, (int)yblock, p.dy8.tiles)];
-          } else {
-            const uint16_t* from = reinterpret_cast<const uint16_t*>(p.dy) + row * p.n + ych;
-            uint32_t o[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-              o[i] = (ych + 2 * i < p.n ? (uint32_t)from[2 * i] : 0u) | (ych + 2 * i + 1 < p.n ? (uint32_t)from[2 * i + 1] << 16 : 0u);
-            yc[0] = make_uint4(o[0], o[1], o[2], o[3]);
-            yc[1] = make_uint4(o[4], o[5], o[6], o[7]);
-          }
-        }
-      }
+      for (int i = 0; i < 8; ++i)
+        o[i] = (row < p.m && ych + 2 * i < p.n ? (uint32_t)from[2 * i] : 0u) | (row < p.m && ych + 2 * i + 1 < p.n ? (uint32_t)from[2 * i + 1] << 16 : 0u);
+      ahead[0] = make_uint4(o[0], o[1], o[2], o[3]);
+      ahead[1] = make_uint4(o[4], o[5], o[6], o[7]);
     };
-    int stage = 0; uint32_t phase = 0;
+    int slot = 0, stage = 0; uint32_t phase = 0, ring_phase = 0;
     bool ok = true;
-    fetch(first);
+    if (p.dy_mode == 1) fetch(first);
     for (int t = first; t < last; ++t) {
-      if (!mbar_wait(&empty[stage], phase ^ 1, abort_flag, p.status, 133)) { ok = false; break; }
-      uint8_t* sA = smem + stage * WG_STAGE;
-      uint8_t* sB = sA + WG_A_BYTES;
-      uint4 codes[kUnits], other[2] = {yc[0], yc[1]};
-      int s[kUnits];
-      const int sy = ys;
+      if (!mbar_wait(&loaded[stage], ring_phase, abort_flag, p.status, 135)) { ok = false; break; }
+      uint4 codes[kUnits], dy_unit[2];
+      int s[kUnits], sy = 1;
+      const uint8_t* e = exponents + stage * WG_EXPONENTS + (t & 1) * 8;      // (rows 64 .. 127 of a tile: words 2 and 3)
 #pragma unroll
-      for (int u = 0; u < kUnits; ++u) { codes[u] = xc[u]; s[u] = xs[u]; }
-      if (t + 1 < last) fetch(t + 1);
+      for (int u = 0; u < kUnits; ++u) {      // row xr + 32 u of the step
+        codes[u] = make_uint4(0, 0, 0, 0);
+        if (x_here) codes[u] = *reinterpret_cast<const uint4*>(x_codes + stage * WG_CODES + (xp >> 3) * (WG_CODES / 2) + swizzle128_offset(xr + 32 * u, xp & 7));
+        s[u] = t * WG_ROWS + xr + 32 * u < p.m ? e[xr * 16 + u * 4 + x_block] : 1;      // (bytes behind the last row are of no account)
+      }
+      if (p.dy_mode == 2) {
+        dy_unit[0] = *reinterpret_cast<const uint4*>(dy_codes + stage * WG_DY_CODES + swizzle128_offset(yr, yp));
+        sy = t * WG_ROWS + yr < p.m ? e[512 + (yr & 31) * 16 + (yr >> 5) * 4 + y_block] : 1;
+      } else if (p.dy_mode == 1) {
+        dy_unit[0] = ahead[0]; dy_unit[1] = ahead[1];
+        if (t + 1 < last) fetch(t + 1);
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&taken[stage]);      // the codes are in registers
+      if (!mbar_wait(&empty[slot], phase ^ 1, abort_flag, p.status, 133)) { ok = false; break; }
+      uint8_t* sA = dy_s + slot * WG_A_BYTES;
+      uint8_t* sB = x_s + slot * WG_B_BYTES;
       // (odd blocks of 64 columns store their second piece first: eight lanes then fill eight different 16-byte columns of the banks)
-      if (xp < groups * 4) {
+      if (x_any) {
         const int swap = xp >> 2 & 1;
 #pragma unroll
         for (int u = 0; u < kUnits; ++u) {
@@ -200,23 +223,24 @@ float8_gradient_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_co
         }
       }
       if (p.dy_mode != 0) {
-        uint4 v[2] = {other[0], other[1]};
-        if (p.dy_mode == 2) convert16(other[0], sy, p.dy8.format, v);
+        uint4 v[2] = {dy_unit[0], dy_unit[1]};
+        if (p.dy_mode == 2) convert16(dy_unit[0], sy, p.dy8.format, v);
         const int swap = yp >> 2 & 1;
         *reinterpret_cast<uint4*>(sA + piece_at(yr, yp * 2 + swap)) = swap ? v[1] : v[0];
         *reinterpret_cast<uint4*>(sA + piece_at(yr, yp * 2 + 1 - swap)) = swap ? v[0] : v[1];
       }
       fence_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&full[stage]);
-      if (++stage == WG_STAGES) { stage = 0; phase ^= 1; }
+      if (lane == 0) mbar_arrive(&full[slot]);
+      if (++slot == WG_OPERANDS) { slot = 0; phase ^= 1; }
+      if (++stage == WG_RING) { stage = 0; ring_phase ^= 1; }
     }
     // The tile: 16 warps, 64 columns of a lane quadrant each.
     ok = ok && mbar_wait(done, 0, abort_flag, p.status, 134);
     tc_fence_after();
     if (ok) {
       const int q = warp & 3, part = (warp - 2) >> 2, row0 = n0 + q * 32, col0 = k0 + part * 64;
-      uint8_t* tile = out_stage + (warp - 2) * 4096;
+      uint8_t* tile = dy_s + (warp - 2) * 4096;      // (every product is done: dy's ring is free)
       float* out = p.out + split * p.split_stride;
       if (row0 < p.n && col0 < p.k) {
         uint32_t r[2][32];
@@ -265,23 +289,55 @@ float8_gradient_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_co
   if (warp == 1) { tc_fence_after(); tmem_dealloc(tmem_base, 512); }
 }
 
-// dW and dbias from the splits' partial tiles, added in order.
+// dW and dbias from the splits' partial tiles, added in a fixed order: four neighbouring columns a thread, STRANDS threads of a block share the splits, eight
+// loads in flight each.
+template <int STRANDS>
 __global__ void __launch_bounds__(256)
-gradient_join_kernel(const float* partial, int64_t ld, int64_t split_stride, int splits, int n, int k, float* out, const float* bias_partial, float* bias) {
+gradient_join_kernel(const float* partial, int ld, int64_t split_stride, int splits, int n, int k, int direct, float* out, const float* bias_partial,
+                     float* bias) {
+  constexpr int kColumns = 256 / STRANDS;
+  __shared__ float4 s[STRANDS][kColumns];
+  const int lane = threadIdx.x % kColumns, strand = threadIdx.x / kColumns;
   lf_chain();
-  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x, total = (int64_t)n * k;
-  if (at < total) {
-    const int64_t row = at / k;
-    const float* from = partial + row * ld + (at - row * k);
-    float t = 0.f;
-#pragma unroll 8
-    for (int s = 0; s < splits; ++s) t += from[s * split_stride];
-    out[at] = t;
+  const uint32_t per_row = ld / 4;
+  const int64_t at = (int64_t)blockIdx.x * kColumns + lane;
+  const int64_t row = at / per_row;
+  const int col = (int)(at - row * per_row) * 4;
+  float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (row < n) {
+    const float4* from = reinterpret_cast<const float4*>(partial + row * ld + col);
+    for (int i = strand; i < splits; i += 8 * STRANDS) {
+      float4 v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = i + j * STRANDS < splits ? from[(i + j * STRANDS) * (split_stride / 4)] : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) { t.x += v[j].x; t.y += v[j].y; t.z += v[j].z; t.w += v[j].w; }
+    }
   }
-  if (at < n && bias) {
-    float t = 0.f;
-    for (int s = 0; s < splits; ++s) t += bias_partial[(int64_t)s * n + at];
-    bias[at] = t;
+  if (STRANDS > 1) {
+    s[strand][lane] = t;
+    __syncthreads();
+    if (strand == 0) {
+#pragma unroll
+      for (int i = 1; i < STRANDS; ++i) { t.x += s[i][lane].x; t.y += s[i][lane].y; t.z += s[i][lane].z; t.w += s[i][lane].w; }
+    }
+  }
+  if (strand == 0 && row < n) {
+    float* to = out + row * k + col;
+    if (direct) *reinterpret_cast<float4*>(to) = t;      // whole, aligned rows
+    else {
+      to[0] = t.x;      // (the row's last group may be in part behind its end)
+      if (col + 1 < k) to[1] = t.y;
+      if (col + 2 < k) to[2] = t.z;
+      if (col + 3 < k) to[3] = t.w;
+    }
+  }
+  const int64_t b = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (b < n && bias) {
+    float u = 0.f;
+#pragma unroll 8
+    for (int i = 0; i < splits; ++i) u += bias_partial[(int64_t)i * n + b];
+    bias[b] = u;
   }
 }
 
@@ -329,8 +385,13 @@ lf_status lf_float8_weight_gradient_run(lf_context* ctx, const lf_float8_weight_
   int splits;
   tc::gradient_plan(ctx, x.rows, p.n, p.k, p.steps, splits, p.per_split);
   p.x = matrix(x);
-  CUtensorMap ma{}, mo{};
-  if (d->encoded_gradient.codes) { p.dy_mode = 2; p.dy8 = matrix(d->encoded_gradient); }
+  CUtensorMap ma{}, mx{}, mo{};
+  LF_TRY(tc::make_map_bytes(ctx, &mx, p.x.codes, p.k, p.m, p.x.pitch, tc::WG_ROWS));
+  if (d->encoded_gradient.codes) {
+    p.dy_mode = 2;
+    p.dy8 = matrix(d->encoded_gradient);
+    LF_TRY(tc::make_map_bytes(ctx, &ma, p.dy8.codes, p.n, p.m, p.dy8.pitch, tc::WG_ROWS));
+  }
   else {
     p.dy = (const bf16*)d->gradient;
     p.dy_mode = lf_aligned16(p.dy) && p.n % 8 == 0 ? 0 : 1;
@@ -348,13 +409,18 @@ lf_status lf_float8_weight_gradient_run(lf_context* ctx, const lf_float8_weight_
     LF_TRY(tc::make_map_f32_any(ctx, &mo, p.out, {(uint64_t)p.k, (uint64_t)p.n, (uint64_t)splits}, {(uint64_t)p.ld * 4, (uint64_t)p.ld * 4 * p.n}, {32, 32, 1}));
   p.status = (tc05::Status*)ctx->tc_status;
   lf_prof_begin(ctx, LF_KERNEL_TRIANGLE_CONTRACT);
-  lf_launch(ctx, tc::float8_gradient_kernel, dim3((p.k + tc::WG_BK - 1) / tc::WG_BK, (p.n + tc::WG_BN - 1) / tc::WG_BN, splits), tc::WG_THREADS, tc::WG_SMEM, ma, mo, p);
+  lf_launch(ctx, tc::float8_gradient_kernel, dim3((p.k + tc::WG_BK - 1) / tc::WG_BK, (p.n + tc::WG_BN - 1) / tc::WG_BN, splits), tc::WG_THREADS, tc::WG_SMEM, ma, mx, mo, p);
   lf_prof_end(ctx);
   ctx->launches++;
   if (!direct) {
     lf_prof_begin(ctx, LF_KERNEL_ELEMENTWISE);
-    lf_launch(ctx, tc::gradient_join_kernel, lf_ceil_div((int64_t)p.n * p.k, 256), 256, 0, p.out, p.ld, p.split_stride, splits, p.n, p.k, d->weight_gradient, bias_partial,
-              d->bias_gradient);
+    const int64_t fours = (int64_t)p.n * (p.ld / 4);
+    const int whole = p.ld == p.k && lf_aligned16(d->weight_gradient);
+    auto join = [&](auto kernel, int per_block) {      // (as many blocks as the bias needs, where the rows are short)
+      lf_launch(ctx, kernel, std::max(lf_ceil_div(fours, per_block), lf_ceil_div(p.n, 256)), 256, 0, p.out, (int)p.ld, p.split_stride, splits, p.n, p.k, whole,
+                d->weight_gradient, bias_partial, d->bias_gradient);
+    };
+    if (splits > 8) join(tc::gradient_join_kernel<8>, 32); else join(tc::gradient_join_kernel<1>, 256);
     lf_prof_end(ctx);
     ctx->launches++;
   }

@@ -9,6 +9,8 @@
 // Blocks stay and walk over the rows, the next row's loads in flight under the present one's arithmetic and the weights in registers; a lane always
 // has the same channels, so dg and db add up in its registers and every block leaves one row of sums, which a second, small kernel
 // adds in a fixed order.
+#include <algorithm>
+
 #include "float8.cuh"
 #include "tc05.cuh"
 
@@ -20,7 +22,7 @@ using tc05::fma2;
 
 struct Forward {
   int64_t rows;
-  int c, access_in, access_out;
+  int c, access_in, access_out, access_weights;
   float epsilon;
   const void* x;
   const float *scale, *offset;
@@ -31,7 +33,7 @@ struct Forward {
 
 struct Backward {
   int64_t rows;
-  int c, access_dy, access_x, access_dx;
+  int c, access_dy, access_x, access_dx, access_weights;
   const void *dy, *x;            // x null: `kept`
   Matrix kept;
   const float *mean, *inverse, *scale;
@@ -64,10 +66,19 @@ __device__ __forceinline__ float2 group_sum(float2 v, float2* slots, int& turn) 
   return v;
 }
 
+template <int LANES>
+__device__ __forceinline__ Share load_weights(const float* p, int left, int access, float* room) {
+  Raw<float> r;
+  load16<float, LANES>(r, p, left, true, access);
+  return unpack<float, LANES>(r, access, room);
+}
+
 template <typename T, int G>
 __global__ void __launch_bounds__(threads_of(G), blocks_of(G))
 forward_kernel(const Forward a) {
-  constexpr int kGroups = threads_of(G) / G, kLanes = G < 8 ? G : 8;
+  constexpr int kGroups = threads_of(G) / G, kLanes = G < 8 ? G : 8, kWarp = G < 32 ? G : 32;
+  __shared__ __align__(16) float rooms[threads_of(G) / 32][kRoom];
+  float* room = rooms[threadIdx.x >> 5];
   __shared__ float2 slots[2 * threads_of(G) / 32];
   const int lane = threadIdx.x % G, group = threadIdx.x / G, first = lane * kShare, left = a.c - first;
   int turn = 0;
@@ -75,14 +86,14 @@ forward_kernel(const Forward a) {
   const int64_t step = (int64_t)gridDim.x * kGroups;
   int64_t row = (int64_t)blockIdx.x * kGroups + group;
   Raw<T> raw;
-  load16(raw, static_cast<const T*>(a.x) + row * a.c + first, row < a.rows ? left : 0, a.access_in);
-  const Share scale = load_weights(a.scale + first, left), offset = load_weights(a.offset + first, left);
+  load16<T, kWarp>(raw, static_cast<const T*>(a.x) + row * a.c + first, left, row < a.rows, a.access_in);
+  const Share scale = load_weights<kWarp>(a.scale + first, left, a.access_weights, room), offset = load_weights<kWarp>(a.offset + first, left, a.access_weights, room);
   const float over = 1.0f / (float)a.c;
   // (the trip count is the same for every lane of a block)
   for (int64_t base = (int64_t)blockIdx.x * kGroups; base < a.rows; base += step, row += step) {
     const bool live = row < a.rows;
-    Share x = unpack(raw);
-    load16(raw, static_cast<const T*>(a.x) + (row + step) * a.c + first, row + step < a.rows ? left : 0, a.access_in);
+    Share x = unpack<T, kWarp>(raw, a.access_in, room);
+    load16<T, kWarp>(raw, static_cast<const T*>(a.x) + (row + step) * a.c + first, left, row + step < a.rows, a.access_in);
     if (a.kept.codes) {
       uint4 codes;
       const int s = encode16<kLanes>(x, a.kept.format, codes);
@@ -106,7 +117,7 @@ forward_kernel(const Forward a) {
     if (a.mean && live && lane == 0) { a.mean[row] = mean; a.inverse[row] = inverse; }
 #pragma unroll
     for (int i = 0; i < kShare / 2; ++i) x.v[i] = fma2(mul2(x.v[i], both(inverse)), scale.v[i], offset.v[i]);
-    if (a.y && live) store16(static_cast<T*>(a.y) + row * a.c + first, left, a.access_out, x);
+    if (a.y) store16<T, kWarp>(static_cast<T*>(a.y) + row * a.c + first, left, live, a.access_out, x, room);
     if (a.encoded.codes) {
       if (left < kShare) {      // (0 * inverse is no zero in a row whose statistics are no numbers)
 #pragma unroll
@@ -125,7 +136,9 @@ forward_kernel(const Forward a) {
 template <typename T, int G, bool KEPT>
 __global__ void __launch_bounds__(threads_of(G), blocks_of(G))
 backward_kernel(const Backward a) {
-  constexpr int kThreads = threads_of(G), kGroups = kThreads / G;
+  constexpr int kThreads = threads_of(G), kGroups = kThreads / G, kWarp = G < 32 ? G : 32;
+  __shared__ __align__(16) float rooms[kThreads / 32][kRoom];
+  float* room = rooms[threadIdx.x >> 5];
   __shared__ float2 slots[2 * kThreads / 32];
   __shared__ float sums[kGroups > 1 ? kThreads * kShare : 1];
   const int lane = threadIdx.x % G, group = threadIdx.x / G, first = lane * kShare, left = a.c - first;
@@ -138,12 +151,11 @@ backward_kernel(const Backward a) {
   float factor, mean, inverse;
   auto fetch = [&](int64_t r) {      // (a row that does not exist is all zeros)
     const bool live = r < a.rows;
-    const int count = live ? left : 0;
-    load16(raw_dy, static_cast<const T*>(a.dy) + r * a.c + first, count, a.access_dy);
+    load16<T, kWarp>(raw_dy, static_cast<const T*>(a.dy) + r * a.c + first, left, live, a.access_dy);
     codes = make_uint4(0, 0, 0, 0);
     factor = 0.f;
-    if (!KEPT) load16(raw_x, static_cast<const T*>(a.x) + r * a.c + first, count, a.access_x);
-    else if (count > 0) {
+    if (!KEPT) load16<T, kWarp>(raw_x, static_cast<const T*>(a.x) + r * a.c + first, left, live, a.access_x);
+    else if (live && left > 0) {
       codes = *reinterpret_cast<const uint4*>(a.kept.codes + r * a.kept.pitch + first);
       factor = up(a.kept.exponents[exponent_at(r, first / kBlock, a.kept.tiles)]);
     }
@@ -151,14 +163,14 @@ backward_kernel(const Backward a) {
     inverse = live ? a.inverse[r] : 0.f;
   };
   fetch(row);
-  const Share scale = load_weights(a.scale + first, left);
+  const Share scale = load_weights<kWarp>(a.scale + first, left, a.access_weights, room);
   Share dg, db;
 #pragma unroll
   for (int i = 0; i < kShare / 2; ++i) dg.v[i] = db.v[i] = make_float2(0.f, 0.f);
   const float over = 1.0f / (float)a.c;
   for (int64_t base = (int64_t)blockIdx.x * kGroups; base < a.rows; base += step, row += step) {
-    const Share dy = unpack(raw_dy);
-    Share u = KEPT ? decode16(codes, a.kept.format) : unpack(raw_x);
+    const Share dy = unpack<T, kWarp>(raw_dy, a.access_dy, room);
+    Share u = KEPT ? decode16(codes, a.kept.format) : unpack<T, kWarp>(raw_x, a.access_x, room);
     const float inv = inverse;
     // (x - mean) rstd; of codes by one multiply-add, their power of two with rstd
     const float2 by = both(KEPT ? factor * inv : inv), from = both(KEPT ? -mean * inv : -mean);
@@ -175,18 +187,16 @@ backward_kernel(const Backward a) {
       s2 = fma2(h, u.v[i], s2);
     }
     const float2 s = group_sum<G>(make_float2(s1.x + s1.y, s2.x + s2.y), slots, turn);
-    if (row < a.rows) {
-      const float2 t1 = both(-s.x * over * inv), t2 = both(-s.y * over * inv);
+    const float2 t1 = both(-s.x * over * inv), t2 = both(-s.y * over * inv);
 #pragma unroll
-      for (int i = 0; i < kShare / 2; ++i) u.v[i] = fma2(u.v[i], t2, fma2(mul2(dy.v[i], scale.v[i]), both(inv), t1));
-      store16(static_cast<T*>(a.dx) + row * a.c + first, left, a.access_dx, u);
-    }
+    for (int i = 0; i < kShare / 2; ++i) u.v[i] = fma2(u.v[i], t2, fma2(mul2(dy.v[i], scale.v[i]), both(inv), t1));
+    store16<T, kWarp>(static_cast<T*>(a.dx) + row * a.c + first, left, row < a.rows, a.access_dx, u, room);
   }
   // this block's row of sums
 #pragma unroll
   for (int which = 0; which < 2; ++which) {
     float* out = a.partial + ((int64_t)blockIdx.x * 2 + which) * a.c;
-    if (kGroups == 1) store16(out + first, left, kElements, which ? db : dg);
+    if (kGroups == 1) store16<float, kWarp>(out + first, left, true, kElements, which ? db : dg, room);
     else {
       __syncthreads();
 #pragma unroll
@@ -292,6 +302,7 @@ lf_status lf_layer_norm_run(lf_context* ctx, const lf_layer_norm_desc* d, lf_res
   a.rows = d->rows; a.c = d->channels; a.epsilon = d->epsilon;
   a.access_in = row_access(d->activations, a.c, d->act_dtype);
   a.access_out = row_access(d->out, a.c, d->act_dtype);
+  a.access_weights = std::min(row_access(d->scale, a.c, LF_DTYPE_F32), row_access(d->offset, a.c, LF_DTYPE_F32));
   a.x = d->activations; a.scale = d->scale; a.offset = d->offset; a.y = d->out; a.mean = d->mean; a.inverse = d->inverse_deviation;
   if (d->checkpoint.codes) a.kept = matrix(d->checkpoint);
   if (d->encoded.codes) a.encoded = matrix(d->encoded);
@@ -325,6 +336,7 @@ lf_status lf_layer_norm_backward_run(lf_context* ctx, const lf_layer_norm_backwa
   a.access_dy = row_access(d->gradient, a.c, d->act_dtype);
   a.access_x = row_access(d->activations, a.c, d->act_dtype);
   a.access_dx = row_access(d->out, a.c, d->act_dtype);
+  a.access_weights = row_access(d->scale, a.c, LF_DTYPE_F32);
   a.dy = d->gradient; a.x = d->activations; a.mean = d->mean; a.inverse = d->inverse_deviation; a.scale = d->scale; a.dx = d->out;
   if (d->checkpoint.codes) a.kept = matrix(d->checkpoint);
   a.partial = (float*)d->workspace;

@@ -37,11 +37,14 @@ def _format(value, name="format"):
 
 
 def _shape(inp, *names):
-    values = [inp[name] for name in names]
-    for name, value in zip(names, values):
+    values = []
+    for name in names:
+        value = inp[name]
         if type(value) is not int or value <= 0:
             _positive(name, value)
-    return [int(value) for value in values]
+            value = int(value)
+        values.append(value)
+    return values
 
 
 _names = {}      # torch dtype -> "f32" | "bf16"
@@ -61,7 +64,7 @@ def _tensor(device, name, value, count, only=None):
         raise ValueError(f"{name} must be a CUDA tensor")
     if value.get_device() != device.ordinal:
         raise ValueError(f"{name} is on {value.device}, the device's GPU is cuda:{device.ordinal}")
-    dtype = _names.get(value.dtype) or _names.get(value.dtype if _torch() else None)
+    dtype = (_names or (_torch(), _names)[1]).get(value.dtype)
     if dtype is None or (only is not None and dtype != only):
         raise ValueError(f"{name} must be {only or 'f32 or bf16'}; received {value.dtype}")
     if not value.is_contiguous():
@@ -215,7 +218,7 @@ class LayerNormGpu:
         if out is not None:
             _tensor(dev, "out", out, rows * c, dtype)
         elif not encode:
-            out = x.new_empty(x.shape)
+            out = _torch().empty_like(x)
         checkpoint = Float8Tensor.empty(rows, c, kept, x) if kept else None
         encoded = Float8Tensor.empty(rows, c, encode, x) if encode else None
         statistics = scale.new_empty((2, rows)) if kept or opts.get("statistics") else None
@@ -250,7 +253,7 @@ class LayerNormGpu:
         if out is not None:
             _tensor(dev, "out", out, rows * c, dtype)
         else:
-            out = dy.new_empty(dy.shape)
+            out = _torch().empty_like(dy)
         nbytes = dev.lib.lf_layer_norm_backward_workspace(dev.handle, rows, c)
         # the two weights' gradients, then the workspace on a 16-byte boundary
         ahead = (2 * c + 3) // 4 * 4
