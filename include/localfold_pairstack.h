@@ -646,9 +646,10 @@ LF_API uint64_t lf_layer_norm_backward_workspace(const lf_context* ctx, int64_t 
 LF_API lf_status lf_layer_norm_backward_run(lf_context* ctx, const lf_layer_norm_backward_desc* d, lf_result* r);
 
 /* out[m][n] = sum_k activations[m][k] weights[n][k] (+ bias[n]), float32 sums, out_dtype rows.  With
- * `source` [rows][channels] of source_dtype its 8-bit form is made first, into the buffers of
- * `activations`.  The gradient of a projection's input is the same call on the encoded gradient and
- * the transposed weights. */
+ * `source` [rows][channels] of source_dtype the operand is its 8-bit form in activations.format, which goes
+ * to the buffers of `activations` where they are set; where they are not, some sizes need the
+ * workspace.  The gradient of a projection's input is the same call on the encoded gradient and the
+ * transposed weights. */
 typedef struct lf_float8_linear_desc {
   lf_float8_matrix activations;   /* [rows][channels] */
   lf_float8_matrix weights;       /* [out channels][channels] */
@@ -656,7 +657,10 @@ typedef struct lf_float8_linear_desc {
   int32_t out_dtype, source_dtype;
   const void* source;             /* or null: activations are encoded already */
   void* out;
+  void* workspace;
+  uint64_t workspace_bytes;
 } lf_float8_linear_desc;
+LF_API uint64_t lf_float8_linear_workspace(int64_t rows, int32_t channels);
 LF_API lf_status lf_float8_linear_run(lf_context* ctx, const lf_float8_linear_desc* d, lf_result* r);
 /* weight_gradient [out channels][channels] = sum over rows of gradient[row][n] activations[row][k], bias_gradient [out channels]
  * (or null) = sum of gradient[row][n], float32.  gradient: bf16 rows, or its 8-bit form; activations: the 8-bit

@@ -166,7 +166,7 @@ class LayerNormBackwardDesc(ctypes.Structure):
 
 class Float8LinearDesc(ctypes.Structure):
     _fields_ = [("activations", Float8Matrix), ("weights", Float8Matrix), ("bias", c_void_p), ("out_dtype", c_int32),
-                ("source_dtype", c_int32), ("source", c_void_p), ("out", c_void_p)]
+                ("source_dtype", c_int32), ("source", c_void_p), ("out", c_void_p), ("workspace", c_void_p), ("workspace_bytes", ctypes.c_uint64)]
 
 
 class Float8WeightGradientDesc(ctypes.Structure):
@@ -187,7 +187,7 @@ EXPORTS = (
     "lf_pair_shard_step", "lf_pair_shard_exchange_step", "lf_pair_planes_scatter", "lf_peer_buffer_create", "lf_peer_buffer_open", "lf_peer_buffer_close",
     "lf_peer_buffer_destroy", "lf_pair_transpose_scatter",
     "lf_float8_code_bytes", "lf_float8_exponent_bytes", "lf_float8_encode", "lf_float8_decode", "lf_layer_norm_run",
-    "lf_layer_norm_backward_workspace", "lf_layer_norm_backward_run", "lf_float8_linear_run",
+    "lf_layer_norm_backward_workspace", "lf_layer_norm_backward_run", "lf_float8_linear_workspace", "lf_float8_linear_run",
     "lf_float8_weight_gradient_workspace", "lf_float8_weight_gradient_run",
 )
 
@@ -252,7 +252,7 @@ def load():
     lib.lf_peer_buffer_destroy.argtypes = [c_void_p, c_void_p]
     lib.lf_pair_transpose_scatter.argtypes = [c_void_p, c_void_p, c_int32, c_int32, c_int32, c_int32, c_int32,
                                               ctypes.POINTER(c_void_p)]
-    for name, args in (("lf_float8_code_bytes", [c_int64, c_int32]), ("lf_float8_exponent_bytes", [c_int64, c_int32]),
+    for name, args in (("lf_float8_code_bytes", [c_int64, c_int32]), ("lf_float8_linear_workspace", [c_int64, c_int32]), ("lf_float8_exponent_bytes", [c_int64, c_int32]),
                        ("lf_layer_norm_backward_workspace", [c_void_p, c_int64, c_int32]),
                        ("lf_float8_weight_gradient_workspace", [c_void_p, c_int64, c_int32, c_int32])):
         getattr(lib, name).argtypes = args

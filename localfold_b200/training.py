@@ -323,22 +323,27 @@ class Float8LinearGpu:
 
     def _product(self, name, value, rows, channels, weights, bias, options, out):
         dev, opts = self.device, options or {}
+        keep, source, operand, workspace, nbytes = bool(opts.get("checkpoint")), None, None, None, 0
         format = _format(opts.get("format", "e4m3"))
-        source = None
         if isinstance(value, Float8Tensor):
             operand, dtype = _matrix(dev, name, value, rows, channels), _output(opts, "bf16")
         else:
             source = _tensor(dev, name, value, rows * channels)
             dtype = _output(opts, source)
-            operand = Float8Tensor.empty(rows, channels, format, value)
+            if keep:
+                operand = Float8Tensor.empty(rows, channels, format, value)
+            else:
+                nbytes = dev.lib.lf_float8_linear_workspace(rows, channels)
+                workspace = weights.memory.new_empty(nbytes) if nbytes else None
         if out is not None:
             _tensor(dev, "out", out, rows * weights.rows, dtype)
         else:
             out = weights.memory.new_empty((rows, weights.rows), dtype=_torch_dtype(dtype))
-        desc = nat.Float8LinearDesc(operand.desc, weights.desc, bias.data_ptr() if bias is not None else None, _DTYPE[dtype],
-                                    _DTYPE[source or "f32"], value.data_ptr() if source else None, out.data_ptr())
-        result = _call(dev, dev.lib.lf_float8_linear_run, desc, (value, operand, weights, bias, out), out)
-        if opts.get("checkpoint"):
+        desc = nat.Float8LinearDesc(operand.desc if operand is not None else nat.Float8Matrix(rows, channels, _FORMAT[format]), weights.desc,
+                                    bias.data_ptr() if bias is not None else None, _DTYPE[dtype], _DTYPE[source or "f32"],
+                                    value.data_ptr() if source else None, out.data_ptr(), workspace.data_ptr() if nbytes else None, nbytes)
+        result = _call(dev, dev.lib.lf_float8_linear_run, desc, (value, operand, weights, bias, workspace, out), out)
+        if keep:
             result["checkpoint"] = operand
         return result
 

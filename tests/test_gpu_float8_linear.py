@@ -14,7 +14,7 @@ TYPES = {"f32": torch.float32, "bf16": torch.bfloat16}
 STEP = 2.0 ** -23
 # rows, channels, outputs: single tokens, partial tiles, all tile widths (64, 128, 256 columns), several groups of 512 channels, odd everything
 SHAPES = [(1, 1, 1), (1, 16, 8), (3, 128, 64), (4, 1536, 384), (16, 384, 1536), (17, 130, 72), (33, 5, 500), (64, 640, 24), (127, 129, 65), (128, 128, 128), (129, 512, 257),
-          (200, 513, 100), (300, 1030, 333), (1000, 64, 1), (2500, 128, 512), (5000, 256, 1000), (20001, 72, 136), (4099, 1200, 640)]
+          (200, 513, 100), (300, 1030, 333), (1000, 64, 1), (2500, 128, 512), (5000, 256, 1000), (20001, 72, 136), (4099, 1200, 640), (30000, 500, 130), (9, 4096, 40), (16, 2000, 33), (8, 5000, 16)]
 
 
 @pytest.fixture(scope="module")
@@ -50,10 +50,13 @@ def test_product(dev, rows, c, n, name, dtype):
     shape = {"rows": rows, "channels": c, "outChannels": n, "weights": weights}
     linear = lf.Float8LinearGpu(dev)
     got = linear.run({**shape, "activations": x}, {"format": name, "checkpoint": True})
+    plain = linear.run({**shape, "activations": x}, {"format": name})
+    kept, encoded = (lf.float8_decode(dev, t, {"output": "f32"}) for t in (got["checkpoint"], lf.float8_encode(dev, x, rows, c, {"format": name})))
     weights.bias = None
     again = linear.run({**shape, "activations": got["checkpoint"]}, {"output": "f32"})
     dev.synchronize()
     assert got["output"].dtype == TYPES[dtype] and again["output"].dtype == torch.float32
+    assert torch.equal(got["output"], plain["output"]) and "checkpoint" not in plain and torch.equal(kept, encoded)
     x8, w8 = ref.decoded(host(x), name), ref.decoded(host(w), "e4m3", 128)
     want, size = x8 @ w8.T, np.abs(x8) @ np.abs(w8).T
     ref.close(again["output"], want, c * STEP * size, "without a bias, float32")
