@@ -10,13 +10,14 @@ namespace f8 {
 
 constexpr int kThreads = 256, kUnits = 2;
 
-template <typename T, int LANES>
+template <typename T, int LANES, bool ELEMENTS>
 __global__ void __launch_bounds__(kThreads)
-encode_kernel(const T* x, const Matrix m, uint32_t units, uint32_t per_row, int access) {
+encode_kernel(const T* x, const Matrix m, uint32_t units, uint32_t per_row, int how) {
+  const int access = ELEMENTS ? (int)kElements : max(how, (int)kSixteen);
   const int lane = threadIdx.x % LANES;
   const uint32_t base = blockIdx.x * (uint32_t)(kThreads / LANES * kUnits) + threadIdx.x / LANES;
-  __shared__ __align__(16) float rooms[kThreads / 32][kRoom];
-  float* room = rooms[threadIdx.x >> 5];
+  __shared__ __align__(16) float rooms[ELEMENTS ? kThreads / 32 : 1][ELEMENTS ? kRoom : 4];
+  float* room = rooms[ELEMENTS ? threadIdx.x >> 5 : 0];
   lf_chain();
   Raw<T> raw[kUnits];
   uint32_t row[kUnits], first[kUnits];
@@ -35,13 +36,14 @@ encode_kernel(const T* x, const Matrix m, uint32_t units, uint32_t per_row, int 
   }
 }
 
-template <typename T, int LANES>
+template <typename T, int LANES, bool ELEMENTS>
 __global__ void __launch_bounds__(kThreads)
-decode_kernel(const Matrix m, T* out, uint32_t units, uint32_t per_row, int access) {
+decode_kernel(const Matrix m, T* out, uint32_t units, uint32_t per_row, int how) {
+  const int access = ELEMENTS ? (int)kElements : max(how, (int)kSixteen);
   const int lane = threadIdx.x % LANES;
   const uint32_t base = blockIdx.x * (uint32_t)(kThreads / LANES * kUnits) + threadIdx.x / LANES;
-  __shared__ __align__(16) float rooms[kThreads / 32][kRoom];
-  float* room = rooms[threadIdx.x >> 5];
+  __shared__ __align__(16) float rooms[ELEMENTS ? kThreads / 32 : 1][ELEMENTS ? kRoom : 4];
+  float* room = rooms[ELEMENTS ? threadIdx.x >> 5 : 0];
   lf_chain();
   uint4 codes[kUnits];
   int s[kUnits];
@@ -90,16 +92,12 @@ encode_square_kernel(const T* x, const Matrix m, const Matrix t, int access) {
     load16<T, 8>(raw[k], x + row * m.channels + first, m.channels - first, row < m.rows, access);
   }
   float most = 0.f, finite = 0.f;
-  Share all[kRows];
+  Share v[kRows];
 #pragma unroll
   for (int k = 0; k < kRows; ++k) {
-    const Share v = all[k] = unpack<T, 8>(raw[k], access, room);
-#pragma unroll
-    for (int i = 0; i < kShare; ++i) {
-      const float a = fabsf(i & 1 ? v.v[i / 2].y : v.v[i / 2].x);
-      most = fmaxf(most, a);
-      if (a < kInfinity) finite = fmaxf(finite, a);
-    }
+    v[k] = unpack<T, 8>(raw[k], access, room);
+    most = fmaxf(most, most_of(v[k]));
+    finite = fmaxf(finite, most_finite_of(v[k]));
   }
 #pragma unroll
   for (int o = 16; o; o >>= 1) { most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o)); finite = fmaxf(finite, __shfl_xor_sync(0xffffffffu, finite, o)); }
@@ -108,22 +106,13 @@ encode_square_kernel(const T* x, const Matrix m, const Matrix t, int access) {
 #pragma unroll
   for (int w = 0; w < kThreads / 32; ++w) { most = fmaxf(most, most_s[0][w]); finite = fmaxf(finite, most_s[1][w]); }
   const int s = exponent_byte(__float_as_uint(finite), m.format);
-  const float f = down(s);
 #pragma unroll
   for (int k = 0; k < kRows; ++k) {
     const int64_t row = row0 + strand + kThreads / 8 * k;
-    const Share& v = all[k];
-    uint32_t w[4] = {0, 0, 0, 0};
-    if (most < kInfinity) {
-#pragma unroll
-      for (int i = 0; i < kShare / 2; ++i) w[i >> 1] |= code2(v.v[i].x * f, v.v[i].y * f, m.format) << (16 * (i & 1));
-    } else {
-#pragma unroll
-      for (int i = 0; i < kShare / 2; ++i)
-        w[i >> 1] |= (code_special(v.v[i].x * f, m.format) | code_special(v.v[i].y * f, m.format) << 8) << (16 * (i & 1));
-    }
-    if (row < m.rows && first < m.channels) *reinterpret_cast<uint4*>(m.codes + row * m.pitch + first) = make_uint4(w[0], w[1], w[2], w[3]);
+    const uint4 codes = code16(v[k], s, m.format, most == kInfinity);
+    if (row < m.rows && first < m.channels) *reinterpret_cast<uint4*>(m.codes + row * m.pitch + first) = codes;
     if (t.codes) {
+      const uint32_t w[4] = {codes.x, codes.y, codes.z, codes.w};
 #pragma unroll
       for (int i = 0; i < kShare; ++i) turned[lane * kShare + i][strand + kThreads / 8 * k] = (uint8_t)(w[i >> 2] >> (8 * (i & 3)));
     }
@@ -140,6 +129,14 @@ encode_square_kernel(const T* x, const Matrix m, const Matrix t, int access) {
       *reinterpret_cast<uint4*>(t.codes + row * t.pitch + tfirst) = *reinterpret_cast<const uint4*>(&turned[strand + kThreads / 8 * k][lane * kShare]);
   }
   if (threadIdx.x < kBlock) t.exponents[exponent_at(trow0 + threadIdx.x, blockIdx.y, t.tiles)] = (uint8_t)s;
+}
+
+// f(T, LANES, ELEMENTS as types)
+template <typename F>
+static void row_forms(int dtype, int channels, int access, F f) {
+  auto last = [&](auto t, auto lanes) { if (access == kElements) f(t, lanes, std::true_type{}); else f(t, lanes, std::false_type{}); };
+  auto with = [&](auto t) { if (channels <= 64) last(t, std::integral_constant<int, 4>{}); else last(t, std::integral_constant<int, 8>{}); };
+  if (dtype == LF_DTYPE_BF16) with(bf16{}); else with(float{});
 }
 
 }  // namespace f8
@@ -202,13 +199,11 @@ lf_status lf_float8_encode(lf_context* ctx, const lf_float8_encode_desc* d, lf_r
     else lf_launch(ctx, encode_square_kernel<float>, grid, kThreads, 0, (const float*)d->source, m, t, access);
   } else {
     const uint32_t per_row = blocks(o.channels), units = (uint32_t)(o.rows * per_row);
-    auto run = [&](auto lanes) {
+    row_forms(d->dtype, o.channels, access, [&](auto t, auto lanes, auto elements) {
+      typedef decltype(t) T;
       constexpr int L = decltype(lanes)::value;
-      const int grid = lf_ceil_div(units, kThreads / L * kUnits);
-      if (d->dtype == LF_DTYPE_BF16) lf_launch(ctx, encode_kernel<bf16, L>, grid, kThreads, 0, (const bf16*)d->source, m, units, per_row, access);
-      else lf_launch(ctx, encode_kernel<float, L>, grid, kThreads, 0, (const float*)d->source, m, units, per_row, access);
-    };
-    if (o.channels <= 64) run(std::integral_constant<int, 4>{}); else run(std::integral_constant<int, 8>{});
+      lf_launch(ctx, encode_kernel<T, L, decltype(elements)::value>, lf_ceil_div(units, kThreads / L * kUnits), kThreads, 0, (const T*)d->source, m, units, per_row, access);
+    });
   }
   lf_prof_end(ctx);
   ctx->launches++;
@@ -226,13 +221,11 @@ lf_status lf_float8_decode(lf_context* ctx, const lf_float8_decode_desc* d, lf_r
   const int access = row_access(d->out, o.channels, d->dtype);
   const uint32_t per_row = blocks(o.channels), units = (uint32_t)(o.rows * per_row);
   lf_prof_begin(ctx, LF_KERNEL_ELEMENTWISE);
-  auto run = [&](auto lanes) {
+  row_forms(d->dtype, o.channels, access, [&](auto t, auto lanes, auto elements) {
+    typedef decltype(t) T;
     constexpr int L = decltype(lanes)::value;
-    const int grid = lf_ceil_div(units, kThreads / L * kUnits);
-    if (d->dtype == LF_DTYPE_BF16) lf_launch(ctx, decode_kernel<bf16, L>, grid, kThreads, 0, m, (bf16*)d->out, units, per_row, access);
-    else lf_launch(ctx, decode_kernel<float, L>, grid, kThreads, 0, m, (float*)d->out, units, per_row, access);
-  };
-  if (o.channels <= 64) run(std::integral_constant<int, 4>{}); else run(std::integral_constant<int, 8>{});
+    lf_launch(ctx, decode_kernel<T, L, decltype(elements)::value>, lf_ceil_div(units, kThreads / L * kUnits), kThreads, 0, m, (T*)d->out, units, per_row, access);
+  });
   lf_prof_end(ctx);
   ctx->launches++;
   return lf_float8_done(ctx, r, 1);

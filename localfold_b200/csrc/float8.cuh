@@ -48,17 +48,26 @@ __device__ __forceinline__ float up(int s) { return __int_as_float(s << 23); }
 
 constexpr float kInfinity = __builtin_huge_valf();
 
+// Formats are template arguments where codes are made and read, behind one branch for many codes: chosen code by code they cost both conversions.
 // Two codes, x in the low byte.  `scaled` values are within the format's range (or not finite: see code_special).
-__device__ __forceinline__ uint32_t code2(float x, float y, int format) {
-  return __nv_cvt_float2_to_fp8x2(make_float2(x, y), __NV_SATFINITE, format == LF_FLOAT8_E4M3 ? __NV_E4M3 : __NV_E5M2);
+template <int FORMAT>
+__device__ __forceinline__ uint32_t code2(float x, float y) {
+  return __nv_cvt_float2_to_fp8x2(make_float2(x, y), __NV_SATFINITE, FORMAT == LF_FLOAT8_E4M3 ? __NV_E4M3 : __NV_E5M2);
 }
 // One code of a value that may be infinite: e4m3 has no infinity, so that it becomes NaN and is not lost in a finite code.
-__device__ __forceinline__ uint32_t code_special(float v, int format) {
-  if (fabsf(v) == kInfinity) return (__float_as_uint(v) >> 24 & 0x80u) | (format == LF_FLOAT8_E4M3 ? 0x7fu : 0x7cu);
-  return code2(v, 0.f, format) & 0xffu;
+template <int FORMAT>
+__device__ __forceinline__ uint32_t code_special(float v) {
+  if (fabsf(v) == kInfinity) return (__float_as_uint(v) >> 24 & 0x80u) | (FORMAT == LF_FLOAT8_E4M3 ? 0x7fu : 0x7cu);
+  return code2<FORMAT>(v, 0.f) & 0xffu;
 }
-__device__ __forceinline__ float2 decode2(uint32_t two, int format) {
-  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)two, format == LF_FLOAT8_E4M3 ? __NV_E4M3 : __NV_E5M2);
+template <int FORMAT>
+__device__ __forceinline__ uint32_t half2_of(uint32_t two) {
+  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)two, FORMAT == LF_FLOAT8_E4M3 ? __NV_E4M3 : __NV_E5M2);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <int FORMAT>
+__device__ __forceinline__ float2 decode2(uint32_t two) {
+  const uint32_t h = half2_of<FORMAT>(two);
   return __half22float2(*reinterpret_cast<const __half2*>(&h));
 }
 
@@ -208,51 +217,73 @@ __device__ __forceinline__ void store16(T* p, int left, bool live, int access, c
   }
 }
 
-// A lane's sixteen codes -> values times `factor`
-__device__ __forceinline__ Share decode16(uint4 codes, int format) {
+// A lane's sixteen codes -> values, without their power of two
+template <int FORMAT>
+__device__ __forceinline__ Share decode16_as(uint4 codes) {
   const uint32_t w[4] = {codes.x, codes.y, codes.z, codes.w};
   Share s;
 #pragma unroll
-  for (int i = 0; i < kShare / 2; ++i) s.v[i] = decode2(w[i >> 1] >> (16 * (i & 1)) & 0xffffu, format);
+  for (int i = 0; i < kShare / 2; ++i) s.v[i] = decode2<FORMAT>(w[i >> 1] >> (16 * (i & 1)) & 0xffffu);
   return s;
 }
+__device__ __forceinline__ Share decode16(uint4 codes, int format) {
+  return format == LF_FLOAT8_E4M3 ? decode16_as<LF_FLOAT8_E4M3>(codes) : decode16_as<LF_FLOAT8_E5M2>(codes);
+}
 
-// The exponent byte of the block that LANES neighbouring lanes hold (eight lanes, or all of a narrower row's), and the lane's codes.  All lanes of
-// the warp call it.  NaN has no say in a maximum; infinities must not have one either.
-template <int LANES>
-__device__ __forceinline__ int encode16(const Share& x, int format, uint4& codes) {
+// A lane's codes of x over the power of two of the byte s; `special`: infinities may be among the values.
+template <int FORMAT>
+__device__ __forceinline__ uint4 code16_as(const Share& x, int s, bool special) {
+  const float2 f = both(down(s));
+  uint32_t w[4];
+  if (special) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      w[i] = code_special<FORMAT>(x.v[2 * i].x * f.x) | code_special<FORMAT>(x.v[2 * i].y * f.x) << 8 | code_special<FORMAT>(x.v[2 * i + 1].x * f.x) << 16 |
+             code_special<FORMAT>(x.v[2 * i + 1].y * f.x) << 24;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 a = mul2(x.v[2 * i], f), b = mul2(x.v[2 * i + 1], f);
+      w[i] = code2<FORMAT>(a.x, a.y) | code2<FORMAT>(b.x, b.y) << 16;
+    }
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+__device__ __forceinline__ uint4 code16(const Share& x, int s, int format, bool special) {
+  return format == LF_FLOAT8_E4M3 ? code16_as<LF_FLOAT8_E4M3>(x, s, special) : code16_as<LF_FLOAT8_E5M2>(x, s, special);
+}
+// The largest magnitude of a lane's values, NaN left out; of its finite ones.
+__device__ __forceinline__ float most_of(const Share& x) {
   float most = 0.f;
 #pragma unroll
   for (int i = 0; i < kShare / 2; ++i) most = fmaxf(most, fmaxf(fabsf(x.v[i].x), fabsf(x.v[i].y)));
+  return most;
+}
+__device__ __forceinline__ float most_finite_of(const Share& x) {
+  float most = 0.f;
+#pragma unroll
+  for (int i = 0; i < kShare / 2; ++i) {
+    if (fabsf(x.v[i].x) < kInfinity) most = fmaxf(most, fabsf(x.v[i].x));
+    if (fabsf(x.v[i].y) < kInfinity) most = fmaxf(most, fabsf(x.v[i].y));
+  }
+  return most;
+}
+
+// The exponent byte of the block that LANES neighbouring lanes hold (eight lanes, or all of a narrower row's), and the lane's codes.  All lanes of
+// the warp call it.
+template <int LANES>
+__device__ __forceinline__ int encode16(const Share& x, int format, uint4& codes) {
+  float most = most_of(x);
 #pragma unroll
   for (int o = LANES / 2; o; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-  uint32_t w[4];
-  if (__any_sync(0xffffffffu, most == kInfinity)) {
-    most = 0.f;
-#pragma unroll
-    for (int i = 0; i < kShare / 2; ++i) {
-      if (fabsf(x.v[i].x) < kInfinity) most = fmaxf(most, fabsf(x.v[i].x));
-      if (fabsf(x.v[i].y) < kInfinity) most = fmaxf(most, fabsf(x.v[i].y));
-    }
+  const bool special = __any_sync(0xffffffffu, most == kInfinity);
+  if (special) {
+    most = most_finite_of(x);
 #pragma unroll
     for (int o = LANES / 2; o; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-    const int s = exponent_byte(__float_as_uint(most), format);
-    const float f = down(s);
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      w[i] = code_special(x.v[2 * i].x * f, format) | code_special(x.v[2 * i].y * f, format) << 8 | code_special(x.v[2 * i + 1].x * f, format) << 16 |
-             code_special(x.v[2 * i + 1].y * f, format) << 24;
-    codes = make_uint4(w[0], w[1], w[2], w[3]);
-    return s;
   }
   const int s = exponent_byte(__float_as_uint(most), format);
-  const float2 f = both(down(s));
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 a = mul2(x.v[2 * i], f), b = mul2(x.v[2 * i + 1], f);
-    w[i] = code2(a.x, a.y, format) | code2(b.x, b.y, format) << 16;
-  }
-  codes = make_uint4(w[0], w[1], w[2], w[3]);
+  codes = code16(x, s, format, special);
   return s;
 }
 

@@ -22,18 +22,14 @@ struct FewParams {
   void* out;
 };
 
-__device__ __forceinline__ uint32_t half2_of(uint32_t two, int format) {
-  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)two, format == LF_FLOAT8_E4M3 ? __NV_E4M3 : __NV_E5M2);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
 __device__ __forceinline__ void mma_16x8x16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// EIGHTS: 8 or 16 rows.  Shared memory: the rows' codes, rows of `room` bytes, then their exponents [row][block].
-template <typename T, int EIGHTS>
+// EIGHTS: 8 or 16 rows; FORMAT of x (weights are e4m3).  Shared memory: the rows' codes, rows of `room` bytes, then their exponents [row][block].
+template <typename T, int EIGHTS, int FORMAT>
 __global__ void __launch_bounds__(FEW_WARPS * 32)
 float8_few_kernel(const FewParams p) {
   constexpr int kRows = EIGHTS * 8;
@@ -57,7 +53,7 @@ float8_few_kernel(const FewParams p) {
     if (p.source) {
       Raw<T> raw;
       load16<T, 8>(raw, static_cast<const T*>(p.source) + (int64_t)row * p.k + first, p.k - first, live, p.access);
-      s = encode16<8>(unpack<T, 8>(raw, p.access, rooms[warp]), p.x.format, codes);
+      s = encode16<8>(unpack<T, 8>(raw, p.access, rooms[warp]), FORMAT, codes);
       if (live && p.x.codes && blockIdx.x == 0) put16(p.x, row, first, codes, s);
     } else if (live) {
       if (first < p.k) codes = *reinterpret_cast<const uint4*>(p.x.codes + row * p.x.pitch + first);
@@ -114,12 +110,12 @@ float8_few_kernel(const FewParams p) {
           const uint32_t w0[4] = {w[i][h][0].x, w[i][h][0].y, w[i][h][0].z, w[i][h][0].w}, w1[4] = {w[i][h][1].x, w[i][h][1].y, w[i][h][1].z, w[i][h][1].w};
 #pragma unroll
           for (int j = 0; j < 4; ++j) {      // four codes a lane are 16 channels of the product
-            const uint32_t a[4] = {half2_of(w0[j] & 0xffffu, p.w.format), half2_of(w1[j] & 0xffffu, p.w.format), half2_of(w0[j] >> 16, p.w.format),
-                                   half2_of(w1[j] >> 16, p.w.format)};
+            const uint32_t a[4] = {half2_of<LF_FLOAT8_E4M3>(w0[j] & 0xffffu), half2_of<LF_FLOAT8_E4M3>(w1[j] & 0xffffu), half2_of<LF_FLOAT8_E4M3>(w0[j] >> 16),
+                                   half2_of<LF_FLOAT8_E4M3>(w1[j] >> 16)};
 #pragma unroll
             for (int e = 0; e < EIGHTS; ++e) {
               const uint32_t xw = j == 0 ? x[e].x : j == 1 ? x[e].y : j == 2 ? x[e].z : x[e].w;
-              mma_16x8x16(c[e], a, half2_of(xw & 0xffffu, p.x.format), half2_of(xw >> 16, p.x.format));
+              mma_16x8x16(c[e], a, half2_of<FORMAT>(xw & 0xffffu), half2_of<FORMAT>(xw >> 16));
             }
           }
         }
@@ -160,12 +156,21 @@ static int few_smem_bytes(int rows8, int k) { return rows8 * 8 * (blocks(k) * kB
 // Rows that the kernel takes: sixteen, and what their codes may have of shared memory.
 bool float8_few_takes(int64_t rows, int k) { return rows <= 16 && k <= 4096; }
 
+// f(T, EIGHTS, FORMAT as types)
+template <typename F>
+static void few_forms(int dtype, int eights, int format, F f) {
+  auto with = [&](auto t, auto e) {
+    if (format == LF_FLOAT8_E4M3) f(t, e, std::integral_constant<int, LF_FLOAT8_E4M3>{}); else f(t, e, std::integral_constant<int, LF_FLOAT8_E5M2>{});
+  };
+  auto typed = [&](auto t) { if (eights == 1) with(t, std::integral_constant<int, 1>{}); else with(t, std::integral_constant<int, 2>{}); };
+  if (dtype == LF_DTYPE_BF16) typed(bf16{}); else typed(float{});
+}
+
 void configure_float8_few() {
-  const int most = few_smem_bytes(2, 4096);
-  cudaFuncSetAttribute(float8_few_kernel<float, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
-  cudaFuncSetAttribute(float8_few_kernel<float, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
-  cudaFuncSetAttribute(float8_few_kernel<bf16, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
-  cudaFuncSetAttribute(float8_few_kernel<bf16, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+  for (int i = 0; i < 8; ++i)
+    few_forms(i & 1, 1 + (i >> 1 & 1), i >> 2, [](auto t, auto e, auto f) {
+      cudaFuncSetAttribute(float8_few_kernel<decltype(t), decltype(e)::value, decltype(f)::value>, cudaFuncAttributeMaxDynamicSharedMemorySize, few_smem_bytes(2, 4096));
+    });
 }
 
 // out = x . w^T + bias; `source` (dtype) or x's codes; x.codes, where set beside a source, receive its 8-bit form.
@@ -174,15 +179,11 @@ lf_status float8_few(lf_context* ctx, const void* source, int dtype, const Matri
   p.rows = (int)x.rows; p.n = (int)w.rows; p.k = x.channels; p.out_f32 = out_dtype == LF_DTYPE_F32;
   p.source = source; p.access = source ? row_access(source, x.channels, dtype) : 0;
   p.x = x; p.w = w; p.bias = bias; p.out = out;
-  const int grid = lf_ceil_div(p.n, FEW_OUT), eights = p.rows > 8 ? 2 : 1, smem = few_smem_bytes(eights, p.k);
+  const int eights = p.rows > 8 ? 2 : 1;
   lf_prof_begin(ctx, LF_KERNEL_SIMT);
-  if (dtype == LF_DTYPE_BF16) {
-    if (eights == 1) lf_launch(ctx, float8_few_kernel<bf16, 1>, grid, FEW_WARPS * 32, smem, p);
-    else lf_launch(ctx, float8_few_kernel<bf16, 2>, grid, FEW_WARPS * 32, smem, p);
-  } else {
-    if (eights == 1) lf_launch(ctx, float8_few_kernel<float, 1>, grid, FEW_WARPS * 32, smem, p);
-    else lf_launch(ctx, float8_few_kernel<float, 2>, grid, FEW_WARPS * 32, smem, p);
-  }
+  few_forms(dtype, eights, x.format, [&](auto t, auto e, auto f) {
+    lf_launch(ctx, float8_few_kernel<decltype(t), decltype(e)::value, decltype(f)::value>, lf_ceil_div(p.n, FEW_OUT), FEW_WARPS * 32, few_smem_bytes(eights, p.k), p);
+  });
   lf_prof_end(ctx);
   ctx->launches++;
   return LF_OK;

@@ -54,17 +54,21 @@ __device__ __forceinline__ uint32_t bf16x2_bits(float lo, float hi) {
 }
 
 // Sixteen neighbouring codes of one row -> two 16-byte pieces of bf16.
-__device__ __forceinline__ void convert16(uint4 codes, int s, int format, uint4 (&out)[2]) {
-  const uint32_t w[4] = {codes.x, codes.y, codes.z, codes.w};
+template <int FORMAT>
+__device__ __forceinline__ void convert16_as(uint4 codes, int s, uint4 (&out)[2]) {
+  const f8::Share v = f8::decode16_as<FORMAT>(codes);
+  const float2 factor = f8::both(f8::up(s));
   uint32_t o[8];
-  const float factor = f8::up(s);
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const float2 v = f8::decode2(w[i >> 1] >> (16 * (i & 1)) & 0xffffu, format);
-    o[i] = bf16x2_bits(v.x * factor, v.y * factor);
+    const float2 t = f8::mul2(v.v[i], factor);
+    o[i] = bf16x2_bits(t.x, t.y);
   }
   out[0] = make_uint4(o[0], o[1], o[2], o[3]);
   out[1] = make_uint4(o[4], o[5], o[6], o[7]);
+}
+__device__ __forceinline__ void convert16(uint4 codes, int s, int format, uint4 (&out)[2]) {
+  if (format == LF_FLOAT8_E4M3) convert16_as<LF_FLOAT8_E4M3>(codes, s, out); else convert16_as<LF_FLOAT8_E5M2>(codes, s, out);
 }
 
 // The place of a piece of eight columns in an MN-major operand: blocks of 64 columns, rows of 128 bytes, 128-byte swizzle.
@@ -138,31 +142,29 @@ float8_gradient_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_co
       }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      int slot = 0, stage = 0; uint32_t phase = 0, ring_phase = 0;
-      bool ok = true;
-      constexpr uint32_t both = (1u << 7) | (1u << 10);      // bf16 operands
-      const uint32_t idesc = make_idesc_f16(WG_BN, groups * 64, 1, 1) | both, idesc_ones = make_idesc_f16(WG_BN, 16, 1, 0) | both;
-      const uint64_t ones_desc = make_smem_desc_plain(smem_u32(ones), 128, 256);
-      for (int t = first; t < last; ++t) {
-        if (!mbar_wait(&full[slot], phase, abort_flag, p.status, 132) || (p.dy_mode == 0 && !mbar_wait(&loaded[stage], ring_phase, abort_flag, p.status, 136))) {
-          ok = false;
-          break;
-        }
-        tc_fence_after();
-        const uint32_t a0 = smem_u32(dy_s + (p.dy_mode == 0 ? stage : slot) * WG_A_BYTES), b0 = smem_u32(x_s + slot * WG_B_BYTES);
+    // (the whole warp walks and waits, so that what the instructions take stays in uniform registers; one lane issues)
+    int slot = 0, stage = 0; uint32_t phase = 0, ring_phase = 0;
+    constexpr uint32_t both = (1u << 7) | (1u << 10);      // bf16 operands
+    const uint32_t idesc = make_idesc_f16(WG_BN, groups * 64, 1, 1) | both, idesc_ones = make_idesc_f16(WG_BN, 16, 1, 0) | both;
+    const uint64_t ones_desc = make_smem_desc_plain(smem_u32(ones), 128, 256);
+    const uint64_t a_first = make_smem_desc(smem_u32(dy_s), WG_ROWS * 128, 1024), b_first = make_smem_desc(smem_u32(x_s), WG_ROWS * 128, 1024);
+    for (int t = first; t < last; ++t) {
+      if (!mbar_wait(&full[slot], phase, abort_flag, p.status, 132) || (p.dy_mode == 0 && !mbar_wait(&loaded[stage], ring_phase, abort_flag, p.status, 136))) break;
+      tc_fence_after();
+      if (elect_one()) {
+        const uint64_t a = a_first + (uint32_t)((p.dy_mode == 0 ? stage : slot) * (WG_A_BYTES >> 4)), b = b_first + (uint32_t)(slot * (WG_B_BYTES >> 4));
 #pragma unroll
         for (int kk = 0; kk < WG_ROWS / 16; ++kk) {
-          const uint64_t a = make_smem_desc(a0 + kk * 2048, WG_ROWS * 128, 1024);
-          umma_f16(tmem_base, a, make_smem_desc(b0 + kk * 2048, WG_ROWS * 128, 1024), idesc, (t != first || kk != 0) ? 1u : 0u);
-          if (sums) umma_f16(tmem_base + WG_BK, a, ones_desc, idesc_ones, (t != first || kk != 0) ? 1u : 0u);
+          umma_f16(tmem_base, a + kk * 128, b + kk * 128, idesc, (t != first || kk != 0) ? 1u : 0u);
+          if (sums) umma_f16(tmem_base + WG_BK, a + kk * 128, ones_desc, idesc_ones, (t != first || kk != 0) ? 1u : 0u);
         }
         umma_commit(&empty[slot]);
         if (p.dy_mode == 0) umma_commit(&taken[stage]);
-        if (++slot == WG_OPERANDS) { slot = 0; phase ^= 1; }
-        if (++stage == WG_RING) { stage = 0; ring_phase ^= 1; }
+        if (t + 1 == last) umma_commit(done);
       }
-      if (ok) umma_commit(done);
+      __syncwarp();
+      if (++slot == WG_OPERANDS) { slot = 0; phase ^= 1; }
+      if (++stage == WG_RING) { stage = 0; ring_phase ^= 1; }
     }
   } else {
     // Rows of a step: x has 16 pieces of 16 channels, dy 8 of 16 outputs; neighbouring lanes take neighbouring pieces of a row.

@@ -58,24 +58,23 @@ __device__ __forceinline__ void tmem_copy_scales(uint32_t taddr, uint64_t desc) 
 // A lane's 32 columns of its row, with the bias, into a staging tile of 32 rows of 128 bytes (128-byte swizzle): half a bf16 row, a whole float32 one.
 template <bool F32>
 __device__ __forceinline__ void stage_columns(uint8_t* stage, const float* bias, const uint32_t (&r)[32], int half, int lane) {
+  constexpr int kPiece = F32 ? 4 : 8;      // columns of 16 bytes
 #pragma unroll
-  for (int c = 0; c < (F32 ? 8 : 4); ++c) {
-    uint4 w;
-    if (F32) {
-      const float4 b = *reinterpret_cast<const float4*>(bias + c * 4);
-      w = make_uint4(__float_as_uint(__uint_as_float(r[(c * 4) % 32]) + b.x), __float_as_uint(__uint_as_float(r[(c * 4 + 1) % 32]) + b.y),
-                     __float_as_uint(__uint_as_float(r[(c * 4 + 2) % 32]) + b.z), __float_as_uint(__uint_as_float(r[(c * 4 + 3) % 32]) + b.w));
-    } else {
-      uint32_t u[4];
+  for (int c = 0; c < 32; c += kPiece) {
+    uint32_t w[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float2 b = *reinterpret_cast<const float2*>(bias + c * 8 + e * 2);
-        const __nv_bfloat162 two = __floats2bfloat162_rn(__uint_as_float(r[(c * 8 + e * 2) % 32]) + b.x, __uint_as_float(r[(c * 8 + e * 2 + 1) % 32]) + b.y);
-        u[e] = *reinterpret_cast<const uint32_t*>(&two);
+    for (int e = 0; e < kPiece; e += 4) {
+      const float4 b = *reinterpret_cast<const float4*>(bias + c + e);
+      const float2 x = add2(make_float2(__uint_as_float(r[c + e]), __uint_as_float(r[c + e + 1])), make_float2(b.x, b.y));
+      const float2 y = add2(make_float2(__uint_as_float(r[c + e + 2]), __uint_as_float(r[c + e + 3])), make_float2(b.z, b.w));
+      if (F32) { w[0] = __float_as_uint(x.x); w[1] = __float_as_uint(x.y); w[2] = __float_as_uint(y.x); w[3] = __float_as_uint(y.y); }
+      else {
+        const __nv_bfloat162 p0 = __floats2bfloat162_rn(x.x, x.y), p1 = __floats2bfloat162_rn(y.x, y.y);
+        w[e / 2] = *reinterpret_cast<const uint32_t*>(&p0);
+        w[e / 2 + 1] = *reinterpret_cast<const uint32_t*>(&p1);
       }
-      w = make_uint4(u[0], u[1], u[2], u[3]);
     }
-    *reinterpret_cast<uint4*>(stage + swizzle128_offset(lane, F32 ? c : half * 4 + c)) = w;
+    *reinterpret_cast<uint4*>(stage + swizzle128_offset(lane, F32 ? c / 4 : half * 4 + c / 8)) = make_uint4(w[0], w[1], w[2], w[3]);
   }
 }
 // The staged rows to columns from c0 on of rows from row0 on (the whole warp): by TMA, or, where no 16-byte access divides the rows, a row after the other.
@@ -181,39 +180,44 @@ float8_linear_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_cons
       }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      int stage = 0; uint32_t phase = 0, it = 0, group = 0;
-      bool ok = true;
-      for (int t = blockIdx.x; t < total && ok; t += gridDim.x, ++it) {
-        const int nj = t % tiles_n;
-        const int left = p.n - nj * BN, columns = left >= BN ? BN : (left + 15) / 16 * 16;
-        const uint32_t acc = it % S::accumulators;
-        if (!mbar_wait(&tmem_empty[acc], ((it / S::accumulators) & 1) ^ 1, abort_flag, p.status, 122)) break;
+    // The whole warp walks and waits and one lane issues, so that the instructions' operands stay in uniform registers (4096 x 4096 x 4096: 58 us, by one lane's
+    // branch 64).
+    const uint64_t a_first = make_smem_desc(smem_u32(smem), 16, 1024), b_first = make_smem_desc(smem_u32(smem) + F8_A_BYTES, 16, 1024);
+    const uint64_t scale_first = make_smem_desc_plain(smem_u32(scale_s), 0, 128);
+    int stage = 0; uint32_t phase = 0, it = 0, group = 0;
+    bool ok = true;
+    for (int t = blockIdx.x; t < total && ok; t += gridDim.x, ++it) {
+      const int nj = t % tiles_n;
+      const int left = p.n - nj * BN, columns = left >= BN ? BN : (left + 15) / 16 * 16;
+      const uint32_t acc = it % S::accumulators;
+      if (!mbar_wait(&tmem_empty[acc], ((it / S::accumulators) & 1) ^ 1, abort_flag, p.status, 122)) break;
+      tc_fence_after();
+      const uint32_t d = tmem_base + acc * BN;
+      const uint32_t idesc = make_idesc_f8(F8_BM, columns, p.formats & 1, p.formats >> 1, 0);
+      uint32_t scales = 0;
+      for (int kb = 0; kb < kblocks; ++kb) {
+        if (!mbar_wait(&full[stage], phase, abort_flag, p.status, 123)) { ok = false; break; }
         tc_fence_after();
-        const uint32_t d = tmem_base + acc * BN;
-        uint32_t scales = 0;
-        for (int kb = 0; kb < kblocks; ++kb) {
-          if (!mbar_wait(&full[stage], phase, abort_flag, p.status, 123)) { ok = false; break; }
-          tc_fence_after();
-          const uint32_t a0 = smem_u32(smem + stage * S::stage), b0 = a0 + F8_A_BYTES;
+        const uint64_t a = a_first + (uint32_t)(stage * S::stage >> 4), b = b_first + (uint32_t)(stage * S::stage >> 4);
+        // Four slots in turn: when a group's first step is here, the step `stages` <= 6 before it is complete, and with it
+        // the group before last; the slot's last reader is four groups back.
+        if ((kb & 3) == 0) scales = tmem_base + 256 + (group++ & 3) * 16;
+        if (elect_one()) {
           if ((kb & 3) == 0) {
-            // Four slots in turn: when a group's first step is here, the step `stages` <= 6 before it is complete, and with it
-            // the group before last; the slot's last reader is four groups back.
-            scales = tmem_base + 256 + (group++ & 3) * 16;
-            const uint32_t sc = smem_u32(scale_s + stage * S::scales);
-            tmem_copy_scales(scales, make_smem_desc_plain(sc, 0, 128));
-            tmem_copy_scales(scales + 8, make_smem_desc_plain(sc + 512, 0, 128));
-            if (BN == 256 && columns > 128) tmem_copy_scales(scales + 12, make_smem_desc_plain(sc + 1024, 0, 128));
+            const uint64_t sc = scale_first + (uint32_t)(stage * S::scales >> 4);
+            tmem_copy_scales(scales, sc);
+            tmem_copy_scales(scales + 8, sc + 32);
+            if (BN == 256 && columns > 128) tmem_copy_scales(scales + 12, sc + 64);
           }
-          const uint32_t idesc = make_idesc_f8(F8_BM, columns, p.formats & 1, p.formats >> 1, kb & 3);
 #pragma unroll
           for (int kk = 0; kk < F8_BK / 32; ++kk)
-            umma_f8_scaled(d, make_smem_desc(a0 + kk * 32, 16, 1024), make_smem_desc(b0 + kk * 32, 16, 1024), idesc, scales,
-                           scales + 8 + (BN == 64 ? 2u * (nj & 1) : 0u), (kb | kk) != 0 ? 1u : 0u);
+            umma_f8_scaled(d, a + kk * 2, b + kk * 2, idesc | (kb & 3) << 4 | (kb & 3) << 29, scales, scales + 8 + (BN == 64 ? 2u * (nj & 1) : 0u),
+                           (kb | kk) != 0 ? 1u : 0u);
           umma_commit(&empty[stage]);
-          if (++stage == S::stages) { stage = 0; phase ^= 1; }
+          if (kb + 1 == kblocks) umma_commit(&tmem_full[acc]);
         }
-        if (ok) umma_commit(&tmem_full[acc]);
+        __syncwarp();
+        if (++stage == S::stages) { stage = 0; phase ^= 1; }
       }
     }
   } else {
@@ -270,234 +274,21 @@ float8_linear_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_cons
   if (warp == 1) { tc_fence_after(); tmem_dealloc(tmem_base, 512); }
 }
 
-// The same product with the encoder in front of it, for rows of at most 512 channels: sixteen warps turn 128 rows of x into a block of codes a
-// time, straight into the tensor core's operand (and, where the codes are kept, to memory), so that x is read once and its codes are never read
-// back.  A block's codes serve all of the item's column tiles; w stays in shared memory where the range's tiles fit its ring (128 -> 512 and 512 -> 128
-// channels do).  Work item: 128 rows and a range of column tiles of 128; three accumulators.
-// (147456 x 128 -> 512, bf16: encoder 12.5 us and product 29.8 us apart.)
-// Warp roles: 0 = w's TMA producer, 1 = MMA issuer (owns TMEM), 2..17 = encoder, 18..25 = epilogue, 64 columns of a lane quadrant each.
-constexpr int FU_BN = 128, FU_A = 5, FU_B = 4, FU_ACC = 3, FU_ENCODE = 16, FU_EPI = 8;
-constexpr int FU_THREADS = 64 + 32 * (FU_ENCODE + FU_EPI), FU_B_BYTES = FU_BN * F8_BK;
-constexpr int FU_ROOM = f8::kRoom * 4;
-constexpr int FU_SMEM = FU_A * (F8_A_BYTES + 512) + FU_B * (FU_B_BYTES + 512) + FU_EPI * (4096 + 256) + FU_ENCODE * FU_ROOM + 256 + 1024;
-constexpr int FU_MOST = 4;           // blocks of 128 channels
-
-struct FusedParams {
-  int m, n, k, ranges, per_range;    // column tiles in `ranges` ranges of per_range
-  int vector_out, access;
-  const void* source;
-  const float* bias;
-  const uint8_t* ew;
-  int64_t ew_tiles;
-  f8::Matrix keep;                   // codes null: not kept; its format
-  int w_e5m2;
-  void* out;
-  Status* status;
-};
-
-template <typename T, bool F32>
-__global__ void __launch_bounds__(FU_THREADS, 1)
-float8_fused_kernel(const __grid_constant__ CUtensorMap mapB, const __grid_constant__ CUtensorMap mapO, const FusedParams p) {
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* a_s = align_shared(smem_raw);
-  uint8_t* b_s = a_s + FU_A * F8_A_BYTES;
-  uint8_t* out_stage = b_s + FU_B * FU_B_BYTES;
-  uint8_t* a_scales = out_stage + FU_EPI * 4096;
-  uint8_t* b_scales = a_scales + FU_A * 512;
-  float* rooms = reinterpret_cast<float*>(b_scales + FU_B * 512);
-  float* bias_s = rooms + FU_ENCODE * f8::kRoom;
-  uint64_t* a_full = reinterpret_cast<uint64_t*>(bias_s + FU_EPI * 64);
-  uint64_t* a_empty = a_full + FU_A;
-  uint64_t* b_full = a_empty + FU_A;
-  uint64_t* b_empty = b_full + FU_B;
-  uint64_t* tmem_full = b_empty + FU_B;
-  uint64_t* tmem_empty = tmem_full + FU_ACC;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tmem_empty + FU_ACC);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int tiles_n = (p.n + FU_BN - 1) / FU_BN, kblocks = (p.k + F8_BK - 1) / F8_BK;
-  const int items = (p.m + F8_BM - 1) / F8_BM * p.ranges;
-  const bool resident = p.per_range * kblocks <= FU_B && p.ranges == 1;
-
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < FU_A; ++s) { mbar_init(&a_full[s], FU_ENCODE); mbar_init(&a_empty[s], 1); }
-    for (int s = 0; s < FU_B; ++s) { mbar_init(&b_full[s], 1); mbar_init(&b_empty[s], 1); }
-    for (int b = 0; b < FU_ACC; ++b) { mbar_init(&tmem_full[b], 1); mbar_init(&tmem_empty[b], FU_EPI); }
-    *abort_flag = 0;
-    fence_barrier_init();
-  }
-  if (warp == 1) { tmem_alloc(tmem_slot, 512); tmem_relinquish(); }
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem_base = *tmem_slot;
-  lf_chain();
-
-  if (warp == 0) {
-    if (lane == 0) {
-      prefetch_tensormap(&mapB);
-      int stage = 0; uint32_t phase = 0;
-      bool ok = true;
-      for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
-        if (resident && item != (int)blockIdx.x) break;
-        const int n_first = item % p.ranges * p.per_range, n_last = min(n_first + p.per_range, tiles_n);
-        for (int nj = n_first; nj < n_last && ok; ++nj)
-          for (int kb = 0; kb < kblocks; ++kb) {
-            if (!mbar_wait(&b_empty[stage], phase ^ 1, abort_flag, p.status, 141)) { ok = false; break; }
-            mbar_expect_tx(&b_full[stage], FU_B_BYTES + (kb == 0 ? 512 : 0));
-            tma_load_3d(b_s + stage * FU_B_BYTES, &mapB, &b_full[stage], kb * F8_BK, nj * FU_BN, 0);
-            if (kb == 0) bulk_load(b_scales + stage * 512, p.ew + (int64_t)nj * 512, 512, &b_full[stage]);
-            if (++stage == FU_B) { stage = 0; phase ^= 1; }
-          }
-      }
-    }
-  } else if (warp == 1) {
-    if (lane == 0) {
-      int stage = 0, slot = 0; uint32_t phase = 0, a_phase = 0, it = 0, blocks = 0;
-      bool ok = true, first = true;
-      for (int item = blockIdx.x; item < items && ok; item += gridDim.x, first = false) {
-        const int n_first = item % p.ranges * p.per_range, n_last = min(n_first + p.per_range, tiles_n);
-        if (resident) { stage = 0; phase = 0; }
-        int held = slot; uint32_t held_phase = a_phase;
-        for (int nj = n_first; nj < n_last && ok; ++nj, ++it) {
-          const int left = p.n - nj * FU_BN, columns = left >= FU_BN ? FU_BN : (left + 15) / 16 * 16;
-          const uint32_t acc = it % FU_ACC, d = tmem_base + acc * FU_BN;
-          if (!mbar_wait(&tmem_empty[acc], ((it / FU_ACC) & 1) ^ 1, abort_flag, p.status, 142)) { ok = false; break; }
-          tc_fence_after();
-          // Scales: w's of a tile in four slots in turn (three accumulators: the slot's last reader is complete), x's of a block in eight (the ring
-          // has five blocks); x's stay for all of the item's tiles.
-          const uint32_t w_scales = tmem_base + FU_ACC * FU_BN + (it & 3) * 4;
-          held = slot; held_phase = a_phase;
-          for (int kb = 0; kb < kblocks; ++kb) {
-            if (nj == n_first && !mbar_wait(&a_full[held], held_phase, abort_flag, p.status, 143)) { ok = false; break; }
-            if ((!resident || first) && !mbar_wait(&b_full[stage], phase, abort_flag, p.status, 144)) { ok = false; break; }
-            tc_fence_after();
-            const uint32_t x_scales = tmem_base + FU_ACC * FU_BN + 16 + ((blocks + kb) & 7) * 4;
-            if (nj == n_first) tmem_copy_scales(x_scales, make_smem_desc_plain(smem_u32(a_scales + held * 512), 0, 128));
-            if (kb == 0) tmem_copy_scales(w_scales, make_smem_desc_plain(smem_u32(b_scales + stage * 512), 0, 128));
-            const uint32_t a0 = smem_u32(a_s + held * F8_A_BYTES), b0 = smem_u32(b_s + stage * FU_B_BYTES);
-            // a word of x's scales holds one byte four times, w's the bytes of four blocks
-            const uint32_t idesc = make_idesc_f8(F8_BM, columns, p.keep.format, p.w_e5m2, 0) | ((uint32_t)kb << 4);
-#pragma unroll
-            for (int kk = 0; kk < F8_BK / 32; ++kk)
-              umma_f8_scaled(d, make_smem_desc(a0 + kk * 32, 16, 1024), make_smem_desc(b0 + kk * 32, 16, 1024), idesc, x_scales, w_scales, (kb | kk) != 0 ? 1u : 0u);
-            if (!resident) umma_commit(&b_empty[stage]);
-            if (nj + 1 == n_last) umma_commit(&a_empty[held]);
-            if (++stage == FU_B) { stage = 0; phase ^= 1; }
-            if (++held == FU_A) { held = 0; held_phase ^= 1; }
-          }
-          if (ok) umma_commit(&tmem_full[acc]);
-        }
-        slot = held; a_phase = held_phase;
-        blocks += kblocks;
-      }
-    }
-  } else if (warp < 2 + FU_ENCODE) {
-    const int thread = threadIdx.x - 64, l8 = thread & 7, r0 = thread >> 3;      // rows r0 and r0 + 64 of the tile
-    float* room = rooms + (warp - 2) * f8::kRoom;
-    f8::Raw<T> raw[2];
-    auto fetch = [&](int item, int kb) {
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int64_t row = (int64_t)(item / p.ranges) * F8_BM + r0 + 64 * u;
-        const int first = kb * F8_BK + l8 * f8::kShare;
-        f8::load16<T, 8>(raw[u], static_cast<const T*>(p.source) + row * p.k + first, p.k - first, row < p.m, p.access);
-      }
-    };
-    int slot = 0; uint32_t phase = 0;
-    bool ok = true;
-    if ((int)blockIdx.x < items) fetch(blockIdx.x, 0);
-    for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
-      const bool keep = p.keep.codes && item % p.ranges == 0;
-      for (int kb = 0; kb < kblocks; ++kb) {
-        uint4 codes[2];
-        int s[2];
-#pragma unroll
-        for (int u = 0; u < 2; ++u) s[u] = f8::encode16<8>(f8::unpack<T, 8>(raw[u], p.access, room), p.keep.format, codes[u]);
-        if (kb + 1 < kblocks) fetch(item, kb + 1);
-        else if (item + (int)gridDim.x < items) fetch(item + gridDim.x, 0);
-        if (!mbar_wait(&a_empty[slot], phase ^ 1, abort_flag, p.status, 145)) { ok = false; break; }
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const int r = r0 + 64 * u;
-          *reinterpret_cast<uint4*>(a_s + slot * F8_A_BYTES + swizzle128_offset(r, l8)) = codes[u];
-          if (l8 == 0) *reinterpret_cast<uint32_t*>(a_scales + slot * 512 + (r & 31) * 16 + (r >> 5) * 4) = 0x01010101u * (uint32_t)s[u];
-          const int64_t row = (int64_t)(item / p.ranges) * F8_BM + r;
-          if (keep && row < p.m) f8::put16(p.keep, row, kb * F8_BK + l8 * f8::kShare, codes[u], s[u]);
-        }
-        fence_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&a_full[slot]);
-        if (++slot == FU_A) { slot = 0; phase ^= 1; }
-      }
-    }
-  } else {
-    const int e = warp - 2 - FU_ENCODE, q = warp & 3, part = e >> 2;      // TMEM lane quadrant, 64 of the tile's columns
-    uint8_t* stage = out_stage + e * 4096;
-    float* bias = bias_s + e * 64;
-    uint32_t it = 0;
-    int held = -1;
-    bool ok = true;
-    if (lane == 0 && p.vector_out) prefetch_tensormap(&mapO);
-    for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
-      const int n_first = item % p.ranges * p.per_range, n_last = min(n_first + p.per_range, tiles_n);
-      for (int nj = n_first; nj < n_last; ++nj, ++it) {
-        const int col0 = nj * FU_BN + part * 64, row0 = item / p.ranges * F8_BM + q * 32;
-        const bool mine = col0 < p.n && row0 < p.m;
-        if (mine && held != col0) {
-          held = col0;
-          __syncwarp();
-#pragma unroll
-          for (int c = 0; c < 64; c += 32) bias[c + lane] = p.bias && col0 + c + lane < p.n ? p.bias[col0 + c + lane] : 0.f;
-          __syncwarp();
-        }
-        const uint32_t acc = it % FU_ACC;
-        if (!mbar_wait(&tmem_full[acc], (it / FU_ACC) & 1, abort_flag, p.status, 146)) { ok = false; break; }
-        tc_fence_after();
-        if (mine) {
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            uint32_t r[32];
-            tmem_ld32(tmem_base + ((uint32_t)(q * 32) << 16) + acc * FU_BN + part * 64 + half * 32, r);
-            if (F32 || half == 0) {
-              if (lane == 0) bulk_wait_read();      // the previous copy has read the staging rows
-              __syncwarp();
-            }
-            tmem_ld_wait();
-            tie32(r);
-            stage_columns<F32>(stage, bias + half * 32, r, half, lane);
-            if (F32 || half == 1) {
-              const int c0 = col0 + (F32 ? half * 32 : 0);
-              if (!F32 || c0 < p.n) send_columns<F32>(stage, &mapO, p.vector_out, p.out, c0, row0, p.m, p.n, lane);
-            }
-          }
-        }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&tmem_empty[acc]);
-      }
-    }
-    if (lane == 0) bulk_wait_all();      // this thread's stores have landed
-  }
-
-  tc_fence_before();
-  __syncthreads();
-  if (*abort_flag) drain_after_abort();
-  if (warp == 1) { tc_fence_after(); tmem_dealloc(tmem_base, 512); }
+// f(BN, F32 as types)
+template <typename F>
+static void linear_forms(int bn, bool f32, F f) {
+  auto with = [&](auto b) { if (f32) f(b, std::true_type{}); else f(b, std::false_type{}); };
+  if (bn == 256) with(std::integral_constant<int, 256>{});
+  else if (bn == 128) with(std::integral_constant<int, 128>{});
+  else with(std::integral_constant<int, 64>{});
 }
 
 void configure_float8_linear() {
-  cudaFuncSetAttribute(float8_linear_kernel<256, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, Float8Shape<256>::smem);
-  cudaFuncSetAttribute(float8_linear_kernel<256, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, Float8Shape<256>::smem);
-  cudaFuncSetAttribute(float8_linear_kernel<128, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, Float8Shape<128>::smem);
-  cudaFuncSetAttribute(float8_linear_kernel<128, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, Float8Shape<128>::smem);
-  cudaFuncSetAttribute(float8_linear_kernel<64, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, Float8Shape<64>::smem);
-  cudaFuncSetAttribute(float8_linear_kernel<64, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, Float8Shape<64>::smem);
-  cudaFuncSetAttribute(float8_fused_kernel<bf16, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, FU_SMEM);
-  cudaFuncSetAttribute(float8_fused_kernel<bf16, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, FU_SMEM);
-  cudaFuncSetAttribute(float8_fused_kernel<float, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, FU_SMEM);
-  cudaFuncSetAttribute(float8_fused_kernel<float, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, FU_SMEM);
+  for (int i = 0; i < 6; ++i)
+    linear_forms(64 << i % 3, i / 3, [](auto bn, auto f32) {
+      constexpr int BN = decltype(bn)::value;
+      cudaFuncSetAttribute(float8_linear_kernel<BN, decltype(f32)::value>, cudaFuncAttributeMaxDynamicSharedMemorySize, Float8Shape<BN>::smem);
+    });
   configure_float8_few();
 }
 
@@ -516,40 +307,15 @@ static lf_status launch_float8(lf_context* ctx, const f8::Matrix& x, const f8::M
   return LF_OK;
 }
 
-template <typename T, bool F32>
-static lf_status launch_fused(lf_context* ctx, const f8::Matrix& w, FusedParams p) {
-  CUtensorMap mb, mo{};
-  LF_TRY(make_map_bytes(ctx, &mb, w.codes, w.channels, w.rows, w.pitch, FU_BN));
-  if (p.vector_out) LF_TRY(make_map_rows(ctx, &mo, p.out, F32, p.n, p.m, 32));
-  // Ranges of column tiles: rows alone where there are enough of them, else the fewest ranges (each encodes its rows again) that shorten the longest
-  // block's work by a tenth.
-  const int tiles_m = (p.m + F8_BM - 1) / F8_BM, tiles_n = (p.n + FU_BN - 1) / FU_BN;
-  int64_t best = INT64_MAX;
-  for (int ranges = 1; ranges <= tiles_n && ranges <= 64; ++ranges) {
-    const int per = (tiles_n + ranges - 1) / ranges, used = (tiles_n + per - 1) / per;
-    const int64_t work = (int64_t)(((int64_t)tiles_m * used + ctx->sm_count - 1) / ctx->sm_count) * (per + 1);      // (a tile's encoding is worth about one product)
-    if (best == INT64_MAX || work * 10 <= best * 9) { best = work; p.ranges = used; p.per_range = per; }
-  }
-  const int64_t items = (int64_t)tiles_m * p.ranges;
-  lf_prof_begin(ctx, LF_KERNEL_LN_GEMM);
-  lf_launch(ctx, float8_fused_kernel<T, F32>, (int)(items < ctx->sm_count ? items : ctx->sm_count), FU_THREADS, FU_SMEM, mb, mo, p);
-  lf_prof_end(ctx);
-  ctx->launches++;
-  return LF_OK;
-}
-
 }  // namespace tc
 
 using namespace f8;
 
-// Which kernel takes a product: by its sizes alone.
-//   few rows: one launch that reads the weights at full width (4 x 1536 -> 384: 8.9 us in two launches)
-//   a source of at most 512 channels: encoder and product in one kernel
-//   else: the encoder, then the tiled product
-static bool encodes_itself(int64_t rows, int channels) { return tc::float8_few_takes(rows, channels) || channels <= tc::FU_MOST * kBlock; }
-
+// Which kernel takes a product: few rows one launch that reads the weights at full width (4 x 1536 -> 384: 4.2 us; encoder and tiled product 2.2 + 6.7), else
+// the encoder, then the tiled product.  (One kernel that encoded its rows on the way into the tiled product was slower than the two: with registers for 16
+// encoding warps a multiprocessor hides too little of their latency, 147456 x 128 -> 512 took 40 us or more.)
 extern "C" uint64_t lf_float8_linear_workspace(int64_t rows, int32_t channels) {
-  if (rows <= 0 || channels <= 0 || encodes_itself(rows, channels)) return 0;
+  if (rows <= 0 || channels <= 0 || tc::float8_few_takes(rows, channels)) return 0;
   return lf_float8_code_bytes(rows, channels) + lf_float8_exponent_bytes(rows, channels);
 }
 
@@ -578,18 +344,6 @@ extern "C" lf_status lf_float8_linear_run(lf_context* ctx, const lf_float8_linea
   }
   const bool f32 = d->out_dtype == LF_DTYPE_F32;
   const int vector_out = lf_aligned16(d->out) && w.rows % (f32 ? 4 : 8) == 0;
-  if (d->source && encodes_itself(x.rows, x.channels)) {
-    tc::FusedParams p{};
-    p.m = (int)x.rows; p.n = (int)w.rows; p.k = x.channels;
-    p.vector_out = vector_out; p.access = row_access(d->source, x.channels, d->source_dtype);
-    p.source = d->source; p.bias = d->bias; p.ew = mw.exponents; p.ew_tiles = mw.tiles; p.keep = mx;
-    p.w_e5m2 = w.format == LF_FLOAT8_E5M2;
-    p.out = d->out;
-    p.status = (tc05::Status*)ctx->tc_status;
-    if (d->source_dtype == LF_DTYPE_BF16) LF_TRY(f32 ? (tc::launch_fused<bf16, true>(ctx, mw, p)) : (tc::launch_fused<bf16, false>(ctx, mw, p)));
-    else LF_TRY(f32 ? (tc::launch_fused<float, true>(ctx, mw, p)) : (tc::launch_fused<float, false>(ctx, mw, p)));
-    return lf_float8_done(ctx, r, 1);
-  }
   int launches = 1;
   if (d->source) {
     lf_float8_encode_desc e{};
@@ -611,8 +365,10 @@ extern "C" lf_status lf_float8_linear_run(lf_context* ctx, const lf_float8_linea
   p.status = (tc05::Status*)ctx->tc_status;
   const int64_t rows = mx.tiles;
   const int bn = rows * ((p.n + 255) / 256) >= ctx->sm_count && p.n > 128 ? 256 : rows * ((p.n + 127) / 128) >= ctx->sm_count && p.n > 64 ? 128 : 64;
-  if (bn == 256) LF_TRY(f32 ? (tc::launch_float8<256, true>(ctx, mx, mw, p)) : (tc::launch_float8<256, false>(ctx, mx, mw, p)));
-  else if (bn == 128) LF_TRY(f32 ? (tc::launch_float8<128, true>(ctx, mx, mw, p)) : (tc::launch_float8<128, false>(ctx, mx, mw, p)));
-  else LF_TRY(f32 ? (tc::launch_float8<64, true>(ctx, mx, mw, p)) : (tc::launch_float8<64, false>(ctx, mx, mw, p)));
+  lf_status status = LF_OK;
+  tc::linear_forms(bn, f32, [&](auto b, auto o) {
+    status = tc::launch_float8<decltype(b)::value, decltype(o)::value>(ctx, mx, mw, p);
+  });
+  LF_TRY(status);
   return lf_float8_done(ctx, r, launches);
 }
