@@ -237,10 +237,7 @@ def load():
                        ("lf_single_attention_run", SingleAttentionDesc), ("lf_msa_attention_run", MsaAttentionDesc),
                        ("lf_global_column_attention_run", GlobalAttentionDesc),
                        ("lf_distogram_logits_run", DistogramDesc), ("lf_pair_stack_run", PairStackDesc),
-                       ("lf_pair_shard_step", ShardStepDesc), ("lf_float8_encode", Float8EncodeDesc),
-                       ("lf_float8_decode", Float8DecodeDesc), ("lf_layer_norm_run", LayerNormDesc),
-                       ("lf_layer_norm_backward_run", LayerNormBackwardDesc), ("lf_float8_linear_run", Float8LinearDesc),
-                       ("lf_float8_weight_gradient_run", Float8WeightGradientDesc)):
+                       ("lf_pair_shard_step", ShardStepDesc)):
         getattr(lib, name).argtypes = [c_void_p, ctypes.POINTER(desc), ctypes.POINTER(Result)]
     lib.lf_pair_stack_run_from.argtypes = [c_void_p, ctypes.POINTER(PairStackDesc), c_void_p, ctypes.POINTER(Result)]
     lib.lf_pair_shard_exchange_step.argtypes = [c_void_p, ctypes.POINTER(ShardStepDesc), ctypes.POINTER(ShardPeers),
@@ -252,6 +249,9 @@ def load():
     lib.lf_peer_buffer_destroy.argtypes = [c_void_p, c_void_p]
     lib.lf_pair_transpose_scatter.argtypes = [c_void_p, c_void_p, c_int32, c_int32, c_int32, c_int32, c_int32,
                                               ctypes.POINTER(c_void_p)]
+    for name in ("lf_float8_encode", "lf_float8_decode", "lf_layer_norm_run", "lf_layer_norm_backward_run", "lf_float8_linear_run",
+                 "lf_float8_weight_gradient_run"):      # descriptors are structures (by reference) or their bytes
+        getattr(lib, name).argtypes = [c_void_p, c_void_p, ctypes.POINTER(Result)]
     for name, args in (("lf_float8_code_bytes", [c_int64, c_int32]), ("lf_float8_linear_workspace", [c_int64, c_int32]), ("lf_float8_exponent_bytes", [c_int64, c_int32]),
                        ("lf_layer_norm_backward_workspace", [c_void_p, c_int64, c_int32]),
                        ("lf_float8_weight_gradient_workspace", [c_void_p, c_int64, c_int32, c_int32])):

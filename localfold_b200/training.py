@@ -18,6 +18,7 @@ allocator, so a call can be captured into a CUDA graph (on the stream that the `
 from __future__ import annotations
 
 import math
+import struct
 
 import numpy as np
 
@@ -27,7 +28,18 @@ from .operators import Device, EncodedTensor, _device, _positive, _torch_stream,
 
 _FORMAT = {"e4m3": nat.FLOAT8_E4M3, "e5m2": nat.FLOAT8_E5M2}
 _DTYPE = {"f32": nat.DTYPE_F32, "bf16": nat.DTYPE_BF16}
-_NO_MATRIX = nat.Float8Matrix()
+
+# The descriptors (the ctypes structures of the same names), packed: small calls take a few microseconds, of which filling a structure
+# field by field was one.  A matrix is its five fields.
+_MATRIX = "qiiQQ"
+_ENCODE = struct.Struct("@" + 2 * _MATRIX + "iiQ")
+_DECODE = struct.Struct("@" + _MATRIX + "iiQ")
+_LAYER_NORM = struct.Struct("@qiiif6Q" + 2 * _MATRIX)
+_LAYER_NORM_BACKWARD = struct.Struct("@qiiQQ" + _MATRIX + "8Q")
+_LINEAR = struct.Struct("@" + 2 * _MATRIX + "QiiQQQQ")
+_WEIGHT_GRADIENT = struct.Struct("@" + _MATRIX + "Q" + _MATRIX + "ii4Q")
+_NO_MATRIX = (0, 0, 0, 0, 0)
+_NO_OPTIONS = {}
 
 
 def _format(value, name="format"):
@@ -36,15 +48,12 @@ def _format(value, name="format"):
     return value
 
 
-def _shape(inp, *names):
-    values = []
-    for name in names:
-        value = inp[name]
-        if type(value) is not int or value <= 0:
-            _positive(name, value)
-            value = int(value)
-        values.append(value)
-    return values
+def _size(inp, name):
+    value = inp[name]
+    if type(value) is not int or value <= 0:
+        _positive(name, value)
+        value = int(value)
+    return value
 
 
 _names = {}      # torch dtype -> "f32" | "bf16"
@@ -60,12 +69,17 @@ def _torch():
 def _tensor(device, name, value, count, only=None):
     """A tensor argument: on the device's GPU, contiguous, float32 or bfloat16 (``only``: one of them), of ``count`` values.
     Returns "f32" or "bf16"."""
+    if getattr(value, "is_cuda", False) and value.get_device() == device.ordinal:
+        dtype = _names.get(value.dtype)
+        if dtype is not None and (only is None or only == dtype) and value.numel() == count and value.is_contiguous():
+            return dtype
     if not getattr(value, "is_cuda", False):
         raise ValueError(f"{name} must be a CUDA tensor")
     if value.get_device() != device.ordinal:
         raise ValueError(f"{name} is on {value.device}, the device's GPU is cuda:{device.ordinal}")
-    dtype = (_names or (_torch(), _names)[1]).get(value.dtype)
-    if dtype is None or (only is not None and dtype != only):
+    _torch()
+    dtype = _names.get(value.dtype)
+    if dtype is None or only not in (None, dtype):
         raise ValueError(f"{name} must be {only or 'f32 or bf16'}; received {value.dtype}")
     if not value.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
@@ -101,7 +115,17 @@ def _call(device, function, desc, tensors, output=None):
 
 def _sizes(rows, channels):
     """Bytes of the codes and of the exponents (``lf_float8_code_bytes``, ``lf_float8_exponent_bytes``)."""
-    return rows * ((channels + 15) // 16 * 16), (channels + 511) // 512 * ((rows + 127) // 128) * 512
+    return rows * ((channels + 15) & -16), ((channels + 511) >> 9) * ((rows + 127) >> 7) * 512
+
+
+_bytes = {}      # GPU -> an empty uint8 tensor there: new memory of that kind takes least time from one
+
+
+def _new_bytes(like, nbytes):
+    proto = _bytes.get(like.get_device())
+    if proto is None:
+        proto = _bytes[like.get_device()] = like.new_empty(0, dtype=_torch().uint8)
+    return proto.new_empty(nbytes)
 
 
 class Float8Tensor:
@@ -117,11 +141,12 @@ class Float8Tensor:
         if memory.numel() != self._codes + exponents:
             raise RangeError(f"memory has {memory.numel()} values; expected {self._codes + exponents}")
         base = memory.data_ptr()
-        self.desc = nat.Float8Matrix(rows, channels, _FORMAT[format], base, base + self._codes)
+        self.fields = (rows, channels, _FORMAT[format], base, base + self._codes)
 
     @classmethod
     def empty(cls, rows, channels, format, like):
-        return cls(rows, channels, format, like.new_empty(sum(_sizes(rows, channels)), dtype=_torch().uint8))
+        codes, exponents = _sizes(rows, channels)
+        return cls(rows, channels, format, _new_bytes(like, codes + exponents))
 
     @property
     def nbytes(self):
@@ -149,7 +174,7 @@ def _matrix(device, name, value, rows, channels):
 
 
 def _encode(device, source, dtype, out, block_rows=1, transposed=None):
-    desc = nat.Float8EncodeDesc(out.desc, transposed.desc if transposed is not None else _NO_MATRIX, _DTYPE[dtype], block_rows, source.data_ptr())
+    desc = _ENCODE.pack(*out.fields, *(transposed.fields if transposed is not None else _NO_MATRIX), _DTYPE[dtype], block_rows, source.data_ptr())
     _call(device, device.lib.lf_float8_encode, desc, (source, out, transposed))
 
 
@@ -157,8 +182,9 @@ def float8_encode(device, activations, rows, channels, options=None):
     """The 8-bit form of ``activations`` ``[rows][channels]`` (float32 or bfloat16).  ``options``: format "e4m3" (default) or "e5m2"
     (more range, less precision: gradients)."""
     dev = _device(device)
-    rows, channels = _shape({"rows": rows, "channels": channels}, "rows", "channels")
-    format = _format((options or {}).get("format", "e4m3"))
+    shape = {"rows": rows, "channels": channels}
+    rows, channels = _size(shape, "rows"), _size(shape, "channels")
+    format = _format((options or _NO_OPTIONS).get("format", "e4m3"))
     dtype = _tensor(dev, "activations", activations, rows * channels)
     out = Float8Tensor.empty(rows, channels, format, activations)
     _encode(dev, activations, dtype, out)
@@ -177,12 +203,12 @@ def float8_decode(device, encoded, options=None, out=None):
         out = encoded.memory.new_empty((encoded.rows, encoded.channels), dtype=_torch_dtype(dtype))
     else:
         _tensor(dev, "out", out, encoded.rows * encoded.channels, dtype)
-    _call(dev, dev.lib.lf_float8_decode, nat.Float8DecodeDesc(encoded.desc, _DTYPE[dtype], 0, out.data_ptr()), (encoded, out))
+    _call(dev, dev.lib.lf_float8_decode, _DECODE.pack(*encoded.fields, _DTYPE[dtype], 0, out.data_ptr()), (encoded, out))
     return out
 
 
 def _output(options, default):
-    value = (options or {}).get("output") or default
+    value = (options or _NO_OPTIONS).get("output") or default
     if value not in _DTYPE:
         raise ValueError(f'output must be "f32" or "bf16"; received {value!r}')
     return value
@@ -200,13 +226,13 @@ class LayerNormGpu:
         ``[rows]`` for ``backward``; checkpoint "e4m3" | "e5m2" - those and the input's 8-bit form as ``checkpoint``; encode "e4m3" |
         "e5m2" - the output is a ``Float8Tensor``, the operand of a ``Float8LinearGpu``; variance "two-pass" | "fast" (two passes
         either way).  ``out`` may be the activations."""
-        dev, opts = self.device, options or {}
-        rows, c = _shape(input, "rows", "channels")
+        dev, opts = self.device, options or _NO_OPTIONS
+        rows, c = _size(input, "rows"), _size(input, "channels")
         x, scale, offset = input["activations"], input["scale"], input["offset"]
         epsilon = input.get("epsilon", 1e-5)
         if not epsilon > 0 or not math.isfinite(epsilon):
             raise RangeError(f"epsilon must be finite and positive; received {epsilon}")
-        variance = _variance(opts, "two-pass")
+        variance = _variance(opts, "two-pass") if opts else nat.VARIANCE_TWO_PASS
         kept, encode = opts.get("checkpoint"), opts.get("encode")
         kept = None if kept is None else _format(kept, "checkpoint")
         encode = None if encode is None else _format(encode, "encode")
@@ -221,14 +247,15 @@ class LayerNormGpu:
             out = _torch().empty_like(x)
         checkpoint = Float8Tensor.empty(rows, c, kept, x) if kept else None
         encoded = Float8Tensor.empty(rows, c, encode, x) if encode else None
-        statistics = scale.new_empty((2, rows)) if kept or opts.get("statistics") else None
-        mean = statistics.data_ptr() if statistics is not None else None
-        desc = nat.LayerNormDesc(rows, c, variance, _DTYPE[dtype], epsilon, x.data_ptr(), scale.data_ptr(), offset.data_ptr(),
-                                 out.data_ptr() if out is not None else None, mean, mean and mean + 4 * rows,
-                                 checkpoint.desc if kept else _NO_MATRIX, encoded.desc if encode else _NO_MATRIX)
-        result = _call(dev, dev.lib.lf_layer_norm_run, desc, (x, scale, offset, out, statistics, checkpoint, encoded), encoded if encode else out)
-        if statistics is not None:
-            result["mean"], result["inverseDeviation"] = statistics.unbind(0)
+        mean = inverse = None
+        if kept or opts.get("statistics"):
+            mean, inverse = scale.new_empty(rows), scale.new_empty(rows)
+        desc = _LAYER_NORM.pack(rows, c, variance, _DTYPE[dtype], epsilon, x.data_ptr(), scale.data_ptr(), offset.data_ptr(),
+                                out.data_ptr() if out is not None else 0, 0 if mean is None else mean.data_ptr(), 0 if mean is None else inverse.data_ptr(),
+                                *(checkpoint.fields if kept else _NO_MATRIX), *(encoded.fields if encode else _NO_MATRIX))
+        result = _call(dev, dev.lib.lf_layer_norm_run, desc, (x, scale, offset, out, mean, inverse, checkpoint, encoded), encoded if encode else out)
+        if mean is not None:
+            result["mean"], result["inverseDeviation"] = mean, inverse
         if kept:
             result["checkpoint"] = checkpoint
         return result
@@ -239,32 +266,28 @@ class LayerNormGpu:
         gradient's type; ``out`` may be the gradient itself), ``scale`` and ``offset`` (float32).  The sums over the rows have a
         fixed order: the same call gives the same bits."""
         dev = self.device
-        rows, c = _shape(input, "rows", "channels")
-        dy, x, scale = input["gradient"], input["activations"], input["scale"]
+        rows, c = _size(input, "rows"), _size(input, "channels")
+        dy, x, scale, mean, inverse = input["gradient"], input["activations"], input["scale"], input["mean"], input["inverseDeviation"]
         dtype = _tensor(dev, "gradient", dy, rows * c)
         encoded = isinstance(x, Float8Tensor)
         if encoded:
             _matrix(dev, "activations", x, rows, c)
         else:
             _tensor(dev, "activations", x, rows * c, dtype)
-        _tensor(dev, "mean", input["mean"], rows, "f32")
-        _tensor(dev, "inverseDeviation", input["inverseDeviation"], rows, "f32")
+        _tensor(dev, "mean", mean, rows, "f32")
+        _tensor(dev, "inverseDeviation", inverse, rows, "f32")
         _tensor(dev, "scale", scale, c, "f32")
         if out is not None:
             _tensor(dev, "out", out, rows * c, dtype)
         else:
             out = _torch().empty_like(dy)
         nbytes = dev.lib.lf_layer_norm_backward_workspace(dev.handle, rows, c)
-        # the two weights' gradients, then the workspace on a 16-byte boundary
-        ahead = (2 * c + 3) // 4 * 4
-        memory = scale.new_empty(ahead + nbytes // 4)
-        base = memory.data_ptr()
-        desc = nat.LayerNormBackwardDesc(rows, c, _DTYPE[dtype], dy.data_ptr(), None if encoded else x.data_ptr(),
-                                         x.desc if encoded else _NO_MATRIX, input["mean"].data_ptr(), input["inverseDeviation"].data_ptr(),
-                                         scale.data_ptr(), out.data_ptr(), base, base + 4 * c, base + 4 * ahead, nbytes)
-        result = _call(dev, dev.lib.lf_layer_norm_backward_run, desc, (dy, x, input["mean"], input["inverseDeviation"], scale, out, memory), out)
+        dscale, doffset, workspace = scale.new_empty(c), scale.new_empty(c), _new_bytes(scale, nbytes)
+        desc = _LAYER_NORM_BACKWARD.pack(rows, c, _DTYPE[dtype], dy.data_ptr(), 0 if encoded else x.data_ptr(), *(x.fields if encoded else _NO_MATRIX),
+                                         mean.data_ptr(), inverse.data_ptr(), scale.data_ptr(), out.data_ptr(), dscale.data_ptr(), doffset.data_ptr(), workspace.data_ptr(), nbytes)
+        result = _call(dev, dev.lib.lf_layer_norm_backward_run, desc, (dy, x, mean, inverse, scale, out, dscale, doffset, workspace), out)
         result["activations"] = result.pop("output")
-        result["scale"], result["offset"] = memory[:c], memory[c:2 * c]
+        result["scale"], result["offset"] = dscale, doffset
         return result
 
 
@@ -297,7 +320,7 @@ class Float8LinearWeights:
     def update(self, weight, bias=None):
         """New values (float32 or bfloat16 CUDA tensors or host arrays).  The bias tensor is used as it is at every call."""
         weight, bias = self._on_device(weight), self._on_device(bias)
-        if tuple(weight.shape) != (self.out_channels, self.channels):
+        if weight.shape != (self.out_channels, self.channels):
             raise RangeError(f"weight is {tuple(weight.shape)}; expected {(self.out_channels, self.channels)}")
         dtype = _tensor(self.device, "weight", weight, self.out_channels * self.channels)
         if bias is not None:
@@ -322,7 +345,7 @@ class Float8LinearGpu:
         self.device = _device(device)
 
     def _product(self, name, value, rows, channels, weights, bias, options, out):
-        dev, opts = self.device, options or {}
+        dev, opts = self.device, options or _NO_OPTIONS
         keep, source, operand, workspace, nbytes = bool(opts.get("checkpoint")), None, None, None, 0
         format = _format(opts.get("format", "e4m3"))
         if isinstance(value, Float8Tensor):
@@ -334,21 +357,21 @@ class Float8LinearGpu:
                 operand = Float8Tensor.empty(rows, channels, format, value)
             else:
                 nbytes = dev.lib.lf_float8_linear_workspace(rows, channels)
-                workspace = weights.memory.new_empty(nbytes) if nbytes else None
+                workspace = _new_bytes(value, nbytes) if nbytes else None
         if out is not None:
             _tensor(dev, "out", out, rows * weights.rows, dtype)
         else:
             out = weights.memory.new_empty((rows, weights.rows), dtype=_torch_dtype(dtype))
-        desc = nat.Float8LinearDesc(operand.desc if operand is not None else nat.Float8Matrix(rows, channels, _FORMAT[format]), weights.desc,
-                                    bias.data_ptr() if bias is not None else None, _DTYPE[dtype], _DTYPE[source or "f32"],
-                                    value.data_ptr() if source else None, out.data_ptr(), workspace.data_ptr() if nbytes else None, nbytes)
+        desc = _LINEAR.pack(*(operand.fields if operand is not None else (rows, channels, _FORMAT[format], 0, 0)), *weights.fields,
+                            bias.data_ptr() if bias is not None else 0, _DTYPE[dtype], _DTYPE[source or "f32"], value.data_ptr() if source else 0,
+                            out.data_ptr(), workspace.data_ptr() if nbytes else 0, nbytes)
         result = _call(dev, dev.lib.lf_float8_linear_run, desc, (value, operand, weights, bias, workspace, out), out)
         if keep:
             result["checkpoint"] = operand
         return result
 
     def _weights(self, input):
-        rows, channels, n = _shape(input, "rows", "channels", "outChannels")
+        rows, channels, n = _size(input, "rows"), _size(input, "channels"), _size(input, "outChannels")
         weights = input["weights"]
         if not isinstance(weights, Float8LinearWeights):
             raise ValueError("weights must come from prepare_float8_linear_weights")
@@ -374,7 +397,7 @@ class Float8LinearGpu:
         encoded first, ``float8_encode``), activations (the ``Float8Tensor`` that the forward pass multiplied with) -> ``weight``
         ``[outChannels][channels]`` and ``bias`` ``[outChannels]``, float32, the same bits at every call."""
         dev = self.device
-        rows, channels, n = _shape(input, "rows", "channels", "outChannels")
+        rows, channels, n = _size(input, "rows"), _size(input, "channels"), _size(input, "outChannels")
         dy, x = input["gradient"], _matrix(dev, "activations", input["activations"], rows, channels)
         encoded = isinstance(dy, Float8Tensor)
         if encoded:
@@ -383,13 +406,10 @@ class Float8LinearGpu:
             _tensor(dev, "gradient", dy, rows * n, "bf16")
         nbytes = dev.lib.lf_float8_weight_gradient_workspace(dev.handle, rows, channels, n)
         weight = x.memory.new_empty((n, channels), dtype=_torch().float32)
-        # the bias' gradient, then the workspace on a 16-byte boundary
-        ahead = (n + 3) // 4 * 4
-        memory = weight.new_empty(ahead + nbytes // 4)
-        base = memory.data_ptr()
-        desc = nat.Float8WeightGradientDesc(x.desc, None if encoded else dy.data_ptr(), dy.desc if encoded else _NO_MATRIX, n, 0, weight.data_ptr(), base,
-                                            base + 4 * ahead, nbytes)
-        result = _call(dev, dev.lib.lf_float8_weight_gradient_run, desc, (dy, x, weight, memory), weight)
+        bias, workspace = weight.new_empty(n), _new_bytes(weight, nbytes) if nbytes else None
+        desc = _WEIGHT_GRADIENT.pack(*x.fields, 0 if encoded else dy.data_ptr(), *(dy.fields if encoded else _NO_MATRIX), n, 0, weight.data_ptr(), bias.data_ptr(),
+                                     workspace.data_ptr() if nbytes else 0, nbytes)
+        result = _call(dev, dev.lib.lf_float8_weight_gradient_run, desc, (dy, x, weight, bias, workspace), weight)
         result["weight"] = result.pop("output")
-        result["bias"] = memory[:n]
+        result["bias"] = bias
         return result
