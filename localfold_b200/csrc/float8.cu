@@ -73,14 +73,19 @@ decode_kernel(const Matrix m, T* out, uint32_t units, uint32_t per_row, int how)
 
 // One 128 x 128 block a block of threads: its largest magnitude, its codes in rows, and (t.codes set) the same codes with rows and
 // channels exchanged - the exponent is the block's, so the transposed matrix stands for the same values.
-template <typename T>
-__global__ void __launch_bounds__(kThreads)
-encode_square_kernel(const T* x, const Matrix m, const Matrix t, int access) {
-  __shared__ float most_s[2][kThreads / 32];
-  __shared__ __align__(16) uint8_t turned[kBlock][kBlock + 16];
-  constexpr int kRows = kBlock * 8 / kThreads;      // of a thread
-  __shared__ __align__(16) float rooms[kThreads / 32][kRoom];
-  float* room = rooms[threadIdx.x >> 5];
+// (1024 threads of sixteen elements: 512 x 128 took 5.8 us with 256 of 64.  Element by element 512, for what their rooms take of shared memory.)
+__host__ __device__ constexpr int square_threads(bool elements) { return elements ? 512 : 1024; }
+template <typename T, bool ELEMENTS>
+__global__ void __launch_bounds__(square_threads(ELEMENTS))
+encode_square_kernel(const T* x, const Matrix m, const Matrix t, int how) {
+  constexpr int kSquareThreads = square_threads(ELEMENTS), kTurned = kBlock * kBlock, kRooms = ELEMENTS ? kSquareThreads / 32 * kRoom * 4 : 0;
+  const int access = ELEMENTS ? (int)kElements : max(how, (int)kSixteen);
+  __shared__ __align__(16) uint8_t shared_s[kTurned > kRooms ? kTurned : kRooms];      // the warps' rooms, then the codes on their way to the other orientation
+  __shared__ float most_s[2][kSquareThreads / 32];
+  // (channel ch's byte of row r; pieces of sixteen rows are exchanged by the channel, so that eight lanes' bytes lie in different banks)
+  auto turned_at = [&](int ch, int r) { return shared_s + ch * kBlock + (r ^ (ch & 0x70)); };
+  constexpr int kRows = kBlock * 8 / kSquareThreads;      // of a thread
+  float* room = reinterpret_cast<float*>(shared_s) + (ELEMENTS ? threadIdx.x >> 5 : 0) * kRoom;
   const int lane = threadIdx.x & 7, strand = threadIdx.x >> 3;
   const int64_t row0 = (int64_t)blockIdx.y * kBlock;
   const int first = blockIdx.x * kBlock + lane * kShare;
@@ -88,7 +93,7 @@ encode_square_kernel(const T* x, const Matrix m, const Matrix t, int access) {
   Raw<T> raw[kRows];
 #pragma unroll
   for (int k = 0; k < kRows; ++k) {
-    const int64_t row = row0 + strand + kThreads / 8 * k;
+    const int64_t row = row0 + strand + kSquareThreads / 8 * k;
     load16<T, 8>(raw[k], x + row * m.channels + first, m.channels - first, row < m.rows, access);
   }
   float most = 0.f, finite = 0.f;
@@ -104,17 +109,17 @@ encode_square_kernel(const T* x, const Matrix m, const Matrix t, int access) {
   if ((threadIdx.x & 31) == 0) { most_s[0][threadIdx.x >> 5] = most; most_s[1][threadIdx.x >> 5] = finite; }
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < kThreads / 32; ++w) { most = fmaxf(most, most_s[0][w]); finite = fmaxf(finite, most_s[1][w]); }
+  for (int w = 0; w < kSquareThreads / 32; ++w) { most = fmaxf(most, most_s[0][w]); finite = fmaxf(finite, most_s[1][w]); }
   const int s = exponent_byte(__float_as_uint(finite), m.format);
 #pragma unroll
   for (int k = 0; k < kRows; ++k) {
-    const int64_t row = row0 + strand + kThreads / 8 * k;
+    const int64_t row = row0 + strand + kSquareThreads / 8 * k;
     const uint4 codes = code16(v[k], s, m.format, most == kInfinity);
     if (row < m.rows && first < m.channels) *reinterpret_cast<uint4*>(m.codes + row * m.pitch + first) = codes;
     if (t.codes) {
       const uint32_t w[4] = {codes.x, codes.y, codes.z, codes.w};
 #pragma unroll
-      for (int i = 0; i < kShare; ++i) turned[lane * kShare + i][strand + kThreads / 8 * k] = (uint8_t)(w[i >> 2] >> (8 * (i & 3)));
+      for (int i = 0; i < kShare; ++i) *turned_at(lane * kShare + i, strand + kSquareThreads / 8 * k) = (uint8_t)(w[i >> 2] >> (8 * (i & 3)));
     }
   }
   if (threadIdx.x < kBlock) m.exponents[exponent_at(row0 + threadIdx.x, blockIdx.x, m.tiles)] = (uint8_t)s;
@@ -124,9 +129,9 @@ encode_square_kernel(const T* x, const Matrix m, const Matrix t, int access) {
   const int tfirst = blockIdx.y * kBlock + lane * kShare;
 #pragma unroll
   for (int k = 0; k < kRows; ++k) {
-    const int64_t row = trow0 + strand + kThreads / 8 * k;
+    const int64_t row = trow0 + strand + kSquareThreads / 8 * k;
     if (row < t.rows && tfirst < t.channels)
-      *reinterpret_cast<uint4*>(t.codes + row * t.pitch + tfirst) = *reinterpret_cast<const uint4*>(&turned[strand + kThreads / 8 * k][lane * kShare]);
+      *reinterpret_cast<uint4*>(t.codes + row * t.pitch + tfirst) = *reinterpret_cast<const uint4*>(turned_at(strand + kSquareThreads / 8 * k, lane * kShare));
   }
   if (threadIdx.x < kBlock) t.exponents[exponent_at(trow0 + threadIdx.x, blockIdx.y, t.tiles)] = (uint8_t)s;
 }
@@ -192,11 +197,16 @@ lf_status lf_float8_encode(lf_context* ctx, const lf_float8_encode_desc* d, lf_r
   const int access = row_access(d->source, o.channels, d->dtype);
   lf_prof_begin(ctx, LF_KERNEL_ELEMENTWISE);
   if (d->block_rows == kBlock) {
-    Matrix t{};
-    if (turned) t = matrix(d->transposed);
+    Matrix t8{};
+    if (turned) t8 = matrix(d->transposed);
     const dim3 grid(blocks(o.channels), (unsigned)row_tiles(o.rows));
-    if (d->dtype == LF_DTYPE_BF16) lf_launch(ctx, encode_square_kernel<bf16>, grid, kThreads, 0, (const bf16*)d->source, m, t, access);
-    else lf_launch(ctx, encode_square_kernel<float>, grid, kThreads, 0, (const float*)d->source, m, t, access);
+    auto run = [&](auto t, auto elements) {
+      typedef decltype(t) T;
+      constexpr bool E = decltype(elements)::value;
+      lf_launch(ctx, encode_square_kernel<T, E>, grid, square_threads(E), 0, (const T*)d->source, m, t8, access);
+    };
+    auto typed = [&](auto t) { if (access == kElements) run(t, std::true_type{}); else run(t, std::false_type{}); };
+    if (d->dtype == LF_DTYPE_BF16) typed(bf16{}); else typed(float{});
   } else {
     const uint32_t per_row = blocks(o.channels), units = (uint32_t)(o.rows * per_row);
     row_forms(d->dtype, o.channels, access, [&](auto t, auto lanes, auto elements) {

@@ -33,7 +33,7 @@ constexpr int WG_THREADS = 64 + 32 * WG_CONVERT;
 // [ring of dy: four bf16 operands, or two that are converted and four times its codes][ring of x's codes][x's operands][exponents][ones]
 constexpr int WG_DY = WG_RING * WG_A_BYTES, WG_EXPONENTS = 2 * 512;
 constexpr int WG_SMEM = WG_DY + WG_RING * (WG_CODES + WG_EXPONENTS) + WG_OPERANDS * WG_B_BYTES + 512 + 256 + 1024;
-static_assert(WG_OPERANDS * WG_A_BYTES + WG_RING * WG_DY_CODES <= WG_DY && WG_CONVERT * 4096 <= WG_DY, "");
+static_assert(WG_OPERANDS * WG_A_BYTES + WG_RING * WG_DY_CODES <= WG_DY && WG_CONVERT * 8192 <= WG_DY + WG_RING * WG_CODES, "");
 
 struct GradientParams {
   int m, n, k;
@@ -242,7 +242,7 @@ float8_gradient_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_co
     tc_fence_after();
     if (ok) {
       const int q = warp & 3, part = (warp - 2) >> 2, row0 = n0 + q * 32, col0 = k0 + part * 64;
-      uint8_t* tile = dy_s + (warp - 2) * 4096;      // (every product is done: dy's ring is free)
+      uint8_t* tiles = dy_s + (warp - 2) * 8192;      // (every product is done: the rings of dy and of x's codes are free)
       float* out = p.out + split * p.split_stride;
       if (row0 < p.n && col0 < p.k) {
         uint32_t r[2][32];
@@ -256,8 +256,7 @@ float8_gradient_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_co
         for (int half = 0; half < 2; ++half) {
           const int c0 = col0 + half * 32;
           if (c0 >= p.k) break;
-          if (lane == 0) bulk_wait_read();
-          __syncwarp();
+          uint8_t* tile = tiles + half * 4096;
 #pragma unroll
           for (int c = 0; c < 8; ++c)
             *reinterpret_cast<uint4*>(tile + lane * 128 + ((c ^ (lane & 7)) << 4)) = make_uint4(r[half][c * 4], r[half][c * 4 + 1], r[half][c * 4 + 2], r[half][c * 4 + 3]);

@@ -363,8 +363,14 @@ extern "C" lf_status lf_float8_linear_run(lf_context* ctx, const lf_float8_linea
   p.formats = (x.format == LF_FLOAT8_E5M2) | (w.format == LF_FLOAT8_E5M2) << 1;
   p.out = d->out;
   p.status = (tc05::Status*)ctx->tc_status;
-  const int64_t rows = mx.tiles;
-  const int bn = rows * ((p.n + 255) / 256) >= ctx->sm_count && p.n > 128 ? 256 : rows * ((p.n + 127) / 128) >= ctx->sm_count && p.n > 64 ? 128 : 64;
+  // The tile width whose longest block is done first: a tile costs about its columns and 64 more (3001 x 449 -> 1283: 256 wide in one turn of the blocks, where 128
+  // takes two; 3001 x 1283 -> 449: 128 wide).
+  int bn = 0;
+  int64_t best = 0;
+  for (int width = 64; width <= 256; width *= 2) {
+    const int64_t turns = (mx.tiles * ((p.n + width - 1) / width) + ctx->sm_count - 1) / ctx->sm_count, work = turns * (width + 64);
+    if (bn == 0 || work < best) { bn = width; best = work; }
+  }
   lf_status status = LF_OK;
   tc::linear_forms(bn, f32, [&](auto b, auto o) {
     status = tc::launch_float8<decltype(b)::value, decltype(o)::value>(ctx, mx, mw, p);

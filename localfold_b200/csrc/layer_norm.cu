@@ -148,16 +148,16 @@ backward_kernel(const Backward a) {
   int64_t row = (int64_t)blockIdx.x * kGroups + group;
   Raw<T> raw_dy, raw_x;
   uint4 codes;
-  float factor, mean, inverse;
+  int power = 1;      // (a byte as it is loaded: what has to wait for it waits when the row's turn comes)
+  float mean, inverse;
   auto fetch = [&](int64_t r) {      // (a row that does not exist is all zeros)
     const bool live = r < a.rows;
     load16<T, kWarp>(raw_dy, static_cast<const T*>(a.dy) + r * a.c + first, left, live, a.access_dy);
     codes = make_uint4(0, 0, 0, 0);
-    factor = 0.f;
     if (!KEPT) load16<T, kWarp>(raw_x, static_cast<const T*>(a.x) + r * a.c + first, left, live, a.access_x);
     else if (live && left > 0) {
       codes = *reinterpret_cast<const uint4*>(a.kept.codes + r * a.kept.pitch + first);
-      factor = up(a.kept.exponents[exponent_at(r, first / kBlock, a.kept.tiles)]);
+      power = a.kept.exponents[exponent_at(r, first / kBlock, a.kept.tiles)];
     }
     mean = live ? a.mean[r] : 0.f;
     inverse = live ? a.inverse[r] : 0.f;
@@ -173,7 +173,7 @@ backward_kernel(const Backward a) {
     Share u = KEPT ? decode16(codes, a.kept.format) : unpack<T, kWarp>(raw_x, a.access_x, room);
     const float inv = inverse;
     // (x - mean) rstd; of codes by one multiply-add, their power of two with rstd
-    const float2 by = both(KEPT ? factor * inv : inv), from = both(KEPT ? -mean * inv : -mean);
+    const float2 by = both(KEPT ? up(power) * inv : inv), from = both(KEPT ? -mean * inv : -mean);
 #pragma unroll
     for (int i = 0; i < kShare / 2; ++i) u.v[i] = KEPT ? fma2(u.v[i], by, from) : mul2(add2(u.v[i], from), by);
     fetch(row + step);
