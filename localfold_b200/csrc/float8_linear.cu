@@ -16,7 +16,7 @@ namespace tc {
 using namespace tc05;
 
 lf_status make_map_bytes(lf_context* ctx, CUtensorMap* map, const void* base, uint64_t width, uint64_t rows, uint64_t pitch, uint32_t box_rows);
-lf_status make_map_rows(lf_context* ctx, CUtensorMap* map, const void* base, bool f32, uint64_t width, uint64_t rows, uint32_t box_rows);
+lf_status make_map_rows(lf_context* ctx, CUtensorMap* map, const void* base, bool f32, uint64_t width, uint64_t rows, uint32_t box_rows, bool narrow = false);
 
 void configure_float8_few();
 bool float8_few_takes(int64_t rows, int k);
@@ -24,6 +24,7 @@ lf_status float8_few(lf_context* ctx, const void* source, int dtype, const f8::M
 
 constexpr int F8_BM = 128, F8_BK = 128;      // a k step is a block of the format, and a row of it 128 bytes of shared memory
 constexpr int F8_A_BYTES = F8_BM * F8_BK;
+constexpr int F8_DEEP = 1024;                // channels from which the deeper ring pays
 
 struct Float8Params {
   int m, n, k;
@@ -55,12 +56,17 @@ __device__ __forceinline__ void tmem_copy_scales(uint32_t taddr, uint64_t desc) 
   asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
 }
 
-// A lane's 32 columns of its row, with the bias, into a staging tile of 32 rows of 128 bytes (128-byte swizzle): half a bf16 row, a whole float32 one.
-template <bool F32>
-__device__ __forceinline__ void stage_columns(uint8_t* stage, const float* bias, const uint32_t (&r)[32], int half, int lane) {
+// Staging tiles of 32 rows: of 128 bytes (128-byte swizzle) or, NARROW, 64 (64-byte swizzle).
+template <bool NARROW>
+__device__ __forceinline__ uint32_t staged_at(int row, int piece) {
+  return NARROW ? row * 64 + ((piece ^ (row >> 1 & 3)) << 4) : swizzle128_offset(row, piece);
+}
+// COUNT of a lane's columns of its row, with the bias, to the tile's pieces from `piece` on.
+template <bool F32, bool NARROW, int COUNT>
+__device__ __forceinline__ void stage_columns(uint8_t* stage, const float* bias, const uint32_t* r, int piece, int lane) {
   constexpr int kPiece = F32 ? 4 : 8;      // columns of 16 bytes
 #pragma unroll
-  for (int c = 0; c < 32; c += kPiece) {
+  for (int c = 0; c < COUNT; c += kPiece) {
     uint32_t w[4];
 #pragma unroll
     for (int e = 0; e < kPiece; e += 4) {
@@ -74,12 +80,13 @@ __device__ __forceinline__ void stage_columns(uint8_t* stage, const float* bias,
         w[e / 2 + 1] = *reinterpret_cast<const uint32_t*>(&p1);
       }
     }
-    *reinterpret_cast<uint4*>(stage + swizzle128_offset(lane, F32 ? c / 4 : half * 4 + c / 8)) = make_uint4(w[0], w[1], w[2], w[3]);
+    *reinterpret_cast<uint4*>(stage + staged_at<NARROW>(lane, piece + c / kPiece)) = make_uint4(w[0], w[1], w[2], w[3]);
   }
 }
 // The staged rows to columns from c0 on of rows from row0 on (the whole warp): by TMA, or, where no 16-byte access divides the rows, a row after the other.
-template <bool F32>
+template <bool F32, bool NARROW>
 __device__ __forceinline__ void send_columns(const uint8_t* stage, const CUtensorMap* map, int vector_out, void* out, int c0, int row0, int m, int n, int lane) {
+  constexpr int kColumns = (F32 ? 32 : 64) >> NARROW, kPiece = F32 ? 4 : 8;
   if (vector_out) {
     fence_async_smem();
     __syncwarp();
@@ -90,12 +97,14 @@ __device__ __forceinline__ void send_columns(const uint8_t* stage, const CUtenso
   const int rows = min(32, m - row0);
   for (int row = 0; row < rows; ++row) {
     const int64_t at = (int64_t)(row0 + row) * n;
-    if (F32) {
-      if (c0 + lane < n) static_cast<float*>(out)[at + c0 + lane] = *reinterpret_cast<const float*>(stage + swizzle128_offset(row, lane >> 2) + (lane & 3) * 4);
-    } else {
 #pragma unroll
-      for (int e = 0; e < 64; e += 32)
-        if (c0 + e + lane < n) static_cast<bf16*>(out)[at + c0 + e + lane] = *reinterpret_cast<const bf16*>(stage + swizzle128_offset(row, (e + lane) >> 3) + (lane & 7) * 2);
+    for (int e = 0; e < kColumns; e += 32) {
+      const int c = e + lane;
+      if (c < kColumns && c0 + c < n) {
+        const uint8_t* from = stage + staged_at<NARROW>(row, c / kPiece);
+        if (F32) static_cast<float*>(out)[at + c0 + c] = *reinterpret_cast<const float*>(from + c % kPiece * 4);
+        else static_cast<bf16*>(out)[at + c0 + c] = *reinterpret_cast<const bf16*>(from + c % kPiece * 2);
+      }
     }
   }
   __syncwarp();
@@ -106,28 +115,30 @@ __device__ __forceinline__ void send_columns(const uint8_t* stage, const CUtenso
 // of 256 columns has no second one beside it and the scales (512 columns in all): the epilogue's warps take their shares into registers with
 // one wait and hand it back, so that the next tile's products run under the stores.  Narrower tiles have two.
 // Warp roles: 0 = TMA producer, 1 = MMA issuer (owns TMEM), 2.. = epilogue, 64 columns of a lane quadrant each.
-template <int BN>
+// DEEP (256 columns, many channels): three steps on their way leave the tensor core waiting a fifth of its time; a fourth takes the room of the wide staging
+// tiles, and the epilogue, which then has a long main loop to hide under, has eight warps of 128 columns and tiles of 64-byte rows.
+template <int BN, bool DEEP>
 struct Float8Shape {
-  static constexpr int stages = BN == 256 ? 3 : BN == 128 ? 5 : 6;
+  static constexpr int stages = DEEP ? 4 : BN == 256 ? 3 : BN == 128 ? 5 : 6;
   static constexpr int b_bytes = BN * F8_BK, stage = F8_A_BYTES + b_bytes;
   static constexpr int b_tiles = (BN + 127) / 128, scales = 512 * (1 + b_tiles);
   static constexpr int accumulators = BN == 256 ? 1 : 2;
-  static constexpr int parts = BN / 64, epi = 4 * parts;
+  static constexpr int share = DEEP ? 128 : 64, epi = 4 * (BN / share), staging = DEEP ? 2048 : 4096;
   static constexpr int threads = 64 + 32 * epi;
-  static constexpr int smem = stages * (stage + scales) + epi * (4096 + 256) + 256 + 1024;
+  static constexpr int smem = stages * (stage + scales) + epi * (staging + share * 4) + 256 + 1024;
 };
 
-template <int BN, bool F32>
-__global__ void __launch_bounds__(Float8Shape<BN>::threads, 1)
+template <int BN, bool F32, bool DEEP>
+__global__ void __launch_bounds__(Float8Shape<BN, DEEP>::threads, 1)
 float8_linear_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant__ CUtensorMap mapB, const __grid_constant__ CUtensorMap mapO,
                      const Float8Params p) {
-  using S = Float8Shape<BN>;
+  using S = Float8Shape<BN, DEEP>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = align_shared(smem_raw);
   uint8_t* out_stage = smem + S::stages * S::stage;
-  uint8_t* scale_s = out_stage + S::epi * 4096;
+  uint8_t* scale_s = out_stage + S::epi * S::staging;
   float* bias_s = reinterpret_cast<float*>(scale_s + S::stages * S::scales);
-  uint64_t* bars = reinterpret_cast<uint64_t*>(bias_s + S::epi * 64);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(bias_s + S::epi * S::share);
   uint64_t* full = bars;
   uint64_t* empty = full + S::stages;
   uint64_t* tmem_full = empty + S::stages;
@@ -222,47 +233,49 @@ float8_linear_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_cons
     }
   } else {
     const int q = warp & 3, part = (warp - 2) >> 2;      // TMEM lane quadrant, 64 of the tile's columns
-    uint8_t* stage = out_stage + (warp - 2) * 4096;
-    float* bias = bias_s + (warp - 2) * 64;
+    uint8_t* stage = out_stage + (warp - 2) * S::staging;
+    float* bias = bias_s + (warp - 2) * S::share;
     uint32_t it = 0;
     int held = -1;      // first column of the bias share in shared memory
     if (lane == 0 && p.vector_out) prefetch_tensormap(&mapO);
     for (int t = blockIdx.x; t < total; t += gridDim.x, ++it) {
       const int mi = t / tiles_n, nj = t - mi * tiles_n;
-      const int col0 = nj * BN + part * 64, row0 = mi * F8_BM + q * 32;
+      const int col0 = nj * BN + part * S::share, row0 = mi * F8_BM + q * 32;
       const bool mine = col0 < p.n && row0 < p.m;
       if (mine && held != col0) {
         held = col0;
         __syncwarp();
 #pragma unroll
-        for (int e = 0; e < 64; e += 32) bias[e + lane] = p.bias && col0 + e + lane < p.n ? p.bias[col0 + e + lane] : 0.f;
+        for (int e = 0; e < S::share; e += 32) bias[e + lane] = p.bias && col0 + e + lane < p.n ? p.bias[col0 + e + lane] : 0.f;
         __syncwarp();
       }
       const uint32_t acc = it % S::accumulators;
       if (!mbar_wait(&tmem_full[acc], (it / S::accumulators) & 1, abort_flag, p.status, 124)) break;
       tc_fence_after();
-      uint32_t r[2][32];
+      uint32_t r[S::share / 32][32];
       if (mine) {
-        const uint32_t d = tmem_base + ((uint32_t)(q * 32) << 16) + acc * BN + part * 64;
-        tmem_ld32(d, r[0]);
-        tmem_ld32(d + 32, r[1]);
+        const uint32_t d = tmem_base + ((uint32_t)(q * 32) << 16) + acc * BN + part * S::share;
+#pragma unroll
+        for (int i = 0; i < S::share / 32; ++i) tmem_ld32(d + i * 32, r[i]);
         tmem_ld_wait();
-        tie32(r[0]);
-        tie32(r[1]);
+#pragma unroll
+        for (int i = 0; i < S::share / 32; ++i) tie32(r[i]);
       }
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&tmem_empty[acc]);      // the share is in registers: the accumulator may be overwritten
       if (!mine) continue;
+      constexpr int kSend = (F32 ? 32 : 64) >> DEEP, kStage = kSend < 32 ? kSend : 32;      // columns of a staging tile, and staged at a time
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        if (F32 || half == 0) {
+      for (int c = 0; c < S::share; c += kStage) {
+        const int within = c % kSend, c0 = col0 + c - within;
+        if (c0 >= p.n) break;
+        if (within == 0) {
           if (lane == 0) bulk_wait_read();      // the previous copy has read the staging rows
           __syncwarp();
         }
-        stage_columns<F32>(stage, bias + half * 32, r[half], half, lane);
-        const int c0 = col0 + (F32 ? half * 32 : 0);
-        if ((F32 || half == 1) && c0 < p.n) send_columns<F32>(stage, &mapO, p.vector_out, p.out, c0, row0, p.m, p.n, lane);
+        stage_columns<F32, DEEP, kStage>(stage, bias + c, &r[c / 32][c % 32], within / (F32 ? 4 : 8), lane);
+        if (within + kStage == kSend) send_columns<F32, DEEP>(stage, &mapO, p.vector_out, p.out, c0, row0, p.m, p.n, lane);
       }
     }
     if (lane == 0) bulk_wait_all();      // this thread's stores have landed
@@ -274,34 +287,36 @@ float8_linear_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_cons
   if (warp == 1) { tc_fence_after(); tmem_dealloc(tmem_base, 512); }
 }
 
-// f(BN, F32 as types)
+// f(BN, F32, DEEP as types)
 template <typename F>
-static void linear_forms(int bn, bool f32, F f) {
-  auto with = [&](auto b) { if (f32) f(b, std::true_type{}); else f(b, std::false_type{}); };
-  if (bn == 256) with(std::integral_constant<int, 256>{});
+static void linear_forms(int bn, bool deep, bool f32, F f) {
+  auto with = [&](auto b) { if (f32) f(b, std::true_type{}, std::false_type{}); else f(b, std::false_type{}, std::false_type{}); };
+  if (deep) { if (f32) f(std::integral_constant<int, 256>{}, std::true_type{}, std::true_type{}); else f(std::integral_constant<int, 256>{}, std::false_type{}, std::true_type{}); }
+  else if (bn == 256) with(std::integral_constant<int, 256>{});
   else if (bn == 128) with(std::integral_constant<int, 128>{});
   else with(std::integral_constant<int, 64>{});
 }
 
 void configure_float8_linear() {
-  for (int i = 0; i < 6; ++i)
-    linear_forms(64 << i % 3, i / 3, [](auto bn, auto f32) {
+  for (int i = 0; i < 8; ++i)
+    linear_forms(64 << i % 4, i % 4 == 3, i / 4, [](auto bn, auto f32, auto deep) {
       constexpr int BN = decltype(bn)::value;
-      cudaFuncSetAttribute(float8_linear_kernel<BN, decltype(f32)::value>, cudaFuncAttributeMaxDynamicSharedMemorySize, Float8Shape<BN>::smem);
+      constexpr bool D = decltype(deep)::value;
+      cudaFuncSetAttribute(float8_linear_kernel<BN, decltype(f32)::value, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Float8Shape<BN, D>::smem);
     });
   configure_float8_few();
 }
 
-template <int BN, bool F32>
+template <int BN, bool F32, bool DEEP>
 static lf_status launch_float8(lf_context* ctx, const f8::Matrix& x, const f8::Matrix& w, Float8Params p) {
-  using S = Float8Shape<BN>;
+  using S = Float8Shape<BN, DEEP>;
   CUtensorMap ma, mb, mo{};
   LF_TRY(make_map_bytes(ctx, &ma, x.codes, x.channels, x.rows, x.pitch, F8_BM));
   LF_TRY(make_map_bytes(ctx, &mb, w.codes, w.channels, w.rows, w.pitch, BN));
-  if (p.vector_out) LF_TRY(make_map_rows(ctx, &mo, p.out, F32, p.n, p.m, 32));
+  if (p.vector_out) LF_TRY(make_map_rows(ctx, &mo, p.out, F32, p.n, p.m, 32, DEEP));
   const int64_t tiles = (int64_t)((p.m + F8_BM - 1) / F8_BM) * ((p.n + BN - 1) / BN);
   lf_prof_begin(ctx, LF_KERNEL_LN_GEMM);
-  lf_launch(ctx, float8_linear_kernel<BN, F32>, (int)(tiles < ctx->sm_count ? tiles : ctx->sm_count), S::threads, S::smem, ma, mb, mo, p);
+  lf_launch(ctx, float8_linear_kernel<BN, F32, DEEP>, (int)(tiles < ctx->sm_count ? tiles : ctx->sm_count), S::threads, S::smem, ma, mb, mo, p);
   lf_prof_end(ctx);
   ctx->launches++;
   return LF_OK;
@@ -363,17 +378,20 @@ extern "C" lf_status lf_float8_linear_run(lf_context* ctx, const lf_float8_linea
   p.formats = (x.format == LF_FLOAT8_E5M2) | (w.format == LF_FLOAT8_E5M2) << 1;
   p.out = d->out;
   p.status = (tc05::Status*)ctx->tc_status;
-  // The tile width whose longest block is done first: a tile costs about its columns and 64 more (3001 x 449 -> 1283: 256 wide in one turn of the blocks, where 128
-  // takes two; 3001 x 1283 -> 449: 128 wide).
+  // The tile width whose longest block is done first: a tile costs about its columns and 64 more, and the last one's stores, which nothing hides, a quarter of
+  // its columns by TMA or three quarters by threads.  (3001 x 1283 -> 449 in float32: 10.8 us 128 wide, 13.7 at 64; 3001 x 449 -> 1283 in bf16: 9.5 at 128,
+  // 11.9 at 256.)
   int bn = 0;
   int64_t best = 0;
   for (int width = 64; width <= 256; width *= 2) {
-    const int64_t turns = (mx.tiles * ((p.n + width - 1) / width) + ctx->sm_count - 1) / ctx->sm_count, work = turns * (width + 64);
+    const int64_t turns = (mx.tiles * ((p.n + width - 1) / width) + ctx->sm_count - 1) / ctx->sm_count;
+    const int64_t work = turns * (width + 64) + width * (vector_out ? 1 : 3) / 4;
     if (bn == 0 || work < best) { bn = width; best = work; }
   }
   lf_status status = LF_OK;
-  tc::linear_forms(bn, f32, [&](auto b, auto o) {
-    status = tc::launch_float8<decltype(b)::value, decltype(o)::value>(ctx, mx, mw, p);
+  // (the deeper ring, 4096 rows and outputs: 57.3 -> 54.2 us at 4096 channels)
+  tc::linear_forms(bn, bn == 256 && p.k >= tc::F8_DEEP, f32, [&](auto b, auto o, auto deep) {
+    status = tc::launch_float8<decltype(b)::value, decltype(o)::value, decltype(deep)::value>(ctx, mx, mw, p);
   });
   LF_TRY(status);
   return lf_float8_done(ctx, r, launches);

@@ -164,14 +164,14 @@ lf_status make_map_bytes(lf_context* ctx, CUtensorMap* map, const void* base, ui
   return LF_OK;
 }
 
-// float32 or bf16 rows (a multiple of 16 bytes), 128-byte swizzled boxes of 128 bytes x `box_rows` rows
-lf_status make_map_rows(lf_context* ctx, CUtensorMap* map, const void* base, bool f32, uint64_t width, uint64_t rows, uint32_t box_rows) {
+// float32 or bf16 rows (a multiple of 16 bytes), 128-byte swizzled boxes of 128 bytes x `box_rows` rows; narrow: 64 bytes, 64-byte swizzle
+lf_status make_map_rows(lf_context* ctx, CUtensorMap* map, const void* base, bool f32, uint64_t width, uint64_t rows, uint32_t box_rows, bool narrow) {
   if (!g_encode) return lf_fail(ctx, LF_ERR_CUDA, "cuTensorMapEncodeTiled is not available from this driver");
   const uint64_t pitch = width * (f32 ? 4 : 2);
   cuuint64_t dims[3] = {width, rows, 1}, strides[2] = {pitch, pitch * rows};
-  cuuint32_t box[3] = {f32 ? 32u : 64u, box_rows, 1}, estr[3] = {1, 1, 1};
+  cuuint32_t box[3] = {(f32 ? 32u : 64u) >> narrow, box_rows, 1}, estr[3] = {1, 1, 1};
   CUresult r = g_encode(map, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, estr,
-                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, narrow ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return lf_fail(ctx, LF_ERR_CUDA, "cuTensorMapEncodeTiled (rows) failed with code %d", (int)r);
   return LF_OK;
 }
