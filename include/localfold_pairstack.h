@@ -652,7 +652,7 @@ LF_API lf_status lf_layer_norm_backward_run(lf_context* ctx, const lf_layer_norm
  * transposed weights. */
 typedef struct lf_float8_linear_desc {
   lf_float8_matrix activations;   /* [rows][channels] */
-  lf_float8_matrix weights;       /* [out channels][channels] */
+  lf_float8_matrix weights;       /* [out channels][channels], e4m3 */
   const float* bias;              /* [out channels] or null */
   int32_t out_dtype, source_dtype;
   const void* source;             /* or null: activations are encoded already */

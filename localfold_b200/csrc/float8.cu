@@ -150,7 +150,7 @@ using namespace f8;
 
 lf_status lf_float8_check_rows(lf_context* ctx, const char* what, int64_t rows, int channels, int dtype) {
   if (rows <= 0 || channels <= 0) return lf_fail(ctx, LF_ERR_SHAPE, "%s: rows and channels must be positive safe integers", what);
-  if (rows > 0x7fffffff || channels > (1 << 24) || (uint64_t)rows * blocks(channels) > 0x7fffffffull)
+  if (rows > 0x7fffff00 || channels > (1 << 24) || (uint64_t)rows * blocks(channels) > 0x7fffffffull)
     return lf_fail(ctx, LF_ERR_UNSUPPORTED, "%s: %lld rows of %d channels are too many", what, (long long)rows, channels);
   if (dtype != LF_DTYPE_F32 && dtype != LF_DTYPE_BF16) return lf_fail(ctx, LF_ERR_ARGUMENT, "unknown activation dtype %d", dtype);
   return LF_OK;
@@ -192,7 +192,7 @@ lf_status lf_float8_encode(lf_context* ctx, const lf_float8_encode_desc* d, lf_r
     if (d->transposed.format != o.format) return lf_fail(ctx, LF_ERR_ARGUMENT, "float8 encode: both forms have one format");
   }
   if (d->block_rows == kBlock && row_tiles(o.rows) > 65535) return lf_fail(ctx, LF_ERR_UNSUPPORTED, "float8 encode: %lld rows are too many for blocks of 128 rows", (long long)o.rows);
-  LF_CUDA(ctx, cudaSetDevice(ctx->device));
+  const lf_device_guard device(ctx);
   const Matrix m = matrix(o);
   const int access = row_access(d->source, o.channels, d->dtype);
   lf_prof_begin(ctx, LF_KERNEL_ELEMENTWISE);
@@ -226,7 +226,7 @@ lf_status lf_float8_decode(lf_context* ctx, const lf_float8_decode_desc* d, lf_r
   const lf_float8_matrix& o = d->source;
   LF_TRY(lf_float8_check_rows(ctx, "float8 decode", o.rows, o.channels, d->dtype));
   LF_TRY(lf_float8_check(ctx, "float8 decode", o, o.rows, o.channels));
-  LF_CUDA(ctx, cudaSetDevice(ctx->device));
+  const lf_device_guard device(ctx);
   const Matrix m = matrix(o);
   const int access = row_access(d->out, o.channels, d->dtype);
   const uint32_t per_row = blocks(o.channels), units = (uint32_t)(o.rows * per_row);

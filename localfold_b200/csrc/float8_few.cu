@@ -75,7 +75,7 @@ float8_few_kernel(const FewParams p) {
     for (int i = 0; i < 4; ++i) total[e][i] = 0.f;
   constexpr int kAhead = 2;      // blocks whose weights are in flight
   uint4 w[kAhead][2][2];         // [block][half of its channels][output row]
-  int sw[kAhead];
+  int sw[kAhead][2];
   auto fetch = [&](int slot, int block) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -86,7 +86,8 @@ float8_few_kernel(const FewParams p) {
         if (r1 < p.n) w[slot][h][1] = *reinterpret_cast<const uint4*>(p.w.codes + r1 * p.w.pitch + c);
       }
     }
-    sw[slot] = p.w.exponents[exponent_at(n0, block, p.w.tiles)];      // a weight's block has 128 outputs: all sixteen share it
+    sw[slot][0] = r0 < p.n ? p.w.exponents[exponent_at(r0, block, p.w.tiles)] : 1;
+    sw[slot][1] = r1 < p.n ? p.w.exponents[exponent_at(r1, block, p.w.tiles)] : 1;
   };
 #pragma unroll
   for (int i = 0; i < kAhead; ++i)
@@ -101,7 +102,7 @@ float8_few_kernel(const FewParams p) {
         for (int e = 0; e < EIGHTS; ++e)
 #pragma unroll
           for (int j = 0; j < 4; ++j) c[e][j] = 0.f;
-        const float fw = up(sw[i]);
+        const float fw0 = up(sw[i][0]), fw1 = up(sw[i][1]);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           uint4 x[EIGHTS];
@@ -123,10 +124,10 @@ float8_few_kernel(const FewParams p) {
 #pragma unroll
         for (int e = 0; e < EIGHTS; ++e) {
           const float f0 = up(exp_s[(e * 8 + 2 * t) * nblk + block]), f1 = up(exp_s[(e * 8 + 2 * t + 1) * nblk + block]);
-          total[e][0] += c[e][0] * f0 * fw;
-          total[e][1] += c[e][1] * f1 * fw;
-          total[e][2] += c[e][2] * f0 * fw;
-          total[e][3] += c[e][3] * f1 * fw;
+          total[e][0] += c[e][0] * f0 * fw0;
+          total[e][1] += c[e][1] * f1 * fw0;
+          total[e][2] += c[e][2] * f0 * fw1;
+          total[e][3] += c[e][3] * f1 * fw1;
         }
       }
     }

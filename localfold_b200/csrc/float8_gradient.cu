@@ -149,7 +149,9 @@ float8_gradient_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_co
     const uint64_t ones_desc = make_smem_desc_plain(smem_u32(ones), 128, 256);
     const uint64_t a_first = make_smem_desc(smem_u32(dy_s), WG_ROWS * 128, 1024), b_first = make_smem_desc(smem_u32(x_s), WG_ROWS * 128, 1024);
     for (int t = first; t < last; ++t) {
-      if (!mbar_wait(&full[slot], phase, abort_flag, p.status, 132) || (p.dy_mode == 0 && !mbar_wait(&loaded[stage], ring_phase, abort_flag, p.status, 136))) break;
+      // (an expired wait ends the loop for all lanes alike)
+      if (!__all_sync(0xffffffffu, mbar_wait(&full[slot], phase, abort_flag, p.status, 132))) break;
+      if (p.dy_mode == 0 && !__all_sync(0xffffffffu, mbar_wait(&loaded[stage], ring_phase, abort_flag, p.status, 136))) break;
       tc_fence_after();
       if (elect_one()) {
         const uint64_t a = a_first + (uint32_t)((p.dy_mode == 0 ? stage : slot) * (WG_A_BYTES >> 4)), b = b_first + (uint32_t)(slot * (WG_B_BYTES >> 4));
@@ -190,7 +192,7 @@ float8_gradient_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_co
     bool ok = true;
     if (p.dy_mode == 1) fetch(first);
     for (int t = first; t < last; ++t) {
-      if (!mbar_wait(&loaded[stage], ring_phase, abort_flag, p.status, 135)) { ok = false; break; }
+      if (!__all_sync(0xffffffffu, mbar_wait(&loaded[stage], ring_phase, abort_flag, p.status, 135))) { ok = false; break; }
       uint4 codes[kUnits], dy_unit[2];
       int s[kUnits], sy = 1;
       const uint8_t* e = exponents + stage * WG_EXPONENTS + (t & 1) * 8;      // (rows 64 .. 127 of a tile: words 2 and 3)
@@ -209,7 +211,7 @@ float8_gradient_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_co
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&taken[stage]);      // the codes are in registers
-      if (!mbar_wait(&empty[slot], phase ^ 1, abort_flag, p.status, 133)) { ok = false; break; }
+      if (!__all_sync(0xffffffffu, mbar_wait(&empty[slot], phase ^ 1, abort_flag, p.status, 133))) { ok = false; break; }
       uint8_t* sA = dy_s + slot * WG_A_BYTES;
       uint8_t* sB = x_s + slot * WG_B_BYTES;
       // (odd blocks of 64 columns store their second piece first: eight lanes then fill eight different 16-byte columns of the banks)
@@ -238,7 +240,7 @@ float8_gradient_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_co
       if (++stage == WG_RING) { stage = 0; ring_phase ^= 1; }
     }
     // The tile: 16 warps, 64 columns of a lane quadrant each.
-    ok = ok && mbar_wait(done, 0, abort_flag, p.status, 134);
+    ok = ok && __all_sync(0xffffffffu, mbar_wait(done, 0, abort_flag, p.status, 134));
     tc_fence_after();
     if (ok) {
       const int q = warp & 3, part = (warp - 2) >> 2, row0 = n0 + q * 32, col0 = k0 + part * 64;
@@ -380,7 +382,7 @@ lf_status lf_float8_weight_gradient_run(lf_context* ctx, const lf_float8_weight_
   const uint64_t need = lf_float8_weight_gradient_workspace(ctx, x.rows, x.channels, d->out_channels);
   if (need && (!d->workspace || d->workspace_bytes < need || !lf_aligned16(d->workspace)))
     return lf_fail(ctx, LF_ERR_ARGUMENT, "float8 weight gradient: a workspace of %llu bytes on a 16-byte boundary is needed", (unsigned long long)need);
-  LF_CUDA(ctx, cudaSetDevice(ctx->device));
+  const lf_device_guard device(ctx);
   tc::GradientParams p{};
   p.m = (int)x.rows; p.n = d->out_channels; p.k = x.channels;
   int splits;

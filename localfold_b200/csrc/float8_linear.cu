@@ -32,7 +32,7 @@ struct Float8Params {
   const float* bias;           // [n] or null
   const uint8_t *ex, *ew;      // exponents
   int64_t ex_tiles, ew_tiles;  // 128-row tiles of each
-  int formats;                 // bit 0: x is e5m2, bit 1: w
+  int x_format;                // w is e4m3
   void* out;
   Status* status;
 };
@@ -201,13 +201,13 @@ float8_linear_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_cons
       const int nj = t % tiles_n;
       const int left = p.n - nj * BN, columns = left >= BN ? BN : (left + 15) / 16 * 16;
       const uint32_t acc = it % S::accumulators;
-      if (!mbar_wait(&tmem_empty[acc], ((it / S::accumulators) & 1) ^ 1, abort_flag, p.status, 122)) break;
+      if (!__all_sync(0xffffffffu, mbar_wait(&tmem_empty[acc], ((it / S::accumulators) & 1) ^ 1, abort_flag, p.status, 122))) break;
       tc_fence_after();
       const uint32_t d = tmem_base + acc * BN;
-      const uint32_t idesc = make_idesc_f8(F8_BM, columns, p.formats & 1, p.formats >> 1, 0);
+      const uint32_t idesc = make_idesc_f8(F8_BM, columns, p.x_format, 0, 0);
       uint32_t scales = 0;
       for (int kb = 0; kb < kblocks; ++kb) {
-        if (!mbar_wait(&full[stage], phase, abort_flag, p.status, 123)) { ok = false; break; }
+        if (!__all_sync(0xffffffffu, mbar_wait(&full[stage], phase, abort_flag, p.status, 123))) { ok = false; break; }      // (for all lanes alike)
         tc_fence_after();
         const uint64_t a = a_first + (uint32_t)(stage * S::stage >> 4), b = b_first + (uint32_t)(stage * S::stage >> 4);
         // Four slots in turn: when a group's first step is here, the step `stages` <= 6 before it is complete, and with it
@@ -250,7 +250,7 @@ float8_linear_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_cons
         __syncwarp();
       }
       const uint32_t acc = it % S::accumulators;
-      if (!mbar_wait(&tmem_full[acc], (it / S::accumulators) & 1, abort_flag, p.status, 124)) break;
+      if (!__all_sync(0xffffffffu, mbar_wait(&tmem_full[acc], (it / S::accumulators) & 1, abort_flag, p.status, 124))) break;
       tc_fence_after();
       uint32_t r[S::share / 32][32];
       if (mine) {
@@ -342,6 +342,7 @@ extern "C" lf_status lf_float8_linear_run(lf_context* ctx, const lf_float8_linea
   LF_TRY(lf_float8_check_rows(ctx, "float8 linear", w.rows, x.channels, d->out_dtype));
   LF_TRY(lf_float8_check(ctx, "float8 linear, weights", w, w.rows, x.channels));
   if (d->source && d->source_dtype != LF_DTYPE_F32 && d->source_dtype != LF_DTYPE_BF16) return lf_fail(ctx, LF_ERR_ARGUMENT, "unknown source dtype %d", d->source_dtype);
+  if (w.format != LF_FLOAT8_E4M3) return lf_fail(ctx, LF_ERR_UNSUPPORTED, "float8 linear: weights are e4m3");
   if (w.rows > (1 << 24)) return lf_fail(ctx, LF_ERR_UNSUPPORTED, "float8 linear: %lld output channels are too many", (long long)w.rows);
   if (row_tiles(x.rows) * ((w.rows + 63) / 64) > 0x7fffffffll) return lf_fail(ctx, LF_ERR_UNSUPPORTED, "float8 linear: %lld x %lld outputs are too many", (long long)x.rows, (long long)w.rows);
   Matrix mx = matrix(x);
@@ -352,7 +353,7 @@ extern "C" lf_status lf_float8_linear_run(lf_context* ctx, const lf_float8_linea
   const uint64_t need = d->source && !kept ? lf_float8_linear_workspace(x.rows, x.channels) : 0;
   if (need && (!d->workspace || d->workspace_bytes < need || !lf_aligned16(d->workspace)))
     return lf_fail(ctx, LF_ERR_ARGUMENT, "float8 linear: a workspace of %llu bytes on a 16-byte boundary is needed", (unsigned long long)need);
-  LF_CUDA(ctx, cudaSetDevice(ctx->device));
+  const lf_device_guard device(ctx);
   if (tc::float8_few_takes(x.rows, x.channels)) {
     LF_TRY(tc::float8_few(ctx, d->source, d->source ? d->source_dtype : LF_DTYPE_F32, mx, mw, d->bias, d->out, d->out_dtype));
     return lf_float8_done(ctx, r, 1);
@@ -375,7 +376,7 @@ extern "C" lf_status lf_float8_linear_run(lf_context* ctx, const lf_float8_linea
   p.m = (int)x.rows; p.n = (int)w.rows; p.k = x.channels;
   p.vector_out = vector_out;
   p.bias = d->bias; p.ex = mx.exponents; p.ew = mw.exponents; p.ex_tiles = mx.tiles; p.ew_tiles = mw.tiles;
-  p.formats = (x.format == LF_FLOAT8_E5M2) | (w.format == LF_FLOAT8_E5M2) << 1;
+  p.x_format = x.format;
   p.out = d->out;
   p.status = (tc05::Status*)ctx->tc_status;
   // The tile width whose longest block is done first: a tile costs about its columns and 64 more, and the last one's stores, which nothing hides, a quarter of

@@ -297,7 +297,7 @@ lf_status lf_layer_norm_run(lf_context* ctx, const lf_layer_norm_desc* d, lf_res
   if (!(d->epsilon > 0.f) || !(d->epsilon < INFINITY)) return lf_fail(ctx, LF_ERR_SHAPE, "epsilon must be finite and positive; received %g", d->epsilon);
   for (const lf_float8_matrix* m : {&d->checkpoint, &d->encoded})
     if (m->codes) LF_TRY(lf_float8_check(ctx, "layer norm", *m, d->rows, d->channels));
-  LF_CUDA(ctx, cudaSetDevice(ctx->device));
+  const lf_device_guard device(ctx);
   Forward a{};
   a.rows = d->rows; a.c = d->channels; a.epsilon = d->epsilon;
   a.access_in = row_access(d->activations, a.c, d->act_dtype);
@@ -330,7 +330,7 @@ lf_status lf_layer_norm_backward_run(lf_context* ctx, const lf_layer_norm_backwa
   const uint64_t need = lf_layer_norm_backward_workspace(ctx, d->rows, d->channels);
   if (d->workspace_bytes < need || !lf_aligned16(d->workspace))
     return lf_fail(ctx, LF_ERR_ARGUMENT, "layer norm backward: a workspace of %llu bytes on a 16-byte boundary is needed", (unsigned long long)need);
-  LF_CUDA(ctx, cudaSetDevice(ctx->device));
+  const lf_device_guard device(ctx);
   Backward a{};
   a.rows = d->rows; a.c = d->channels;
   a.access_dy = row_access(d->gradient, a.c, d->act_dtype);

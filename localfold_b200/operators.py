@@ -12,6 +12,7 @@ Where the reference takes ``precision: "f32" | "f16"``, this library takes
 """
 from __future__ import annotations
 
+import collections
 import ctypes
 import weakref
 
@@ -84,6 +85,7 @@ class Device:
         self._own_stream = stream is None
         self._uploads = None
         self._scratch_limit = 0
+        self._held = collections.deque()
 
     def wait_for_torch(self):
         """Makes the context's own stream wait (on the device, no host wait) for the work torch has enqueued so
@@ -111,8 +113,19 @@ class Device:
     def check(self, status):
         nat.check(self.lib, self.handle, status)
 
+    def hold(self, tensors):
+        """Keeps ``tensors`` until the work enqueued so far on the context's stream is done: until a later ``hold`` or ``synchronize`` finds it so.
+        For tensors of torch's allocator, which knows nothing of this stream."""
+        import torch
+        while self._held and self._held[0][0].query():
+            self._held.popleft()
+        event = torch.cuda.Event()
+        event.record(torch.cuda.ExternalStream(self.stream, device=f"cuda:{self.ordinal}"))
+        self._held.append((event, tensors))
+
     def synchronize(self):
         self.check(self.lib.lf_context_synchronize(self.handle))
+        self._held.clear()
 
     def launch_count(self) -> int:
         """Kernels launched so far, those that prepared weights on ``uploads()`` among them."""
@@ -164,7 +177,8 @@ class Device:
         if self._uploads is not None:
             self._uploads.close()
             self._uploads = None
-        self._finalizer()
+        self._finalizer()      # (waits for the stream)
+        self._held.clear()
 
 
 _default_device = None

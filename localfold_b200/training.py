@@ -40,6 +40,7 @@ _LINEAR = struct.Struct("@" + 2 * _MATRIX + "QiiQQQQ")
 _WEIGHT_GRADIENT = struct.Struct("@" + _MATRIX + "Q" + _MATRIX + "ii4Q")
 _NO_MATRIX = (0, 0, 0, 0, 0)
 _NO_OPTIONS = {}
+_AS_IT_WAS = object()
 
 
 def _format(value, name="format"):
@@ -94,8 +95,9 @@ def _torch_dtype(name):
 
 
 def _call(device, function, desc, tensors, output=None):
-    """One library call and its result object.  Where torch's current stream is not the device's: the tensors' memory stays theirs until
-    the device's stream is done with it, and a device with a stream of its own waits for torch's work first."""
+    """One library call and its result object.  Where torch's current stream is not the device's: a device with a stream of its own waits for
+    torch's work first, and the device holds the call's tensors until its stream is done with them, so that torch does not
+    give their memory away before."""
     current = _torch_stream(device.ordinal)
     if current != device.stream and device._own_stream:
         device.check(device.lib.lf_context_await(device.handle, current))
@@ -104,12 +106,7 @@ def _call(device, function, desc, tensors, output=None):
     if status != nat.LF_OK:
         device.check(status)
     if current != device.stream:
-        torch = _torch()
-        stream = torch.cuda.ExternalStream(device.stream, device=f"cuda:{device.ordinal}")
-        for t in tensors:
-            t = t.memory if isinstance(t, Float8Tensor) else t
-            if t is not None:
-                t.record_stream(stream)
+        device.hold(tensors)
     return {"output": output, "elapsedMilliseconds": 0.0, "memory": {"peakBytes": res.peak_bytes}, "launches": res.launches}
 
 
@@ -136,8 +133,10 @@ class Float8Tensor:
 
     def __init__(self, rows: int, channels: int, format: str, memory):
         """``memory``: contiguous uint8 CUDA tensor with the codes, then the exponents, 16-byte aligned (``lf_float8_matrix``)."""
-        self.rows, self.channels, self.format, self.memory = rows, channels, format, memory
+        self.rows, self.channels, self.format, self.memory = rows, channels, _format(format), memory
         self._codes, exponents = _sizes(rows, channels)
+        if memory.element_size() != 1 or not memory.is_cuda or not memory.is_contiguous():
+            raise ValueError("memory must be a contiguous uint8 CUDA tensor")
         if memory.numel() != self._codes + exponents:
             raise RangeError(f"memory has {memory.numel()} values; expected {self._codes + exponents}")
         base = memory.data_ptr()
@@ -229,7 +228,8 @@ class LayerNormGpu:
         dev, opts = self.device, options or _NO_OPTIONS
         rows, c = _size(input, "rows"), _size(input, "channels")
         x, scale, offset = input["activations"], input["scale"], input["offset"]
-        epsilon = input.get("epsilon", 1e-5)
+        epsilon = input.get("epsilon")
+        epsilon = 1e-5 if epsilon is None else epsilon
         if not epsilon > 0 or not math.isfinite(epsilon):
             raise RangeError(f"epsilon must be finite and positive; received {epsilon}")
         variance = _variance(opts, "two-pass") if opts else nat.VARIANCE_TWO_PASS
@@ -304,8 +304,9 @@ class Float8LinearWeights:
         self.out_channels, self.channels = int(shape[0]), int(shape[1])
         _positive("outChannels", self.out_channels)
         _positive("channels", self.channels)
-        weight, bias = self._on_device(weight), self._on_device(bias)
+        weight = self._on_device(weight)
         _tensor(device, "weight", weight, self.out_channels * self.channels)
+        self.bias = None
         self.forward = Float8Tensor.empty(self.out_channels, self.channels, "e4m3", weight)
         self.transposed = Float8Tensor.empty(self.channels, self.out_channels, "e4m3", weight)
         self.update(weight, bias)
@@ -317,9 +318,10 @@ class Float8LinearWeights:
         host = value.decode() if isinstance(value, EncodedTensor) else np.ascontiguousarray(np.asarray(value, np.float32))
         return torch.as_tensor(host).to(f"cuda:{self.device.ordinal}")
 
-    def update(self, weight, bias=None):
-        """New values (float32 or bfloat16 CUDA tensors or host arrays).  The bias tensor is used as it is at every call."""
-        weight, bias = self._on_device(weight), self._on_device(bias)
+    def update(self, weight, bias=_AS_IT_WAS):
+        """A new weight (float32 or bfloat16 CUDA tensor, or host array) and, if given, a new bias (float32, or None).  The bias tensor is
+        not copied: calls read what it holds."""
+        weight, bias = self._on_device(weight), self.bias if bias is _AS_IT_WAS else self._on_device(bias)
         if weight.shape != (self.out_channels, self.channels):
             raise RangeError(f"weight is {tuple(weight.shape)}; expected {(self.out_channels, self.channels)}")
         dtype = _tensor(self.device, "weight", weight, self.out_channels * self.channels)
