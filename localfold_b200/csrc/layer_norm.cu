@@ -38,7 +38,7 @@ struct Backward {
   Matrix kept;
   const float *mean, *inverse, *scale;
   void* dx;
-  float* partial;                // [blocks][2][c]
+  float *partial_g, *partial_b;  // [blocks][2][c] and its second rows; of one block the gradients themselves
 };
 
 __host__ __device__ constexpr int threads_of(int G) { return G <= 256 ? 256 : G; }
@@ -195,7 +195,7 @@ backward_kernel(const Backward a) {
   // this block's row of sums
 #pragma unroll
   for (int which = 0; which < 2; ++which) {
-    float* out = a.partial + ((int64_t)blockIdx.x * 2 + which) * a.c;
+    float* out = (which ? a.partial_b : a.partial_g) + (int64_t)blockIdx.x * 2 * a.c;
     if (kGroups == 1) store16<float, kWarp>(out + first, left, true, kElements, which ? db : dg, room);
     else {
       __syncthreads();
@@ -259,8 +259,12 @@ static auto by_width(int c, F f) {
   return f(std::integral_constant<int, 512>{});
 }
 
+// Few rows take one block, whose sums are the gradients: three more turns of it cost less than the launch that joins blocks.
 static int backward_blocks(const lf_context* ctx, int64_t rows, int c) {
-  return by_width(c, [&](auto g) { constexpr int G = decltype(g)::value; return grid_of(ctx, rows, threads_of(G) / G, blocks_of(G)); });
+  return by_width(c, [&](auto g) {
+    constexpr int G = decltype(g)::value, kGroups = threads_of(G) / G;
+    return rows <= 4 * kGroups ? 1 : grid_of(ctx, rows, kGroups, blocks_of(G));
+  });
 }
 
 template <typename T>
@@ -315,20 +319,21 @@ lf_status lf_layer_norm_run(lf_context* ctx, const lf_layer_norm_desc* d, lf_res
 
 uint64_t lf_layer_norm_backward_workspace(const lf_context* ctx, int64_t rows, int32_t channels) {
   if (!ctx || rows <= 0 || channels <= 0 || channels > kMostChannels) return 0;
-  return (uint64_t)backward_blocks(ctx, rows, channels) * 2 * channels * sizeof(float);
+  const int blocks = backward_blocks(ctx, rows, channels);
+  return blocks == 1 ? 0 : (uint64_t)blocks * 2 * channels * sizeof(float);
 }
 
 lf_status lf_layer_norm_backward_run(lf_context* ctx, const lf_layer_norm_backward_desc* d, lf_result* r) {
   if (!ctx) return LF_ERR_ARGUMENT;
   if (!d || !d->gradient || (!d->activations && !d->checkpoint.codes) || !d->mean || !d->inverse_deviation || !d->scale || !d->out ||
-      !d->scale_gradient || !d->offset_gradient || !d->workspace)
+      !d->scale_gradient || !d->offset_gradient)
     return lf_fail(ctx, LF_ERR_ARGUMENT, "layer norm backward: null argument");
   if (d->activations && d->checkpoint.codes) return lf_fail(ctx, LF_ERR_ARGUMENT, "layer norm backward: activations or a checkpoint, not both");
   LF_TRY(lf_float8_check_rows(ctx, "layer norm backward", d->rows, d->channels, d->act_dtype));
   if (d->channels > kMostChannels) return lf_fail(ctx, LF_ERR_UNSUPPORTED, "layer norm of %d channels: at most %d", d->channels, kMostChannels);
   if (d->checkpoint.codes) LF_TRY(lf_float8_check(ctx, "layer norm backward", d->checkpoint, d->rows, d->channels));
   const uint64_t need = lf_layer_norm_backward_workspace(ctx, d->rows, d->channels);
-  if (d->workspace_bytes < need || !lf_aligned16(d->workspace))
+  if (need && (!d->workspace || d->workspace_bytes < need || !lf_aligned16(d->workspace)))
     return lf_fail(ctx, LF_ERR_ARGUMENT, "layer norm backward: a workspace of %llu bytes on a 16-byte boundary is needed", (unsigned long long)need);
   const lf_device_guard device(ctx);
   Backward a{};
@@ -339,15 +344,18 @@ lf_status lf_layer_norm_backward_run(lf_context* ctx, const lf_layer_norm_backwa
   a.access_weights = row_access(d->scale, a.c, LF_DTYPE_F32);
   a.dy = d->gradient; a.x = d->activations; a.mean = d->mean; a.inverse = d->inverse_deviation; a.scale = d->scale; a.dx = d->out;
   if (d->checkpoint.codes) a.kept = matrix(d->checkpoint);
-  a.partial = (float*)d->workspace;
   const int blocks = backward_blocks(ctx, a.rows, a.c);
+  a.partial_g = blocks == 1 ? d->scale_gradient : (float*)d->workspace;
+  a.partial_b = blocks == 1 ? d->offset_gradient : a.partial_g + a.c;
   lf_prof_begin(ctx, LF_KERNEL_ELEMENTWISE);
   if (d->act_dtype == LF_DTYPE_BF16) launch_backward<bf16>(ctx, a, blocks); else launch_backward<float>(ctx, a, blocks);
   lf_prof_end(ctx);
+  ctx->launches++;
+  if (blocks == 1) return lf_float8_done(ctx, r, 1);
   lf_prof_begin(ctx, LF_KERNEL_ELEMENTWISE);
-  lf_launch(ctx, join_kernel, dim3(lf_ceil_div(a.c, 32), 2), 1024, 0, a.partial, blocks, a.c, d->scale_gradient, d->offset_gradient);
+  lf_launch(ctx, join_kernel, dim3(lf_ceil_div(a.c, 32), 2), 1024, 0, a.partial_g, blocks, a.c, d->scale_gradient, d->offset_gradient);
   lf_prof_end(ctx);
-  ctx->launches += 2;
+  ctx->launches++;
   return lf_float8_done(ctx, r, 2);
 }
 

@@ -115,14 +115,15 @@ def _sizes(rows, channels):
     return rows * ((channels + 15) & -16), ((channels + 511) >> 9) * ((rows + 127) >> 7) * 512
 
 
-_bytes = {}      # GPU -> an empty uint8 tensor there: new memory of that kind takes least time from one
+_empty = {}      # (GPU, dtype) -> an empty tensor: new memory of that kind takes least time from one
 
 
-def _new_bytes(like, nbytes):
-    proto = _bytes.get(like.get_device())
+def _new(like, dtype, shape):
+    key = (like.get_device(), dtype)
+    proto = _empty.get(key)
     if proto is None:
-        proto = _bytes[like.get_device()] = like.new_empty(0, dtype=_torch().uint8)
-    return proto.new_empty(nbytes)
+        proto = _empty[key] = like.new_empty(0, dtype=_torch().uint8 if dtype == "bytes" else _torch_dtype(dtype))
+    return proto.new_empty(shape)
 
 
 class Float8Tensor:
@@ -145,7 +146,7 @@ class Float8Tensor:
     @classmethod
     def empty(cls, rows, channels, format, like):
         codes, exponents = _sizes(rows, channels)
-        return cls(rows, channels, format, _new_bytes(like, codes + exponents))
+        return cls(rows, channels, format, _new(like, "bytes", codes + exponents))
 
     @property
     def nbytes(self):
@@ -199,7 +200,7 @@ def float8_decode(device, encoded, options=None, out=None):
     _matrix(dev, "encoded", encoded, encoded.rows, encoded.channels)
     dtype = _output(options, "bf16")
     if out is None:
-        out = encoded.memory.new_empty((encoded.rows, encoded.channels), dtype=_torch_dtype(dtype))
+        out = _new(encoded.memory, dtype, (encoded.rows, encoded.channels))
     else:
         _tensor(dev, "out", out, encoded.rows * encoded.channels, dtype)
     _call(dev, dev.lib.lf_float8_decode, _DECODE.pack(*encoded.fields, _DTYPE[dtype], 0, out.data_ptr()), (encoded, out))
@@ -282,9 +283,9 @@ class LayerNormGpu:
         else:
             out = _torch().empty_like(dy)
         nbytes = dev.lib.lf_layer_norm_backward_workspace(dev.handle, rows, c)
-        dscale, doffset, workspace = scale.new_empty(c), scale.new_empty(c), _new_bytes(scale, nbytes)
+        dscale, doffset, workspace = scale.new_empty(c), scale.new_empty(c), _new(scale, "bytes", nbytes) if nbytes else None
         desc = _LAYER_NORM_BACKWARD.pack(rows, c, _DTYPE[dtype], dy.data_ptr(), 0 if encoded else x.data_ptr(), *(x.fields if encoded else _NO_MATRIX),
-                                         mean.data_ptr(), inverse.data_ptr(), scale.data_ptr(), out.data_ptr(), dscale.data_ptr(), doffset.data_ptr(), workspace.data_ptr(), nbytes)
+                                         mean.data_ptr(), inverse.data_ptr(), scale.data_ptr(), out.data_ptr(), dscale.data_ptr(), doffset.data_ptr(), workspace.data_ptr() if nbytes else 0, nbytes)
         result = _call(dev, dev.lib.lf_layer_norm_backward_run, desc, (dy, x, mean, inverse, scale, out, dscale, doffset, workspace), out)
         result["activations"] = result.pop("output")
         result["scale"], result["offset"] = dscale, doffset
@@ -359,11 +360,11 @@ class Float8LinearGpu:
                 operand = Float8Tensor.empty(rows, channels, format, value)
             else:
                 nbytes = dev.lib.lf_float8_linear_workspace(rows, channels)
-                workspace = _new_bytes(value, nbytes) if nbytes else None
+                workspace = _new(value, "bytes", nbytes) if nbytes else None
         if out is not None:
             _tensor(dev, "out", out, rows * weights.rows, dtype)
         else:
-            out = weights.memory.new_empty((rows, weights.rows), dtype=_torch_dtype(dtype))
+            out = _new(weights.memory, dtype, (rows, weights.rows))
         desc = _LINEAR.pack(*(operand.fields if operand is not None else (rows, channels, _FORMAT[format], 0, 0)), *weights.fields,
                             bias.data_ptr() if bias is not None else 0, _DTYPE[dtype], _DTYPE[source or "f32"], value.data_ptr() if source else 0,
                             out.data_ptr(), workspace.data_ptr() if nbytes else 0, nbytes)
@@ -407,8 +408,8 @@ class Float8LinearGpu:
         else:
             _tensor(dev, "gradient", dy, rows * n, "bf16")
         nbytes = dev.lib.lf_float8_weight_gradient_workspace(dev.handle, rows, channels, n)
-        weight = x.memory.new_empty((n, channels), dtype=_torch().float32)
-        bias, workspace = weight.new_empty(n), _new_bytes(weight, nbytes) if nbytes else None
+        weight = _new(x.memory, "f32", (n, channels))
+        bias, workspace = weight.new_empty(n), _new(weight, "bytes", nbytes) if nbytes else None
         desc = _WEIGHT_GRADIENT.pack(*x.fields, 0 if encoded else dy.data_ptr(), *(dy.fields if encoded else _NO_MATRIX), n, 0, weight.data_ptr(), bias.data_ptr(),
                                      workspace.data_ptr() if nbytes else 0, nbytes)
         result = _call(dev, dev.lib.lf_float8_weight_gradient_run, desc, (dy, x, weight, bias, workspace), weight)

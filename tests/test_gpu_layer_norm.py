@@ -14,7 +14,7 @@ U = 128 * ref.U32
 TYPES = {"f32": torch.float32, "bf16": torch.bfloat16}
 # widths: one channel, narrow, one vector, whole blocks, odd, each form's last width and the next one's first
 SHAPES = [(1, 1), (3, 5), (129, 8), (1, 128), (65, 64), (300, 65), (77, 100), (64, 128), (1000, 128), (33, 129), (50, 256), (41, 257), (17, 384), (21, 512),
-          (9, 513), (13, 1000), (5, 1024), (6, 1025), (3, 2048), (2, 2049), (3, 4096), (2, 4097), (1, 8192), (7, 8191), (40000, 16), (20011, 72)]
+          (9, 513), (13, 1000), (5, 1024), (6, 1025), (3, 2048), (2, 2049), (3, 4096), (2, 4097), (1, 8192), (7, 8191), (40000, 16), (20011, 72), (256, 60), (257, 60), (32, 512), (33, 500)]      # (the last four: one block and two)
 
 
 @pytest.fixture(scope="module")
@@ -77,7 +77,9 @@ def test_gradients(dev, rows, c, dtype, kept):
     dev.synchronize()
     if kept:
         values = ref.decoded(host(x), kept)
-        ref.close(lf.float8_decode(dev, forward["checkpoint"], {"output": "f32"}), values, 0.0, "checkpoint")
+        decoded = lf.float8_decode(dev, forward["checkpoint"], {"output": "f32"})
+        dev.synchronize()
+        ref.close(decoded, values, 0.0, "checkpoint")
     else:
         values = host(x)
     mean, inverse = host(forward["mean"]), host(forward["inverseDeviation"])

@@ -324,8 +324,9 @@ def test_library_refusals(dev):
                                                            workspace_bytes=x.numel() * 4), **k})
     refuse("lf_layer_norm_backward_run", back(activations=None), A, "null argument")
     refuse("lf_layer_norm_backward_run", back(checkpoint=M()), A, "not both")
-    refuse("lf_layer_norm_backward_run", back(workspace_bytes=16), A, "workspace")
-    refuse("lf_layer_norm_backward_run", back(workspace=p + 4), A, "workspace")
+    many = dict(rows=4096, channels=1)      # (more rows than one block takes; refused before any of them is read)
+    refuse("lf_layer_norm_backward_run", back(**many, workspace_bytes=16), A, "workspace")
+    refuse("lf_layer_norm_backward_run", back(**many, workspace=p + 4), A, "workspace")
     lin = lambda **k: nat.Float8LinearDesc(**{**dict(activations=M(), weights=M(w8), out_dtype=0, out=out.data_ptr()), **k})      # noqa: E731
     refuse("lf_float8_linear_run", lin(out=None), A, "null argument")
     refuse("lf_float8_linear_run", lin(weights=M(w8, channels=63)), S, "expected 64 x 64")
