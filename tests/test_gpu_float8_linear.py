@@ -81,6 +81,22 @@ def test_gradients(dev, rows, c, n, name, dtype):
     xv, wv, dyv = ref.decoded(host(x), "e4m3"), ref.decoded(host(w), "e4m3", 128), ref.decoded(host(dy), name)
     ref.close(dx["output"], dyv @ wv, n * STEP * (np.abs(dyv) @ np.abs(wv)), "input")
     dv = dyv if dtype == "f32" else host(dy)
-    chain = (rows / 16 + 16 + 148) * STEP
+    chain = (min(rows, 4096) / 16 + 16 + max(rows / 4096, 148)) * STEP
     ref.close(grads["weight"], dv.T @ xv, chain * (np.abs(dv).T @ np.abs(xv)), "weight")
     ref.close(grads["bias"], dv.sum(0), chain * np.abs(dv).sum(0), "bias")
+
+
+def test_long_sums(dev):
+    """Values of one sign over many rows, several chains a tile: the bound of a chain holds, and what the tests' shorter sums allow."""
+    import localfold_b200 as lf
+    rows, c, n = 40000, 300, 1200
+    x = torch.rand(rows, c, device="cuda") + 0.5
+    dy = (torch.rand(rows, n, device="cuda") + 0.5).bfloat16()
+    x8 = lf.float8_encode(dev, x, rows, c)
+    values = lf.float8_decode(dev, x8, {"output": "f32"})
+    got = lf.Float8LinearGpu(dev).weight_gradient({"rows": rows, "channels": c, "outChannels": n, "gradient": dy, "activations": x8})
+    dev.synchronize()
+    want = (dy.double().T @ values.double()).cpu().numpy()
+    ref.close(got["weight"], want, (4096 / 16 + 16 + 148) * STEP * want, "weight")
+    sums = dy.double().sum(0).cpu().numpy()
+    ref.close(got["bias"], sums, (4096 / 16 + 16 + 148) * STEP * sums, "bias")
