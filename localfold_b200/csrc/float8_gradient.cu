@@ -6,8 +6,11 @@
 // or comes from codes the same way.  Both operands lie with the summed index outside (MN-major), as they are in memory; nothing is transposed.
 // The column sums of dy are one more product, with a tile of ones of 16 columns, on the blocks of the first column tile.
 //
-// Products are dW's n x k in tiles of 128 x 256 over all rows; there are few tiles and many rows, so the rows are split over as many
+// Products are dW's n x k in tiles of 128 x 256 or 256 x 256 over all rows; there are few tiles and many rows, so the rows are split over as many
 // blocks as the GPU has room for, each writes its float32 partial tile, and a second kernel adds them in order.
+//
+// What bounds it beside the loads is shared memory: of a step of 64 rows and 128 outputs, 144 KB pass through it (codes in and out, operands in, both operands
+// to the tensor core, dy twice with the ones), 1150 cycles for 512 of products.  Two blocks of 128 outputs share x's conversion and operand: 96 KB a block.
 #include <cuda.h>
 
 #include <algorithm>
@@ -24,16 +27,22 @@ lf_status make_map_bytes(lf_context* ctx, CUtensorMap* map, const void* base, ui
 lf_status make_map_rows(lf_context* ctx, CUtensorMap* map, const void* base, bool f32, uint64_t width, uint64_t rows, uint32_t box_rows, bool narrow = false);
 lf_status make_map_f32_any(lf_context* ctx, CUtensorMap* map, const void* base, const uint64_t (&dims)[3], const uint64_t (&strides)[2], const uint32_t (&box)[3]);
 
-constexpr int WG_BN = 128, WG_BK = 256, WG_ROWS = 64;      // outputs, channels, rows of a step
+constexpr int WG_BN = 128, WG_BK = 256, WG_ROWS = 64;      // outputs of a block (a tile has one or two), channels, rows of a step
 constexpr int WG_A_BYTES = WG_BN * WG_ROWS * 2, WG_B_BYTES = WG_BK * WG_ROWS * 2;
 constexpr int WG_CODES = WG_BK * WG_ROWS, WG_DY_CODES = WG_BN * WG_ROWS;
-constexpr int WG_RING = 4, WG_OPERANDS = 2;                // steps on their way from memory, converted ones
+constexpr int WG_OPERANDS = 2;                             // converted steps
 constexpr int WG_CONVERT = 16;                             // warps that convert, and store the tile
 constexpr int WG_THREADS = 64 + 32 * WG_CONVERT;
-// [ring of dy: four bf16 operands, or two that are converted and four times its codes][ring of x's codes][x's operands][exponents][ones]
-constexpr int WG_DY = WG_RING * WG_A_BYTES, WG_EXPONENTS = 2 * 512;
-constexpr int WG_SMEM = WG_DY + WG_RING * (WG_CODES + WG_EXPONENTS) + WG_OPERANDS * WG_B_BYTES + 512 + 256 + 1024;
-static_assert(WG_OPERANDS * WG_A_BYTES + WG_RING * WG_DY_CODES <= WG_DY && WG_CONVERT * 8192 <= WG_DY + WG_RING * WG_CODES, "");
+constexpr int WG_EXPONENTS = 2 * 512;
+// [dy: a ring of bf16 operands, or two that are converted and a ring of its codes][ring of x's codes][x's operands][exponents][ones]
+template <int NB>
+struct GradientShape {
+  static constexpr int a_bytes = NB * WG_A_BYTES, dy_codes = NB * WG_DY_CODES;
+  static constexpr int ring = NB == 1 ? 4 : 3, ring_codes = NB == 1 ? 4 : 2;      // steps on their way from memory; of a dy in codes
+  static constexpr int dy = ring * a_bytes;
+  static constexpr int smem = dy + ring * (WG_CODES + WG_EXPONENTS) + WG_OPERANDS * WG_B_BYTES + 512 + 256 + 1024;
+  static_assert(WG_OPERANDS * a_bytes + ring_codes * dy_codes <= dy && WG_CONVERT * 8192 <= dy + ring * WG_CODES, "");
+};
 
 struct GradientParams {
   int m, n, k;
@@ -75,16 +84,20 @@ __device__ __forceinline__ void convert16(uint4 codes, int s, int format, uint4 
 __device__ __forceinline__ uint32_t piece_at(int row, int piece) { return (piece >> 3) * (WG_ROWS * 128) + row * 128 + (((piece & 7) ^ (row & 7)) << 4); }
 
 // Warp roles: 0 = loads (dy, x's codes, the exponents that belong to them), 1 = MMA issuer (owns TMEM), 2.. = conversion, then the tile's stores.
+template <int NB>
 __global__ void __launch_bounds__(WG_THREADS, 1)
 float8_gradient_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant__ CUtensorMap mapX, const __grid_constant__ CUtensorMap mapO,
                        const GradientParams p) {
+  using S = GradientShape<NB>;
+  constexpr int WG_RING = S::ring;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* dy_s = align_shared(smem_raw);
-  uint8_t* dy_codes = dy_s + WG_OPERANDS * WG_A_BYTES;
-  uint8_t* x_codes = dy_s + WG_DY;
+  uint8_t* dy_codes = dy_s + WG_OPERANDS * S::a_bytes;
+  uint8_t* x_codes = dy_s + S::dy;
   uint8_t* x_s = x_codes + WG_RING * WG_CODES;
   uint8_t* exponents = x_s + WG_OPERANDS * WG_B_BYTES;
   uint8_t* ones = exponents + WG_RING * WG_EXPONENTS;
+  const int ring = p.dy_mode == 2 ? S::ring_codes : S::ring;
   uint64_t* loaded = reinterpret_cast<uint64_t*>(ones + 512);      // [RING] codes, exponents and a bf16 dy are here
   uint64_t* taken = loaded + WG_RING;                              // [RING] their codes are read (and a bf16 dy multiplied)
   uint64_t* full = taken + WG_RING;                                // [OPERANDS]
@@ -94,11 +107,13 @@ float8_gradient_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_co
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int n0 = blockIdx.y * WG_BN, k0 = blockIdx.x * WG_BK, split = blockIdx.z;
+  const int n0 = blockIdx.y * (NB * WG_BN), k0 = blockIdx.x * WG_BK, split = blockIdx.z;
   const int first = split * p.per_split, last = min(first + p.per_split, p.steps);
   const int columns = min(WG_BK, p.k - k0);
   const int groups = (columns + 63) / 64;                   // 64-channel blocks of x that exist
-  const bool sums = blockIdx.x == 0;
+  // dy's sums: in tensor memory behind the products of one block of outputs, or of two, where their channels leave room (else see column_sums_kernel)
+  const bool sums = blockIdx.x == 0 && (NB == 1 || p.k <= 192);
+  const uint32_t sums_at = NB == 1 ? WG_BK : 192;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < WG_RING; ++s) { mbar_init(&loaded[s], 1); mbar_init(&taken[s], WG_CONVERT + (p.dy_mode == 0)); }
@@ -121,7 +136,7 @@ float8_gradient_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_co
       if (p.dy_mode != 1) prefetch_tensormap(&mapA);
       prefetch_tensormap(&mapX);
       const uint32_t x_boxes = columns > 128 ? 2 : 1;
-      const uint32_t bytes = x_boxes * (WG_CODES / 2) + 512 + (p.dy_mode == 0 ? WG_A_BYTES : p.dy_mode == 2 ? WG_DY_CODES + 512 : 0);
+      const uint32_t bytes = x_boxes * (WG_CODES / 2) + 512 + (p.dy_mode == 0 ? S::a_bytes : p.dy_mode == 2 ? S::dy_codes + 512 : 0);
       const uint8_t* ex = p.x.exponents + (int64_t)(k0 >> 9) * p.x.tiles * 512;
       const uint8_t* ey = p.dy8.exponents + (int64_t)(n0 >> 9) * p.dy8.tiles * 512;
       int stage = 0; uint32_t phase = 0;
@@ -132,13 +147,14 @@ float8_gradient_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_co
         for (uint32_t i = 0; i < x_boxes; ++i) tma_load_3d(x_codes + stage * WG_CODES + i * (WG_CODES / 2), &mapX, bar, k0 + i * 128, t * WG_ROWS, 0);
         bulk_load(exponents + stage * WG_EXPONENTS, ex + (int64_t)(t >> 1) * 512, 512, bar);
         if (p.dy_mode == 0) {
-          tma_load_3d(dy_s + stage * WG_A_BYTES, &mapA, bar, n0, t * WG_ROWS, 0);
-          tma_load_3d(dy_s + stage * WG_A_BYTES + WG_A_BYTES / 2, &mapA, bar, n0 + 64, t * WG_ROWS, 0);
+#pragma unroll
+          for (int i = 0; i < 2 * NB; ++i) tma_load_3d(dy_s + stage * S::a_bytes + i * (WG_A_BYTES / 2), &mapA, bar, n0 + 64 * i, t * WG_ROWS, 0);
         } else if (p.dy_mode == 2) {
-          tma_load_3d(dy_codes + stage * WG_DY_CODES, &mapA, bar, n0, t * WG_ROWS, 0);
+#pragma unroll
+          for (int i = 0; i < NB; ++i) tma_load_3d(dy_codes + stage * S::dy_codes + i * WG_DY_CODES, &mapA, bar, n0 + 128 * i, t * WG_ROWS, 0);
           bulk_load(exponents + stage * WG_EXPONENTS + 512, ey + (int64_t)(t >> 1) * 512, 512, bar);
         }
-        if (++stage == WG_RING) { stage = 0; phase ^= 1; }
+        if (++stage == ring) { stage = 0; phase ^= 1; }
       }
     }
   } else if (warp == 1) {
@@ -154,11 +170,15 @@ float8_gradient_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_co
       if (p.dy_mode == 0 && !__all_sync(0xffffffffu, mbar_wait(&loaded[stage], ring_phase, abort_flag, p.status, 136))) break;
       tc_fence_after();
       if (elect_one()) {
-        const uint64_t a = a_first + (uint32_t)((p.dy_mode == 0 ? stage : slot) * (WG_A_BYTES >> 4)), b = b_first + (uint32_t)(slot * (WG_B_BYTES >> 4));
+        const uint64_t a = a_first + (uint32_t)((p.dy_mode == 0 ? stage : slot) * (S::a_bytes >> 4)), b = b_first + (uint32_t)(slot * (WG_B_BYTES >> 4));
 #pragma unroll
         for (int kk = 0; kk < WG_ROWS / 16; ++kk) {
-          umma_f16(tmem_base, a + kk * 128, b + kk * 128, idesc, (t != first || kk != 0) ? 1u : 0u);
-          if (sums) umma_f16(tmem_base + WG_BK, a + kk * 128, ones_desc, idesc_ones, (t != first || kk != 0) ? 1u : 0u);
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb) {
+            const uint64_t ab = a + kk * 128 + nb * (WG_A_BYTES >> 4);
+            umma_f16(tmem_base + nb * WG_BK, ab, b + kk * 128, idesc, (t != first || kk != 0) ? 1u : 0u);
+            if (sums) umma_f16(tmem_base + nb * WG_BK + sums_at, ab, ones_desc, idesc_ones, (t != first || kk != 0) ? 1u : 0u);
+          }
         }
         umma_commit(&empty[slot]);
         if (p.dy_mode == 0) umma_commit(&taken[stage]);
@@ -166,35 +186,39 @@ float8_gradient_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_co
       }
       __syncwarp();
       if (++slot == WG_OPERANDS) { slot = 0; phase ^= 1; }
-      if (++stage == WG_RING) { stage = 0; ring_phase ^= 1; }
+      if (++stage == ring) { stage = 0; ring_phase ^= 1; }
     }
   } else {
     // Rows of a step: x has 16 pieces of 16 channels, dy 8 of 16 outputs; neighbouring lanes take neighbouring pieces of a row.
     const int thread = threadIdx.x - 64;
     constexpr int kUnits = WG_ROWS * 16 / (32 * WG_CONVERT);      // of x a thread
     const int xp = thread & 15, xr = thread >> 4;                 // piece, first row (rows xr + 32 u)
-    const int yp = thread & 7, yr = thread >> 3;                  // of dy, one unit a thread
+    constexpr int kPerRow = 8 * NB, kStep = 32 * WG_CONVERT / kPerRow;      // of dy: NB units a thread, rows yr + kStep u
+    const int yp = thread % kPerRow, yr = thread / kPerRow;
     const int ych = n0 + yp * 16;
-    const int x_block = (k0 >> 7 & 3) + (xp >> 3), y_block = n0 >> 7 & 3;
+    const int x_block = (k0 >> 7 & 3) + (xp >> 3), y_block = (n0 >> 7 & 3) + (yp >> 3);
     const bool x_any = xp < groups * 4, x_here = xp * 16 < (columns > 128 ? 256 : 128);
-    uint4 ahead[2];      // dy_mode 1: the next step's unit
+    uint4 ahead[NB][2];      // dy_mode 1: the next step's units
     auto fetch = [&](int t) {
-      const int64_t row = (int64_t)t * WG_ROWS + yr;
-      const uint16_t* from = reinterpret_cast<const uint16_t*>(p.dy) + row * p.n + ych;
-      uint32_t o[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        o[i] = (row < p.m && ych + 2 * i < p.n ? (uint32_t)from[2 * i] : 0u) | (row < p.m && ych + 2 * i + 1 < p.n ? (uint32_t)from[2 * i + 1] << 16 : 0u);
-      ahead[0] = make_uint4(o[0], o[1], o[2], o[3]);
-      ahead[1] = make_uint4(o[4], o[5], o[6], o[7]);
+      for (int u = 0; u < NB; ++u) {
+        const int64_t row = (int64_t)t * WG_ROWS + yr + kStep * u;
+        const uint16_t* from = reinterpret_cast<const uint16_t*>(p.dy) + row * p.n + ych;
+        uint32_t o[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          o[i] = (row < p.m && ych + 2 * i < p.n ? (uint32_t)from[2 * i] : 0u) | (row < p.m && ych + 2 * i + 1 < p.n ? (uint32_t)from[2 * i + 1] << 16 : 0u);
+        ahead[u][0] = make_uint4(o[0], o[1], o[2], o[3]);
+        ahead[u][1] = make_uint4(o[4], o[5], o[6], o[7]);
+      }
     };
     int slot = 0, stage = 0; uint32_t phase = 0, ring_phase = 0;
     bool ok = true;
     if (p.dy_mode == 1) fetch(first);
     for (int t = first; t < last; ++t) {
       if (!__all_sync(0xffffffffu, mbar_wait(&loaded[stage], ring_phase, abort_flag, p.status, 135))) { ok = false; break; }
-      uint4 codes[kUnits], dy_unit[2];
-      int s[kUnits], sy = 1;
+      uint4 codes[kUnits], dy_unit[NB][2];
+      int s[kUnits], sy[NB];
       const uint8_t* e = exponents + stage * WG_EXPONENTS + (t & 1) * 8;      // (rows 64 .. 127 of a tile: words 2 and 3)
 #pragma unroll
       for (int u = 0; u < kUnits; ++u) {      // row xr + 32 u of the step
@@ -202,17 +226,19 @@ float8_gradient_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_co
         if (x_here) codes[u] = *reinterpret_cast<const uint4*>(x_codes + stage * WG_CODES + (xp >> 3) * (WG_CODES / 2) + swizzle128_offset(xr + 32 * u, xp & 7));
         s[u] = t * WG_ROWS + xr + 32 * u < p.m ? e[xr * 16 + u * 4 + x_block] : 1;      // (bytes behind the last row are of no account)
       }
-      if (p.dy_mode == 2) {
-        dy_unit[0] = *reinterpret_cast<const uint4*>(dy_codes + stage * WG_DY_CODES + swizzle128_offset(yr, yp));
-        sy = t * WG_ROWS + yr < p.m ? e[512 + (yr & 31) * 16 + (yr >> 5) * 4 + y_block] : 1;
-      } else if (p.dy_mode == 1) {
-        dy_unit[0] = ahead[0]; dy_unit[1] = ahead[1];
-        if (t + 1 < last) fetch(t + 1);
+#pragma unroll
+      for (int u = 0; u < NB; ++u) {
+        const int r = yr + kStep * u;
+        if (p.dy_mode == 2) {
+          dy_unit[u][0] = *reinterpret_cast<const uint4*>(dy_codes + stage * S::dy_codes + (yp >> 3) * WG_DY_CODES + swizzle128_offset(r, yp & 7));
+          sy[u] = t * WG_ROWS + r < p.m ? e[512 + (r & 31) * 16 + (r >> 5) * 4 + y_block] : 1;
+        } else if (p.dy_mode == 1) { dy_unit[u][0] = ahead[u][0]; dy_unit[u][1] = ahead[u][1]; }
       }
+      if (p.dy_mode == 1 && t + 1 < last) fetch(t + 1);
       __syncwarp();
       if (lane == 0) mbar_arrive(&taken[stage]);      // the codes are in registers
       if (!__all_sync(0xffffffffu, mbar_wait(&empty[slot], phase ^ 1, abort_flag, p.status, 133))) { ok = false; break; }
-      uint8_t* sA = dy_s + slot * WG_A_BYTES;
+      uint8_t* sA = dy_s + slot * S::a_bytes;
       uint8_t* sB = x_s + slot * WG_B_BYTES;
       // (odd blocks of 64 columns store their second piece first: eight lanes then fill eight different 16-byte columns of the banks)
       if (x_any) {
@@ -227,59 +253,69 @@ float8_gradient_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_co
         }
       }
       if (p.dy_mode != 0) {
-        uint4 v[2] = {dy_unit[0], dy_unit[1]};
-        if (p.dy_mode == 2) convert16(dy_unit[0], sy, p.dy8.format, v);
         const int swap = yp >> 2 & 1;
-        *reinterpret_cast<uint4*>(sA + piece_at(yr, yp * 2 + swap)) = swap ? v[1] : v[0];
-        *reinterpret_cast<uint4*>(sA + piece_at(yr, yp * 2 + 1 - swap)) = swap ? v[0] : v[1];
+#pragma unroll
+        for (int u = 0; u < NB; ++u) {
+          uint4 v[2] = {dy_unit[u][0], dy_unit[u][1]};
+          if (p.dy_mode == 2) convert16(dy_unit[u][0], sy[u], p.dy8.format, v);
+          const int row = yr + kStep * u;
+          *reinterpret_cast<uint4*>(sA + piece_at(row, yp * 2 + swap)) = swap ? v[1] : v[0];
+          *reinterpret_cast<uint4*>(sA + piece_at(row, yp * 2 + 1 - swap)) = swap ? v[0] : v[1];
+        }
       }
       fence_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&full[slot]);
       if (++slot == WG_OPERANDS) { slot = 0; phase ^= 1; }
-      if (++stage == WG_RING) { stage = 0; ring_phase ^= 1; }
+      if (++stage == ring) { stage = 0; ring_phase ^= 1; }
     }
     // The tile: 16 warps, 64 columns of a lane quadrant each.
     ok = ok && __all_sync(0xffffffffu, mbar_wait(done, 0, abort_flag, p.status, 134));
     tc_fence_after();
     if (ok) {
-      const int q = warp & 3, part = (warp - 2) >> 2, row0 = n0 + q * 32, col0 = k0 + part * 64;
+      const int q = warp & 3, part = (warp - 2) >> 2, col0 = k0 + part * 64;
       uint8_t* tiles = dy_s + (warp - 2) * 8192;      // (every product is done: the rings of dy and of x's codes are free)
       float* out = p.out + split * p.split_stride;
-      if (row0 < p.n && col0 < p.k) {
-        uint32_t r[2][32];
-        const uint32_t d = tmem_base + ((uint32_t)(q * 32) << 16) + part * 64;
-        tmem_ld32(d, r[0]);
-        tmem_ld32(d + 32, r[1]);
-        tmem_ld_wait();
-        tie32(r[0]);
-        tie32(r[1]);
+#pragma unroll 1
+      for (int nb = 0; nb < NB; ++nb) {
+        const int row0 = n0 + nb * WG_BN + q * 32;
+        const uint32_t d = tmem_base + ((uint32_t)(q * 32) << 16) + nb * WG_BK;
+        if (row0 < p.n && col0 < p.k) {
+          uint32_t r[2][32];
+          tmem_ld32(d + part * 64, r[0]);
+          tmem_ld32(d + part * 64 + 32, r[1]);
+          if (lane == 0) bulk_wait_read();      // the copies of the block before have read the staging rows
+          __syncwarp();
+          tmem_ld_wait();
+          tie32(r[0]);
+          tie32(r[1]);
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const int c0 = col0 + half * 32;
-          if (c0 >= p.k) break;
-          uint8_t* tile = tiles + half * 4096;
+          for (int half = 0; half < 2; ++half) {
+            const int c0 = col0 + half * 32;
+            if (c0 >= p.k) break;
+            uint8_t* tile = tiles + half * 4096;
 #pragma unroll
-          for (int c = 0; c < 8; ++c)
-            *reinterpret_cast<uint4*>(tile + lane * 128 + ((c ^ (lane & 7)) << 4)) = make_uint4(r[half][c * 4], r[half][c * 4 + 1], r[half][c * 4 + 2], r[half][c * 4 + 3]);
-          if (p.vector_out) {
-            fence_async_smem();
-            __syncwarp();
-            if (lane == 0) { tma_store_3d(&mapO, tile, c0, row0, split); bulk_commit(); }
-          } else {
-            __syncwarp();
-            const int rows = min(32, p.n - row0);
-            for (int row = 0; row < rows; ++row)
-              if (c0 + lane < p.k) out[(int64_t)(row0 + row) * p.ld + c0 + lane] = *reinterpret_cast<const float*>(tile + row * 128 + (((lane >> 2) ^ (row & 7)) << 4) + (lane & 3) * 4);
-            __syncwarp();
+            for (int c = 0; c < 8; ++c)
+              *reinterpret_cast<uint4*>(tile + swizzle128_offset(lane, c)) = make_uint4(r[half][c * 4], r[half][c * 4 + 1], r[half][c * 4 + 2], r[half][c * 4 + 3]);
+            if (p.vector_out) {
+              fence_async_smem();
+              __syncwarp();
+              if (lane == 0) { tma_store_3d(&mapO, tile, c0, row0, split); bulk_commit(); }
+            } else {
+              __syncwarp();
+              const int rows = min(32, p.n - row0);
+              for (int row = 0; row < rows; ++row)
+                if (c0 + lane < p.k) out[(int64_t)(row0 + row) * p.ld + c0 + lane] = *reinterpret_cast<const float*>(tile + swizzle128_offset(row, lane >> 2) + (lane & 3) * 4);
+              __syncwarp();
+            }
           }
         }
-      }
-      if (sums && part == 0) {
-        uint32_t r[8];
-        tmem_ld8(tmem_base + ((uint32_t)(q * 32) << 16) + WG_BK, r);
-        tmem_ld_wait();
-        if (p.bias && row0 + lane < p.n) p.bias[split * p.bias_stride + row0 + lane] = __uint_as_float(r[0]);
+        if (sums && part == 0) {
+          uint32_t r[8];
+          tmem_ld8(d + sums_at, r);
+          tmem_ld_wait();
+          if (p.bias && row0 + lane < p.n) p.bias[split * p.bias_stride + row0 + lane] = __uint_as_float(r[0]);
+        }
       }
     }
     if (lane == 0) bulk_wait_all();
@@ -344,13 +380,62 @@ gradient_join_kernel(const float* partial, int ld, int64_t split_stride, int spl
   }
 }
 
-void configure_float8_gradient() { cudaFuncSetAttribute(float8_gradient_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, WG_SMEM); }
+// The column sums of a split's rows of dy for tiles of two blocks of outputs, which have no columns of tensor memory left for them: 32 columns a block; MODE
+// as dy_mode.  A thread has 8, 1 or 16 neighbouring columns of every kStrands-th row.
+template <int MODE>
+__global__ void __launch_bounds__(MODE == 2 ? 512 : 1024)
+column_sums_kernel(const GradientParams p) {
+  constexpr int kThreads = MODE == 2 ? 512 : 1024, kColumns = MODE == 0 ? 8 : MODE == 1 ? 1 : 16, kLanes = 32 / kColumns, kStrands = kThreads / kLanes;
+  __shared__ float s[kStrands][33];
+  const int lane = threadIdx.x % kLanes, strand = threadIdx.x / kLanes, col = blockIdx.x * 32 + lane * kColumns;
+  const int64_t first = (int64_t)blockIdx.y * p.per_split * WG_ROWS, last = min(first + (int64_t)p.per_split * WG_ROWS, (int64_t)p.m);
+  lf_chain();
+  float t[kColumns];
+#pragma unroll
+  for (int i = 0; i < kColumns; ++i) t[i] = 0.f;
+  if (col < p.n) {
+#pragma unroll 8
+    for (int64_t row = first + strand; row < last; row += kStrands) {
+      if (MODE == 0) {
+        const uint4 u = *reinterpret_cast<const uint4*>(p.dy + row * p.n + col);
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { t[(2 * i) % kColumns] += __uint_as_float(w[i] << 16); t[(2 * i + 1) % kColumns] += __uint_as_float(w[i] & 0xffff0000u); }
+      } else if (MODE == 1) t[0] += __bfloat162float(p.dy[row * p.n + col]);
+      else {
+        const f8::Share v = f8::decode16(*reinterpret_cast<const uint4*>(p.dy8.codes + row * p.dy8.pitch + col), p.dy8.format);
+        const float factor = f8::up(p.dy8.exponents[f8::exponent_at(row, col / f8::kBlock, p.dy8.tiles)]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) { t[(2 * i) % kColumns] = fmaf(v.v[i].x, factor, t[(2 * i) % kColumns]); t[(2 * i + 1) % kColumns] = fmaf(v.v[i].y, factor, t[(2 * i + 1) % kColumns]); }
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kColumns; ++i) s[strand][lane * kColumns + i] = t[i];
+  __syncthreads();
+  for (int c = threadIdx.x >> 5; c < 32; c += kThreads / 32) {
+    float u = 0.f;
+    for (int i = threadIdx.x & 31; i < kStrands; i += 32) u += s[i][c];
+#pragma unroll
+    for (int o = 16; o; o >>= 1) u += __shfl_xor_sync(0xffffffffu, u, o);
+    if ((threadIdx.x & 31) == 0 && blockIdx.x * 32 + c < p.n) p.bias[blockIdx.y * p.bias_stride + blockIdx.x * 32 + c] = u;
+  }
+}
+
+void configure_float8_gradient() {
+  cudaFuncSetAttribute(float8_gradient_kernel<1>, cudaFuncAttributeMaxDynamicSharedMemorySize, GradientShape<1>::smem);
+  cudaFuncSetAttribute(float8_gradient_kernel<2>, cudaFuncAttributeMaxDynamicSharedMemorySize, GradientShape<2>::smem);
+}
+
+// Blocks of outputs of a tile: two where there are two and the sums of dy come with the products (at most 192 channels), or where a launch of their own is little
+// beside them (2^32 multiplications: about 20 us).
+static int gradient_blocks(int64_t m, int n, int k) { return n > WG_BN && (k <= 192 || (double)m * n * k >= 4294967296.0) ? 2 : 1; }
 
 // Blocks of rows: as many as the GPU has multiprocessors for beside the tiles, with four steps of 64 rows each at least - and 64 at most: the tensor core's
-// additions truncate, and 65536 x 1024 x 1024 with values of one sign was 3.5e-5 off in sums of 16384 rows (9e-6 in 4096).
+// additions truncate, and 65536 x 1024 x 1024 with values of one sign was 3.5e-5 off in sums of 16384 rows (5.8e-6 in 4096).
 static void gradient_plan(const lf_context* ctx, int64_t m, int n, int k, int& steps, int& splits, int& per_split) {
   constexpr int kMostSteps = 64, kMostSplits = 65535;
-  const int tiles = ((n + WG_BN - 1) / WG_BN) * ((k + WG_BK - 1) / WG_BK);
+  const int outputs = WG_BN * gradient_blocks(m, n, k), tiles = ((n + outputs - 1) / outputs) * ((k + WG_BK - 1) / WG_BK);
   steps = (int)((m + WG_ROWS - 1) / WG_ROWS);
   const int want = std::max(1, std::min(ctx->sm_count / tiles, steps / 4)), most = std::max(kMostSteps, (steps + kMostSplits - 1) / kMostSplits);
   per_split = (steps + want - 1) / want;
@@ -418,9 +503,23 @@ lf_status lf_float8_weight_gradient_run(lf_context* ctx, const lf_float8_weight_
     LF_TRY(tc::make_map_f32_any(ctx, &mo, p.out, {(uint64_t)p.k, (uint64_t)p.n, (uint64_t)splits}, {(uint64_t)p.ld * 4, (uint64_t)p.ld * 4 * p.n}, {32, 32, 1}));
   p.status = (tc05::Status*)ctx->tc_status;
   lf_prof_begin(ctx, LF_KERNEL_TRIANGLE_CONTRACT);
-  lf_launch(ctx, tc::float8_gradient_kernel, dim3((p.k + tc::WG_BK - 1) / tc::WG_BK, (p.n + tc::WG_BN - 1) / tc::WG_BN, splits), tc::WG_THREADS, tc::WG_SMEM, ma, mx, mo, p);
+  const int blocks = tc::gradient_blocks(x.rows, p.n, p.k), outputs = tc::WG_BN * blocks;
+  const dim3 grid((p.k + tc::WG_BK - 1) / tc::WG_BK, (p.n + outputs - 1) / outputs, splits);
+  if (blocks == 2) lf_launch(ctx, tc::float8_gradient_kernel<2>, grid, tc::WG_THREADS, tc::GradientShape<2>::smem, ma, mx, mo, p);
+  else lf_launch(ctx, tc::float8_gradient_kernel<1>, grid, tc::WG_THREADS, tc::GradientShape<1>::smem, ma, mx, mo, p);
   lf_prof_end(ctx);
   ctx->launches++;
+  int launches = 1;
+  if (blocks == 2 && p.k > 192 && p.bias) {
+    const dim3 grid2((p.n + 31) / 32, splits);
+    lf_prof_begin(ctx, LF_KERNEL_ELEMENTWISE);
+    if (p.dy_mode == 0) lf_launch(ctx, tc::column_sums_kernel<0>, grid2, 1024, 0, p);
+    else if (p.dy_mode == 1) lf_launch(ctx, tc::column_sums_kernel<1>, grid2, 1024, 0, p);
+    else lf_launch(ctx, tc::column_sums_kernel<2>, grid2, 512, 0, p);
+    lf_prof_end(ctx);
+    ctx->launches++;
+    ++launches;
+  }
   if (!direct) {
     lf_prof_begin(ctx, LF_KERNEL_ELEMENTWISE);
     const int64_t fours = (int64_t)p.n * (p.ld / 4);
@@ -433,7 +532,7 @@ lf_status lf_float8_weight_gradient_run(lf_context* ctx, const lf_float8_weight_
     lf_prof_end(ctx);
     ctx->launches++;
   }
-  return lf_float8_done(ctx, r, direct ? 1 : 2);
+  return lf_float8_done(ctx, r, launches + !direct);
 }
 
 }  // extern "C"
