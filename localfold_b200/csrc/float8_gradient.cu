@@ -4,13 +4,18 @@
 // The sum runs over the rows, whose exponents differ, so the exponent has to be in the operand: codes become bf16 values on the way to
 // shared memory (exactly: four significant bits times a power of two), and tcgen05.mma of kind f16 multiplies them with dy, which is bf16
 // or comes from codes the same way.  Both operands lie with the summed index outside (MN-major), as they are in memory; nothing is transposed.
-// The column sums of dy are one more product, with a tile of ones of 16 columns, on the blocks of the first column tile.
+// The column sums of dy are added up by two warps of the first column tile's blocks, from the operand in shared memory.  (By the converting warps: 262144 x 128 -> 512
+// 66 -> 88 us, from codes 78 -> 175.)
+//
+// The tensor core's additions to an accumulator truncate: their error grows with how many there are (one for 16 rows).  So all of the 512 columns of tensor
+// memory are accumulators that take steps in turn (two of 256 channels, or four of 128, for one block of outputs), added up in registers at the end, and
+// a split has 4096 rows at most.
 //
 // Products are dW's n x k in tiles of 128 x 256 or 256 x 256 over all rows; there are few tiles and many rows, so the rows are split over as many
 // blocks as the GPU has room for, each writes its float32 partial tile, and a second kernel adds them in order.
 //
-// What bounds it beside the loads is shared memory: of a step of 64 rows and 128 outputs, 144 KB pass through it (codes in and out, operands in, both operands
-// to the tensor core, dy twice with the ones), 1150 cycles for 512 of products.  Two blocks of 128 outputs share x's conversion and operand: 96 KB a block.
+// What bounds it beside the loads is shared memory: of a step of 64 rows and 128 outputs, 128 KB pass through it (codes in and out, operands in, both operands
+// to the tensor core), 1000 cycles for 512 of products.  Two blocks of 128 outputs share x's conversion and operand: 96 KB a block.
 #include <cuda.h>
 
 #include <algorithm>
@@ -32,22 +37,22 @@ constexpr int WG_A_BYTES = WG_BN * WG_ROWS * 2, WG_B_BYTES = WG_BK * WG_ROWS * 2
 constexpr int WG_CODES = WG_BK * WG_ROWS, WG_DY_CODES = WG_BN * WG_ROWS;
 constexpr int WG_OPERANDS = 2;                             // converted steps
 constexpr int WG_CONVERT = 16;                             // warps that convert, and store the tile
-constexpr int WG_THREADS = 64 + 32 * WG_CONVERT;
+constexpr int WG_SUMS = 2;                                 // warps that add up dy's columns
+constexpr int WG_THREADS = 64 + 32 * (WG_CONVERT + WG_SUMS);
 constexpr int WG_EXPONENTS = 2 * 512;
-// [dy: a ring of bf16 operands, or two that are converted and a ring of its codes][ring of x's codes][x's operands][exponents][ones]
+// [dy: a ring of bf16 operands, or two that are converted and a ring of its codes][ring of x's codes][x's operands][exponents]
 template <int NB>
 struct GradientShape {
   static constexpr int a_bytes = NB * WG_A_BYTES, dy_codes = NB * WG_DY_CODES;
   static constexpr int ring = NB == 1 ? 4 : 3, ring_codes = NB == 1 ? 4 : 2;      // steps on their way from memory; of a dy in codes
   static constexpr int dy = ring * a_bytes;
-  static constexpr int smem = dy + ring * (WG_CODES + WG_EXPONENTS) + WG_OPERANDS * WG_B_BYTES + 512 + 256 + 1024;
+  static constexpr int smem = dy + ring * (WG_CODES + WG_EXPONENTS) + WG_OPERANDS * WG_B_BYTES + 256 + 1024;
   static_assert(WG_OPERANDS * a_bytes + ring_codes * dy_codes <= dy && WG_CONVERT * 8192 <= dy + ring * WG_CODES, "");
 };
 
 struct GradientParams {
   int m, n, k;
   int steps, per_split;          // steps of 64 rows in all, and of a split
-  int dy_mode;                   // 0: by TMA, 1: bf16 rows that no 16-byte access divides, 2: codes
   const bf16* dy;
   f8::Matrix dy8, x;
   float* out;                    // [split][n][ld] partial tiles, or dW itself
@@ -83,8 +88,10 @@ __device__ __forceinline__ void convert16(uint4 codes, int s, int format, uint4 
 // The place of a piece of eight columns in an MN-major operand: blocks of 64 columns, rows of 128 bytes, 128-byte swizzle.
 __device__ __forceinline__ uint32_t piece_at(int row, int piece) { return (piece >> 3) * (WG_ROWS * 128) + row * 128 + (((piece & 7) ^ (row & 7)) << 4); }
 
-// Warp roles: 0 = loads (dy, x's codes, the exponents that belong to them), 1 = MMA issuer (owns TMEM), 2.. = conversion, then the tile's stores.
-template <int NB>
+// Warp roles: 0 = loads (dy, x's codes, the exponents that belong to them), 1 = MMA issuer (owns TMEM), 2..17 = conversion, then the tile's stores, 18 and 19 =
+// dy's sums.
+// MODE: how dy comes, by TMA (0), as bf16 rows that no 16-byte access divides (1), as codes (2).
+template <int NB, int MODE>
 __global__ void __launch_bounds__(WG_THREADS, 1)
 float8_gradient_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant__ CUtensorMap mapX, const __grid_constant__ CUtensorMap mapO,
                        const GradientParams p) {
@@ -96,9 +103,8 @@ float8_gradient_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_co
   uint8_t* x_codes = dy_s + S::dy;
   uint8_t* x_s = x_codes + WG_RING * WG_CODES;
   uint8_t* exponents = x_s + WG_OPERANDS * WG_B_BYTES;
-  uint8_t* ones = exponents + WG_RING * WG_EXPONENTS;
-  const int ring = p.dy_mode == 2 ? S::ring_codes : S::ring;
-  uint64_t* loaded = reinterpret_cast<uint64_t*>(ones + 512);      // [RING] codes, exponents and a bf16 dy are here
+  const int ring = MODE == 2 ? S::ring_codes : S::ring;
+  uint64_t* loaded = reinterpret_cast<uint64_t*>(exponents + WG_RING * WG_EXPONENTS);      // [RING] codes, exponents and a bf16 dy are here
   uint64_t* taken = loaded + WG_RING;                              // [RING] their codes are read (and a bf16 dy multiplied)
   uint64_t* full = taken + WG_RING;                                // [OPERANDS]
   uint64_t* empty = full + WG_OPERANDS;
@@ -111,19 +117,16 @@ float8_gradient_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_co
   const int first = split * p.per_split, last = min(first + p.per_split, p.steps);
   const int columns = min(WG_BK, p.k - k0);
   const int groups = (columns + 63) / 64;                   // 64-channel blocks of x that exist
-  // dy's sums: in tensor memory behind the products of one block of outputs, or of two, where their channels leave room (else see column_sums_kernel)
-  const bool sums = blockIdx.x == 0 && (NB == 1 || p.k <= 192);
-  const uint32_t sums_at = NB == 1 ? WG_BK : 192;
+  const bool sums = blockIdx.x == 0 && p.bias;              // dy's, too
+  const int wide = columns > 128 ? 256 : 128, accumulators = 512 / (NB * wide);
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < WG_RING; ++s) { mbar_init(&loaded[s], 1); mbar_init(&taken[s], WG_CONVERT + (p.dy_mode == 0)); }
-    for (int s = 0; s < WG_OPERANDS; ++s) { mbar_init(&full[s], WG_CONVERT); mbar_init(&empty[s], 1); }
+    for (int s = 0; s < WG_RING; ++s) { mbar_init(&loaded[s], 1); mbar_init(&taken[s], WG_CONVERT + (MODE == 0 ? 1 + (sums ? WG_SUMS : 0) : 0)); }
+    for (int s = 0; s < WG_OPERANDS; ++s) { mbar_init(&full[s], WG_CONVERT); mbar_init(&empty[s], 1 + (MODE != 0 && sums ? WG_SUMS : 0)); }
     mbar_init(done, 1);
     *abort_flag = 0;
     fence_barrier_init();
   }
-  if (threadIdx.x < 128) reinterpret_cast<uint32_t*>(ones)[threadIdx.x] = 0x3f803f80u;
-  fence_async_smem();
   if (warp == 1) { tmem_alloc(tmem_slot, 512); tmem_relinquish(); }
   tc_fence_before();
   __syncthreads();
@@ -133,10 +136,10 @@ float8_gradient_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_co
 
   if (warp == 0) {
     if (lane == 0) {
-      if (p.dy_mode != 1) prefetch_tensormap(&mapA);
+      if (MODE != 1) prefetch_tensormap(&mapA);
       prefetch_tensormap(&mapX);
       const uint32_t x_boxes = columns > 128 ? 2 : 1;
-      const uint32_t bytes = x_boxes * (WG_CODES / 2) + 512 + (p.dy_mode == 0 ? S::a_bytes : p.dy_mode == 2 ? S::dy_codes + 512 : 0);
+      const uint32_t bytes = x_boxes * (WG_CODES / 2) + 512 + (MODE == 0 ? S::a_bytes : MODE == 2 ? S::dy_codes + 512 : 0);
       const uint8_t* ex = p.x.exponents + (int64_t)(k0 >> 9) * p.x.tiles * 512;
       const uint8_t* ey = p.dy8.exponents + (int64_t)(n0 >> 9) * p.dy8.tiles * 512;
       int stage = 0; uint32_t phase = 0;
@@ -146,10 +149,10 @@ float8_gradient_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_co
         mbar_expect_tx(bar, bytes);
         for (uint32_t i = 0; i < x_boxes; ++i) tma_load_3d(x_codes + stage * WG_CODES + i * (WG_CODES / 2), &mapX, bar, k0 + i * 128, t * WG_ROWS, 0);
         bulk_load(exponents + stage * WG_EXPONENTS, ex + (int64_t)(t >> 1) * 512, 512, bar);
-        if (p.dy_mode == 0) {
+        if (MODE == 0) {
 #pragma unroll
           for (int i = 0; i < 2 * NB; ++i) tma_load_3d(dy_s + stage * S::a_bytes + i * (WG_A_BYTES / 2), &mapA, bar, n0 + 64 * i, t * WG_ROWS, 0);
-        } else if (p.dy_mode == 2) {
+        } else if (MODE == 2) {
 #pragma unroll
           for (int i = 0; i < NB; ++i) tma_load_3d(dy_codes + stage * S::dy_codes + i * WG_DY_CODES, &mapA, bar, n0 + 128 * i, t * WG_ROWS, 0);
           bulk_load(exponents + stage * WG_EXPONENTS + 512, ey + (int64_t)(t >> 1) * 512, 512, bar);
@@ -159,34 +162,68 @@ float8_gradient_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_co
     }
   } else if (warp == 1) {
     // (the whole warp walks and waits, so that what the instructions take stays in uniform registers; one lane issues)
-    int slot = 0, stage = 0; uint32_t phase = 0, ring_phase = 0;
+    int slot = 0, stage = 0, acc = 0; uint32_t phase = 0, ring_phase = 0;
     constexpr uint32_t both = (1u << 7) | (1u << 10);      // bf16 operands
-    const uint32_t idesc = make_idesc_f16(WG_BN, groups * 64, 1, 1) | both, idesc_ones = make_idesc_f16(WG_BN, 16, 1, 0) | both;
-    const uint64_t ones_desc = make_smem_desc_plain(smem_u32(ones), 128, 256);
+    const uint32_t idesc = make_idesc_f16(WG_BN, groups * 64, 1, 1) | both;
     const uint64_t a_first = make_smem_desc(smem_u32(dy_s), WG_ROWS * 128, 1024), b_first = make_smem_desc(smem_u32(x_s), WG_ROWS * 128, 1024);
     for (int t = first; t < last; ++t) {
       // (an expired wait ends the loop for all lanes alike)
       if (!__all_sync(0xffffffffu, mbar_wait(&full[slot], phase, abort_flag, p.status, 132))) break;
-      if (p.dy_mode == 0 && !__all_sync(0xffffffffu, mbar_wait(&loaded[stage], ring_phase, abort_flag, p.status, 136))) break;
+      if (MODE == 0 && !__all_sync(0xffffffffu, mbar_wait(&loaded[stage], ring_phase, abort_flag, p.status, 136))) break;
       tc_fence_after();
       if (elect_one()) {
-        const uint64_t a = a_first + (uint32_t)((p.dy_mode == 0 ? stage : slot) * (S::a_bytes >> 4)), b = b_first + (uint32_t)(slot * (WG_B_BYTES >> 4));
+        const uint64_t a = a_first + (uint32_t)((MODE == 0 ? stage : slot) * (S::a_bytes >> 4)), b = b_first + (uint32_t)(slot * (WG_B_BYTES >> 4));
 #pragma unroll
         for (int kk = 0; kk < WG_ROWS / 16; ++kk) {
 #pragma unroll
-          for (int nb = 0; nb < NB; ++nb) {
-            const uint64_t ab = a + kk * 128 + nb * (WG_A_BYTES >> 4);
-            umma_f16(tmem_base + nb * WG_BK, ab, b + kk * 128, idesc, (t != first || kk != 0) ? 1u : 0u);
-            if (sums) umma_f16(tmem_base + nb * WG_BK + sums_at, ab, ones_desc, idesc_ones, (t != first || kk != 0) ? 1u : 0u);
-          }
+          for (int nb = 0; nb < NB; ++nb)
+            umma_f16(tmem_base + (acc * NB + nb) * wide, a + kk * 128 + nb * (WG_A_BYTES >> 4), b + kk * 128, idesc, (t - first >= accumulators || kk != 0) ? 1u : 0u);
         }
         umma_commit(&empty[slot]);
-        if (p.dy_mode == 0) umma_commit(&taken[stage]);
+        if (MODE == 0) umma_commit(&taken[stage]);
         if (t + 1 == last) umma_commit(done);
       }
       __syncwarp();
+      if (++acc == accumulators) acc = 0;
       if (++slot == WG_OPERANDS) { slot = 0; phase ^= 1; }
       if (++stage == ring) { stage = 0; ring_phase ^= 1; }
+    }
+  } else if (warp >= 2 + WG_CONVERT) {
+    // A warp has NB blocks of 64 outputs: eight columns a lane, every fourth row.
+    if (sums) {
+      const int w = warp - 2 - WG_CONVERT, piece = lane & 7, r0 = lane >> 3;
+      float2 total[NB][4];
+#pragma unroll
+      for (int i = 0; i < NB * 4; ++i) total[i / 4][i % 4] = make_float2(0.f, 0.f);
+      int slot = 0, stage = 0; uint32_t phase = 0, ring_phase = 0;
+      for (int t = first; t < last; ++t) {
+        const bool here = MODE == 0 ? mbar_wait(&loaded[stage], ring_phase, abort_flag, p.status, 137) : mbar_wait(&full[slot], phase, abort_flag, p.status, 138);
+        if (!__all_sync(0xffffffffu, here)) break;
+        const uint8_t* sA = dy_s + (MODE == 0 ? stage : slot) * S::a_bytes;
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll 8
+          for (int r = r0; r < WG_ROWS; r += 4) {
+            const uint4 u = *reinterpret_cast<const uint4*>(sA + piece_at(r, (w * NB + b) * 8 + piece));
+            const uint32_t v[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) total[b][i] = add2(total[b][i], make_float2(__uint_as_float(v[i] << 16), __uint_as_float(v[i] & 0xffff0000u)));
+          }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(MODE == 0 ? &taken[stage] : &empty[slot]);
+        if (++slot == WG_OPERANDS) { slot = 0; phase ^= 1; }
+        if (++stage == ring) { stage = 0; ring_phase ^= 1; }
+      }
+#pragma unroll
+      for (int i = 0; i < NB * 4; ++i) {
+        float2 v = total[i / 4][i % 4];
+#pragma unroll
+        for (int o = 8; o < 32; o *= 2) { v.x += __shfl_xor_sync(0xffffffffu, v.x, o); v.y += __shfl_xor_sync(0xffffffffu, v.y, o); }
+        const int n = n0 + (w * NB + i / 4) * 64 + piece * 8 + i % 4 * 2;
+        float* to = p.bias + split * p.bias_stride + n;
+        if (r0 == 0 && n < p.n) to[0] = v.x;
+        if (r0 == 0 && n + 1 < p.n) to[1] = v.y;
+      }
     }
   } else {
     // Rows of a step: x has 16 pieces of 16 channels, dy 8 of 16 outputs; neighbouring lanes take neighbouring pieces of a row.
@@ -198,7 +235,7 @@ float8_gradient_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_co
     const int ych = n0 + yp * 16;
     const int x_block = (k0 >> 7 & 3) + (xp >> 3), y_block = (n0 >> 7 & 3) + (yp >> 3);
     const bool x_any = xp < groups * 4, x_here = xp * 16 < (columns > 128 ? 256 : 128);
-    uint4 ahead[NB][2];      // dy_mode 1: the next step's units
+    uint4 ahead[NB][2];      // MODE 1: the next step's units
     auto fetch = [&](int t) {
 #pragma unroll
       for (int u = 0; u < NB; ++u) {
@@ -214,7 +251,7 @@ float8_gradient_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_co
     };
     int slot = 0, stage = 0; uint32_t phase = 0, ring_phase = 0;
     bool ok = true;
-    if (p.dy_mode == 1) fetch(first);
+    if (MODE == 1) fetch(first);
     for (int t = first; t < last; ++t) {
       if (!__all_sync(0xffffffffu, mbar_wait(&loaded[stage], ring_phase, abort_flag, p.status, 135))) { ok = false; break; }
       uint4 codes[kUnits], dy_unit[NB][2];
@@ -229,12 +266,12 @@ float8_gradient_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_co
 #pragma unroll
       for (int u = 0; u < NB; ++u) {
         const int r = yr + kStep * u;
-        if (p.dy_mode == 2) {
+        if (MODE == 2) {
           dy_unit[u][0] = *reinterpret_cast<const uint4*>(dy_codes + stage * S::dy_codes + (yp >> 3) * WG_DY_CODES + swizzle128_offset(r, yp & 7));
           sy[u] = t * WG_ROWS + r < p.m ? e[512 + (r & 31) * 16 + (r >> 5) * 4 + y_block] : 1;
-        } else if (p.dy_mode == 1) { dy_unit[u][0] = ahead[u][0]; dy_unit[u][1] = ahead[u][1]; }
+        } else if (MODE == 1) { dy_unit[u][0] = ahead[u][0]; dy_unit[u][1] = ahead[u][1]; }
       }
-      if (p.dy_mode == 1 && t + 1 < last) fetch(t + 1);
+      if (MODE == 1 && t + 1 < last) fetch(t + 1);
       __syncwarp();
       if (lane == 0) mbar_arrive(&taken[stage]);      // the codes are in registers
       if (!__all_sync(0xffffffffu, mbar_wait(&empty[slot], phase ^ 1, abort_flag, p.status, 133))) { ok = false; break; }
@@ -252,12 +289,12 @@ float8_gradient_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_co
           *reinterpret_cast<uint4*>(sB + piece_at(row, xp * 2 + 1 - swap)) = swap ? v[0] : v[1];
         }
       }
-      if (p.dy_mode != 0) {
+      if (MODE != 0) {
         const int swap = yp >> 2 & 1;
 #pragma unroll
         for (int u = 0; u < NB; ++u) {
           uint4 v[2] = {dy_unit[u][0], dy_unit[u][1]};
-          if (p.dy_mode == 2) convert16(dy_unit[u][0], sy[u], p.dy8.format, v);
+          if (MODE == 2) convert16(dy_unit[u][0], sy[u], p.dy8.format, v);
           const int row = yr + kStep * u;
           *reinterpret_cast<uint4*>(sA + piece_at(row, yp * 2 + swap)) = swap ? v[1] : v[0];
           *reinterpret_cast<uint4*>(sA + piece_at(row, yp * 2 + 1 - swap)) = swap ? v[0] : v[1];
@@ -276,19 +313,30 @@ float8_gradient_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_co
       const int q = warp & 3, part = (warp - 2) >> 2, col0 = k0 + part * 64;
       uint8_t* tiles = dy_s + (warp - 2) * 8192;      // (every product is done: the rings of dy and of x's codes are free)
       float* out = p.out + split * p.split_stride;
+      const int used = min(accumulators, last - first);
 #pragma unroll 1
       for (int nb = 0; nb < NB; ++nb) {
         const int row0 = n0 + nb * WG_BN + q * 32;
-        const uint32_t d = tmem_base + ((uint32_t)(q * 32) << 16) + nb * WG_BK;
+        const uint32_t d = tmem_base + ((uint32_t)(q * 32) << 16) + nb * wide + part * 64;
         if (row0 < p.n && col0 < p.k) {
           uint32_t r[2][32];
-          tmem_ld32(d + part * 64, r[0]);
-          tmem_ld32(d + part * 64 + 32, r[1]);
+          tmem_ld32(d, r[0]);
+          tmem_ld32(d + 32, r[1]);
           if (lane == 0) bulk_wait_read();      // the copies of the block before have read the staging rows
           __syncwarp();
           tmem_ld_wait();
           tie32(r[0]);
           tie32(r[1]);
+          for (int i = 1; i < used; ++i)
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              uint32_t more[32];
+              tmem_ld32(d + i * NB * wide + half * 32, more);
+              tmem_ld_wait();
+              tie32(more);
+#pragma unroll
+              for (int c = 0; c < 32; ++c) r[half][c] = __float_as_uint(__uint_as_float(r[half][c]) + __uint_as_float(more[c]));
+            }
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
             const int c0 = col0 + half * 32;
@@ -309,12 +357,6 @@ float8_gradient_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_co
               __syncwarp();
             }
           }
-        }
-        if (sums && part == 0) {
-          uint32_t r[8];
-          tmem_ld8(d + sums_at, r);
-          tmem_ld_wait();
-          if (p.bias && row0 + lane < p.n) p.bias[split * p.bias_stride + row0 + lane] = __uint_as_float(r[0]);
         }
       }
     }
@@ -380,56 +422,28 @@ gradient_join_kernel(const float* partial, int ld, int64_t split_stride, int spl
   }
 }
 
-// The column sums of a split's rows of dy for tiles of two blocks of outputs, which have no columns of tensor memory left for them: 32 columns a block; MODE
-// as dy_mode.  A thread has 8, 1 or 16 neighbouring columns of every kStrands-th row.
-template <int MODE>
-__global__ void __launch_bounds__(MODE == 2 ? 512 : 1024)
-column_sums_kernel(const GradientParams p) {
-  constexpr int kThreads = MODE == 2 ? 512 : 1024, kColumns = MODE == 0 ? 8 : MODE == 1 ? 1 : 16, kLanes = 32 / kColumns, kStrands = kThreads / kLanes;
-  __shared__ float s[kStrands][33];
-  const int lane = threadIdx.x % kLanes, strand = threadIdx.x / kLanes, col = blockIdx.x * 32 + lane * kColumns;
-  const int64_t first = (int64_t)blockIdx.y * p.per_split * WG_ROWS, last = min(first + (int64_t)p.per_split * WG_ROWS, (int64_t)p.m);
-  lf_chain();
-  float t[kColumns];
-#pragma unroll
-  for (int i = 0; i < kColumns; ++i) t[i] = 0.f;
-  if (col < p.n) {
-#pragma unroll 8
-    for (int64_t row = first + strand; row < last; row += kStrands) {
-      if (MODE == 0) {
-        const uint4 u = *reinterpret_cast<const uint4*>(p.dy + row * p.n + col);
-        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) { t[(2 * i) % kColumns] += __uint_as_float(w[i] << 16); t[(2 * i + 1) % kColumns] += __uint_as_float(w[i] & 0xffff0000u); }
-      } else if (MODE == 1) t[0] += __bfloat162float(p.dy[row * p.n + col]);
-      else {
-        const f8::Share v = f8::decode16(*reinterpret_cast<const uint4*>(p.dy8.codes + row * p.dy8.pitch + col), p.dy8.format);
-        const float factor = f8::up(p.dy8.exponents[f8::exponent_at(row, col / f8::kBlock, p.dy8.tiles)]);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) { t[(2 * i) % kColumns] = fmaf(v.v[i].x, factor, t[(2 * i) % kColumns]); t[(2 * i + 1) % kColumns] = fmaf(v.v[i].y, factor, t[(2 * i + 1) % kColumns]); }
-      }
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < kColumns; ++i) s[strand][lane * kColumns + i] = t[i];
-  __syncthreads();
-  for (int c = threadIdx.x >> 5; c < 32; c += kThreads / 32) {
-    float u = 0.f;
-    for (int i = threadIdx.x & 31; i < kStrands; i += 32) u += s[i][c];
-#pragma unroll
-    for (int o = 16; o; o >>= 1) u += __shfl_xor_sync(0xffffffffu, u, o);
-    if ((threadIdx.x & 31) == 0 && blockIdx.x * 32 + c < p.n) p.bias[blockIdx.y * p.bias_stride + blockIdx.x * 32 + c] = u;
-  }
+// f(NB, MODE as types)
+template <typename F>
+static void gradient_forms(int blocks, int mode, F f) {
+  auto with = [&](auto nb) {
+    if (mode == 0) f(nb, std::integral_constant<int, 0>{});
+    else if (mode == 1) f(nb, std::integral_constant<int, 1>{});
+    else f(nb, std::integral_constant<int, 2>{});
+  };
+  if (blocks == 1) with(std::integral_constant<int, 1>{}); else with(std::integral_constant<int, 2>{});
 }
 
 void configure_float8_gradient() {
-  cudaFuncSetAttribute(float8_gradient_kernel<1>, cudaFuncAttributeMaxDynamicSharedMemorySize, GradientShape<1>::smem);
-  cudaFuncSetAttribute(float8_gradient_kernel<2>, cudaFuncAttributeMaxDynamicSharedMemorySize, GradientShape<2>::smem);
+  for (int i = 0; i < 6; ++i)
+    gradient_forms(1 + i / 3, i % 3, [](auto nb, auto mode) {
+      constexpr int NB = decltype(nb)::value;
+      cudaFuncSetAttribute(float8_gradient_kernel<NB, decltype(mode)::value>, cudaFuncAttributeMaxDynamicSharedMemorySize, GradientShape<NB>::smem);
+    });
 }
 
-// Blocks of outputs of a tile: two where there are two and the sums of dy come with the products (at most 192 channels), or where a launch of their own is little
-// beside them (2^32 multiplications: about 20 us).
-static int gradient_blocks(int64_t m, int n, int k) { return n > WG_BN && (k <= 192 || (double)m * n * k >= 4294967296.0) ? 2 : 1; }
+// Blocks of outputs of a tile: two where there are two.  Beside more than 128 channels they leave room for one accumulator, so fewer rows than make a difference (2^32
+// multiplications, some 20 us) keep the two of a single block.
+static int gradient_blocks(int64_t m, int n, int k) { return n > WG_BN && (k <= 128 || (double)m * n * k >= 4294967296.0) ? 2 : 1; }
 
 // Blocks of rows: as many as the GPU has multiprocessors for beside the tiles, with four steps of 64 rows each at least - and 64 at most: the tensor core's
 // additions truncate, and 65536 x 1024 x 1024 with values of one sign was 3.5e-5 off in sums of 16384 rows (5.8e-6 in 4096).
@@ -479,17 +493,18 @@ lf_status lf_float8_weight_gradient_run(lf_context* ctx, const lf_float8_weight_
   int splits;
   tc::gradient_plan(ctx, x.rows, p.n, p.k, p.steps, splits, p.per_split);
   p.x = matrix(x);
+  int mode;
   CUtensorMap ma{}, mx{}, mo{};
   LF_TRY(tc::make_map_bytes(ctx, &mx, p.x.codes, p.k, p.m, p.x.pitch, tc::WG_ROWS));
   if (d->encoded_gradient.codes) {
-    p.dy_mode = 2;
+    mode = 2;
     p.dy8 = matrix(d->encoded_gradient);
     LF_TRY(tc::make_map_bytes(ctx, &ma, p.dy8.codes, p.n, p.m, p.dy8.pitch, tc::WG_ROWS));
   }
   else {
     p.dy = (const bf16*)d->gradient;
-    p.dy_mode = lf_aligned16(p.dy) && p.n % 8 == 0 ? 0 : 1;
-    if (p.dy_mode == 0) LF_TRY(tc::make_map_rows(ctx, &ma, p.dy, false, p.n, p.m, tc::WG_ROWS));
+    mode = lf_aligned16(p.dy) && p.n % 8 == 0 ? 0 : 1;
+    if (mode == 0) LF_TRY(tc::make_map_rows(ctx, &ma, p.dy, false, p.n, p.m, tc::WG_ROWS));
   }
   const bool direct = splits == 1;
   p.out = direct ? d->weight_gradient : (float*)d->workspace;
@@ -505,21 +520,12 @@ lf_status lf_float8_weight_gradient_run(lf_context* ctx, const lf_float8_weight_
   lf_prof_begin(ctx, LF_KERNEL_TRIANGLE_CONTRACT);
   const int blocks = tc::gradient_blocks(x.rows, p.n, p.k), outputs = tc::WG_BN * blocks;
   const dim3 grid((p.k + tc::WG_BK - 1) / tc::WG_BK, (p.n + outputs - 1) / outputs, splits);
-  if (blocks == 2) lf_launch(ctx, tc::float8_gradient_kernel<2>, grid, tc::WG_THREADS, tc::GradientShape<2>::smem, ma, mx, mo, p);
-  else lf_launch(ctx, tc::float8_gradient_kernel<1>, grid, tc::WG_THREADS, tc::GradientShape<1>::smem, ma, mx, mo, p);
+  tc::gradient_forms(blocks, mode, [&](auto nb, auto how) {
+    constexpr int NB = decltype(nb)::value;
+    lf_launch(ctx, tc::float8_gradient_kernel<NB, decltype(how)::value>, grid, tc::WG_THREADS, tc::GradientShape<NB>::smem, ma, mx, mo, p);
+  });
   lf_prof_end(ctx);
   ctx->launches++;
-  int launches = 1;
-  if (blocks == 2 && p.k > 192 && p.bias) {
-    const dim3 grid2((p.n + 31) / 32, splits);
-    lf_prof_begin(ctx, LF_KERNEL_ELEMENTWISE);
-    if (p.dy_mode == 0) lf_launch(ctx, tc::column_sums_kernel<0>, grid2, 1024, 0, p);
-    else if (p.dy_mode == 1) lf_launch(ctx, tc::column_sums_kernel<1>, grid2, 1024, 0, p);
-    else lf_launch(ctx, tc::column_sums_kernel<2>, grid2, 512, 0, p);
-    lf_prof_end(ctx);
-    ctx->launches++;
-    ++launches;
-  }
   if (!direct) {
     lf_prof_begin(ctx, LF_KERNEL_ELEMENTWISE);
     const int64_t fours = (int64_t)p.n * (p.ld / 4);
@@ -532,7 +538,7 @@ lf_status lf_float8_weight_gradient_run(lf_context* ctx, const lf_float8_weight_
     lf_prof_end(ctx);
     ctx->launches++;
   }
-  return lf_float8_done(ctx, r, launches + !direct);
+  return lf_float8_done(ctx, r, direct ? 1 : 2);
 }
 
 }  // extern "C"
