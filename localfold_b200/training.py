@@ -378,8 +378,10 @@ class Float8LinearGpu:
         weights = input["weights"]
         if not isinstance(weights, Float8LinearWeights):
             raise ValueError("weights must come from prepare_float8_linear_weights")
-        if weights.device.ordinal != self.device.ordinal:
-            raise ValueError(f"weights are on cuda:{weights.device.ordinal}, the device's GPU is cuda:{self.device.ordinal}")
+        if weights.device is not self.device:
+            if weights.device.ordinal != self.device.ordinal:
+                raise ValueError(f"weights are on cuda:{weights.device.ordinal}, the device's GPU is cuda:{self.device.ordinal}")
+            self.device.check(self.device.lib.lf_context_await(self.device.handle, weights.device.stream))      # (encoded on its stream)
         if (weights.out_channels, weights.channels) != (n, channels):
             raise RangeError(f"weights are {weights.out_channels} x {weights.channels}; expected {n} x {channels}")
         return rows, channels, n, weights

@@ -135,6 +135,26 @@ def test_one_stream_and_another(dev):
     other.close()
 
 
+def test_weights_of_another_device(dev):
+    """Weights encoded on one device's stream and used on another's: the second waits for them."""
+    import localfold_b200 as lf
+    other = lf.Device(0)
+    x = torch.randn(64, 2048, device="cuda")
+    shape = {"rows": 64, "channels": 2048, "outChannels": 4096}
+    first = torch.randn(4096, 2048, device="cuda")
+    weights = lf.prepare_float8_linear_weights(other, first)
+    other.synchronize()
+    for _ in range(10):
+        w = torch.randn(4096, 2048, device="cuda")
+        weights.update(w)
+        got = lf.Float8LinearGpu(dev).run({**shape, "activations": x, "weights": weights})["output"]
+        dev.synchronize()
+        want = lf.Float8LinearGpu(other).run({**shape, "activations": x, "weights": weights})["output"]
+        other.synchronize()
+        assert torch.equal(got, want)
+    other.close()
+
+
 def test_memory_is_not_reused_too_early():
     """A device with a stream of its own: results dropped at once, their memory used again by torch while the calls may still run."""
     import localfold_b200 as lf
