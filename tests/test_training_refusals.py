@@ -113,7 +113,7 @@ def test_float8():
 
 def weights(n, c, gpu=0):
     w = object.__new__(lf.Float8LinearWeights)
-    w.device, w.out_channels, w.channels, w.bias = SimpleNamespace(ordinal=gpu), n, c, None
+    w.device, w.out_channels, w.channels, w.bias = SimpleNamespace(ordinal=gpu) if gpu else DEVICE, n, c, None
     w.forward, w.transposed = float8(n, c), float8(c, n)
     return w
 
