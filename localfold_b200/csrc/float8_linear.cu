@@ -84,8 +84,10 @@ __device__ __forceinline__ void stage_columns(uint8_t* stage, const float* bias,
     *reinterpret_cast<uint4*>(stage + staged_at<NARROW>(lane, piece + c / kPiece)) = make_uint4(w[0], w[1], w[2], w[3]);
   }
 }
-// The staged rows to columns from c0 on of rows from row0 on (the whole warp): by TMA, or, where no 16-byte access divides the rows, a row after the other.
-template <bool F32, bool NARROW>
+// The staged rows to columns from c0 on of rows from row0 on (the whole warp): by TMA, or, where no 16-byte access divides the rows, AHEAD at a time: the loads of
+// that many, then their stores.  (Eight: 3001 x 449 x 1283 in float32, forward and input gradient, 12.9 -> 11.9 us.  The kernels of 256 columns have no registers for it: eight
+// there cost aligned rows, that never come here, 147456 x 128 x 512 43.1 -> 43.9 us.)
+template <bool F32, bool NARROW, int AHEAD>
 __device__ __forceinline__ void send_columns(const uint8_t* stage, const CUtensorMap* map, int vector_out, void* out, int c0, int row0, int m, int n, int lane) {
   constexpr int kColumns = (F32 ? 32 : 64) >> NARROW, kPiece = F32 ? 4 : 8;
   if (vector_out) {
@@ -96,15 +98,19 @@ __device__ __forceinline__ void send_columns(const uint8_t* stage, const CUtenso
   }
   __syncwarp();
   const int rows = min(32, m - row0);
-  for (int row = 0; row < rows; ++row) {
-    const int64_t at = (int64_t)(row0 + row) * n;
+  for (int row = 0; row < rows; row += AHEAD) {
 #pragma unroll
     for (int e = 0; e < kColumns; e += 32) {
       const int c = e + lane;
-      if (c < kColumns && c0 + c < n) {
-        const uint8_t* from = stage + staged_at<NARROW>(row, c / kPiece);
-        if (F32) static_cast<float*>(out)[at + c0 + c] = *reinterpret_cast<const float*>(from + c % kPiece * 4);
-        else static_cast<bf16*>(out)[at + c0 + c] = *reinterpret_cast<const bf16*>(from + c % kPiece * 2);
+      const bool here = c < kColumns && c0 + c < n;
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) {
+        const uint8_t* from = stage + staged_at<NARROW>(row + k, c / kPiece);
+        const int64_t at = (int64_t)(row0 + row + k) * n + c0 + c;
+        if (here && row + k < rows) {
+          if (F32) static_cast<float*>(out)[at] = *reinterpret_cast<const float*>(from + c % kPiece * 4);
+          else static_cast<bf16*>(out)[at] = *reinterpret_cast<const bf16*>(from + c % kPiece * 2);
+        }
       }
     }
   }
@@ -276,7 +282,7 @@ float8_linear_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_cons
           __syncwarp();
         }
         stage_columns<F32, DEEP, kStage>(stage, bias + c, &r[c / 32][c % 32], within / (F32 ? 4 : 8), lane);
-        if (within + kStage == kSend) send_columns<F32, DEEP>(stage, &mapO, p.vector_out, p.out, c0, row0, p.m, p.n, lane);
+        if (within + kStage == kSend) send_columns<F32, DEEP, BN == 256 ? 1 : 8>(stage, &mapO, p.vector_out, p.out, c0, row0, p.m, p.n, lane);
       }
     }
     if (lane == 0) bulk_wait_all();      // this thread's stores have landed
