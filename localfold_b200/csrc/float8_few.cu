@@ -28,6 +28,10 @@ __device__ __forceinline__ void mma_16x8x16(float (&c)[4], const uint32_t (&a)[4
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// total + c 2^(s - 254), s the sum of the two powers' bytes.  By halves of the power: the rows' whole power may take c out of float32's range where the
+// weights' brings it back.
+__device__ __forceinline__ float scaled_sum(float total, float c, int s) { return fmaf(c * up(s >> 1), up(s - (s >> 1)), total); }
+
 // EIGHTS: 8 or 16 rows; FORMAT of x (weights are e4m3).  Shared memory: the rows' codes, rows of `room` bytes, then their exponents [row][block].
 template <typename T, int EIGHTS, int FORMAT>
 __global__ void __launch_bounds__(FEW_WARPS * 32)
@@ -102,7 +106,7 @@ float8_few_kernel(const FewParams p) {
         for (int e = 0; e < EIGHTS; ++e)
 #pragma unroll
           for (int j = 0; j < 4; ++j) c[e][j] = 0.f;
-        const float fw0 = up(sw[i][0]), fw1 = up(sw[i][1]);
+        const int w0_power = sw[i][0], w1_power = sw[i][1];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           uint4 x[EIGHTS];
@@ -123,11 +127,11 @@ float8_few_kernel(const FewParams p) {
         if (block + FEW_WARPS * kAhead < nblk) fetch(i, block + FEW_WARPS * kAhead);
 #pragma unroll
         for (int e = 0; e < EIGHTS; ++e) {
-          const float f0 = up(exp_s[(e * 8 + 2 * t) * nblk + block]), f1 = up(exp_s[(e * 8 + 2 * t + 1) * nblk + block]);
-          total[e][0] += c[e][0] * f0 * fw0;
-          total[e][1] += c[e][1] * f1 * fw0;
-          total[e][2] += c[e][2] * f0 * fw1;
-          total[e][3] += c[e][3] * f1 * fw1;
+          const int x0_power = exp_s[(e * 8 + 2 * t) * nblk + block], x1_power = exp_s[(e * 8 + 2 * t + 1) * nblk + block];
+          total[e][0] = scaled_sum(total[e][0], c[e][0], x0_power + w0_power);
+          total[e][1] = scaled_sum(total[e][1], c[e][1], x1_power + w0_power);
+          total[e][2] = scaled_sum(total[e][2], c[e][2], x0_power + w1_power);
+          total[e][3] = scaled_sum(total[e][3], c[e][3], x1_power + w1_power);
         }
       }
     }

@@ -86,6 +86,24 @@ def test_gradients(dev, rows, c, n, name, dtype):
     ref.close(grads["bias"], dv.sum(0), chain * np.abs(dv).sum(0), "bias")
 
 
+@pytest.mark.parametrize("power", [115, -115])
+@pytest.mark.parametrize("rows,c,n", [(3, 128, 64), (16, 384, 160), (200, 513, 100), (300, 1030, 700), (300, 4100, 700)])
+def test_powers_that_cancel(dev, rows, c, n, power):
+    """Activations near one end of float32's range and weights near the other: the products are ordinary numbers, and neither power of two alone
+    may take a sum out of the range.  (Powers of two are exact: the bounds are those of ordinary operands.)"""
+    import localfold_b200 as lf
+    x, w, dy, _ = operands(rows + c + n, rows, c, n, "f32")
+    x, w = x * 2.0 ** power, w * 2.0 ** -power
+    linear, weights = lf.Float8LinearGpu(dev), lf.prepare_float8_linear_weights(dev, w)
+    shape = {"rows": rows, "channels": c, "outChannels": n, "weights": weights}
+    y = linear.run({**shape, "activations": x})
+    dx = linear.input_gradient({**shape, "gradient": dy * 2.0 ** power})
+    dev.synchronize()
+    x8, w8, dy8 = ref.decoded(host(x)), ref.decoded(host(w), "e4m3", 128), ref.decoded(host(dy * 2.0 ** power))
+    ref.close(y["output"], x8 @ w8.T, c * STEP * (np.abs(x8) @ np.abs(w8).T), "output")
+    ref.close(dx["output"], dy8 @ w8, n * STEP * (np.abs(dy8) @ np.abs(w8)), "gradient")
+
+
 def test_long_sums(dev):
     """Values of one sign over many rows, several chains a tile: the bound of a chain holds, and what the tests' shorter sums allow."""
     import localfold_b200 as lf
