@@ -19,6 +19,7 @@ from __future__ import annotations
 
 import math
 import struct
+import weakref
 
 import numpy as np
 
@@ -295,7 +296,9 @@ class LayerNormGpu:
 class Float8LinearWeights:
     """A projection's weight ``[outChannels][channels]`` on the device in e4m3, one power of two for every 128 x 128 elements, in both
     orientations (the transposed one multiplies gradients), and its bias.  ``update`` encodes new values into the same memory, as
-    a training step does; calls enqueued before it have read the old ones."""
+    a training step does; calls enqueued before it, on this device or another of the same GPU, have read the old ones."""
+
+    _readers = None      # other devices of the GPU whose calls may still be reading
 
     def __init__(self, device: Device, weight, bias=None):
         self.device = device
@@ -329,6 +332,10 @@ class Float8LinearWeights:
         if bias is not None:
             _tensor(self.device, "bias", bias, self.out_channels, "f32")
         self.bias = bias
+        for reader in self._readers or ():
+            if reader._finalizer.alive:      # (a closed device has finished)
+                self.device.check(self.device.lib.lf_context_await(self.device.handle, reader.stream))
+        self._readers = None
         _encode(self.device, weight, dtype, self.forward, 128, self.transposed)
 
 
@@ -381,7 +388,11 @@ class Float8LinearGpu:
         if weights.device is not self.device:
             if weights.device.ordinal != self.device.ordinal:
                 raise ValueError(f"weights are on cuda:{weights.device.ordinal}, the device's GPU is cuda:{self.device.ordinal}")
-            self.device.check(self.device.lib.lf_context_await(self.device.handle, weights.device.stream))      # (encoded on its stream)
+            if weights.device._finalizer.alive:      # (encoded on its stream)
+                self.device.check(self.device.lib.lf_context_await(self.device.handle, weights.device.stream))
+            if weights._readers is None:
+                weights._readers = weakref.WeakSet()
+            weights._readers.add(self.device)
         if (weights.out_channels, weights.channels) != (n, channels):
             raise RangeError(f"weights are {weights.out_channels} x {weights.channels}; expected {n} x {channels}")
         return rows, channels, n, weights

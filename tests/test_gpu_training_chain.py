@@ -364,3 +364,28 @@ def test_library_refusals(dev):
     refuse("lf_float8_weight_gradient_run", grad(activations=M(big)), A, "workspace")
     dev.synchronize()
     assert dev.launch_count() == launched and not out.any()
+
+
+def test_update_while_another_device_reads(dev):
+    """Weights of one device, multiplied on another's stream behind a queue of products, and updated at once: the products have the old values."""
+    import localfold_b200 as lf
+    n = 2048
+    x, first, second = (torch.randn(n, n, device="cuda") for _ in range(3))
+    weights, other = lf.prepare_float8_linear_weights(dev, first), lf.Device(0)
+    dev.synchronize()
+    linear, call = lf.Float8LinearGpu(other), {"rows": n, "channels": n, "outChannels": n, "activations": x, "weights": weights}
+    want = linear.run(call)["output"]
+    other.synchronize()
+    got = [linear.run(call)["output"] for _ in range(40)]
+    weights.update(second)
+    new = linear.run(call)["output"]
+    other.synchronize()
+    assert all(torch.equal(t, want) for t in got) and not torch.equal(new, want)
+    renewed = lf.Float8LinearGpu(dev).run(call)["output"]
+    dev.synchronize()
+    assert torch.equal(new, renewed)
+    other.close()
+    weights.update(first)
+    again = lf.Float8LinearGpu(dev).run(call)["output"]
+    dev.synchronize()
+    assert torch.equal(again, want)

@@ -135,6 +135,49 @@ def test_linear(changes, options, error, text):
         lf.Float8LinearGpu(DEVICE).run({**good, **changes}, options)
 
 
+class FakeDevice:
+    """A device whose library calls are written down."""
+
+    def __init__(self, log, stream):
+        self.ordinal, self.stream, self.handle, self._own_stream, self._finalizer = 0, stream, stream, False, SimpleNamespace(alive=True)
+        answer = lambda name: lambda *args: log.append((name, self.stream) + args[1:2]) or nat.LF_OK
+        self.lib = SimpleNamespace(**{name: answer(name) for name in ("lf_context_await", "lf_float8_encode", "lf_float8_linear_run")})
+
+    def check(self, status):
+        assert status == nat.LF_OK
+
+    def hold(self, tensors):
+        pass
+
+
+def test_weights_of_another_device(monkeypatch):
+    """Calls wait for the weights' device, a later update for the calls; a device that was closed is not waited for."""
+    monkeypatch.setattr(training, "_torch_stream", lambda ordinal: 1)
+    log = []
+    owner, user = FakeDevice(log, 1), FakeDevice(log, 2)
+    w = weights(6, 8)
+    w.device, value = owner, Fake(48)
+    value.shape = (6, 8)
+    call = {"rows": 4, "channels": 8, "outChannels": 6, "activations": float8(4, 8), "weights": w}
+    out = Fake(24, torch.bfloat16)
+    names = lambda: [e[:3] if e[0] == "lf_context_await" else e[:2] for e in log]
+    lf.Float8LinearGpu(user).run(call, None, out)
+    w.update(value)
+    assert names() == [("lf_context_await", 2, 1), ("lf_float8_linear_run", 2), ("lf_context_await", 1, 2), ("lf_float8_encode", 1)]
+    log.clear()
+    w.update(value)      # (nothing has read since)
+    lf.Float8LinearGpu(owner).run(call, None, out)
+    w.update(value)
+    assert names() == [("lf_float8_encode", 1), ("lf_float8_linear_run", 1), ("lf_float8_encode", 1)]
+    log.clear()
+    lf.Float8LinearGpu(user).run(call, None, out)
+    user._finalizer.alive = False
+    w.update(value)
+    user._finalizer.alive, owner._finalizer.alive = True, False
+    lf.Float8LinearGpu(user).run(call, None, out)
+    assert names() == [("lf_context_await", 2, 1), ("lf_float8_linear_run", 2), ("lf_float8_encode", 1), ("lf_float8_linear_run", 2)]
+
+
 def test_linear_gradients():
     linear = lf.Float8LinearGpu(DEVICE)
     good = {"rows": 4, "channels": 8, "outChannels": 6, "weights": weights(6, 8)}
