@@ -17,7 +17,6 @@ allocator, so a call can be captured into a CUDA graph (on the stream that the `
 """
 from __future__ import annotations
 
-import math
 import struct
 import weakref
 
@@ -41,6 +40,8 @@ _LINEAR = struct.Struct("@" + 2 * _MATRIX + "QiiQQQQ")
 _WEIGHT_GRADIENT = struct.Struct("@" + _MATRIX + "Q" + _MATRIX + "ii4Q")
 _NO_MATRIX = (0, 0, 0, 0, 0)
 _NO_OPTIONS = {}
+_MOST = 2 ** 31 - 1                                # rows and channels are 32-bit numbers in the kernels
+_LARGEST = (2 - 2.0 ** -23) * 2.0 ** 127           # of float32
 _AS_IT_WAS = object()
 
 
@@ -52,8 +53,10 @@ def _format(value, name="format"):
 
 def _size(inp, name):
     value = inp[name]
-    if type(value) is not int or value <= 0:
+    if type(value) is not int or not 0 < value <= _MOST:
         _positive(name, value)
+        if value > _MOST:
+            raise RangeError(f"{name} must be at most {_MOST}; received {value}")
         value = int(value)
     return value
 
@@ -232,7 +235,7 @@ class LayerNormGpu:
         x, scale, offset = input["activations"], input["scale"], input["offset"]
         epsilon = input.get("epsilon")
         epsilon = 1e-5 if epsilon is None else epsilon
-        if not epsilon > 0 or not math.isfinite(epsilon):
+        if not 0 < epsilon <= _LARGEST:
             raise RangeError(f"epsilon must be finite and positive; received {epsilon}")
         variance = _variance(opts, "two-pass") if opts else nat.VARIANCE_TWO_PASS
         kept, encode = opts.get("checkpoint"), opts.get("encode")

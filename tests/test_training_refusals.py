@@ -56,6 +56,10 @@ def norm_input(**changes):
     ({"activations": Fake(32, contiguous=False)}, None, ValueError, "activations must be contiguous"),
     ({"scale": Fake(8, torch.bfloat16)}, None, ValueError, "scale must be f32"),
     ({"offset": Fake(7)}, None, RangeError, "offset has 7 values; expected 8"),
+    ({"rows": 2 ** 31}, None, RangeError, "rows must be at most 2147483647; received 2147483648"),
+    ({"rows": 1, "channels": 2 ** 40, "activations": Fake(2 ** 40)}, None, RangeError, "channels must be at most 2147483647"),
+    ({"epsilon": 1e39}, None, RangeError, "epsilon must be finite and positive"),
+    ({"epsilon": float("inf")}, None, RangeError, "epsilon must be finite and positive"),
     ({"epsilon": 0.0}, None, RangeError, "epsilon must be finite and positive"),
     ({"epsilon": float("nan")}, None, RangeError, "epsilon must be finite and positive"),
     ({}, {"checkpoint": "int8"}, ValueError, 'checkpoint must be "e4m3" or "e5m2"'),
@@ -93,6 +97,8 @@ def test_layer_norm_backward(changes, error, text):
 def test_float8():
     with pytest.raises(RangeError, match="rows must be a positive safe integer"):
         lf.float8_encode(DEVICE, Fake(8), 0, 8)
+    with pytest.raises(RangeError, match="channels must be at most 2147483647"):
+        lf.float8_encode(DEVICE, Fake(2 ** 33), 1, 2 ** 33)
     with pytest.raises(ValueError, match='format must be "e4m3" or "e5m2"'):
         lf.float8_encode(DEVICE, Fake(8), 1, 8, {"format": "e3m4"})
     with pytest.raises(RangeError, match="activations has 8 values; expected 16"):
