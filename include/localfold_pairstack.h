@@ -596,7 +596,9 @@ typedef struct lf_float8_encode_desc {
   const void* source;
 } lf_float8_encode_desc;
 LF_API lf_status lf_float8_encode(lf_context* ctx, const lf_float8_encode_desc* d, lf_result* r);
-/* out [source.rows][source.channels] of `dtype` = the values of source (exact in either type). */
+/* out [source.rows][source.channels] of `dtype` = the values of source: exact in either type, but that bf16's least step
+ * 2^-133 rounds values of blocks below about 2^-115 (E4M3) or 2^-101 (E5M2), and that a magnitude which the encoder rounded
+ * up to 2^128 is infinite. */
 typedef struct lf_float8_decode_desc {
   lf_float8_matrix source;
   int32_t dtype, reserved;

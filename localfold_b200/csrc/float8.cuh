@@ -4,7 +4,8 @@
 // amax = the largest finite magnitude of the block = m 2^p, 1 <= m < 2.  The largest finite code is 1.75 2^8 (e4m3) or 1.75 2^15 (e5m2), so
 // the least power of two that brings amax to it is 2^(p - 8), or 2^(p - 7) where m > 1.75: the exponent field of amax less 8, plus a
 // carry out of the mantissa.  It is kept as that biased byte, at least 1 (2^-126, the least normal number).  Scaling by it
-// rounds nothing, so a code is one rounding of the value, and a decoded value (at most four significant bits) is exact in float32 and bf16.
+// rounds nothing, so a code is one rounding of the value, and a decoded value (at most four significant bits) is exact in float32, and in bf16 down to its least step 2^-133 (powers
+// of two below 2^-124, e5m2 2^-117, have codes beneath it).
 //
 // Exponent bytes lie as the tensor cores read them as scales: [512 channels][128 rows] tiles of 512 bytes, in a tile
 // [row % 32][row / 32][block % 4].

@@ -85,7 +85,7 @@ __device__ __forceinline__ void stage_columns(uint8_t* stage, const float* bias,
   }
 }
 // The staged rows to columns from c0 on of rows from row0 on (the whole warp): by TMA, or, where no 16-byte access divides the rows, AHEAD at a time: the loads of
-// that many, then their stores.  (Eight: 3001 x 449 x 1283 in float32, forward and input gradient, 12.9 -> 11.9 us.  The kernels of 256 columns have no registers for it: eight
+// that many, then their stores.  (Eight: 3001 x 449 x 1283 in float32 13.1 -> 12.1 us, its input's gradient 10.8 -> 10.1.  The kernels of 256 columns have no registers for it: eight
 // there cost aligned rows, that never come here, 147456 x 128 x 512 43.1 -> 43.9 us.)
 template <bool F32, bool NARROW, int AHEAD>
 __device__ __forceinline__ void send_columns(const uint8_t* stage, const CUtensorMap* map, int vector_out, void* out, int c0, int row0, int m, int n, int lane) {
@@ -387,8 +387,8 @@ extern "C" lf_status lf_float8_linear_run(lf_context* ctx, const lf_float8_linea
   p.out = d->out;
   p.status = (tc05::Status*)ctx->tc_status;
   // The tile width whose longest block is done first: a tile costs about its columns and 64 more, and the last one's stores, which nothing hides, a quarter of
-  // its columns by TMA or three quarters by threads.  (3001 x 1283 -> 449 in float32: 10.8 us 128 wide, 13.7 at 64; 3001 x 449 -> 1283 in bf16: 9.5 at 128,
-  // 11.9 at 256.)
+  // its columns by TMA or three quarters by threads.  (3001 x 1283 -> 449 in float32: 10.4 us 128 wide, 12.9 at 64, 24 at 256; 3001 x 449 -> 1283 in bf16: 9.6 at 128,
+  // 12.0 at 64, 11.7 at 256; 1000 x 1000 -> 1001 in float32: 8.1 at 64, 9.2 at 128.)
   int bn = 0;
   int64_t best = 0;
   for (int width = 64; width <= 256; width *= 2) {

@@ -8,8 +8,8 @@
 // and eight lanes are a block of the 8-bit form (float8.cuh), which leaves or comes back in the same pass.  G lanes hold a row in registers.
 // Blocks stay and walk over the rows, the next row's loads in flight under the present one's arithmetic and the weights in registers; a lane always
 // has the same channels, so dg and db add up in its registers and every block leaves one row of sums, which a second, small kernel
-// adds in a fixed order.  205824 x 64 in float32: forward 18.2 us, 5.8 TB/s; 147456 x 128 in bf16 with an e4m3 checkpoint: forward 19.7, backward 21.5 and 3.4
-// to join, 4.8 and 4.4 TB/s (copies of such sizes reach 5.7).
+// adds in a fixed order.  205824 x 64 in float32: forward 18.2 us, 5.8 TB/s; 147456 x 128 in bf16 with an e4m3 checkpoint: forward 19.1, backward 21.5 and 3.4
+// to join, 5.0 and 4.4 TB/s (copies of such sizes reach 5.7).
 #include <algorithm>
 
 #include "float8.cuh"
@@ -44,7 +44,7 @@ struct Backward {
 
 __host__ __device__ constexpr int threads_of(int G) { return G <= 256 ? 256 : G; }
 __host__ __device__ constexpr int blocks_of(int G) { return 512 / threads_of(G); }      // a multiprocessor's
-// (rows in 16 bits leave the forward pass registers for three blocks: 147456 x 128 with a checkpoint 19.7 -> 19.1 us; float32 is slower so, 102400 x 64
+// (rows in 16 bits leave the forward pass registers for three blocks: 147456 x 128 with a checkpoint 19.7 -> 19.1 us; float32 is slower so, 205824 x 64
 // 18.3 -> 19.4)
 template <typename T>
 __host__ __device__ constexpr int forward_blocks_of(int G) { return sizeof(T) == 2 && threads_of(G) == 256 ? 3 : blocks_of(G); }

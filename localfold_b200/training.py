@@ -197,7 +197,7 @@ def float8_encode(device, activations, rows, channels, options=None):
 
 def float8_decode(device, encoded, options=None, out=None):
     """The values of a ``Float8Tensor`` as a tensor ``[rows][channels]``.  ``options``: output "bf16" (default) or "f32"; both hold them
-    exactly."""
+    exactly (bf16 with its least step of 2^-133: blocks below about 2^-101 are rounded to it)."""
     dev = _device(device)
     if not isinstance(encoded, Float8Tensor):
         raise ValueError("encoded must be a Float8Tensor")

@@ -74,6 +74,19 @@ def test_special_values(dev, name):
     assert torch.signbit(got[8]).all()
 
 
+@pytest.mark.parametrize("name", ["e4m3", "e5m2"])
+def test_least_values(dev, name):
+    """Blocks whose codes lie beneath bf16's least step: exact in float32, rounded to nearest in bf16."""
+    import localfold_b200 as lf
+    x = torch.as_tensor(np.ldexp(np.random.default_rng(5).standard_normal((40, 300)), np.arange(-145, -105)[:, None])).float().cuda()
+    kept = lf.float8_encode(dev, x, 40, 300, {"format": name})
+    exact, rounded = (lf.float8_decode(dev, kept, {"output": out}) for out in ("f32", "bf16"))
+    dev.synchronize()
+    ref.close(exact, ref.decoded(host(x), name), 0.0, "f32")
+    ref.close(rounded, host(exact.bfloat16()), 0.0, "bf16")
+    assert (rounded.float() != exact).any()
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("shift", [1, 2, 3, 8])
 def test_any_address(dev, shift, dtype):
