@@ -186,9 +186,9 @@ def test_captured(dev):
             graph = torch.cuda.CUDAGraph()
             with torch.cuda.graph(graph, stream=stream):
                 results = step(d, *args, weights)
-            graphs.append((graph, results))
+            graphs.append((graph, results, weights))      # (what a graph reads and writes lives as long as it)
     for turn in range(3):
-        for args, (graph, results) in zip(cases, graphs):
+        for args, (graph, results, _) in zip(cases, graphs):
             fresh = problem(100 + turn, args[0].shape[0], args[0].shape[1], args[3].shape[0])
             for old, new in zip(args, fresh):
                 old.copy_(new)
@@ -219,16 +219,16 @@ def test_replayed_at_the_same_time(dev):
             graph = torch.cuda.CUDAGraph()
             with torch.cuda.graph(graph, stream=stream):
                 results = step(d, *args, weights)
-            graphs.append((graph, results))
+            graphs.append((graph, results, weights))      # (what a graph reads and writes lives as long as it)
     wants = [step(dev, *args) for args in cases]
     dev.synchronize()
     streams = [torch.cuda.Stream(), torch.cuda.Stream()]
     for _ in range(20):
-        for s, (graph, _) in zip(streams, graphs):
+        for s, (graph, *_) in zip(streams, graphs):
             with torch.cuda.stream(s):
                 graph.replay()
     torch.cuda.synchronize()
-    for want, (_, results) in zip(wants, graphs):
+    for want, (_, results, _) in zip(wants, graphs):
         for name, value in want.items():
             assert torch.equal(results[name], value), name
     d.close()
