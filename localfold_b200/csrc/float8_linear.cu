@@ -4,8 +4,8 @@
 // exponent bytes as they lie in the matrices, one byte for four instructions (a block of 128 channels).  No product is scaled by an
 // instruction of ours, and partial sums of different blocks meet in one float32 accumulator.
 //
-// 147456 x 128 -> 512 in bf16: 30 us, bound by its 151 MB of writes (5.7 TB/s in all); 4096 x 4096 -> 4096: 54 to 58 us, 2370 to 2550 TFLOP/s, bound by the tensor
-// core and the steps' way from L2.
+// 147456 x 128 -> 512 in bf16: 30 us, bound by its 151 MB of writes (5.7 TB/s in all); 4096 x 4096 -> 4096: 53.4 us, 2570 TFLOP/s, bound by the tensor core
+// and by the turns of its tiles.
 #include <cuda.h>
 
 #include "float8.cuh"
@@ -18,6 +18,7 @@ using namespace tc05;
 
 lf_status make_map_bytes(lf_context* ctx, CUtensorMap* map, const void* base, uint64_t width, uint64_t rows, uint64_t pitch, uint32_t box_rows);
 lf_status make_map_rows(lf_context* ctx, CUtensorMap* map, const void* base, bool f32, uint64_t width, uint64_t rows, uint32_t box_rows, bool narrow = false);
+lf_status make_map_tiles(lf_context* ctx, CUtensorMap* map, const void* base, uint64_t tiles, uint32_t box_tiles);
 
 void configure_float8_few();
 bool float8_few_takes(int64_t rows, int k);
@@ -25,7 +26,7 @@ lf_status float8_few(lf_context* ctx, const void* source, int dtype, const f8::M
 
 constexpr int F8_BM = 128, F8_BK = 128;      // a k step is a block of the format, and a row of it 128 bytes of shared memory
 constexpr int F8_A_BYTES = F8_BM * F8_BK;
-constexpr int F8_DEEP = 1024;                // channels from which the deeper ring pays
+constexpr int F8_DEEP = 1024;                // channels from which the deeper ring pays (4096 x 4096 -> 4096: 57.3 -> 54.2 us)
 
 struct Float8Params {
   int m, n, k;
@@ -43,18 +44,20 @@ __device__ __forceinline__ uint32_t make_idesc_f8(int M, int N, int a_format, in
   return ((uint32_t)id << 4) | ((uint32_t)a_format << 7) | ((uint32_t)b_format << 10) | ((uint32_t)(N >> 3) << 17) | (1u << 23) |
          ((uint32_t)(M >> 4) << 24) | ((uint32_t)id << 29);
 }
+template <int CTAS>
 __device__ __forceinline__ void umma_f8_scaled(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t a_scale, uint32_t b_scale,
                                                uint32_t accumulate) {
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
       "setp.ne.b32 p, %6, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d_tmem),
-      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(a_scale), "r"(b_scale), "r"(accumulate)
+      "tcgen05.mma.cta_group::%7.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(a_scale), "r"(b_scale), "r"(accumulate), "n"(CTAS)
       : "memory");
 }
 // 32 rows of 16 bytes of shared memory -> four columns of tensor memory, the same for each quarter of the lanes
+template <int CTAS>
 __device__ __forceinline__ void tmem_copy_scales(uint32_t taddr, uint64_t desc) {
-  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+  asm volatile("tcgen05.cp.cta_group::%2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc), "n"(CTAS) : "memory");
 }
 
 // Staging tiles of 32 rows: of 128 bytes (128-byte swizzle) or, NARROW, 64 (64-byte swizzle).
@@ -115,6 +118,24 @@ __device__ __forceinline__ void send_columns(const uint8_t* stage, const CUtenso
     }
   }
   __syncwarp();
+}
+
+// A warp's COLUMNS columns of 32 rows from (row0, col0) on, from registers, with the bias.
+template <int COLUMNS, bool F32, bool NARROW, int AHEAD>
+__device__ __forceinline__ void send_share(const uint32_t (&r)[COLUMNS / 32][32], uint8_t* stage, const float* bias, const CUtensorMap* map, const Float8Params& p, int col0,
+                                           int row0, int lane) {
+  constexpr int kSend = (F32 ? 32 : 64) >> NARROW, kStage = kSend < 32 ? kSend : 32;      // columns of a staging tile, and staged at a time
+#pragma unroll
+  for (int c = 0; c < COLUMNS; c += kStage) {
+    const int within = c % kSend, c0 = col0 + c - within;
+    if (c0 >= p.n) break;
+    if (within == 0) {
+      if (lane == 0) bulk_wait_read();      // the previous copy has read the staging rows
+      __syncwarp();
+    }
+    stage_columns<F32, NARROW, kStage>(stage, bias + c, &r[c / 32][c % 32], within / (F32 ? 4 : 8), lane);
+    if (within + kStage == kSend) send_columns<F32, NARROW, AHEAD>(stage, map, p.vector_out, p.out, c0, row0, p.m, p.n, lane);
+  }
 }
 
 // One 128 x BN tile per work item, k stepped by 128 through a TMA ring.  A step that opens a group of four brings the group's exponent tiles
@@ -223,13 +244,13 @@ float8_linear_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_cons
         if (elect_one()) {
           if ((kb & 3) == 0) {
             const uint64_t sc = scale_first + (uint32_t)(stage * S::scales >> 4);
-            tmem_copy_scales(scales, sc);
-            tmem_copy_scales(scales + 8, sc + 32);
-            if (BN == 256 && columns > 128) tmem_copy_scales(scales + 12, sc + 64);
+            tmem_copy_scales<1>(scales, sc);
+            tmem_copy_scales<1>(scales + 8, sc + 32);
+            if (BN == 256 && columns > 128) tmem_copy_scales<1>(scales + 12, sc + 64);
           }
 #pragma unroll
           for (int kk = 0; kk < F8_BK / 32; ++kk)
-            umma_f8_scaled(d, a + kk * 2, b + kk * 2, idesc | (kb & 3) << 4 | (kb & 3) << 29, scales, scales + 8 + (BN == 64 ? 2u * (nj & 1) : 0u),
+            umma_f8_scaled<1>(d, a + kk * 2, b + kk * 2, idesc | (kb & 3) << 4 | (kb & 3) << 29, scales, scales + 8 + (BN == 64 ? 2u * (nj & 1) : 0u),
                            (kb | kk) != 0 ? 1u : 0u);
           umma_commit(&empty[stage]);
           if (kb + 1 == kblocks) umma_commit(&tmem_full[acc]);
@@ -272,18 +293,7 @@ float8_linear_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_cons
       __syncwarp();
       if (lane == 0) mbar_arrive(&tmem_empty[acc]);      // the share is in registers: the accumulator may be overwritten
       if (!mine) continue;
-      constexpr int kSend = (F32 ? 32 : 64) >> DEEP, kStage = kSend < 32 ? kSend : 32;      // columns of a staging tile, and staged at a time
-#pragma unroll
-      for (int c = 0; c < S::share; c += kStage) {
-        const int within = c % kSend, c0 = col0 + c - within;
-        if (c0 >= p.n) break;
-        if (within == 0) {
-          if (lane == 0) bulk_wait_read();      // the previous copy has read the staging rows
-          __syncwarp();
-        }
-        stage_columns<F32, DEEP, kStage>(stage, bias + c, &r[c / 32][c % 32], within / (F32 ? 4 : 8), lane);
-        if (within + kStage == kSend) send_columns<F32, DEEP, BN == 256 ? 1 : 8>(stage, &mapO, p.vector_out, p.out, c0, row0, p.m, p.n, lane);
-      }
+      send_share<S::share, F32, DEEP, BN == 256 ? 1 : 8>(r, stage, bias, &mapO, p, col0, row0, lane);
     }
     if (lane == 0) bulk_wait_all();      // this thread's stores have landed
   }
@@ -292,6 +302,169 @@ float8_linear_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_cons
   __syncthreads();
   if (*abort_flag) drain_after_abort();
   if (warp == 1) { tc_fence_after(); tmem_dealloc(tmem_base, 512); }
+}
+
+// Tiles of 256 x BN for two multiprocessors (a cluster of two CTAs), for products of many channels.  Of a pair each CTA loads its own 128 rows of x and half of the
+// weights' rows, and the pair's MMA reads both halves: at 256 columns 32 KB a step instead of 48, and a step takes 0.33 us instead of 0.38.  192 columns, at 0.29, have two
+// accumulators and divide what 256 do not: 5000 x 4096 -> 2048 takes 35 us (256: 41, 256 without pairs: 41), 12000 x 4096 -> 400 25 (29, 29).  4096 x 4096 -> 4096:
+// 53.4 us at 256 (192: 55.2, without pairs 55.9), 2570 TFLOP/s, 256 tiles in four turns of 74 pairs.  A pair starts about 1 us later and its accumulator changes hands
+// across two CTAs, so few channels have nothing of it.
+// Each CTA's producer fills its own shared memory and the leader's barriers count both; the leader's MMA warp multiplies for both and its commits arrive in both.
+// Exponents come by TMA like the rest: a CTA needs those of its own rows and of all the tile's outputs.
+template <int BN>
+struct PairShape {
+  static constexpr int stages = 6, stage = F8_A_BYTES + BN / 2 * F8_BK, scales = 512 * 3;
+  static constexpr int accumulators = BN == 256 ? 1 : 2, scale_columns = accumulators * BN;      // (and where the scales begin)
+  static constexpr int share = BN == 256 ? 128 : 64, epi = 4 * (BN / share), staging = 2048, threads = 64 + 32 * epi;
+  static constexpr int smem = stages * (stage + scales) + epi * (staging + share * 4) + 256 + 1024;
+};
+
+template <int BN, bool F32>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairShape<BN>::threads, 1)
+float8_pair_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant__ CUtensorMap mapB, const __grid_constant__ CUtensorMap mapEx,
+                   const __grid_constant__ CUtensorMap mapEw, const __grid_constant__ CUtensorMap mapO, const Float8Params p) {
+  using S = PairShape<BN>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = align_shared(smem_raw);
+  uint8_t* out_stage = smem + S::stages * S::stage;
+  uint8_t* scale_s = out_stage + S::epi * S::staging;
+  float* bias_s = reinterpret_cast<float*>(scale_s + S::stages * S::scales);
+  uint64_t* full = reinterpret_cast<uint64_t*>(bias_s + S::epi * S::share);      // [stages] the leader's: both CTAs' loads are here
+  uint64_t* empty = full + S::stages;            // [stages] multiplied
+  uint64_t* tmem_full = empty + S::stages;
+  uint64_t* tmem_empty = tmem_full + S::accumulators;          // the leader's: both CTAs' shares are in registers
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tmem_empty + S::accumulators);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = pair_rank();
+  const int tiles_m = (p.m + 255) / 256, tiles_n = (p.n + BN - 1) / BN, total = tiles_m * tiles_n;
+  const int kblocks = (p.k + F8_BK - 1) / F8_BK;
+  const int first = blockIdx.x >> 1, step = gridDim.x >> 1;
+
+  if (threadIdx.x == 32) { prefetch_tensormap(&mapA); prefetch_tensormap(&mapB); prefetch_tensormap(&mapEx); prefetch_tensormap(&mapEw); }
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S::stages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+    for (int b = 0; b < S::accumulators; ++b) { mbar_init(&tmem_full[b], 1); mbar_init(&tmem_empty[b], 2 * S::epi); }
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  __syncwarp();
+  if (warp == 1) tmem_alloc_pair(tmem_slot, 512);
+  tc_fence_before();
+  pair_sync();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  lf_chain();
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int stage = 0; uint32_t phase = 0;
+      bool ok = true;
+      for (int t = first; t < total && ok; t += step) {
+        const int mi = t / tiles_n, nj = t - mi * tiles_n;
+        for (int kb = 0; kb < kblocks; ++kb) {
+          if (!mbar_wait_cluster(&empty[stage], phase ^ 1, abort_flag, p.status, 141)) { ok = false; break; }
+          const bool opens = (kb & 3) == 0;
+          if (rank == 0) mbar_expect_tx(&full[stage], 2 * (S::stage + (opens ? S::scales : 0)));
+          const uint32_t bar = leader_bar(&full[stage]);
+          uint8_t* sA = smem + stage * S::stage;
+          tma_load_3d_pair(sA, &mapA, bar, kb * F8_BK, mi * 256 + (int)rank * 128, 0);
+          tma_load_3d_pair(sA + F8_A_BYTES, &mapB, bar, kb * F8_BK, nj * BN + (int)rank * (BN / 2), 0);
+          if (opens) {      // (tiles that do not exist: other rows' bytes or zeros, for rows and outputs that are not stored)
+            uint8_t* sc = scale_s + stage * S::scales;
+            tma_load_3d_pair(sc, &mapEx, bar, 0, (int)((kb >> 2) * p.ex_tiles) + mi * 2 + (int)rank, 0);
+            tma_load_3d_pair(sc + 512, &mapEw, bar, 0, (int)((kb >> 2) * p.ew_tiles) + nj * BN / 128, 0);
+          }
+          if (++stage == S::stages) { stage = 0; phase ^= 1; }
+        }
+      }
+      // the leader's arrivals have landed before this CTA may end
+      for (int s = 0; s < S::stages && ok; ++s) {
+        ok = mbar_wait_cluster(&empty[stage], phase ^ 1, abort_flag, p.status, 145);
+        if (++stage == S::stages) { stage = 0; phase ^= 1; }
+      }
+    }
+  } else if (warp == 1) {
+    if (rank == 0) {
+      const uint64_t a_first = make_smem_desc(smem_u32(smem), 16, 1024), b_first = make_smem_desc(smem_u32(smem) + F8_A_BYTES, 16, 1024);
+      const uint64_t scale_first = make_smem_desc_plain(smem_u32(scale_s), 0, 128);
+      const uint32_t idesc = make_idesc_f8(256, BN, p.x_format, 0, 0);
+      int stage = 0; uint32_t phase = 0, it = 0, group = 0;
+      bool ok = true;
+      for (int t = first; t < total && ok; t += step, ++it) {
+        const uint32_t acc = it % S::accumulators, within = t % tiles_n * BN & 127;      // (the tile's first output in its 128 exponents)
+        if (!__all_sync(0xffffffffu, mbar_wait_cluster(&tmem_empty[acc], ((it / S::accumulators) & 1) ^ 1, abort_flag, p.status, 142))) break;
+        tc_fence_after();
+        uint32_t scales = 0;
+        for (int kb = 0; kb < kblocks; ++kb) {
+          if (!__all_sync(0xffffffffu, mbar_wait_cluster(&full[stage], phase, abort_flag, p.status, 143))) { ok = false; break; }
+          tc_fence_after();
+          const uint64_t a = a_first + (uint32_t)(stage * S::stage >> 4), b = b_first + (uint32_t)(stage * S::stage >> 4);
+          if ((kb & 3) == 0) scales = tmem_base + S::scale_columns + (group++ & 3) * 16;      // (four slots in turn, as above)
+          if (elect_one()) {
+            if ((kb & 3) == 0) {
+              const uint64_t sc = scale_first + (uint32_t)(stage * S::scales >> 4);
+              tmem_copy_scales<2>(scales, sc);
+              tmem_copy_scales<2>(scales + 8, sc + 32);
+              tmem_copy_scales<2>(scales + 12, sc + 64);
+            }
+#pragma unroll
+            for (int kk = 0; kk < F8_BK / 32; ++kk)
+              umma_f8_scaled<2>(tmem_base + acc * BN, a + kk * 2, b + kk * 2, idesc | (kb & 3) << 4 | (kb & 3) << 29, scales, scales + 8 + within / 32,
+                                (kb | kk) != 0 ? 1u : 0u);
+            umma_commit_pair(&empty[stage]);
+            if (kb + 1 == kblocks) umma_commit_pair(&tmem_full[acc]);
+          }
+          __syncwarp();
+          if (++stage == S::stages) { stage = 0; phase ^= 1; }
+        }
+      }
+    }
+  } else {
+    const int q = warp & 3, part = (warp - 2) >> 2;      // TMEM lane quadrant, share of the tile's columns
+    uint8_t* stage = out_stage + (warp - 2) * S::staging;
+    float* bias = bias_s + (warp - 2) * S::share;
+    uint32_t it = 0;
+    int held = -1;      // first column of the bias share in shared memory
+    if (lane == 0 && p.vector_out) prefetch_tensormap(&mapO);
+    for (int t = first; t < total; t += step, ++it) {
+      const int mi = t / tiles_n, nj = t - mi * tiles_n;
+      const int col0 = nj * BN + part * S::share, row0 = mi * 256 + (int)rank * 128 + q * 32;
+      const bool mine = col0 < p.n && row0 < p.m;
+      if (mine && held != col0) {
+        held = col0;
+        __syncwarp();
+#pragma unroll
+        for (int e = 0; e < S::share; e += 32) bias[e + lane] = p.bias && col0 + e + lane < p.n ? p.bias[col0 + e + lane] : 0.f;
+        __syncwarp();
+      }
+      const uint32_t acc = it % S::accumulators;
+      if (!__all_sync(0xffffffffu, mbar_wait_cluster(&tmem_full[acc], (it / S::accumulators) & 1, abort_flag, p.status, 144))) break;
+      tc_fence_after();
+      uint32_t r[S::share / 32][32];
+      if (mine) {
+        const uint32_t d = tmem_base + ((uint32_t)(q * 32) << 16) + acc * BN + part * S::share;
+#pragma unroll
+        for (int i = 0; i < S::share / 32; ++i) tmem_ld32(d + i * 32, r[i]);
+        tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < S::share / 32; ++i) tie32(r[i]);
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(leader_bar(&tmem_empty[acc]));
+      if (mine) send_share<S::share, F32, true, 1>(r, stage, bias, &mapO, p, col0, row0, lane);
+    }
+    if (lane == 0) bulk_wait_all();
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (*abort_flag) drain_after_abort();
+  __syncwarp();
+  pair_sync();      // neither CTA's memory goes before both are through
+  if (warp == 1) { tc_fence_after(); tmem_dealloc_pair(tmem_base, 512); }
 }
 
 // f(BN, F32, DEEP as types)
@@ -304,6 +477,13 @@ static void linear_forms(int bn, bool deep, bool f32, F f) {
   else with(std::integral_constant<int, 64>{});
 }
 
+// f(BN, F32 as types)
+template <typename F>
+static void pair_forms(int bn, bool f32, F f) {
+  auto with = [&](auto b) { if (f32) f(b, std::true_type{}); else f(b, std::false_type{}); };
+  if (bn == 256) with(std::integral_constant<int, 256>{}); else with(std::integral_constant<int, 192>{});
+}
+
 void configure_float8_linear() {
   for (int i = 0; i < 8; ++i)
     linear_forms(64 << i % 4, i % 4 == 3, i / 4, [](auto bn, auto f32, auto deep) {
@@ -311,7 +491,30 @@ void configure_float8_linear() {
       constexpr bool D = decltype(deep)::value;
       cudaFuncSetAttribute(float8_linear_kernel<BN, decltype(f32)::value, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Float8Shape<BN, D>::smem);
     });
+  for (int i = 0; i < 4; ++i)
+    pair_forms(i & 1 ? 256 : 192, i >> 1, [](auto bn, auto f32) {
+      constexpr int BN = decltype(bn)::value;
+      cudaFuncSetAttribute(float8_pair_kernel<BN, decltype(f32)::value>, cudaFuncAttributeMaxDynamicSharedMemorySize, PairShape<BN>::smem);
+    });
   configure_float8_few();
+}
+
+template <int BN, bool F32>
+static lf_status launch_pair(lf_context* ctx, const f8::Matrix& x, const f8::Matrix& w, const Float8Params& p) {
+  using S = PairShape<BN>;
+  CUtensorMap ma, mb, mex, mew, mo{};
+  LF_TRY(make_map_bytes(ctx, &ma, x.codes, x.channels, x.rows, x.pitch, 128));
+  LF_TRY(make_map_bytes(ctx, &mb, w.codes, w.channels, w.rows, w.pitch, BN / 2));
+  const int groups = (f8::blocks(p.k) + 3) / 4;
+  LF_TRY(make_map_tiles(ctx, &mex, x.exponents, groups * x.tiles, 1));
+  LF_TRY(make_map_tiles(ctx, &mew, w.exponents, groups * w.tiles, 2));
+  if (p.vector_out) LF_TRY(make_map_rows(ctx, &mo, p.out, F32, p.n, p.m, 32, true));
+  const int64_t tiles = (int64_t)((p.m + 255) / 256) * ((p.n + BN - 1) / BN), pairs = ctx->sm_count / 2;
+  lf_prof_begin(ctx, LF_KERNEL_LN_GEMM);
+  lf_launch(ctx, float8_pair_kernel<BN, F32>, 2 * (int)(tiles < pairs ? tiles : pairs), S::threads, S::smem, ma, mb, mex, mew, mo, p);
+  lf_prof_end(ctx);
+  ctx->launches++;
+  return LF_OK;
 }
 
 template <int BN, bool F32, bool DEEP>
@@ -328,6 +531,16 @@ static lf_status launch_float8(lf_context* ctx, const f8::Matrix& x, const f8::M
   ctx->launches++;
   return LF_OK;
 }
+
+// What the forms take, in nanoseconds: at the start, for a turn, and for a step of a turn; a turn more where rows are float32, or odd (stored by threads).  Least squares over
+// 172 products of 100 to 65536 rows, 40 to 4096 channels and 100 to 4096 outputs, each timed in every form: the form that they choose is 0.7 % slower than the
+// fastest on average and 15 % at most.  (A rule on widths and turns alone was 7.7 % slower, 88 % at most; without pairs 3.6 %.)
+struct FormCost { int ctas, bn; bool deep; int start, turn, step, turn_f32, odd_start, odd_turn; };
+constexpr FormCost kForms[] = {
+    {1, 64, false, 3100, 500, 264, 360, 0, 1100},    {1, 128, false, 3200, 630, 305, 570, 0, 1700},
+    {1, 256, false, 4050, 1230, 349, 1120, 1100, 3230}, {1, 256, true, 3300, 1010, 362, 1940, 5000, 4300},      // DEEP: from F8_DEEP channels on
+    {2, 192, false, 4000, 1720, 247, 1210, 2100, 2660}, {2, 256, false, 3900, 2230, 301, 1610, 3250, 4400},
+};
 
 }  // namespace tc
 
@@ -386,21 +599,22 @@ extern "C" lf_status lf_float8_linear_run(lf_context* ctx, const lf_float8_linea
   p.x_format = x.format;
   p.out = d->out;
   p.status = (tc05::Status*)ctx->tc_status;
-  // The tile width whose longest block is done first: a tile costs about its columns and 64 more, and the last one's stores, which nothing hides, a quarter of
-  // its columns by TMA or three quarters by threads.  (3001 x 1283 -> 449 in float32: 10.4 us 128 wide, 12.9 at 64, 24 at 256; 3001 x 449 -> 1283 in bf16: 9.6 at 128,
-  // 12.0 at 64, 11.7 at 256; 1000 x 1000 -> 1001 in float32: 8.1 at 64, 9.2 at 128.)
-  int bn = 0;
+  // The form that is done first.  Which that is depends on the turns (tiles over multiprocessors or pairs) and the steps of 128 channels.
+  const int64_t steps = (p.k + tc::F8_BK - 1) / tc::F8_BK;
+  const tc::FormCost* form = nullptr;
   int64_t best = 0;
-  for (int width = 64; width <= 256; width *= 2) {
-    const int64_t turns = (mx.tiles * ((p.n + width - 1) / width) + ctx->sm_count - 1) / ctx->sm_count;
-    const int64_t work = turns * (width + 64) + width * (vector_out ? 1 : 3) / 4;
-    if (bn == 0 || work < best) { bn = width; best = work; }
+  for (const tc::FormCost& f : tc::kForms) {
+    if (f.bn == 256 && f.ctas == 1 && f.deep != (p.k >= tc::F8_DEEP)) continue;
+    const int64_t tiles = (mx.tiles + f.ctas - 1) / f.ctas * ((p.n + f.bn - 1) / f.bn), at_once = ctx->sm_count / f.ctas, turns = (tiles + at_once - 1) / at_once;
+    const int64_t cost = f.start + (vector_out ? 0 : f.odd_start) + turns * (f.turn + steps * f.step + (f32 ? f.turn_f32 : 0) + (vector_out ? 0 : f.odd_turn));
+    if (!form || cost < best) { form = &f; best = cost; }
   }
   lf_status status = LF_OK;
-  // (the deeper ring, 4096 rows and outputs: 57.3 -> 54.2 us at 4096 channels)
-  tc::linear_forms(bn, bn == 256 && p.k >= tc::F8_DEEP, f32, [&](auto b, auto o, auto deep) {
-    status = tc::launch_float8<decltype(b)::value, decltype(o)::value, decltype(deep)::value>(ctx, mx, mw, p);
-  });
+  if (form->ctas == 2) tc::pair_forms(form->bn, f32, [&](auto b, auto o) { status = tc::launch_pair<decltype(b)::value, decltype(o)::value>(ctx, mx, mw, p); });
+  else
+    tc::linear_forms(form->bn, form->deep, f32, [&](auto b, auto o, auto deep) {
+      status = tc::launch_float8<decltype(b)::value, decltype(o)::value, decltype(deep)::value>(ctx, mx, mw, p);
+    });
   LF_TRY(status);
   return lf_float8_done(ctx, r, launches);
 }

@@ -164,6 +164,17 @@ lf_status make_map_bytes(lf_context* ctx, CUtensorMap* map, const void* base, ui
   return LF_OK;
 }
 
+// `tiles` pieces of 512 contiguous bytes, boxes of `box_tiles`, no swizzle
+lf_status make_map_tiles(lf_context* ctx, CUtensorMap* map, const void* base, uint64_t tiles, uint32_t box_tiles) {
+  if (!g_encode) return lf_fail(ctx, LF_ERR_CUDA, "cuTensorMapEncodeTiled is not available from this driver");
+  cuuint64_t dims[3] = {128, tiles, 1}, strides[2] = {512, 512 * tiles};
+  cuuint32_t box[3] = {128, box_tiles, 1}, estr[3] = {1, 1, 1};
+  CUresult r = g_encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return lf_fail(ctx, LF_ERR_CUDA, "cuTensorMapEncodeTiled (tiles) failed with code %d", (int)r);
+  return LF_OK;
+}
+
 // float32 or bf16 rows (a multiple of 16 bytes), 128-byte swizzled boxes of 128 bytes x `box_rows` rows; narrow: 64 bytes, 64-byte swizzle
 lf_status make_map_rows(lf_context* ctx, CUtensorMap* map, const void* base, bool f32, uint64_t width, uint64_t rows, uint32_t box_rows, bool narrow) {
   if (!g_encode) return lf_fail(ctx, LF_ERR_CUDA, "cuTensorMapEncodeTiled is not available from this driver");

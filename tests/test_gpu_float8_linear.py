@@ -86,6 +86,55 @@ def test_gradients(dev, rows, c, n, name, dtype):
     ref.close(grads["bias"], dv.sum(0), chain * np.abs(dv).sum(0), "bias")
 
 
+@pytest.mark.parametrize("rows,c,n", [(2048, 4096, 4096), (4000, 4000, 4096), (1500, 2500, 2001), (5000, 1024, 2048), (1999, 1155, 1537), (12001, 2048, 400), (9000, 1000, 333),
+                                      (4096, 2048, 1024), (20000, 640, 640), (40000, 1536, 384), (700, 2048, 3000)])
+@pytest.mark.parametrize("out", ["f32", "bf16"])
+def test_many_channels(dev, rows, c, n, out):
+    """Products of every form of the kernel, pairs of multiprocessors among them; the references are 64-bit products of the decoded operands."""
+    import localfold_b200 as lf
+    x, w, _, bias = operands(rows + c + n, rows, c, n, "bf16")
+    linear, weights = lf.Float8LinearGpu(dev), lf.prepare_float8_linear_weights(dev, w, bias)
+    x8 = lf.float8_encode(dev, x, rows, c, {"format": "e5m2" if rows % 2 else "e4m3"})
+    call = {"rows": rows, "channels": c, "outChannels": n, "activations": x8, "weights": weights}
+    room = torch.full((rows * n + 64,), 7.0, dtype=TYPES[out], device="cuda")
+    got, same = linear.run(call, {"output": out}, out=room[:rows * n].view(rows, n))["output"], linear.run(call, {"output": out})["output"]
+    a, b = lf.float8_decode(dev, x8, {"output": "f32"}), lf.float8_decode(dev, weights.forward, {"output": "f32"})
+    dev.synchronize()
+    assert torch.equal(got, same) and (room[rows * n:] == 7).all()
+    size, want = a.double().abs() @ b.double().abs().T, a.double() @ b.double().T + bias.double()
+    off = c * STEP * size
+    bound = off + (STEP + ref.half_step(out)) * (want.abs() + off)
+    assert ((got.double() - want).abs() <= bound).all()
+
+
+def test_forms_at_the_same_time():
+    """Captured and replayed, and beside products of other forms on another stream: every form has all of a multiprocessor's tensor memory to itself."""
+    import localfold_b200 as lf
+    first, second = torch.cuda.Stream(), torch.cuda.Stream()
+    runs = []
+    for stream, sizes in ((first, [(3000, 2048, 2048), (2000, 4096, 4000), (3000, 300, 500)]), (second, [(2500, 2048, 384), (700, 256, 200), (4000, 128, 512)])):
+        with torch.cuda.stream(stream):
+            device = lf.Device(0, stream=stream.cuda_stream)
+            linear, calls = lf.Float8LinearGpu(device), []
+            for rows, c, n in sizes:
+                weights = lf.prepare_float8_linear_weights(device, torch.randn(n, c, device="cuda"))
+                calls.append({"rows": rows, "channels": c, "outChannels": n, "activations": torch.randn(rows, c, device="cuda"), "weights": weights})
+            want = [linear.run(call)["output"] for call in calls]
+            stream.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=stream):
+                got = [linear.run(call)["output"] for call in calls for _ in range(2)]
+            runs.append((stream, device, graph, want, got, calls))      # (a graph reads its inputs where they were: they live as long)
+    for _ in range(20):
+        for stream, _, graph, *_ in runs:
+            with torch.cuda.stream(stream):
+                graph.replay()
+    torch.cuda.synchronize()
+    for _, device, _, want, got, _ in runs:
+        assert all(torch.equal(got[2 * i], want[i]) and torch.equal(got[2 * i + 1], want[i]) for i in range(len(want)))
+        device.synchronize()
+
+
 @pytest.mark.parametrize("power", [115, -115])
 @pytest.mark.parametrize("rows,c,n", [(3, 128, 64), (16, 384, 160), (200, 513, 100), (300, 1030, 700), (300, 4100, 700)])
 def test_powers_that_cancel(dev, rows, c, n, power):
