@@ -86,6 +86,43 @@ __device__ __forceinline__ void convert16(uint4 codes, int s, int format, uint4 
   if (format == LF_FLOAT8_E4M3) convert16_as<LF_FLOAT8_E4M3>(codes, s, out); else convert16_as<LF_FLOAT8_E5M2>(codes, s, out);
 }
 
+// Sixteen neighbouring elements from `first` on of a bf16 tensor of `all`, wherever they start: the aligned 8-byte words that they lie in, and element by element (`count` of
+// them) where those would reach beyond the tensor's ends.  (By elements alone a warp's load touched 32 sectors: 65536 x 256 -> 1283 took 164 us,
+// now 99, and 100000 x 300 -> 300 152, now 93.)
+__device__ __forceinline__ void fetch_unaligned(uint2 (&raw)[5], const bf16* tensor, int64_t all, int64_t first, int count) {
+#pragma unroll
+  for (int i = 0; i < 5; ++i) raw[i] = make_uint2(0, 0);
+  if (count <= 0) return;
+  const uintptr_t base = reinterpret_cast<uintptr_t>(tensor), at = base + 2 * first, from = at & ~(uintptr_t)7;
+  if (from >= base && from + 40 <= base + 2 * all) {
+#pragma unroll
+    for (int i = 0; i < 5; ++i) raw[i] = *reinterpret_cast<const uint2*>(from + 8 * i);
+  } else {
+    const int skip = (int)(at - from) / 2;
+    auto half = [&](int h) { return h >= skip && h < skip + count ? (uint32_t)*reinterpret_cast<const uint16_t*>(from + 2 * h) : 0u; };
+#pragma unroll
+    for (int i = 0; i < 5; ++i) raw[i] = make_uint2(half(4 * i) | half(4 * i + 1) << 16, half(4 * i + 2) | half(4 * i + 3) << 16);
+  }
+}
+// The elements in their places, zeros from `count` on.
+__device__ __forceinline__ void place_unaligned(const uint2 (&raw)[5], const bf16* tensor, int64_t first, int count, uint4 (&out)[2]) {
+  const uint32_t off = ((uint32_t)reinterpret_cast<uintptr_t>(tensor) + 2 * (uint32_t)first) & 7;      // bytes in front of the first
+  uint32_t w[9], o[8];
+#pragma unroll
+  for (int i = 0; i < 9; ++i) {
+    const uint32_t near = i & 1 ? raw[i / 2].y : raw[i / 2].x, next = i & 1 ? raw[i / 2 + 1].x : raw[i / 2].y;
+    w[i] = off & 4 ? next : near;
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) o[i] = __funnelshift_r(w[i], w[i + 1], (off & 2) * 8);
+  if (count < 16) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i] = 2 * i + 1 < count ? o[i] : 2 * i < count ? o[i] & 0xffffu : 0u;
+  }
+  out[0] = make_uint4(o[0], o[1], o[2], o[3]);
+  out[1] = make_uint4(o[4], o[5], o[6], o[7]);
+}
+
 // The place of a piece of eight columns in an MN-major operand: blocks of 64 columns, rows of 128 bytes, 128-byte swizzle.
 __device__ __forceinline__ uint32_t piece_at(int row, int piece) { return (piece >> 3) * (WG_ROWS * 128) + row * 128 + (((piece & 7) ^ (row & 7)) << 4); }
 
@@ -236,18 +273,13 @@ float8_gradient_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_co
     const int ych = n0 + yp * 16;
     const int x_block = (k0 >> 7 & 3) + (xp >> 3), y_block = (n0 >> 7 & 3) + (yp >> 3);
     const bool x_any = xp < groups * 4, x_here = xp * 16 < (columns > 128 ? 256 : 128);
-    uint4 ahead[NB][2];      // MODE 1: the next step's units
+    // MODE 1: the next step's units, each as the five 8-byte words that its sixteen elements lie in
+    uint2 ahead[MODE == 1 ? NB : 1][5];
     auto fetch = [&](int t) {
 #pragma unroll
       for (int u = 0; u < NB; ++u) {
         const int64_t row = (int64_t)t * WG_ROWS + yr + kStep * u;
-        const uint16_t* from = reinterpret_cast<const uint16_t*>(p.dy) + row * p.n + ych;
-        uint32_t o[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          o[i] = (row < p.m && ych + 2 * i < p.n ? (uint32_t)from[2 * i] : 0u) | (row < p.m && ych + 2 * i + 1 < p.n ? (uint32_t)from[2 * i + 1] << 16 : 0u);
-        ahead[u][0] = make_uint4(o[0], o[1], o[2], o[3]);
-        ahead[u][1] = make_uint4(o[4], o[5], o[6], o[7]);
+        fetch_unaligned(ahead[u], p.dy, (int64_t)p.m * p.n, row * p.n + ych, row < p.m ? min(16, p.n - ych) : 0);
       }
     };
     int slot = 0, stage = 0; uint32_t phase = 0, ring_phase = 0;
@@ -270,7 +302,10 @@ float8_gradient_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_co
         if (MODE == 2) {
           dy_unit[u][0] = *reinterpret_cast<const uint4*>(dy_codes + stage * S::dy_codes + (yp >> 3) * WG_DY_CODES + swizzle128_offset(r, yp & 7));
           sy[u] = t * WG_ROWS + r < p.m ? e[512 + (r & 31) * 16 + (r >> 5) * 4 + y_block] : 1;
-        } else if (MODE == 1) { dy_unit[u][0] = ahead[u][0]; dy_unit[u][1] = ahead[u][1]; }
+        } else if (MODE == 1) {
+          const int64_t row = (int64_t)t * WG_ROWS + r;
+          place_unaligned(ahead[u], p.dy, row * p.n + ych, row < p.m ? min(16, p.n - ych) : 0, dy_unit[u]);
+        }
       }
       if (MODE == 1 && t + 1 < last) fetch(t + 1);
       __syncwarp();
@@ -442,9 +477,9 @@ void configure_float8_gradient() {
     });
 }
 
-// Blocks of outputs of a tile: two where there are two.  Beside more than 128 channels they leave room for one accumulator, so fewer rows than make a difference (2^32
-// multiplications, some 20 us) keep the two of a single block.
-static int gradient_blocks(int64_t m, int n, int k) { return n > WG_BN && (k <= 128 || (double)m * n * k >= 4294967296.0) ? 2 : 1; }
+// Blocks of outputs of a tile: two where there are two and work enough that sharing x's conversion pays (2^31 multiplications; 12000 x 128 -> 512 takes 14.2 us with
+// one block and 17.0 with two, 12000 x 100 -> 2000 26.1 and 22.4).  Beside more than 128 channels they leave room for one accumulator: from 2^32 on, some 20 us.
+static int gradient_blocks(int64_t m, int n, int k) { return n > WG_BN && (double)m * n * k >= (k <= 128 ? 2147483648.0 : 4294967296.0) ? 2 : 1; }
 
 // Blocks of rows: as many as the GPU has multiprocessors for beside the tiles, with four steps of 64 rows each at least - and 64 at most: the tensor core's
 // additions truncate, and 65536 x 1024 x 1024 with values of one sign was 3.5e-5 off in sums of 16384 rows (5.8e-6 in 4096).

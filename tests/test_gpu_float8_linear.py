@@ -153,6 +153,27 @@ def test_powers_that_cancel(dev, rows, c, n, power):
     ref.close(dx["output"], dy8 @ w8, n * STEP * (np.abs(dy8) @ np.abs(w8)), "gradient")
 
 
+@pytest.mark.parametrize("rows,c,n", [(1, 16, 1), (5, 40, 3), (64, 128, 17), (65, 100, 131), (300, 300, 77), (9000, 128, 2001)])
+def test_gradient_at_any_address(dev, rows, c, n):
+    """A bf16 gradient that starts at any element, with numbers that are none in front of it and behind: the same bits as from memory of its own."""
+    import localfold_b200 as lf
+    x8 = lf.float8_encode(dev, torch.randn(rows, c, device="cuda"), rows, c)
+    dy = torch.randn(rows, n, device="cuda").bfloat16()
+    linear, call = lf.Float8LinearGpu(dev), {"rows": rows, "channels": c, "outChannels": n, "activations": x8}
+    want = linear.weight_gradient({**call, "gradient": dy})
+    for shift in range(1, 9):
+        room = torch.full((rows * n + 32,), float("nan"), dtype=torch.bfloat16, device="cuda")
+        view = room[shift:shift + rows * n].view(rows, n)
+        view.copy_(dy)
+        got = linear.weight_gradient({**call, "gradient": view})
+        dev.synchronize()
+        assert torch.equal(got["weight"], want["weight"]) and torch.equal(got["bias"], want["bias"]), shift
+    values = lf.float8_decode(dev, x8, {"output": "f32"})
+    dev.synchronize()
+    chain = (min(rows, 4096) / 16 + 16 + max(rows / 4096, 148)) * STEP
+    ref.close(want["weight"], host(dy).T @ host(values), chain * (np.abs(host(dy)).T @ np.abs(host(values))), "weight")
+
+
 def test_long_sums(dev):
     """Values of one sign over many rows, several chains a tile: the bound of a chain holds, and what the tests' shorter sums allow."""
     import localfold_b200 as lf
