@@ -146,7 +146,7 @@ float8_gradient_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_co
   uint64_t* taken = loaded + WG_RING;                              // [RING] their codes are read (and a bf16 dy multiplied)
   uint64_t* full = taken + WG_RING;                                // [OPERANDS]
   uint64_t* empty = full + WG_OPERANDS;
-  uint64_t* done = empty + WG_OPERANDS;
+  uint64_t* done = empty + WG_OPERANDS;                            // every product, and every step's sums
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
@@ -161,7 +161,7 @@ float8_gradient_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_co
   if (threadIdx.x == 0) {
     for (int s = 0; s < WG_RING; ++s) { mbar_init(&loaded[s], 1); mbar_init(&taken[s], WG_CONVERT + (MODE == 0 ? 1 + (sums ? WG_SUMS : 0) : 0)); }
     for (int s = 0; s < WG_OPERANDS; ++s) { mbar_init(&full[s], WG_CONVERT); mbar_init(&empty[s], 1 + (MODE != 0 && sums ? WG_SUMS : 0)); }
-    mbar_init(done, 1);
+    mbar_init(done, 1 + (sums ? WG_SUMS : 0));
     *abort_flag = 0;
     fence_barrier_init();
   }
@@ -252,6 +252,8 @@ float8_gradient_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_co
         if (++slot == WG_OPERANDS) { slot = 0; phase ^= 1; }
         if (++stage == ring) { stage = 0; ring_phase ^= 1; }
       }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(done);      // (the last steps' slots are not filled again: nothing else waits for these reads of them)
 #pragma unroll
       for (int i = 0; i < NB * 4; ++i) {
         float2 v = total[i / 4][i % 4];
@@ -347,7 +349,7 @@ float8_gradient_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_co
     tc_fence_after();
     if (ok) {
       const int q = warp & 3, part = (warp - 2) >> 2, col0 = k0 + part * 64;
-      uint8_t* tiles = dy_s + (warp - 2) * 8192;      // (every product is done: the rings of dy and of x's codes are free)
+      uint8_t* tiles = dy_s + (warp - 2) * 8192;      // (every product is done and dy's columns are added up: the rings of dy and of x's codes are free)
       float* out = p.out + split * p.split_stride;
       const int used = min(accumulators, last - first);
 #pragma unroll 1
