@@ -3,7 +3,9 @@ projection on 8-bit operands with its gradients.  The reference runs the stack f
 
 They stand beside the operators of ``operators.py`` and are called alike (``run(input[, options])`` on a ``Device``), but take
 and return CUDA tensors only.  A call enqueues on the device's stream and returns.  Results and workspaces come from torch's
-allocator, so a call can be captured into a CUDA graph (on the stream that the ``Device`` was made on) and graphs share nothing.
+allocator, so a call can be captured into a CUDA graph (on the stream that the ``Device`` was made on) and graphs share nothing.  A device whose
+stream is not torch's current one waits for the work enqueued there before it writes into such memory; its inputs are ordered as for
+every operator (``Device``).
 
     norm, linear = lf.LayerNormGpu(dev), lf.Float8LinearGpu(dev)
     weights = lf.prepare_float8_linear_weights(dev, weight, bias)                 # [out][in], encoded once (update() after a step)
@@ -98,12 +100,13 @@ def _torch_dtype(name):
     return torch.float32 if name == "f32" else torch.bfloat16
 
 
-def _call(device, function, desc, tensors, output=None):
+def _call(device, function, desc, tensors, output=None, fresh=True):
     """One library call and its result object.  Where torch's current stream is not the device's: a device with a stream of its own waits for
-    torch's work first, and the device holds the call's tensors until its stream is done with them, so that torch does not
+    torch's work first, and so does any device where the call has taken memory from torch's allocator (``fresh``), which torch's work may still
+    be using for what it held before.  The device holds the call's tensors until its stream is done with them, so that torch does not
     give their memory away before."""
     current = _torch_stream(device.ordinal)
-    if current != device.stream and device._own_stream:
+    if current != device.stream and (device._own_stream or fresh):
         device.check(device.lib.lf_context_await(device.handle, current))
     res = nat.Result()
     status = function(device.handle, desc, res)
@@ -202,12 +205,12 @@ def float8_decode(device, encoded, options=None, out=None):
     if not isinstance(encoded, Float8Tensor):
         raise ValueError("encoded must be a Float8Tensor")
     _matrix(dev, "encoded", encoded, encoded.rows, encoded.channels)
-    dtype = _output(options, "bf16")
-    if out is None:
+    dtype, fresh = _output(options, "bf16"), out is None
+    if fresh:
         out = _new(encoded.memory, dtype, (encoded.rows, encoded.channels))
     else:
         _tensor(dev, "out", out, encoded.rows * encoded.channels, dtype)
-    _call(dev, dev.lib.lf_float8_decode, _DECODE.pack(*encoded.fields, _DTYPE[dtype], 0, out.data_ptr()), (encoded, out))
+    _call(dev, dev.lib.lf_float8_decode, _DECODE.pack(*encoded.fields, _DTYPE[dtype], 0, out.data_ptr()), (encoded, out), fresh=fresh)
     return out
 
 
@@ -246,19 +249,21 @@ class LayerNormGpu:
         _tensor(dev, "offset", offset, c, "f32")
         if encode and out is not None:
             raise ValueError("an encoded output is a new Float8Tensor; out is for the other kind")
-        if out is not None:
+        given = out is not None
+        if given:
             _tensor(dev, "out", out, rows * c, dtype)
         elif not encode:
             out = _torch().empty_like(x)
         checkpoint = Float8Tensor.empty(rows, c, kept, x) if kept else None
         encoded = Float8Tensor.empty(rows, c, encode, x) if encode else None
+        fresh = not given or kept is not None or encode is not None or bool(opts.get("statistics"))
         mean = inverse = None
         if kept or opts.get("statistics"):
             mean, inverse = scale.new_empty(rows), scale.new_empty(rows)
         desc = _LAYER_NORM.pack(rows, c, variance, _DTYPE[dtype], epsilon, x.data_ptr(), scale.data_ptr(), offset.data_ptr(),
                                 out.data_ptr() if out is not None else 0, 0 if mean is None else mean.data_ptr(), 0 if mean is None else inverse.data_ptr(),
                                 *(checkpoint.fields if kept else _NO_MATRIX), *(encoded.fields if encode else _NO_MATRIX))
-        result = _call(dev, dev.lib.lf_layer_norm_run, desc, (x, scale, offset, out, mean, inverse, checkpoint, encoded), encoded if encode else out)
+        result = _call(dev, dev.lib.lf_layer_norm_run, desc, (x, scale, offset, out, mean, inverse, checkpoint, encoded), encoded if encode else out, fresh)
         if mean is not None:
             result["mean"], result["inverseDeviation"] = mean, inverse
         if kept:
@@ -371,6 +376,7 @@ class Float8LinearGpu:
             else:
                 nbytes = dev.lib.lf_float8_linear_workspace(rows, channels)
                 workspace = _new(value, "bytes", nbytes) if nbytes else None
+        fresh = out is None or keep or nbytes > 0
         if out is not None:
             _tensor(dev, "out", out, rows * weights.rows, dtype)
         else:
@@ -378,7 +384,7 @@ class Float8LinearGpu:
         desc = _LINEAR.pack(*(operand.fields if operand is not None else (rows, channels, _FORMAT[format], 0, 0)), *weights.fields,
                             bias.data_ptr() if bias is not None else 0, _DTYPE[dtype], _DTYPE[source or "f32"], value.data_ptr() if source else 0,
                             out.data_ptr(), workspace.data_ptr() if nbytes else 0, nbytes)
-        result = _call(dev, dev.lib.lf_float8_linear_run, desc, (value, operand, weights, bias, workspace, out), out)
+        result = _call(dev, dev.lib.lf_float8_linear_run, desc, (value, operand, weights, bias, workspace, out), out, fresh)
         if keep:
             result["checkpoint"] = operand
         return result
