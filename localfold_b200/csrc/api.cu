@@ -85,7 +85,7 @@ void* lf_context_stream(const lf_context* ctx) { return ctx ? (void*)ctx->stream
 lf_status lf_context_await(lf_context* ctx, void* stream) {
   if (!ctx) return LF_ERR_ARGUMENT;
   if ((cudaStream_t)stream == ctx->stream) return LF_OK;
-  cudaSetDevice(ctx->device);
+  const lf_device_guard device(ctx);
   LF_CUDA(ctx, cudaEventRecord(ctx->inputs, (cudaStream_t)stream));
   LF_CUDA(ctx, cudaStreamWaitEvent(ctx->stream, ctx->inputs, 0));
   return LF_OK;

@@ -49,6 +49,18 @@ struct lf_context {
   uint64_t family_launches[LF_KERNEL_FAMILY_COUNT] = {0};
 };
 
+// The context's GPU is the thread's current one while a call lasts.
+struct lf_device_guard {
+  int before = 0;
+  bool moved = false;
+  explicit lf_device_guard(const lf_context* ctx) {
+    if (cudaGetDevice(&before) == cudaSuccess && before != ctx->device) moved = cudaSetDevice(ctx->device) == cudaSuccess;
+  }
+  ~lf_device_guard() { if (moved) cudaSetDevice(before); }
+  lf_device_guard(const lf_device_guard&) = delete;
+  lf_device_guard& operator=(const lf_device_guard&) = delete;
+};
+
 static inline void lf_prof_begin(lf_context* ctx, int family) {
   if (!ctx->profiling) return;
   lf_context::Timed t{family, nullptr, nullptr};

@@ -23,17 +23,6 @@
 lf_status lf_float8_check_rows(lf_context* ctx, const char* what, int64_t rows, int channels, int dtype);
 lf_status lf_float8_check(lf_context* ctx, const char* what, const lf_float8_matrix& m, int64_t rows, int channels);
 lf_status lf_float8_done(lf_context* ctx, lf_result* r, int launches);
-// The context's GPU is the thread's current one while a call lasts.
-struct lf_device_guard {
-  int before = 0;
-  bool moved = false;
-  explicit lf_device_guard(const lf_context* ctx) {
-    if (cudaGetDevice(&before) == cudaSuccess && before != ctx->device) moved = cudaSetDevice(ctx->device) == cudaSuccess;
-  }
-  ~lf_device_guard() { if (moved) cudaSetDevice(before); }
-  lf_device_guard(const lf_device_guard&) = delete;
-  lf_device_guard& operator=(const lf_device_guard&) = delete;
-};
 
 namespace f8 {
 
