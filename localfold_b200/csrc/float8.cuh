@@ -28,8 +28,8 @@ namespace f8 {
 
 constexpr int kBlock = 128;      // channels that share an exponent
 
-__host__ __device__ inline int64_t pitch(int channels) { return (channels + 15) & ~15; }
-__host__ __device__ inline int blocks(int channels) { return (channels + kBlock - 1) / kBlock; }
+__host__ __device__ inline int64_t pitch(int channels) { return ((int64_t)channels + 15) & ~(int64_t)15; }
+__host__ __device__ inline int blocks(int channels) { return (int)(((uint32_t)channels + (kBlock - 1)) / kBlock); }
 __host__ __device__ inline int64_t row_tiles(int64_t rows) { return (rows + 127) >> 7; }
 __host__ __device__ inline int64_t exponent_bytes(int64_t rows, int channels) { return (int64_t)((blocks(channels) + 3) / 4) * row_tiles(rows) * 512; }
 // `tiles` = row_tiles(rows)

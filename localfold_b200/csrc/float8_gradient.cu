@@ -487,9 +487,10 @@ static int gradient_blocks(int64_t m, int n, int k) { return n > WG_BN && (doubl
 // additions truncate, and 65536 x 1024 x 1024 with values of one sign was 3.5e-5 off in sums of 16384 rows (5.8e-6 in 4096).
 static void gradient_plan(const lf_context* ctx, int64_t m, int n, int k, int& steps, int& splits, int& per_split) {
   constexpr int kMostSteps = 64, kMostSplits = 65535;
-  const int outputs = WG_BN * gradient_blocks(m, n, k), tiles = ((n + outputs - 1) / outputs) * ((k + WG_BK - 1) / WG_BK);
+  const int outputs = WG_BN * gradient_blocks(m, n, k);
+  const int64_t tiles = (int64_t)((n + outputs - 1) / outputs) * ((k + WG_BK - 1) / WG_BK);
   steps = (int)((m + WG_ROWS - 1) / WG_ROWS);
-  const int want = std::max(1, std::min(ctx->sm_count / tiles, steps / 4)), most = std::max(kMostSteps, (steps + kMostSplits - 1) / kMostSplits);
+  const int want = std::max(1, std::min((int)(ctx->sm_count / tiles), steps / 4)), most = std::max(kMostSteps, (steps + kMostSplits - 1) / kMostSplits);
   per_split = (steps + want - 1) / want;
   if (per_split > most) {      // whole turns of the blocks
     const int turns = (per_split + most - 1) / most;
@@ -498,6 +499,7 @@ static void gradient_plan(const lf_context* ctx, int64_t m, int n, int k, int& s
   splits = (steps + per_split - 1) / per_split;
 }
 static int64_t partial_ld(int k) { return (k + 3) / 4 * 4; }
+constexpr int kMostChannels = 1 << 22;      // of either side; blocks of 128 outputs then number 32768
 
 }  // namespace tc
 
@@ -506,7 +508,7 @@ using namespace f8;
 extern "C" {
 
 uint64_t lf_float8_weight_gradient_workspace(const lf_context* ctx, int64_t rows, int32_t channels, int32_t out_channels) {
-  if (!ctx || rows <= 0 || rows > 0x7fffffff || channels <= 0 || out_channels <= 0) return 0;
+  if (!ctx || rows <= 0 || rows > 0x7fffff00 || channels <= 0 || out_channels <= 0 || channels > tc::kMostChannels || out_channels > tc::kMostChannels) return 0;
   int steps, splits, per_split;
   tc::gradient_plan(ctx, rows, out_channels, channels, steps, splits, per_split);
   return splits == 1 ? 0 : (uint64_t)splits * out_channels * (tc::partial_ld(channels) + 1) * sizeof(float);
@@ -519,7 +521,7 @@ lf_status lf_float8_weight_gradient_run(lf_context* ctx, const lf_float8_weight_
   const lf_float8_matrix& x = d->activations;
   LF_TRY(lf_float8_check_rows(ctx, "float8 weight gradient", x.rows, x.channels, LF_DTYPE_BF16));
   LF_TRY(lf_float8_check_rows(ctx, "float8 weight gradient", x.rows, d->out_channels, LF_DTYPE_BF16));
-  if (d->out_channels > (1 << 22) || x.channels > (1 << 22)) return lf_fail(ctx, LF_ERR_UNSUPPORTED, "float8 weight gradient: %d x %d are too many channels", d->out_channels, x.channels);
+  if (d->out_channels > tc::kMostChannels || x.channels > tc::kMostChannels) return lf_fail(ctx, LF_ERR_UNSUPPORTED, "float8 weight gradient: %d x %d are too many channels", d->out_channels, x.channels);
   LF_TRY(lf_float8_check(ctx, "float8 weight gradient, activations", x, x.rows, x.channels));
   if (d->encoded_gradient.codes) LF_TRY(lf_float8_check(ctx, "float8 weight gradient, gradient", d->encoded_gradient, x.rows, d->out_channels));
   const uint64_t need = lf_float8_weight_gradient_workspace(ctx, x.rows, x.channels, d->out_channels);

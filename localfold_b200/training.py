@@ -43,6 +43,7 @@ _WEIGHT_GRADIENT = struct.Struct("@" + _MATRIX + "Q" + _MATRIX + "ii4Q")
 _NO_MATRIX = (0, 0, 0, 0, 0)
 _NO_OPTIONS = {}
 _MOST = 2 ** 31 - 1                                # rows and channels are 32-bit numbers in the kernels
+_MOST_GRADIENT = 2 ** 22                           # channels of either side of a weight's gradient
 _LARGEST = (2 - 2.0 ** -23) * 2.0 ** 127           # of float32
 _AS_IT_WAS = object()
 
@@ -423,6 +424,8 @@ class Float8LinearGpu:
         ``[outChannels][channels]`` and ``bias`` ``[outChannels]``, float32, the same bits at every call."""
         dev = self.device
         rows, channels, n = _size(input, "rows"), _size(input, "channels"), _size(input, "outChannels")
+        if max(channels, n) > _MOST_GRADIENT:
+            raise NotImplementedError(f"the weight's gradient of {n} x {channels} channels: at most {_MOST_GRADIENT} of either")
         dy, x = input["gradient"], _matrix(dev, "activations", input["activations"], rows, channels)
         encoded = isinstance(dy, Float8Tensor)
         if encoded:
