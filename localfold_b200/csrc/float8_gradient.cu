@@ -486,15 +486,15 @@ static int gradient_blocks(int64_t m, int n, int k) { return n > WG_BN && (doubl
 // Blocks of rows: as many as the GPU has multiprocessors for beside the tiles, with four steps of 64 rows each at least - and 64 at most: the tensor core's
 // additions truncate, and 65536 x 1024 x 1024 with values of one sign was 3.5e-5 off in sums of 16384 rows (5.8e-6 in 4096).
 static void gradient_plan(const lf_context* ctx, int64_t m, int n, int k, int& steps, int& splits, int& per_split) {
-  constexpr int kMostSteps = 64, kMostSplits = 65535;
+  constexpr int kMostSteps = 64, kMostSplits = 65535;      // (of the grid; beyond 64 * 65535 steps splits are longer)
   const int outputs = WG_BN * gradient_blocks(m, n, k);
   const int64_t tiles = (int64_t)((n + outputs - 1) / outputs) * ((k + WG_BK - 1) / WG_BK);
   steps = (int)((m + WG_ROWS - 1) / WG_ROWS);
-  const int want = std::max(1, std::min((int)(ctx->sm_count / tiles), steps / 4)), most = std::max(kMostSteps, (steps + kMostSplits - 1) / kMostSplits);
+  const int want = std::max(1, std::min((int)(ctx->sm_count / tiles), steps / 4)), least = (steps + kMostSplits - 1) / kMostSplits, most = std::max(kMostSteps, least);
   per_split = (steps + want - 1) / want;
   if (per_split > most) {      // whole turns of the blocks
     const int turns = (per_split + most - 1) / most;
-    per_split = (steps + want * turns - 1) / (want * turns);
+    per_split = std::max(least, (steps + want * turns - 1) / (want * turns));
   }
   splits = (steps + per_split - 1) / per_split;
 }

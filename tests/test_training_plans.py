@@ -41,6 +41,22 @@ def test_workspace_at_the_limits():
     assert ask("lf_float8_weight_gradient_workspace", 148 * 256, 128, 128) == 148 * 128 * 129 * 4
 
 
+@pytest.mark.parametrize("rows", [64 * 65535 * 64 + 1, 1_860_000_000, 1_859_838_912 + 64 * 148, 2_000_000_000, 2 ** 31 - 257, 2 ** 31 - 256])
+@pytest.mark.parametrize("channels,outputs", [(8, 8), (8, 128), (256, 300)])
+def test_splits_fit_the_grid(rows, channels, outputs):
+    size = outputs * (channels + 1) * 4
+    nbytes = ask("lf_float8_weight_gradient_workspace", rows, channels, outputs)
+    assert nbytes % size == 0 and 148 < nbytes // size <= 65535
+
+
+def test_splits_over_the_whole_range():
+    """... and at every 64th thousand of rows, in one process."""
+    many = ASK.replace("print(getattr(lib, name)(*arguments))", "call = getattr(lib, name)\n"
+                       "print(max(call(arguments[0], rows, 8, 8) for rows in range(1 << 20, 2 ** 31 - 256, 64000)) // (8 * 9 * 4))")
+    out = subprocess.run([sys.executable, "-c", many, "lf_float8_weight_gradient_workspace"], capture_output=True, text=True, env={**os.environ, "PYTHONPATH": ROOT})
+    assert out.returncode == 0 and 60000 < int(out.stdout) <= 65535, (out.stdout, out.stderr)
+
+
 @pytest.mark.parametrize("rows,channels", [(17, 2 ** 31 - 1), (17, 2 ** 31 - 16), (100, 1 << 24), (2 ** 31 - 1, 8)])
 def test_bytes_of_an_operand(rows, channels):
     codes = rows * (-(-channels // 16) * 16)
