@@ -74,13 +74,26 @@ def _torch():
     return torch
 
 
+def _has_memory(name, value):
+    """A fake tensor or one that a function transform has wrapped passes every other check; the library would take it for one that was left out."""
+    try:
+        if value.data_ptr():
+            return
+    except RuntimeError:
+        pass
+    raise ValueError(f"{name} must be a tensor with memory of its own; received {type(value).__name__}")
+
+
 def _tensor(device, name, value, count, only=None):
     """A tensor argument: on the device's GPU, contiguous, float32 or bfloat16 (``only``: one of them), of ``count`` values.
     Returns "f32" or "bf16"."""
     if getattr(value, "is_cuda", False) and value.get_device() == device.ordinal:
         dtype = _names.get(value.dtype)
-        if dtype is not None and (only is None or only == dtype) and value.numel() == count and value.is_contiguous():
-            return dtype
+        try:
+            if dtype is not None and (only is None or only == dtype) and value.numel() == count and value.is_contiguous() and value.data_ptr():
+                return dtype
+        except RuntimeError:      # (no address: below)
+            pass
     if not getattr(value, "is_cuda", False):
         raise ValueError(f"{name} must be a CUDA tensor")
     if value.get_device() != device.ordinal:
@@ -93,6 +106,7 @@ def _tensor(device, name, value, count, only=None):
         raise ValueError(f"{name} must be contiguous")
     if value.numel() != count:
         raise RangeError(f"{name} has {value.numel()} values; expected {count}")
+    _has_memory(name, value)
     return dtype
 
 
@@ -129,9 +143,20 @@ _empty = {}      # (GPU, dtype) -> an empty tensor: new memory of that kind take
 def _new(like, dtype, shape):
     key = (like.get_device(), dtype)
     proto = _empty.get(key)
-    if proto is None:
-        proto = _empty[key] = like.new_empty(0, dtype=_torch().uint8 if dtype == "bytes" else _torch_dtype(dtype))
-    return proto.new_empty(shape)
+    if proto is None:      # (a plain tensor, whatever the call's own are and whichever mode it is made in)
+        torch = _torch()
+        with torch.inference_mode(False):
+            proto = _plain(torch.empty(0, dtype=torch.uint8 if dtype == "bytes" else _torch_dtype(dtype), device=like.device))
+        proto.data_ptr()
+        _empty[key] = proto
+    value = proto.new_empty(shape)
+    return value if type(value) is type(proto) else _plain(value)
+
+
+def _plain(value):
+    if type(value) is not _torch().Tensor:
+        raise ValueError(f"the operators allocate memory of their own, not {type(value).__name__}s")
+    return value
 
 
 class Float8Tensor:
@@ -148,6 +173,7 @@ class Float8Tensor:
             raise ValueError("memory must be a contiguous uint8 CUDA tensor")
         if memory.numel() != self._codes + exponents:
             raise RangeError(f"memory has {memory.numel()} values; expected {self._codes + exponents}")
+        _has_memory("memory", memory)
         base = memory.data_ptr()
         self.fields = (rows, channels, _FORMAT[format], base, base + self._codes)
 
@@ -254,13 +280,13 @@ class LayerNormGpu:
         if given:
             _tensor(dev, "out", out, rows * c, dtype)
         elif not encode:
-            out = _torch().empty_like(x)
+            out = _new(x, dtype, x.shape)
         checkpoint = Float8Tensor.empty(rows, c, kept, x) if kept else None
         encoded = Float8Tensor.empty(rows, c, encode, x) if encode else None
         fresh = not given or kept is not None or encode is not None or bool(opts.get("statistics"))
         mean = inverse = None
         if kept or opts.get("statistics"):
-            mean, inverse = scale.new_empty(rows), scale.new_empty(rows)
+            mean, inverse = _new(scale, "f32", rows), _new(scale, "f32", rows)
         desc = _LAYER_NORM.pack(rows, c, variance, _DTYPE[dtype], epsilon, x.data_ptr(), scale.data_ptr(), offset.data_ptr(),
                                 out.data_ptr() if out is not None else 0, 0 if mean is None else mean.data_ptr(), 0 if mean is None else inverse.data_ptr(),
                                 *(checkpoint.fields if kept else _NO_MATRIX), *(encoded.fields if encode else _NO_MATRIX))
@@ -291,9 +317,9 @@ class LayerNormGpu:
         if out is not None:
             _tensor(dev, "out", out, rows * c, dtype)
         else:
-            out = _torch().empty_like(dy)
+            out = _new(dy, dtype, dy.shape)
         nbytes = dev.lib.lf_layer_norm_backward_workspace(dev.handle, rows, c)
-        dscale, doffset, workspace = scale.new_empty(c), scale.new_empty(c), _new(scale, "bytes", nbytes) if nbytes else None
+        dscale, doffset, workspace = _new(scale, "f32", c), _new(scale, "f32", c), _new(scale, "bytes", nbytes) if nbytes else None
         desc = _LAYER_NORM_BACKWARD.pack(rows, c, _DTYPE[dtype], dy.data_ptr(), 0 if encoded else x.data_ptr(), *(x.fields if encoded else _NO_MATRIX),
                                          mean.data_ptr(), inverse.data_ptr(), scale.data_ptr(), out.data_ptr(), dscale.data_ptr(), doffset.data_ptr(), workspace.data_ptr() if nbytes else 0, nbytes)
         result = _call(dev, dev.lib.lf_layer_norm_backward_run, desc, (dy, x, mean, inverse, scale, out, dscale, doffset, workspace), out)
@@ -434,7 +460,7 @@ class Float8LinearGpu:
             _tensor(dev, "gradient", dy, rows * n, "bf16")
         nbytes = dev.lib.lf_float8_weight_gradient_workspace(dev.handle, rows, channels, n)
         weight = _new(x.memory, "f32", (n, channels))
-        bias, workspace = weight.new_empty(n), _new(weight, "bytes", nbytes) if nbytes else None
+        bias, workspace = _new(weight, "f32", n), _new(weight, "bytes", nbytes) if nbytes else None
         desc = _WEIGHT_GRADIENT.pack(*x.fields, 0 if encoded else dy.data_ptr(), *(dy.fields if encoded else _NO_MATRIX), n, 0, weight.data_ptr(), bias.data_ptr(),
                                      workspace.data_ptr() if nbytes else 0, nbytes)
         result = _call(dev, dev.lib.lf_float8_weight_gradient_run, desc, (dy, x, weight, bias, workspace), weight)
