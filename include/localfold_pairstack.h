@@ -567,6 +567,7 @@ LF_API lf_status lf_pair_transpose_scatter(lf_context* ctx, const void* src, int
  * `workspace` that its *_workspace function gives the size of (16-byte aligned; its content
  * means nothing between calls).  So a call can be captured into a CUDA graph as it is, and two
  * graphs with workspaces of their own are independent.  Rows of tensors follow one another without gaps.
+ * What a call writes overlaps nothing that it reads or writes besides, but where it says so.
  * ------------------------------------------------------------------------------------------ */
 
 /* The 8-bit form of a float matrix [rows][channels].  128 consecutive channels of a row share one
@@ -626,7 +627,7 @@ typedef struct lf_layer_norm_desc {
 } lf_layer_norm_desc;
 LF_API lf_status lf_layer_norm_run(lf_context* ctx, const lf_layer_norm_desc* d, lf_result* r);
 /* Its gradients from gradient = dL/dy (act_dtype) and the statistics of the forward pass: out = dL/dx
- * (act_dtype; may be gradient itself), dL/dscale and dL/doffset [channels] float32.  The input is given whole
+ * (act_dtype; may be gradient itself, or activations), dL/dscale and dL/doffset [channels] float32.  The input is given whole
  * (activations, act_dtype) or as the checkpoint.  Results do not depend on how the GPU schedules the
  * blocks. */
 typedef struct lf_layer_norm_backward_desc {

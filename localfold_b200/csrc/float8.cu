@@ -166,6 +166,17 @@ lf_status lf_float8_check(lf_context* ctx, const char* what, const lf_float8_mat
   return LF_OK;
 }
 
+lf_status lf_float8_apart(lf_context* ctx, const char* what, const void* out, uint64_t bytes, const void* operand, uint64_t operand_bytes) {
+  const uintptr_t a = (uintptr_t)out, b = (uintptr_t)operand;
+  if (a && b && a < b + operand_bytes && b < a + bytes) return lf_fail(ctx, LF_ERR_ARGUMENT, "%s: the output overlaps an operand", what);
+  return LF_OK;
+}
+lf_status lf_float8_apart(lf_context* ctx, const char* what, const void* out, uint64_t bytes, const lf_float8_matrix& m) {
+  if (!m.codes) return LF_OK;
+  LF_TRY(lf_float8_apart(ctx, what, out, bytes, m.codes, lf_float8_code_bytes(m.rows, m.channels)));
+  return lf_float8_apart(ctx, what, out, bytes, m.exponents, lf_float8_exponent_bytes(m.rows, m.channels));
+}
+
 lf_status lf_float8_done(lf_context* ctx, lf_result* r, int launches) {
   LF_CUDA(ctx, cudaGetLastError());
   if (r) { r->elapsed_ms = 0.f; r->peak_bytes = ctx->arena_peak; r->launches = (uint32_t)launches; }
@@ -226,6 +237,7 @@ lf_status lf_float8_decode(lf_context* ctx, const lf_float8_decode_desc* d, lf_r
   const lf_float8_matrix& o = d->source;
   LF_TRY(lf_float8_check_rows(ctx, "float8 decode", o.rows, o.channels, d->dtype));
   LF_TRY(lf_float8_check(ctx, "float8 decode", o, o.rows, o.channels));
+  LF_TRY(lf_float8_apart(ctx, "float8 decode", d->out, (uint64_t)o.rows * o.channels * (d->dtype == LF_DTYPE_BF16 ? 2 : 4), o));
   const lf_device_guard device(ctx);
   const Matrix m = matrix(o);
   const int access = row_access(d->out, o.channels, d->dtype);

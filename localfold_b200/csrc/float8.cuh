@@ -22,6 +22,9 @@
 // Checks that several entry points share (float8.cu).
 lf_status lf_float8_check_rows(lf_context* ctx, const char* what, int64_t rows, int channels, int dtype);
 lf_status lf_float8_check(lf_context* ctx, const char* what, const lf_float8_matrix& m, int64_t rows, int channels);
+// A result's memory is apart from an operand's: its first blocks store while others still read.
+lf_status lf_float8_apart(lf_context* ctx, const char* what, const void* out, uint64_t bytes, const void* operand, uint64_t operand_bytes);
+lf_status lf_float8_apart(lf_context* ctx, const char* what, const void* out, uint64_t bytes, const lf_float8_matrix& operand);
 lf_status lf_float8_done(lf_context* ctx, lf_result* r, int launches);
 
 namespace f8 {

@@ -573,6 +573,13 @@ extern "C" lf_status lf_float8_linear_run(lf_context* ctx, const lf_float8_linea
   const uint64_t need = d->source && !kept ? lf_float8_linear_workspace(x.rows, x.channels) : 0;
   if (need && (!d->workspace || d->workspace_bytes < need || !lf_aligned16(d->workspace)))
     return lf_fail(ctx, LF_ERR_ARGUMENT, "float8 linear: a workspace of %llu bytes on a 16-byte boundary is needed", (unsigned long long)need);
+  const uint64_t out_bytes = (uint64_t)x.rows * w.rows * (d->out_dtype == LF_DTYPE_BF16 ? 2 : 4);
+  if (d->source)
+    LF_TRY(lf_float8_apart(ctx, "float8 linear", d->out, out_bytes, d->source, (uint64_t)x.rows * x.channels * (d->source_dtype == LF_DTYPE_BF16 ? 2 : 4)));
+  LF_TRY(lf_float8_apart(ctx, "float8 linear", d->out, out_bytes, x));
+  LF_TRY(lf_float8_apart(ctx, "float8 linear", d->out, out_bytes, w));
+  if (d->bias) LF_TRY(lf_float8_apart(ctx, "float8 linear", d->out, out_bytes, d->bias, (uint64_t)w.rows * 4));
+  if (need) LF_TRY(lf_float8_apart(ctx, "float8 linear", d->out, out_bytes, d->workspace, need));
   const lf_device_guard device(ctx);
   if (tc::float8_few_takes(x.rows, x.channels)) {
     LF_TRY(tc::float8_few(ctx, d->source, d->source ? d->source_dtype : LF_DTYPE_F32, mx, mw, d->bias, d->out, d->out_dtype));

@@ -259,7 +259,7 @@ class LayerNormGpu:
         ``[channels]`` (float32), epsilon (default 1e-5).  ``options``: statistics - also return ``mean`` and ``inverseDeviation``
         ``[rows]`` for ``backward``; checkpoint "e4m3" | "e5m2" - those and the input's 8-bit form as ``checkpoint``; encode "e4m3" |
         "e5m2" - the output is a ``Float8Tensor``, the operand of a ``Float8LinearGpu``; variance "two-pass" | "fast" (two passes
-        either way).  ``out`` may be the activations."""
+        either way).  ``out`` may be the activations; it may not overlap them otherwise."""
         dev, opts = self.device, options or _NO_OPTIONS
         rows, c = _size(input, "rows"), _size(input, "channels")
         x, scale, offset = input["activations"], input["scale"], input["offset"]
@@ -300,7 +300,7 @@ class LayerNormGpu:
     def backward(self, input, options=None, out=None):
         """``input``: rows, channels, gradient (of the output, ``[rows][channels]``), activations (the forward pass' input: a tensor of
         the gradient's type, or its checkpoint), mean, inverseDeviation, scale.  Returns the gradients of ``activations`` (of the
-        gradient's type; ``out`` may be the gradient itself), ``scale`` and ``offset`` (float32).  The sums over the rows have a
+        gradient's type; ``out`` may be the gradient or the activations, and may not overlap them otherwise), ``scale`` and ``offset`` (float32).  The sums over the rows have a
         fixed order: the same call gives the same bits."""
         dev = self.device
         rows, c = _size(input, "rows"), _size(input, "channels")
@@ -384,7 +384,7 @@ class Float8LinearGpu:
 
     ``run`` and ``input_gradient`` encode a float32 or bfloat16 operand in the call (``options``: format "e4m3" (default) | "e5m2") or take
     a ``Float8Tensor``; with the option checkpoint the encoded operand is returned as ``checkpoint``.  Option output "f32" | "bf16":
-    the result's type, by default the operand's (bf16 for a ``Float8Tensor``)."""
+    the result's type, by default the operand's (bf16 for a ``Float8Tensor``).  ``out`` may not overlap what the call reads."""
 
     def __init__(self, device: Device | None = None):
         self.device = _device(device)
