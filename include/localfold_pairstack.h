@@ -105,7 +105,8 @@ LF_API lf_status lf_context_create_on_stream(int device_ordinal, void* stream, l
  * not ordered with the library's: use this stream, or events, or lf_context_synchronize. */
 LF_API void* lf_context_stream(const lf_context* ctx);
 /* Work enqueued on the context's stream from here on comes after what `stream` holds now (no host wait).  For inputs
- * that other code produces on a stream of its own. */
+ * that other code produces on a stream of its own.  Refused (LF_ERR_UNSUPPORTED) while the context's stream is captured into a graph
+ * and `stream` is not. */
 LF_API lf_status lf_context_await(lf_context* ctx, void* stream);
 LF_API void lf_context_destroy(lf_context* ctx);
 LF_API const char* lf_last_error(const lf_context* ctx);

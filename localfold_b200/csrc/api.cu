@@ -86,6 +86,14 @@ lf_status lf_context_await(lf_context* ctx, void* stream) {
   if (!ctx) return LF_ERR_ARGUMENT;
   if ((cudaStream_t)stream == ctx->stream) return LF_OK;
   const lf_device_guard device(ctx);
+  // (a wait for work outside would end the capture with an error; asking does not)
+  auto captured = [](cudaStream_t s) {
+    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing(s, &status) != cudaSuccess) cudaGetLastError();
+    return status != cudaStreamCaptureStatusNone;
+  };
+  if (captured(ctx->stream) && !captured((cudaStream_t)stream))
+    return lf_fail(ctx, LF_ERR_UNSUPPORTED, "a call that is being captured cannot wait for work on a stream that is not");
   LF_CUDA(ctx, cudaEventRecord(ctx->inputs, (cudaStream_t)stream));
   LF_CUDA(ctx, cudaStreamWaitEvent(ctx->stream, ctx->inputs, 0));
   return LF_OK;

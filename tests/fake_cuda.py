@@ -28,10 +28,15 @@ int cudaStreamCreateWithFlags(void** s, unsigned f) { *s = calloc(1, 8); return 
 int cudaStreamDestroy(void* s) { free(s); return 0; }
 int cudaStreamSynchronize(void* s) { return 0; }
 int cudaStreamWaitEvent(void* s, void* e, unsigned f) { return 0; }
+static void* capturing = (void*)-1;      /* the stream that is */
+static int recorded;
+void fake_capture(void* s) { capturing = s; }
+int fake_recorded(void) { return recorded; }
+int cudaStreamIsCapturing(void* s, int* status) { *status = s == capturing; return 0; }
 int cudaEventCreate(void** e) { *e = calloc(1, 8); return 0; }
 int cudaEventCreateWithFlags(void** e, unsigned f) { *e = calloc(1, 8); return 0; }
 int cudaEventDestroy(void* e) { free(e); return 0; }
-int cudaEventRecord(void* e, void* s) { return 0; }
+int cudaEventRecord(void* e, void* s) { ++recorded; return 0; }
 int cudaLaunchKernelExC(const void* c, const void* f, void** a) { ++launches; return 0; }
 """
 OPEN = """
@@ -39,8 +44,8 @@ import ctypes
 from localfold_b200 import _native as nat
 lib, context = nat.load(), ctypes.c_void_p()
 assert lib.lf_context_create(0, None, ctypes.byref(context)) == nat.LF_OK
-context = context.value
-launches = ctypes.CDLL({fake!r}).fake_launches
+context, fake = context.value, ctypes.CDLL({fake!r})
+launches = fake.fake_launches
 
 
 def call(function, desc):

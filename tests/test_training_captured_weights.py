@@ -1,0 +1,82 @@
+"""Weights of one device in calls of another that are captured into a graph."""
+import pytest
+import torch
+
+import fake_cuda
+import localfold_b200 as lf
+from localfold_b200 import training
+from test_training_refusals import Fake, FakeDevice, float8, weights
+
+WAIT = """
+stream, other = lib.lf_context_stream(context), 64
+fake.fake_capture.argtypes = [ctypes.c_void_p]
+assert lib.lf_context_await(context, other) == nat.LF_OK and fake.fake_recorded() == 1
+fake.fake_capture(stream)
+assert lib.lf_context_await(context, other) == nat.LF_ERR_UNSUPPORTED and fake.fake_recorded() == 1
+print(lib.lf_last_error(context).decode())
+assert lib.lf_context_await(context, stream) == nat.LF_OK
+fake.fake_capture(other)      # (work of this context joins a capture elsewhere)
+assert lib.lf_context_await(context, other) == nat.LF_OK and fake.fake_recorded() == 2
+"""
+
+
+def test_wait_in_a_capture_is_refused(tmp_path):
+    assert "a call that is being captured cannot wait" in fake_cuda.run(tmp_path, WAIT)
+
+
+def test_one_wait_an_update(monkeypatch):
+    """A device waits for the weights once after each update, so that what follows can be captured."""
+    monkeypatch.setattr(training, "_torch_stream", lambda ordinal: 1)
+    log = []
+    owner, users = FakeDevice(log, 1), [FakeDevice(log, 2), FakeDevice(log, 3)]
+    w, value = weights(6, 8), Fake(48)
+    w.device, value.shape = owner, (6, 8)
+    call = {"rows": 4, "channels": 8, "outChannels": 6, "activations": float8(4, 8), "weights": w}
+    back = {"rows": 4, "channels": 8, "outChannels": 6, "gradient": float8(4, 6), "weights": w}
+    for _ in range(3):
+        log.clear()
+        for _ in range(3):
+            for user in users:
+                lf.Float8LinearGpu(user).run(call, None, Fake(24, torch.bfloat16))
+                lf.Float8LinearGpu(user).input_gradient(back, None, Fake(32, torch.bfloat16))
+        assert [e[1:3] for e in log if e[0] == "lf_context_await"] == [(2, 1), (3, 1)]
+        log.clear()
+        w.update(value)
+        assert sorted(e[1:3] for e in log if e[0] == "lf_context_await") == [(1, 2), (1, 3)] and log[-1][0] == "lf_float8_encode"
+
+
+@pytest.mark.gpu
+def test_captured_on_another_device():
+    stream = torch.cuda.Stream()
+    owner, user = lf.Device(0), lf.Device(0, stream=stream.cuda_stream)
+    x, first, second = torch.randn(300, 512, device="cuda"), torch.randn(400, 512, device="cuda"), torch.randn(400, 512, device="cuda")
+    w = lf.prepare_float8_linear_weights(owner, first)
+    call = {"rows": 300, "channels": 512, "outChannels": 400, "activations": x, "weights": w}
+    owner.synchronize()
+    torch.cuda.synchronize()
+    linear = lf.Float8LinearGpu(user)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(stream):
+        linear.run({**call, "weights": lf.prepare_float8_linear_weights(user, first)})      # (modules are loaded)
+        stream.synchronize()
+        with torch.cuda.graph(graph, stream=stream):
+            with pytest.raises(NotImplementedError, match="a call that is being captured cannot wait"):
+                linear.run(call)
+            x.add_(0)      # (the capture goes on)
+        graph = torch.cuda.CUDAGraph()
+        want = linear.run(call)["output"]
+        stream.synchronize()
+        with torch.cuda.graph(graph, stream=stream):
+            got = linear.run(call)["output"]
+        graph.replay()
+    stream.synchronize()
+    assert torch.equal(got, want)
+    w.update(second)
+    owner.synchronize()
+    with torch.cuda.stream(stream):
+        graph.replay()
+        new = linear.run(call)["output"]
+    stream.synchronize()
+    assert torch.equal(got, new) and not torch.equal(got, want)
+    owner.close()
+    user.close()
