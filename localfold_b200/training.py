@@ -20,6 +20,7 @@ every operator (``Device``).
 from __future__ import annotations
 
 import struct
+import sys
 import weakref
 
 import numpy as np
@@ -115,7 +116,12 @@ def _torch_dtype(name):
     return torch.float32 if name == "f32" else torch.bfloat16
 
 
-def _call(device, function, desc, tensors, output=None, fresh=True):
+def _capturing():
+    torch = _torch()
+    return torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing()
+
+
+def _call(device, function, desc, tensors, output=None, fresh=True, weights=None):
     """One library call and its result object.  Where torch's current stream is not the device's: a device with a stream of its own waits for
     torch's work first, and so does any device where the call has taken memory from torch's allocator (``fresh``), which torch's work may still
     be using for what it held before.  The device holds the call's tensors until its stream is done with them, so that torch does not
@@ -129,6 +135,8 @@ def _call(device, function, desc, tensors, output=None, fresh=True):
         device.check(status)
     if current != device.stream:
         device.hold(tensors)
+    elif weights is not None and weights._origin != current:
+        weights._read_on(device)
     return {"output": output, "elapsedMilliseconds": 0.0, "memory": {"peakBytes": res.peak_bytes}, "launches": res.launches}
 
 
@@ -207,9 +215,9 @@ def _matrix(device, name, value, rows, channels):
     return value
 
 
-def _encode(device, source, dtype, out, block_rows=1, transposed=None):
+def _encode(device, source, dtype, out, block_rows=1, transposed=None, weights=None):
     desc = _ENCODE.pack(*out.fields, *(transposed.fields if transposed is not None else _NO_MATRIX), _DTYPE[dtype], block_rows, source.data_ptr())
-    _call(device, device.lib.lf_float8_encode, desc, (source, out, transposed))
+    _call(device, device.lib.lf_float8_encode, desc, (source, out, transposed), weights=weights)
 
 
 def float8_encode(device, activations, rows, channels, options=None):
@@ -336,6 +344,8 @@ class Float8LinearWeights:
     who replays."""
 
     _readers = None      # other devices of the GPU that have waited for the weights, and may still be reading
+    _origin = None       # torch's current stream when the memory was allocated
+    _elsewhere = None    # devices with calls on other streams, made while those were torch's current ones
 
     def __init__(self, device: Device, weight, bias=None):
         self.device = device
@@ -347,10 +357,23 @@ class Float8LinearWeights:
         _positive("channels", self.channels)
         weight = self._on_device(weight)
         _tensor(device, "weight", weight, self.out_channels * self.channels)
-        self.bias = None
+        self.bias, self._origin = None, _torch_stream(device.ordinal)
         self.forward = Float8Tensor.empty(self.out_channels, self.channels, "e4m3", weight)
         self.transposed = Float8Tensor.empty(self.channels, self.out_channels, "e4m3", weight)
         self.update(weight, bias)
+
+    def _read_on(self, device):
+        if self._elsewhere is None:
+            self._elsewhere = weakref.WeakSet()
+        self._elsewhere.add(device)
+
+    def __del__(self):
+        """The memory goes back to the stream that it came from, which knows nothing of calls on others: their devices keep it until they are through.
+        (What a graph reads, its caller keeps.)"""
+        if self._elsewhere and not sys.is_finalizing() and not _capturing():
+            for device in self._elsewhere:
+                if device._finalizer.alive:
+                    device.hold((self.forward, self.transposed))
 
     def _on_device(self, value):
         if value is None or getattr(value, "is_cuda", False):
@@ -373,7 +396,7 @@ class Float8LinearWeights:
             if reader._finalizer.alive:      # (a closed device has finished)
                 self.device.check(self.device.lib.lf_context_await(self.device.handle, reader.stream))
         self._readers = None
-        _encode(self.device, weight, dtype, self.forward, 128, self.transposed)
+        _encode(self.device, weight, dtype, self.forward, 128, self.transposed, self)
 
 
 def prepare_float8_linear_weights(device, weight, bias=None):
@@ -391,7 +414,7 @@ class Float8LinearGpu:
     def __init__(self, device: Device | None = None):
         self.device = _device(device)
 
-    def _product(self, name, value, rows, channels, weights, bias, options, out):
+    def _product(self, name, value, rows, channels, prepared, weights, bias, options, out):
         dev, opts = self.device, options or _NO_OPTIONS
         keep, source, operand, workspace, nbytes = bool(opts.get("checkpoint")), None, None, None, 0
         format = _format(opts.get("format", "e4m3"))
@@ -413,7 +436,7 @@ class Float8LinearGpu:
         desc = _LINEAR.pack(*(operand.fields if operand is not None else (rows, channels, _FORMAT[format], 0, 0)), *weights.fields,
                             bias.data_ptr() if bias is not None else 0, _DTYPE[dtype], _DTYPE[source or "f32"], value.data_ptr() if source else 0,
                             out.data_ptr(), workspace.data_ptr() if nbytes else 0, nbytes)
-        result = _call(dev, dev.lib.lf_float8_linear_run, desc, (value, operand, weights, bias, workspace, out), out, fresh)
+        result = _call(dev, dev.lib.lf_float8_linear_run, desc, (value, operand, weights, bias, workspace, out), out, fresh, prepared)
         if keep:
             result["checkpoint"] = operand
         return result
@@ -439,13 +462,13 @@ class Float8LinearGpu:
     def run(self, input, options=None, out=None):
         """``input``: rows, channels, outChannels, activations ``[rows][channels]``, weights -> ``output`` ``[rows][outChannels]``."""
         rows, channels, _, weights = self._weights(input)
-        return self._product("activations", input["activations"], rows, channels, weights.forward, weights.bias, options, out)
+        return self._product("activations", input["activations"], rows, channels, weights, weights.forward, weights.bias, options, out)
 
     def input_gradient(self, input, options=None, out=None):
         """``input``: rows, channels, outChannels, gradient ``[rows][outChannels]``, weights -> ``output`` ``[rows][channels]``, the
         gradient of the activations."""
         rows, _, n, weights = self._weights(input)
-        return self._product("gradient", input["gradient"], rows, n, weights.transposed, None, options, out)
+        return self._product("gradient", input["gradient"], rows, n, weights, weights.transposed, None, options, out)
 
     def weight_gradient(self, input, options=None):
         """``input``: rows, channels, outChannels, gradient ``[rows][outChannels]`` (bfloat16 or a ``Float8Tensor``; a float32 gradient is

@@ -90,6 +90,77 @@ def test_memory_of_the_caller_is_ordered_by_the_caller(host):
     assert order(log) == ["lf_float8_decode"]
 
 
+@pytest.mark.parametrize("current,held", [(2, True), (T, False)])
+@pytest.mark.parametrize("what", ["run", "input_gradient", "update"])
+def test_memory_of_weights_is_held(host, monkeypatch, what, current, held):
+    """Their memory came from the pool of the stream that was torch's current one then, and goes back to it when they are dropped.  Calls that were made with
+    the device's stream as the current one are unknown there: the device keeps the memory."""
+    log = []
+    d, value = Device(log, 2), Memory(48)
+    value.shape = (6, 8)
+
+    def used():
+        mine = weights(6, 8)
+        mine.device, mine._origin = d, T
+        call, linear = {"rows": 4, "channels": 8, "outChannels": 6, "weights": mine}, lf.Float8LinearGpu(d)
+        for _ in range(3):
+            if what == "update":
+                mine.update(value)
+            elif what == "run":
+                linear.run({**call, "activations": float8(4, 8)})
+            else:
+                linear.input_gradient({**call, "gradient": float8(4, 6)})
+
+    monkeypatch.setattr(training, "_torch_stream", lambda ordinal: current)
+    used()
+    # by the device, with each call, where its stream is not the current one; else when they are dropped
+    assert order(log).count("hold") == (1 if held else 3) and order(log)[-1] == "hold"
+    log.clear()
+    d._finalizer = SimpleNamespace(alive=False)      # (a closed device is through)
+    used()
+    assert order(log).count("hold") == (0 if held else 3)
+
+
+def test_memory_of_weights_of_one_stream(host, monkeypatch):
+    log = []
+    d = Device(log, T)
+    for capturing in (False, True):
+        mine = weights(6, 8)
+        mine.device, mine._origin = d, 5 if capturing else T
+        monkeypatch.setattr(training, "_capturing", lambda: capturing)
+        lf.Float8LinearGpu(d).run({"rows": 4, "channels": 8, "outChannels": 6, "weights": mine, "activations": float8(4, 8)})
+        del mine
+        assert order(log).count("hold") == 0
+
+
+@pytest.mark.gpu
+def test_weights_dropped_while_they_are_read():
+    """Weights made under one stream, multiplied on another behind a queue, and dropped at once; their memory is written again under the first."""
+    n = 4096
+    stream = torch.cuda.Stream()
+    d = lf.Device(0, stream=stream.cuda_stream)
+    x8 = lf.float8_encode(d, torch.randn(n, n, device="cuda"), n, n)
+    w = torch.randn(n, n, device="cuda")
+    linear, call = lf.Float8LinearGpu(d), {"rows": n, "channels": n, "outChannels": n, "activations": x8}
+    want = linear.run({**call, "weights": lf.prepare_float8_linear_weights(d, w)})["output"]
+    a = torch.randn(n, n, device="cuda")
+    for _ in range(5):
+        torch.cuda.synchronize()
+        mine = lf.prepare_float8_linear_weights(d, w)
+        torch.cuda.synchronize()
+        d.synchronize()
+        with torch.cuda.stream(stream):
+            for _ in range(10):
+                a = (a @ a) * 1e-2
+            got = linear.run({**call, "weights": mine})["output"]
+        del mine
+        junk = [torch.full((n * n + 4096 * k,), 255, dtype=torch.uint8, device="cuda") for k in (0, 32, 64)]
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+        del junk
+    d.close()
+
+
 OPERATORS = ["encode", "decode", "norm", "backward", "linear", "weight gradient"]
 
 
