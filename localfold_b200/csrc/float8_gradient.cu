@@ -9,7 +9,7 @@
 //
 // The tensor core's additions to an accumulator truncate: their error grows with how many there are (one for 16 rows).  So all of the 512 columns of tensor
 // memory are accumulators that take steps in turn (two of 256 channels, or four of 128, for one block of outputs), added up in registers at the end, and
-// a split has 4096 rows at most.
+// a split has 4096 rows at most (more only beyond 65535 such splits).
 //
 // Products are dW's n x k in tiles of 128 x 256 or 256 x 256 over all rows; there are few tiles and many rows, so the rows are split over as many
 // blocks as the GPU has room for, each writes its float32 partial tile, and a second kernel adds them in order.
@@ -484,7 +484,7 @@ void configure_float8_gradient() {
 static int gradient_blocks(int64_t m, int n, int k) { return n > WG_BN && (double)m * n * k >= (k <= 128 ? 2147483648.0 : 4294967296.0) ? 2 : 1; }
 
 // Blocks of rows: as many as the GPU has multiprocessors for beside the tiles, with four steps of 64 rows each at least - and 64 at most: the tensor core's
-// additions truncate, and 65536 x 1024 x 1024 with values of one sign was 3.5e-5 off in sums of 16384 rows (5.8e-6 in 4096).
+// additions truncate, and 65536 x 1024 x 1024 with values of one sign was 3.5e-5 off in sums of 16384 rows (4.8e-6 in 4096).
 static void gradient_plan(const lf_context* ctx, int64_t m, int n, int k, int& steps, int& splits, int& per_split) {
   constexpr int kMostSteps = 64, kMostSplits = 65535;      // (of the grid; beyond 64 * 65535 steps splits are longer)
   const int outputs = WG_BN * gradient_blocks(m, n, k);

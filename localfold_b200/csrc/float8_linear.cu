@@ -28,6 +28,13 @@ constexpr int F8_BM = 128, F8_BK = 128;      // a k step is a block of the forma
 constexpr int F8_A_BYTES = F8_BM * F8_BK;
 constexpr int F8_DEEP = 1024;                // channels from which the deeper ring pays (4096 x 4096 -> 4096: 57.3 -> 54.2 us)
 
+// Places in tensor memory for a group's exponents, in turn.  A group writes its place when its first step's loads are here and its tile's accumulator is free; the products that
+// read the place before it, F8_SLOTS groups back, have to be done then.  If they belong to a tile `accumulators` or more back, the accumulator's wait says so (a tile has
+// at least one group).  Otherwise the groups between lie in at most two tiles, so that all but one of them have four steps, and the last of those products is
+// 4 (F8_SLOTS - 2) + 2 steps back or more: the ring's wait for the step `stages` back says so.
+constexpr int F8_SLOTS = 4;
+__host__ __device__ constexpr bool slots_suffice(int stages, int accumulators) { return accumulators <= 2 && accumulators <= F8_SLOTS && stages <= 4 * (F8_SLOTS - 2) + 2; }
+
 struct Float8Params {
   int m, n, k;
   int vector_out;              // rows start on 16-byte boundaries: they leave by TMA
@@ -154,6 +161,7 @@ struct Float8Shape {
   static constexpr int share = DEEP ? 128 : 64, epi = 4 * (BN / share), staging = DEEP ? 2048 : 4096;
   static constexpr int threads = 64 + 32 * epi;
   static constexpr int smem = stages * (stage + scales) + epi * (staging + share * 4) + 256 + 1024;
+  static_assert(slots_suffice(stages, accumulators), "");
 };
 
 template <int BN, bool F32, bool DEEP>
@@ -238,9 +246,8 @@ float8_linear_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_cons
         if (!__all_sync(0xffffffffu, mbar_wait(&full[stage], phase, abort_flag, p.status, 123))) { ok = false; break; }      // (for all lanes alike)
         tc_fence_after();
         const uint64_t a = a_first + (uint32_t)(stage * S::stage >> 4), b = b_first + (uint32_t)(stage * S::stage >> 4);
-        // Four slots in turn: when a group's first step is here, the step `stages` <= 6 before it is complete, and with it
-        // the group before last; the slot's last reader is four groups back.
-        if ((kb & 3) == 0) scales = tmem_base + 256 + (group++ & 3) * 16;
+        // Slots in turn (see F8_SLOTS): the slot's last reader, four groups back, is done.
+        if ((kb & 3) == 0) scales = tmem_base + 256 + (group++ % F8_SLOTS) * 16;
         if (elect_one()) {
           if ((kb & 3) == 0) {
             const uint64_t sc = scale_first + (uint32_t)(stage * S::scales >> 4);
@@ -317,6 +324,7 @@ struct PairShape {
   static constexpr int accumulators = BN == 256 ? 1 : 2, scale_columns = accumulators * BN;      // (and where the scales begin)
   static constexpr int share = BN == 256 ? 128 : 64, epi = 4 * (BN / share), staging = 2048, threads = 64 + 32 * epi;
   static constexpr int smem = stages * (stage + scales) + epi * (staging + share * 4) + 256 + 1024;
+  static_assert(slots_suffice(stages, accumulators), "");
 };
 
 template <int BN, bool F32>
@@ -401,7 +409,7 @@ float8_pair_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_consta
           if (!__all_sync(0xffffffffu, mbar_wait_cluster(&full[stage], phase, abort_flag, p.status, 143))) { ok = false; break; }
           tc_fence_after();
           const uint64_t a = a_first + (uint32_t)(stage * S::stage >> 4), b = b_first + (uint32_t)(stage * S::stage >> 4);
-          if ((kb & 3) == 0) scales = tmem_base + S::scale_columns + (group++ & 3) * 16;      // (four slots in turn, as above)
+          if ((kb & 3) == 0) scales = tmem_base + S::scale_columns + (group++ % F8_SLOTS) * 16;      // (as above)
           if (elect_one()) {
             if ((kb & 3) == 0) {
               const uint64_t sc = scale_first + (uint32_t)(stage * S::scales >> 4);
