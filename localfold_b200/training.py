@@ -66,17 +66,21 @@ def _size(inp, name):
 
 
 _names = {}      # torch dtype -> "f32" | "bf16"
+_Tensor = None   # torch.Tensor, with the first
 
 
 def _torch():
+    global _Tensor
     import torch
     if not _names:
+        _Tensor = torch.Tensor
         _names.update({torch.float32: "f32", torch.bfloat16: "bf16"})
     return torch
 
 
 def _has_memory(name, value):
-    """A fake tensor or one that a function transform has wrapped passes every other check; the library would take it for one that was left out."""
+    """A fake tensor passes every other check; the library would take it for one that was left out.  (One that a function transform has wrapped raises as soon as its
+    address is asked for.)"""
     try:
         if value.data_ptr():
             return
@@ -91,7 +95,7 @@ def _tensor(device, name, value, count, only=None):
     if getattr(value, "is_cuda", False) and value.get_device() == device.ordinal:
         dtype = _names.get(value.dtype)
         try:
-            if dtype is not None and (only is None or only == dtype) and value.numel() == count and value.is_contiguous() and value.data_ptr():
+            if dtype is not None and (only is None or only == dtype) and value.numel() == count and value.is_contiguous() and (type(value) is _Tensor or value.data_ptr()):
                 return dtype
         except RuntimeError:      # (no address: below)
             pass
@@ -158,11 +162,23 @@ def _new(like, dtype, shape):
         proto.data_ptr()
         _empty[key] = proto
     value = proto.new_empty(shape)
-    return value if type(value) is type(proto) else _plain(value)
+    return value if type(value) is _Tensor else _plain(value)
+
+
+def _like(value, dtype):
+    """New memory of a tensor's kind and shape.  (For a plain tensor in half the time of ``_new``.)"""
+    out = _torch().empty_like(value)
+    return out if type(out) is _Tensor else _new(value, dtype, value.shape)
+
+
+def _two(like, count):
+    """Twice ``count`` new values of a float32 tensor's kind."""
+    one, two = like.new_empty(count), like.new_empty(count)
+    return (one, two) if type(one) is _Tensor else (_new(like, "f32", count), _new(like, "f32", count))
 
 
 def _plain(value):
-    if type(value) is not _torch().Tensor:
+    if type(value) is not _Tensor:
         raise ValueError(f"the operators allocate memory of their own, not {type(value).__name__}s")
     return value
 
@@ -181,7 +197,8 @@ class Float8Tensor:
             raise ValueError("memory must be a contiguous uint8 CUDA tensor")
         if memory.numel() != self._codes + exponents:
             raise RangeError(f"memory has {memory.numel()} values; expected {self._codes + exponents}")
-        _has_memory("memory", memory)
+        if type(memory) is not _Tensor:
+            _has_memory("memory", memory)
         base = memory.data_ptr()
         self.fields = (rows, channels, _FORMAT[format], base, base + self._codes)
 
@@ -288,17 +305,17 @@ class LayerNormGpu:
         if given:
             _tensor(dev, "out", out, rows * c, dtype)
         elif not encode:
-            out = _new(x, dtype, x.shape)
+            out = _like(x, dtype)
         checkpoint = Float8Tensor.empty(rows, c, kept, x) if kept else None
         encoded = Float8Tensor.empty(rows, c, encode, x) if encode else None
-        fresh = not given or kept is not None or encode is not None or bool(opts.get("statistics"))
         mean = inverse = None
-        if kept or opts.get("statistics"):
-            mean, inverse = _new(scale, "f32", rows), _new(scale, "f32", rows)
+        statistics = kept or opts.get("statistics")
+        if statistics:
+            mean, inverse = _two(scale, rows)
         desc = _LAYER_NORM.pack(rows, c, variance, _DTYPE[dtype], epsilon, x.data_ptr(), scale.data_ptr(), offset.data_ptr(),
                                 out.data_ptr() if out is not None else 0, 0 if mean is None else mean.data_ptr(), 0 if mean is None else inverse.data_ptr(),
                                 *(checkpoint.fields if kept else _NO_MATRIX), *(encoded.fields if encode else _NO_MATRIX))
-        result = _call(dev, dev.lib.lf_layer_norm_run, desc, (x, scale, offset, out, mean, inverse, checkpoint, encoded), encoded if encode else out, fresh)
+        result = _call(dev, dev.lib.lf_layer_norm_run, desc, (x, scale, offset, out, mean, inverse, checkpoint, encoded), encoded if encode else out, not given or bool(statistics))
         if mean is not None:
             result["mean"], result["inverseDeviation"] = mean, inverse
         if kept:
@@ -325,9 +342,10 @@ class LayerNormGpu:
         if out is not None:
             _tensor(dev, "out", out, rows * c, dtype)
         else:
-            out = _new(dy, dtype, dy.shape)
+            out = _like(dy, dtype)
         nbytes = dev.lib.lf_layer_norm_backward_workspace(dev.handle, rows, c)
-        dscale, doffset, workspace = _new(scale, "f32", c), _new(scale, "f32", c), _new(scale, "bytes", nbytes) if nbytes else None
+        dscale, doffset = _two(scale, c)
+        workspace = _new(scale, "bytes", nbytes) if nbytes else None
         desc = _LAYER_NORM_BACKWARD.pack(rows, c, _DTYPE[dtype], dy.data_ptr(), 0 if encoded else x.data_ptr(), *(x.fields if encoded else _NO_MATRIX),
                                          mean.data_ptr(), inverse.data_ptr(), scale.data_ptr(), out.data_ptr(), dscale.data_ptr(), doffset.data_ptr(), workspace.data_ptr() if nbytes else 0, nbytes)
         result = _call(dev, dev.lib.lf_layer_norm_backward_run, desc, (dy, x, mean, inverse, scale, out, dscale, doffset, workspace), out)
@@ -486,7 +504,7 @@ class Float8LinearGpu:
             _tensor(dev, "gradient", dy, rows * n, "bf16")
         nbytes = dev.lib.lf_float8_weight_gradient_workspace(dev.handle, rows, channels, n)
         weight = _new(x.memory, "f32", (n, channels))
-        bias, workspace = _new(weight, "f32", n), _new(weight, "bytes", nbytes) if nbytes else None
+        bias, workspace = weight.new_empty(n), _new(weight, "bytes", nbytes) if nbytes else None
         desc = _WEIGHT_GRADIENT.pack(*x.fields, 0 if encoded else dy.data_ptr(), *(dy.fields if encoded else _NO_MATRIX), n, 0, weight.data_ptr(), bias.data_ptr(),
                                      workspace.data_ptr() if nbytes else 0, nbytes)
         result = _call(dev, dev.lib.lf_float8_weight_gradient_run, desc, (dy, x, weight, bias, workspace), weight)
