@@ -131,6 +131,8 @@ def _call(device, function, desc, tensors, output=None, fresh=True, weights=None
     be using for what it held before.  The device holds the call's tensors until its stream is done with them, so that torch does not
     give their memory away before."""
     current = _torch_stream(device.ordinal)
+    if current != device.stream and _capturing():      # (the device's stream would run outside the graph, or be left in it)
+        raise RuntimeError(f"a call is captured on its device's stream ({device.stream:#x}); torch's current stream ({current:#x}) is being captured: make the Device on it")
     if current != device.stream and (device._own_stream or fresh):
         device.check(device.lib.lf_context_await(device.handle, current))
     res = nat.Result()

@@ -45,6 +45,46 @@ def test_one_wait_an_update(monkeypatch):
         assert sorted(e[1:3] for e in log if e[0] == "lf_context_await") == [(1, 2), (1, 3)] and log[-1][0] == "lf_float8_encode"
 
 
+@pytest.mark.parametrize("own", [False, True])
+def test_capture_on_another_stream_is_refused(monkeypatch, own):
+    """... before anything of the call has reached the device's stream."""
+    monkeypatch.setattr(training, "_torch_stream", lambda ordinal: 1)
+    monkeypatch.setattr(training, "_capturing", lambda: True)
+    log = []
+    d, w = FakeDevice(log, 2), weights(6, 8)
+    d._own_stream, w.device = own, d
+    call = {"rows": 4, "channels": 8, "outChannels": 6, "activations": float8(4, 8), "weights": w}
+    with pytest.raises(RuntimeError, match="a call is captured on its device's stream"):
+        lf.Float8LinearGpu(d).run(call, None, Fake(24, torch.bfloat16))
+    assert not log
+    d.stream = 1
+    lf.Float8LinearGpu(d).run(call, None, Fake(24, torch.bfloat16))
+    assert [e[0] for e in log] == ["lf_float8_linear_run"]
+
+
+@pytest.mark.gpu
+def test_capture_goes_on_after_a_refusal():
+    """A device with a stream of its own, called while torch captures another: refused, the graph holds the rest, and the device works as before."""
+    d = lf.Device(0)
+    x = torch.randn(64, 128, device="cuda")
+    want = lf.float8_decode(d, lf.float8_encode(d, x, 64, 128), {"output": "f32"})
+    d.synchronize()
+    stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=stream):
+        y = x * 2
+        with pytest.raises(RuntimeError, match="a call is captured on its device's stream"):
+            lf.float8_encode(d, x, 64, 128)
+        z = y + 1
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(z, x * 2 + 1)
+    got = lf.float8_decode(d, lf.float8_encode(d, x, 64, 128), {"output": "f32"})
+    d.synchronize()
+    assert torch.equal(got, want)
+    d.close()
+
+
 @pytest.mark.gpu
 def test_captured_on_another_device():
     stream = torch.cuda.Stream()
