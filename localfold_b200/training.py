@@ -405,6 +405,8 @@ class Float8LinearWeights:
     def update(self, weight, bias=_AS_IT_WAS):
         """A new weight (float32 or bfloat16 CUDA tensor, or host array) and, if given, a new bias (float32, or None).  The bias tensor is
         not copied: calls read what it holds."""
+        if not self.device._finalizer.alive:
+            raise ValueError("the weights' device is closed: they can be read, by other devices, and not updated")
         weight, bias = self._on_device(weight), self.bias if bias is _AS_IT_WAS else self._on_device(bias)
         if weight.shape != (self.out_channels, self.channels):
             raise RangeError(f"weight is {tuple(weight.shape)}; expected {(self.out_channels, self.channels)}")

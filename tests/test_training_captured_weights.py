@@ -45,6 +45,19 @@ def test_one_wait_an_update(monkeypatch):
         assert sorted(e[1:3] for e in log if e[0] == "lf_context_await") == [(1, 2), (1, 3)] and log[-1][0] == "lf_float8_encode"
 
 
+def test_update_after_close_is_refused(monkeypatch):
+    """The context that would encode the values is gone."""
+    monkeypatch.setattr(training, "_torch_stream", lambda ordinal: 1)
+    log = []
+    owner, w, value = FakeDevice(log, 1), weights(6, 8), Fake(48)
+    w.device, value.shape = owner, (6, 8)
+    w.update(value)
+    owner._finalizer.alive = False
+    with pytest.raises(ValueError, match="the weights' device is closed"):
+        w.update(value)
+    assert [e[0] for e in log] == ["lf_float8_encode"]
+
+
 @pytest.mark.parametrize("own", [False, True])
 def test_capture_on_another_stream_is_refused(monkeypatch, own):
     """... before anything of the call has reached the device's stream."""

@@ -99,7 +99,7 @@ def test_memory_of_weights_is_held(host, monkeypatch, what, current, held):
     d, value = Device(log, 2), Memory(48)
     value.shape = (6, 8)
 
-    def used():
+    def used(closed=False):
         mine = weights(6, 8)
         mine.device, mine._origin = d, T
         call, linear = {"rows": 4, "channels": 8, "outChannels": 6, "weights": mine}, lf.Float8LinearGpu(d)
@@ -110,14 +110,15 @@ def test_memory_of_weights_is_held(host, monkeypatch, what, current, held):
                 linear.run({**call, "activations": float8(4, 8)})
             else:
                 linear.input_gradient({**call, "gradient": float8(4, 6)})
+        if closed:
+            d._finalizer = SimpleNamespace(alive=False)      # (a closed device is through)
 
     monkeypatch.setattr(training, "_torch_stream", lambda ordinal: current)
     used()
     # by the device, with each call, where its stream is not the current one; else when they are dropped
     assert order(log).count("hold") == (1 if held else 3) and order(log)[-1] == "hold"
     log.clear()
-    d._finalizer = SimpleNamespace(alive=False)      # (a closed device is through)
-    used()
+    used(closed=True)
     assert order(log).count("hold") == (0 if held else 3)
 
 
