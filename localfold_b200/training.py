@@ -359,11 +359,11 @@ class LayerNormGpu:
 class Float8LinearWeights:
     """A projection's weight ``[outChannels][channels]`` on the device in e4m3, one power of two for every 128 x 128 elements, in both
     orientations (the transposed one multiplies gradients), and its bias.  ``update`` encodes new values into the same memory, as
-    a training step does; calls enqueued before it, on this device or another of the same GPU, have read the old ones.  Another device waits for the
-    weights at its first call after an update; that call cannot be captured, later ones can.  Replays are ordered with updates by
+    a training step does; calls enqueued before it, on this device or another of the same GPU, have read the old ones.  Calls of another device wait for the
+    weights; one that is captured cannot, and takes them as the first call after an update has found them.  Replays are ordered with updates by
     who replays."""
 
-    _readers = None      # other devices of the GPU that have waited for the weights, and may still be reading
+    _readers = None      # other devices of the GPU that have waited for the weights since the last update, and may still be reading
     _origin = None       # torch's current stream when the memory was allocated
     _elsewhere = None    # devices with calls on other streams, made while those were torch's current ones
 
@@ -474,10 +474,10 @@ class Float8LinearGpu:
                 raise ValueError(f"weights are on cuda:{weights.device.ordinal}, the device's GPU is cuda:{self.device.ordinal}")
             if weights._readers is None:
                 weights._readers = weakref.WeakSet()
-            if self.device not in weights._readers:
-                if weights.device._finalizer.alive:      # (encoded on its stream)
-                    self.device.check(self.device.lib.lf_context_await(self.device.handle, weights.device.stream))
-                weights._readers.add(self.device)
+            # (encoded on its stream, by a replayed graph perhaps; a captured call cannot wait and need not where one before it has)
+            if weights.device._finalizer.alive and not (self.device in weights._readers and _capturing()):
+                self.device.check(self.device.lib.lf_context_await(self.device.handle, weights.device.stream))
+            weights._readers.add(self.device)
         if (weights.out_channels, weights.channels) != (n, channels):
             raise RangeError(f"weights are {weights.out_channels} x {weights.channels}; expected {n} x {channels}")
         return rows, channels, n, weights

@@ -24,9 +24,11 @@ def test_wait_in_a_capture_is_refused(tmp_path):
     assert "a call that is being captured cannot wait" in fake_cuda.run(tmp_path, WAIT)
 
 
-def test_one_wait_an_update(monkeypatch):
-    """A device waits for the weights once after each update, so that what follows can be captured."""
-    monkeypatch.setattr(training, "_torch_stream", lambda ordinal: 1)
+def test_captured_calls_do_not_wait(monkeypatch):
+    """A device waits for the weights with every call (their own may replay a graph that encodes them), but for captured ones after the first since an update."""
+    capturing = []
+    monkeypatch.setattr(training, "_torch_stream", lambda ordinal: 1 if not capturing else capturing[0])
+    monkeypatch.setattr(training, "_capturing", lambda: bool(capturing))
     log = []
     owner, users = FakeDevice(log, 1), [FakeDevice(log, 2), FakeDevice(log, 3)]
     w, value = weights(6, 8), Fake(48)
@@ -34,15 +36,22 @@ def test_one_wait_an_update(monkeypatch):
     call = {"rows": 4, "channels": 8, "outChannels": 6, "activations": float8(4, 8), "weights": w}
     back = {"rows": 4, "channels": 8, "outChannels": 6, "gradient": float8(4, 6), "weights": w}
     for _ in range(3):
-        log.clear()
-        for _ in range(3):
-            for user in users:
+        for user in users:
+            log.clear()
+            for captured in (False, True, False, True):
+                capturing[:] = [user.stream] if captured else []
                 lf.Float8LinearGpu(user).run(call, None, Fake(24, torch.bfloat16))
                 lf.Float8LinearGpu(user).input_gradient(back, None, Fake(32, torch.bfloat16))
-        assert [e[1:3] for e in log if e[0] == "lf_context_await"] == [(2, 1), (3, 1)]
+            assert [e[1:3] for e in log if e[0] == "lf_context_await"] == 4 * [(user.stream, 1)]
+        capturing.clear()
         log.clear()
         w.update(value)
         assert sorted(e[1:3] for e in log if e[0] == "lf_context_await") == [(1, 2), (1, 3)] and log[-1][0] == "lf_float8_encode"
+        log.clear()
+        capturing[:] = [2]      # (the first call after an update: the library refuses the wait)
+        lf.Float8LinearGpu(users[0]).run(call, None, Fake(24, torch.bfloat16))
+        assert [e[1:3] for e in log if e[0] == "lf_context_await"] == [(2, 1)]
+        capturing.clear()
 
 
 def test_update_after_close_is_refused(monkeypatch):
@@ -131,5 +140,41 @@ def test_captured_on_another_device():
         new = linear.run(call)["output"]
     stream.synchronize()
     assert torch.equal(got, new) and not torch.equal(got, want)
+    owner.close()
+    user.close()
+
+
+@pytest.mark.gpu
+def test_weights_that_a_graph_encodes():
+    """A graph on the weights' stream encodes them anew at each replay, behind a queue; another device's next call has the new values."""
+    n = 2048
+    stream = torch.cuda.Stream()
+    owner, user = lf.Device(0, stream=stream.cuda_stream), lf.Device(0)
+    source, x = torch.zeros(n, n, device="cuda"), torch.randn(64, n, device="cuda")
+    w = lf.prepare_float8_linear_weights(owner, source)
+    call, linear = {"rows": 64, "channels": n, "outChannels": n, "activations": x, "weights": w}, lf.Float8LinearGpu(user)
+    torch.cuda.synchronize()
+    a, graph = torch.randn(n, n, device="cuda"), torch.cuda.CUDAGraph()
+    with torch.cuda.stream(stream):
+        w.update(source)
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph, stream=stream):
+            w.update(source)
+    linear.run(call)
+    user.synchronize()
+    for _ in range(5):
+        fresh = torch.randn(n, n, device="cuda")
+        want = linear.run({**call, "weights": lf.prepare_float8_linear_weights(user, fresh)})["output"]
+        user.synchronize()
+        source.copy_(fresh)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            for _ in range(30):
+                a = (a @ a) * 1e-2
+            graph.replay()
+        got = linear.run(call)["output"]
+        user.synchronize()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
     owner.close()
     user.close()
