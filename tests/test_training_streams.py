@@ -214,3 +214,18 @@ def test_memory_in_use_on_another_stream(name, own):
         del got
     assert met, "the result never took the memory: this shows nothing"
     d.close()
+
+
+@pytest.mark.gpu
+def test_default_stream_device_beside_a_side_stream():
+    """A device on CUDA's default stream, called while torch's current stream is another."""
+    d, side = lf.Device(0, stream=0), torch.cuda.Stream()
+    x = torch.randn(3000, 256, device="cuda")
+    want = lf.float8_decode(d, lf.float8_encode(d, x, 3000, 256), {"output": "f32"})
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        for _ in range(5):
+            got = lf.float8_decode(d, lf.float8_encode(d, x, 3000, 256), {"output": "f32"})
+            d.synchronize()
+            assert torch.equal(got, want)
+    d.close()
