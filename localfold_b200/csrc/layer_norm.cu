@@ -308,6 +308,7 @@ lf_status lf_layer_norm_run(lf_context* ctx, const lf_layer_norm_desc* d, lf_res
     if (m->codes) LF_TRY(lf_float8_check(ctx, "layer norm", *m, d->rows, d->channels));
   const uint64_t bytes = (uint64_t)d->rows * d->channels * (d->act_dtype == LF_DTYPE_BF16 ? 2 : 4);
   if (d->out && d->out != d->activations) LF_TRY(lf_float8_apart(ctx, "layer norm", d->out, bytes, d->activations, bytes));
+  for (const float* operand : {d->scale, d->offset}) LF_TRY(lf_float8_apart(ctx, "layer norm", d->out, bytes, operand, (uint64_t)d->channels * 4));
   const lf_device_guard device(ctx);
   Forward a{};
   a.rows = d->rows; a.c = d->channels; a.epsilon = d->epsilon;
@@ -343,6 +344,8 @@ lf_status lf_layer_norm_backward_run(lf_context* ctx, const lf_layer_norm_backwa
   for (const void* operand : {d->gradient, d->activations})      // (a row is read by the lanes that store it, before they do)
     if (operand && d->out != operand) LF_TRY(lf_float8_apart(ctx, "layer norm backward", d->out, bytes, operand, bytes));
   LF_TRY(lf_float8_apart(ctx, "layer norm backward", d->out, bytes, d->checkpoint));
+  for (const float* operand : {d->mean, d->inverse_deviation}) LF_TRY(lf_float8_apart(ctx, "layer norm backward", d->out, bytes, operand, (uint64_t)d->rows * 4));
+  LF_TRY(lf_float8_apart(ctx, "layer norm backward", d->out, bytes, d->scale, (uint64_t)d->channels * 4));
   const uint64_t need = lf_layer_norm_backward_workspace(ctx, d->rows, d->channels);
   if (need && (!d->workspace || d->workspace_bytes < need || !lf_aligned16(d->workspace)))
     return lf_fail(ctx, LF_ERR_ARGUMENT, "layer norm backward: a workspace of %llu bytes on a 16-byte boundary is needed", (unsigned long long)need);

@@ -50,16 +50,16 @@ for rows in (1, 4, 16, 17, 5000):
         for at in (kept.codes, kept.codes + 16 * rows - 8, kept.exponents):
             refused("lf_float8_decode", decode(at))
 
-        norm = lambda out: nat.LayerNormDesc(rows=rows, channels=c, variance=1, act_dtype=dtype, epsilon=1e-5, activations=x, scale=ones, offset=ones, out=out)
-        back = lambda out, **k: nat.LayerNormBackwardDesc(**{**dict(rows=rows, channels=c, act_dtype=dtype, gradient=x, activations=w, mean=ones, inverse_deviation=ones, scale=ones, out=out,
-                                                                     scale_gradient=ones, offset_gradient=ones, workspace=room, workspace_bytes=1 << 24), **k})
+        norm = lambda out: nat.LayerNormDesc(rows=rows, channels=c, variance=1, act_dtype=dtype, epsilon=1e-5, activations=x, scale=ones, offset=ones + (1 << 20), out=out)
+        back = lambda out, **k: nat.LayerNormBackwardDesc(**{**dict(rows=rows, channels=c, act_dtype=dtype, gradient=x, activations=w, mean=ones, inverse_deviation=ones + (1 << 20), scale=ones + (1 << 21), out=out,
+                                                                     scale_gradient=ones + (1 << 22), offset_gradient=ones + (1 << 23), workspace=room, workspace_bytes=1 << 24), **k})
         taken("lf_layer_norm_run", norm(out))
         taken("lf_layer_norm_run", norm(x))
-        for at in (x + size, x - size, x + whole - size):
+        for at in (x + size, x - size, x + whole - size, ones, ones + 4 * c - size, ones + (1 << 20) + 4):
             refused("lf_layer_norm_run", norm(at))
         for at in (out, x, w):
             taken("lf_layer_norm_backward_run", back(at))
-        for at in (x + size, x - size, w + size, w + whole - size):
+        for at in (x + size, x - size, w + size, w + whole - size, ones, ones + 4 * rows - size, ones + (1 << 20), ones + (1 << 21) + 4):
             refused("lf_layer_norm_backward_run", back(at))
         kept = matrix(rows, c, w)
         taken("lf_layer_norm_backward_run", back(x, activations=None, checkpoint=kept))
